@@ -50,6 +50,9 @@ typedef struct vh_block vh_block;         /* prepared DA3-BASE encoder block */
 typedef struct vh_linear_q8 vh_linear_q8; /* projection with BlockQ8_0 weights */
 typedef struct vh_conv2d vh_conv2d;       /* prepared 2-D convolution (DPT head) */
 typedef struct vh_conv_transpose2d vh_conv_transpose2d; /* prepared transposed convolution */
+typedef struct vh_index vh_index;         /* device int32 values */
+typedef struct vh_rope vh_rope;           /* prepared rotation of several position axes */
+typedef struct vh_kv_cache vh_kv_cache;   /* paged cache of keys and values */
 
 /* ---- errors --------------------------------------------------------------- */
 /* Message of the calling thread's last failure ("" if none). */
@@ -396,6 +399,93 @@ vh_status vh_bilinear_resize_f32(const vh_runtime *rt, const vh_tensor *input, s
 vh_status vh_bilinear_resize_align_corners_f32(const vh_runtime *rt, const vh_tensor *input,
                                                size_t c, size_t ih, size_t iw, size_t oh,
                                                size_t ow, const vh_tensor *add, vh_tensor **out);
+
+/* ---- streams of frames: index tensors ---------------------------------------- */
+/* No counterpart in the reference, here and down to the profiling section: what a
+ * program needs that feeds the encoder frame after frame, or token after token.
+ * Every handle of a call has to belong to one runtime (clones count as one);
+ * others are refused with VH_ERR_INVALID_ARGUMENT, as is an output that is also
+ * an input or another output, unless the call allows it. */
+/* Device int32 values: positions, slots, lengths, page tables. */
+vh_status vh_upload_i32(const vh_runtime *rt, const int *values, size_t len, vh_index **out);
+/* Synchronising; out_len must equal the index's length. */
+vh_status vh_download_i32(const vh_runtime *rt, const vh_index *index, int *out, size_t out_len);
+/* Uninitialised. */
+vh_status vh_index_alloc(const vh_runtime *rt, size_t len, vh_index **out);
+void vh_index_free(vh_index *index);
+size_t vh_index_len(const vh_index *index);
+int *vh_index_device_ptr(const vh_index *index);
+
+/* ---- rotary positions of several axes ----------------------------------------- */
+/* vh_rope2d_f32_in_place for 1 to 4 axes (time, height, width, ...): axis a owns
+ * pairs[a] >= 1 rotated pairs, together at most head_dim / 2; the other dims pass.
+ * shared_spectrum = 0: axis a has the 2 pairs[a] dims from o = 2 (pairs[0] + .. +
+ * pairs[a-1]); its pair j is dims (o + j, o + pairs[a] + j), turned by
+ * position[a] * frequency^(-j / pairs[a]).  With two axes of head_dim / 4 pairs that
+ * is rope2d.  shared_spectrum = 1: with n pairs in all, pair i is dims (i, n + i),
+ * turned by position[axis of i] * frequency^(-i / n), where the first pairs[0] are
+ * axis 0's, the next pairs[1] axis 1's and so on.
+ * Angles are formed in 64 bits, so far positions of a long stream keep theirs.
+ * head_dim is a multiple of 4 up to 256, frequency finite and positive.  One call
+ * here takes at most 2^27 tokens, and so do the cache's. */
+vh_status vh_prepare_rope_axes(const vh_runtime *rt, size_t head_dim, size_t axes, const size_t *pairs,
+                               float frequency, int shared_spectrum, vh_rope **out);
+void vh_rope_free(vh_rope *rope);
+/* x and out [heads, tokens, head_dim], or [tokens, heads, head_dim] when
+ * token_major; out may be x.  positions [tokens * axes], all axes of a token
+ * together; any int32. */
+vh_status vh_rope_axes_run(const vh_rope *rope, const vh_tensor *x, size_t heads, size_t tokens,
+                           int token_major, const vh_index *positions, vh_tensor *out);
+
+/* ---- paged cache of keys and values --------------------------------------------- */
+/* `pages` pages of page_tokens (a power of two up to 4096) tokens, each with
+ * kv_heads rows of head_dim (a multiple of 4 up to 128) of K and of V, all zeros at
+ * first.  Row i of page p is slot p * page_tokens + i.  type 0: floats; 1: bfloat16
+ * (rounded to nearest even; any finite float short of the last half step keeps
+ * finite); 2: BlockQ8_0 blocks of a row's dims (quantize_row_q8_0, src/q8_0_dot.rs:
+ * 27-46, bit-exact; head_dim % 32 == 0).  Rows are stored 64 or 128 wide.  At most
+ * 2^31 - 4096 slots.  Not to be made inside a stream capture. */
+vh_status vh_kv_cache_new(const vh_runtime *rt, int type, size_t pages, size_t page_tokens,
+                          size_t kv_heads, size_t head_dim, vh_kv_cache **out);
+void vh_kv_cache_free(vh_kv_cache *cache);
+size_t vh_kv_cache_slots(const vh_kv_cache *cache);
+/* Writes K and V rows of `tokens` tokens ([kv_heads, tokens, head_dim], or
+ * [tokens, kv_heads, head_dim] when token_major) to slots[token]; a slot below 0 or
+ * past the cache is not written.  `slots` holds at least `tokens` values; the
+ * same slot twice leaves either token's values or a mixture. */
+vh_status vh_kv_cache_append_f32(vh_kv_cache *cache, const vh_tensor *k, const vh_tensor *v,
+                                 size_t tokens, int token_major, const vh_index *slots);
+/* The same from rows of a QKV projection, [tokens, (heads + 2 kv_heads) *
+ * head_dim] as vh_linear_run writes them (Q, then K, then V, heads in order): Q
+ * and K are rotated when `rope` is non-NULL (positions as in vh_rope_axes_run; NULL
+ * without it), K and V go to their slots and Q to q_out [tokens, heads, head_dim],
+ * in one launch.  heads % kv_heads == 0.  Every Q row is written, whatever its slot. */
+vh_status vh_kv_cache_append_qkv_f32(vh_kv_cache *cache, const vh_rope *rope, const vh_tensor *qkv,
+                                     size_t heads, size_t tokens, const vh_index *positions,
+                                     const vh_index *slots, vh_tensor *q_out);
+/* The stored rows of `tokens` slots as floats: k and v [tokens, kv_heads,
+ * head_dim]; zeros where a slot is below 0 or past the cache. */
+vh_status vh_kv_cache_gather_f32(const vh_kv_cache *cache, const vh_index *slots, size_t tokens,
+                                 vh_tensor *k, vh_tensor *v);
+/* Block tables and slot maps of one step, built on the device from the requests'
+ * lengths: request r has cached[r] tokens and gets added[r] (values below 0 count as
+ * 0) that take the next places of a padded batch of `tokens`.
+ *   starts [requests + 1]   first new token of each request; the last is their sum
+ *   lens [requests]         cached[r] and the new tokens of r
+ *   slots [tokens]          slot of each new token; -1 behind the last request
+ *   table [requests, max_pages]  in and out: a request's pages in order, of which
+ *                           the first ceil(cached[r] / page_tokens) are read and those
+ *                           that it gets now are written
+ *   free_next [1]           free_start and the number of pages taken
+ * Pages come from free_pages[free_start ..] in the order of the requests.  Where the
+ * list ends, page -1 is entered and the tokens get slot -1 (free_next past the list's
+ * length says so), as tokens past the table's row and past `tokens` (which then do not
+ * count in starts and lens) do.  The next step passes lens as cached and free_next as
+ * free_start.  At most 4096 requests and 2^31 - 1 tokens. */
+vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const vh_index *added,
+                             size_t requests, const vh_index *free_pages, const vh_index *free_start,
+                             size_t page_tokens, vh_index *table, size_t max_pages, vh_index *starts,
+                             vh_index *lens, vh_index *slots, size_t tokens, vh_index *free_next);
 
 /* ---- profiling (device twin of DA3_FLASH_PROFILE, src/specialized.rs:1324) - */
 /* When enabled, every kernel launch is bracketed by HIP events on the

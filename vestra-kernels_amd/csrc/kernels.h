@@ -313,4 +313,56 @@ hipError_t launch_gemm_q8_0_qkv(hipStream_t s, const int8_t *a_qs, const uint16_
                                 const float *bias, float *q, float *kk, float *v, size_t tokens,
                                 size_t heads, const float *rot);
 
+// ---- paged cache of keys and values (k_cache.hip) ---------------------------
+// What a cache holds a value in.
+constexpr int kCacheF32 = 0, kCacheBf16 = 1, kCacheQ8 = 2;
+// K and V rows [page][kv_head][token of the page][width], width = 64 or 128
+// (columns past head_dim are zeros): rows of one head and page are consecutive.
+// Q8_0: the values as int8, the scales of their blocks of 32 as kd and vd
+// [row][width / 32] (binary16 bits).
+struct CacheView {
+    void *k, *v;
+    uint16_t *kd, *vd;
+    int kind, kv_heads, width, page_shift;
+    int slots;  // pages << page_shift
+};
+// The row of a slot (page * page_tokens + token of the page) and head.
+__host__ __device__ inline size_t cache_row(const CacheView &c, int slot, int g) {
+    const int page = slot >> c.page_shift, in = slot & ((1 << c.page_shift) - 1);
+    return (((size_t)page * c.kv_heads + g) << c.page_shift) + in;
+}
+// Rotation pairs on the device; pairs == 0: no rotation.
+struct RopePlan {
+    int axes, pairs;
+    const double *turns;  // [pairs] turns per unit of position
+    const int *axis;      // [pairs]
+    const int *dims;      // [head_dim] pair << 9 | first << 8 | the other dim, or -1
+};
+struct CacheRows {
+    const float *q, *k, *v;  // rows of head_dim floats; strides in floats
+    size_t q_token, q_head, kv_token, kv_head;
+    float *q_out;            // rotated rows of q
+    size_t o_token, o_head;
+    int tokens, heads, kv_heads, head_dim;  // kv_heads == 0: q alone
+    const int *positions;    // [tokens][axes]
+    const int *slots;        // [tokens]; outside [0, cache.slots): not stored
+    RopePlan rope;
+    CacheView cache;
+    int per_group;           // set by the launcher
+};
+hipError_t launch_cache_rows(hipStream_t s, CacheRows a);
+hipError_t launch_cache_gather(hipStream_t s, const CacheView &cache, const int *slots, float *k, float *v,
+                               size_t n, size_t head_dim);
+// Requests of one launch_pages_assign (8 bytes of LDS each).
+constexpr size_t kMaxRequests = 4096;
+struct PagesAssign {
+    const int *cached, *added;     // [requests]
+    const int *free_list, *free_start;
+    int *table;                    // [requests][max_pages]
+    int *starts, *lens, *slots, *free_next;
+    int requests, free_pages, tokens, page_shift;
+    long long max_pages;
+};
+hipError_t launch_pages_assign(hipStream_t s, const PagesAssign &a);
+
 }  // namespace vh

@@ -70,6 +70,14 @@ vh_status null_arg(const char *what) {
     return fail(VH_ERR_INVALID_ARGUMENT, std::string(what) + ": null handle or pointer");
 }
 
+vh_status other_runtime(const char *what) {
+    return fail(VH_ERR_INVALID_ARGUMENT, std::string(what) + ": a handle belongs to another runtime");
+}
+
+vh_status aliased(const char *what) {
+    return fail(VH_ERR_INVALID_ARGUMENT, std::string(what) + ": an output is also an input or another output");
+}
+
 // Of a failed HIP call.  The error is also left as the thread's last one, which
 // the next launch's own check would take for its own: cleared.
 std::string hip_msg(const char *what, hipError_t e) {
@@ -292,6 +300,42 @@ struct vh_linear_q8 {
         if (!rt) return;
         hipSetDevice(rt->device);
         L.release(rt->stream);
+    }
+};
+
+struct vh_index {
+    Rt rt;
+    int *ptr = nullptr;
+    size_t len = 0;
+    ~vh_index() {
+        if (!rt || !ptr) return;
+        hipSetDevice(rt->device);
+        hipFreeAsync(ptr, rt->stream);
+    }
+};
+
+// Rotation pairs (kernels.h RopePlan), resident on the device in one block.
+struct vh_rope {
+    Rt rt;
+    size_t head_dim = 0;
+    char *block = nullptr;
+    vh::RopePlan plan{};
+    ~vh_rope() {
+        if (!rt || !block) return;
+        hipSetDevice(rt->device);
+        hipFreeAsync(block, rt->stream);
+    }
+};
+
+struct vh_kv_cache {
+    Rt rt;
+    size_t head_dim = 0;
+    vh::CacheView view{};
+    ~vh_kv_cache() {
+        if (!rt) return;
+        hipSetDevice(rt->device);
+        for (void *p : {view.k, view.v, (void *)view.kd, (void *)view.vd})
+            if (p) hipFreeAsync(p, rt->stream);
     }
 };
 
@@ -3228,6 +3272,389 @@ extern "C" vh_status vh_bilinear_resize_align_corners_f32(const vh_runtime *rt,
                                                           vh_tensor **out) {
     return resize_new(rt, input, c, ih, iw, oh, ow, add, true, out,
                       "vh_bilinear_resize_align_corners_f32");
+}
+
+// =============================================================================
+// streams of frames: index tensors, rotary positions, paged cache
+// =============================================================================
+
+// Tokens of one call, so that its grid stays within a launch (one workgroup to
+// 16 tokens at most).
+constexpr size_t kMaxCacheTokens = (size_t)1 << 27;
+
+static vh_status new_index(const Rt &rt, size_t len, vh_index **out, const char *what) {
+    auto t = std::make_unique<vh_index>();
+    if (len > (SIZE_MAX >> 3)) return fail(VH_ERR_UPLOAD, std::string(what) + ": length overflows");
+    TRY(dalloc(*rt, len, &t->ptr, what));
+    t->rt = rt;
+    t->len = len;
+    *out = t.release();
+    return VH_OK;
+}
+
+extern "C" vh_status vh_upload_i32(const vh_runtime *rt, const int *values, size_t len, vh_index **out) {
+    const char *what = "vh_upload_i32";
+    NEED(rt, what);
+    NEED(out, what);
+    if (len && !values) return null_arg("vh_upload_i32 values");
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    vh_index *t = nullptr;
+    TRY(new_index(rt->s, len, &t, what));
+    vh_status st = h2d(s, t->ptr, values, len * sizeof(int), what);
+    if (st) {
+        delete t;
+        return st;
+    }
+    *out = t;
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" vh_status vh_download_i32(const vh_runtime *rt, const vh_index *index, int *out, size_t out_len) {
+    const char *what = "vh_download_i32";
+    NEED(rt, what);
+    NEED(index, what);
+    if (out_len != index->len) return mismatch(out_len, index->len, what);
+    if (out_len && !out) return null_arg("vh_download_i32 out");
+    if (index->rt != rt->s) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    if (out_len == 0) return VH_OK;
+    hipError_t e = hipMemcpyAsync(out, index->ptr, out_len * sizeof(int), hipMemcpyDeviceToHost, s.stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(s.stream);
+    if (e != hipSuccess) return fail(VH_ERR_DOWNLOAD, hip_msg("device-to-host transfer", e));
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" vh_status vh_index_alloc(const vh_runtime *rt, size_t len, vh_index **out) {
+    NEED(rt, "vh_index_alloc");
+    NEED(out, "vh_index_alloc");
+    GUARD_BEGIN
+    TRY(set_device(*rt->s));
+    return new_index(rt->s, len, out, "index allocation");
+    GUARD_END
+}
+
+extern "C" void vh_index_free(vh_index *index) { delete index; }
+extern "C" size_t vh_index_len(const vh_index *index) { return index ? index->len : 0; }
+extern "C" int *vh_index_device_ptr(const vh_index *index) { return index ? index->ptr : nullptr; }
+
+extern "C" vh_status vh_prepare_rope_axes(const vh_runtime *rt, size_t head_dim, size_t axes, const size_t *pairs,
+                                          float frequency, int shared_spectrum, vh_rope **out) {
+    const char *what = "vh_prepare_rope_axes";
+    NEED(rt, what);
+    NEED(pairs, what);
+    NEED(out, what);
+    if (head_dim == 0 || head_dim % 4 != 0 || head_dim > 256)
+        return fail(VH_ERR_KERNEL, "rope axes: head_dim must be a multiple of 4 up to 256, got " +
+                                       std::to_string(head_dim));
+    if (axes < 1 || axes > 4)
+        return fail(VH_ERR_KERNEL, "rope axes: 1 to 4 axes, got " + std::to_string(axes));
+    size_t n = 0;
+    for (size_t a = 0; a < axes; a++) {
+        if (pairs[a] < 1 || pairs[a] > head_dim / 2 - n)
+            return fail(VH_ERR_KERNEL, "rope axes: axis " + std::to_string(a) + " has " + std::to_string(pairs[a]) +
+                                           " pairs, with " + std::to_string(head_dim / 2 - n) + " left");
+        n += pairs[a];
+    }
+    if (!(frequency > 0.0f) || !std::isfinite(frequency))
+        return fail(VH_ERR_KERNEL, "rope axes: the frequency must be finite and positive");
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    std::vector<double> turns(n);
+    std::vector<int> ints(n + head_dim, -1);  // axis of each pair, then the dims
+    int *dims = ints.data() + n;
+    size_t i = 0, o = 0;
+    for (size_t a = 0; a < axes; a++) {
+        for (size_t j = 0; j < pairs[a]; j++, i++) {
+            const double e = shared_spectrum ? (double)i / (double)n : (double)j / (double)pairs[a];
+            const size_t first = shared_spectrum ? i : o + j, second = shared_spectrum ? n + i : o + pairs[a] + j;
+            turns[i] = std::pow((double)frequency, -e) / 6.283185307179586476925286766559;
+            ints[i] = (int)a;
+            dims[first] = (int)(i << 9 | 1 << 8 | second);
+            dims[second] = (int)(i << 9 | first);
+        }
+        o += 2 * pairs[a];
+    }
+    auto r = std::make_unique<vh_rope>();
+    const size_t tb = n * sizeof(double), ib = ints.size() * sizeof(int);
+    TRY(dalloc(s, tb + ib, &r->block, "rope plan allocation"));
+    r->rt = rt->s;
+    TRY(h2d(s, r->block, turns.data(), tb, "rope plan upload"));
+    TRY(h2d(s, r->block + tb, ints.data(), ib, "rope plan upload"));
+    r->head_dim = head_dim;
+    r->plan.axes = (int)axes;
+    r->plan.pairs = (int)n;
+    r->plan.turns = reinterpret_cast<const double *>(r->block);
+    r->plan.axis = reinterpret_cast<const int *>(r->block + tb);
+    r->plan.dims = r->plan.axis + n;
+    *out = r.release();
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" void vh_rope_free(vh_rope *rope) { delete rope; }
+
+extern "C" vh_status vh_rope_axes_run(const vh_rope *rope, const vh_tensor *x, size_t heads, size_t tokens,
+                                      int token_major, const vh_index *positions, vh_tensor *out) {
+    const char *what = "vh_rope_axes_run";
+    NEED(rope, what);
+    NEED(x, what);
+    NEED(positions, what);
+    NEED(out, what);
+    size_t rows = 0, expected = 0, places = 0;
+    if (mul_overflows(heads, tokens, &rows) || mul_overflows(rows, rope->head_dim, &expected) ||
+        x->len != expected)
+        return mismatch(x->len, expected, what);
+    if (out->len != expected) return mismatch(out->len, expected, what);
+    if (mul_overflows(tokens, (size_t)rope->plan.axes, &places) || positions->len < places)
+        return mismatch(positions->len, places, what);
+    if (tokens > kMaxCacheTokens || heads > 65535)
+        return fail(VH_ERR_KERNEL, "rope axes: more than 2^27 tokens or 65535 heads");
+    if (x->rt != rope->rt || positions->rt != rope->rt || out->rt != rope->rt) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *rope->rt;
+    TRY(set_device(s));
+    if (expected == 0) return VH_OK;
+    const size_t hd = rope->head_dim;
+    vh::CacheRows a{};
+    a.q = x->ptr;
+    a.q_out = out->ptr;
+    a.q_token = a.o_token = token_major ? heads * hd : hd;
+    a.q_head = a.o_head = token_major ? hd : tokens * hd;
+    a.tokens = (int)tokens;
+    a.heads = (int)heads;
+    a.head_dim = (int)hd;
+    a.positions = positions->ptr;
+    a.rope = rope->plan;
+    return launch(s, "rope_axes", [&] { return vh::launch_cache_rows(s.stream, a); });
+    GUARD_END
+}
+
+extern "C" vh_status vh_kv_cache_new(const vh_runtime *rt, int type, size_t pages, size_t page_tokens,
+                                     size_t kv_heads, size_t head_dim, vh_kv_cache **out) {
+    const char *what = "vh_kv_cache_new";
+    NEED(rt, what);
+    NEED(out, what);
+    if (type < vh::kCacheF32 || type > vh::kCacheQ8)
+        return fail(VH_ERR_KERNEL, "kv cache: type " + std::to_string(type) + " is none of 0 (f32), 1 (bf16), 2 (Q8_0)");
+    if (page_tokens == 0 || page_tokens > 4096 || (page_tokens & (page_tokens - 1)))
+        return fail(VH_ERR_KERNEL, "kv cache: page_tokens must be a power of two up to 4096, got " +
+                                       std::to_string(page_tokens));
+    if (head_dim == 0 || head_dim > 128 || head_dim % (type == vh::kCacheQ8 ? 32 : 4))
+        return fail(VH_ERR_KERNEL, "kv cache: head_dim must be a multiple of 4 (32 for Q8_0) up to 128, got " +
+                                       std::to_string(head_dim));
+    size_t slots = 0, rows = 0, bytes = 0;
+    if (kv_heads == 0 || kv_heads > 65535 || mul_overflows(pages, page_tokens, &slots) ||
+        slots > (size_t)INT32_MAX - 4095 || mul_overflows(slots, kv_heads, &rows) || mul_overflows(rows, 1024, &bytes))
+        return fail(VH_ERR_KERNEL, "kv cache: " + std::to_string(pages) + " pages of " + std::to_string(page_tokens) +
+                                       " tokens and " + std::to_string(kv_heads) + " heads are out of range");
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    if (capturing(s.stream)) return fail(VH_ERR_KERNEL, "kv cache: not to be made inside a stream capture");
+    auto c = std::make_unique<vh_kv_cache>();
+    c->rt = rt->s;
+    c->head_dim = head_dim;
+    vh::CacheView &w = c->view;
+    w.kind = type;
+    w.kv_heads = (int)kv_heads;
+    w.width = head_dim <= 64 ? 64 : 128;
+    while ((size_t)1 << w.page_shift < page_tokens) w.page_shift++;
+    w.slots = (int)slots;
+    const size_t value = type == vh::kCacheF32 ? 4 : type == vh::kCacheBf16 ? 2 : 1;
+    for (void **p : {&w.k, &w.v}) {
+        char *q = nullptr;
+        TRY(dalloc(s, rows * w.width * value, &q, "kv cache allocation"));
+        *p = q;
+        if (rows && hipMemsetAsync(q, 0, rows * w.width * value, s.stream) != hipSuccess)
+            return fail(VH_ERR_UPLOAD, hip_msg(what, hipGetLastError()));
+    }
+    if (type == vh::kCacheQ8)
+        for (uint16_t **p : {&w.kd, &w.vd}) {
+            TRY(dalloc(s, rows * (w.width / 32), p, "kv cache allocation"));
+            if (rows && hipMemsetAsync(*p, 0, rows * (w.width / 32) * 2, s.stream) != hipSuccess)
+                return fail(VH_ERR_UPLOAD, hip_msg(what, hipGetLastError()));
+        }
+    *out = c.release();
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" void vh_kv_cache_free(vh_kv_cache *cache) { delete cache; }
+extern "C" size_t vh_kv_cache_slots(const vh_kv_cache *cache) { return cache ? (size_t)cache->view.slots : 0; }
+
+extern "C" vh_status vh_kv_cache_append_f32(vh_kv_cache *cache, const vh_tensor *k, const vh_tensor *v,
+                                            size_t tokens, int token_major, const vh_index *slots) {
+    const char *what = "vh_kv_cache_append_f32";
+    NEED(cache, what);
+    NEED(k, what);
+    NEED(v, what);
+    NEED(slots, what);
+    const size_t hd = cache->head_dim, kvh = (size_t)cache->view.kv_heads;
+    size_t expected = 0;
+    if (mul_overflows(tokens, kvh * hd, &expected) || k->len != expected) return mismatch(k->len, expected, what);
+    if (v->len != expected) return mismatch(v->len, expected, what);
+    if (slots->len < tokens) return mismatch(slots->len, tokens, what);
+    if (tokens > kMaxCacheTokens) return fail(VH_ERR_KERNEL, "kv cache: more than 2^27 tokens");
+    if (k->rt != cache->rt || v->rt != cache->rt || slots->rt != cache->rt) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *cache->rt;
+    TRY(set_device(s));
+    if (expected == 0) return VH_OK;
+    vh::CacheRows a{};
+    a.k = k->ptr;
+    a.v = v->ptr;
+    a.kv_token = token_major ? kvh * hd : hd;
+    a.kv_head = token_major ? hd : tokens * hd;
+    a.tokens = (int)tokens;
+    a.kv_heads = (int)kvh;
+    a.head_dim = (int)hd;
+    a.slots = slots->ptr;
+    a.cache = cache->view;
+    return launch(s, "kv_append", [&] { return vh::launch_cache_rows(s.stream, a); });
+    GUARD_END
+}
+
+extern "C" vh_status vh_kv_cache_append_qkv_f32(vh_kv_cache *cache, const vh_rope *rope, const vh_tensor *qkv,
+                                                size_t heads, size_t tokens, const vh_index *positions,
+                                                const vh_index *slots, vh_tensor *q_out) {
+    const char *what = "vh_kv_cache_append_qkv_f32";
+    NEED(cache, what);
+    NEED(qkv, what);
+    NEED(slots, what);
+    NEED(q_out, what);
+    if (rope) NEED(positions, what);
+    const size_t hd = cache->head_dim, kvh = (size_t)cache->view.kv_heads;
+    if (heads == 0 || heads > 65535 || heads % kvh != 0)
+        return fail(VH_ERR_KERNEL, "kv cache: " + std::to_string(heads) + " query heads over " + std::to_string(kvh) +
+                                       " heads of the cache");
+    if (rope && rope->head_dim != hd)
+        return fail(VH_ERR_KERNEL, "kv cache: a rotation of head_dim " + std::to_string(rope->head_dim) +
+                                       " for rows of " + std::to_string(hd));
+    const size_t per = (heads + 2 * kvh) * hd;
+    size_t expected = 0, places = 0;
+    if (mul_overflows(tokens, per, &expected) || qkv->len != expected) return mismatch(qkv->len, expected, what);
+    if (q_out->len != tokens * heads * hd) return mismatch(q_out->len, tokens * heads * hd, what);
+    if (slots->len < tokens) return mismatch(slots->len, tokens, what);
+    if (rope && (mul_overflows(tokens, (size_t)rope->plan.axes, &places) || positions->len < places))
+        return mismatch(positions->len, places, what);
+    if (tokens > kMaxCacheTokens) return fail(VH_ERR_KERNEL, "kv cache: more than 2^27 tokens");
+    if (qkv->rt != cache->rt || slots->rt != cache->rt || q_out->rt != cache->rt ||
+        (rope && (rope->rt != cache->rt || positions->rt != cache->rt)))
+        return other_runtime(what);
+    if (q_out == qkv) return aliased(what);
+    GUARD_BEGIN
+    RtState &s = *cache->rt;
+    TRY(set_device(s));
+    if (expected == 0) return VH_OK;
+    vh::CacheRows a{};
+    a.q = qkv->ptr;
+    a.k = qkv->ptr + heads * hd;
+    a.v = qkv->ptr + (heads + kvh) * hd;
+    a.q_token = a.kv_token = per;
+    a.q_head = a.kv_head = a.o_head = hd;
+    a.q_out = q_out->ptr;
+    a.o_token = heads * hd;
+    a.tokens = (int)tokens;
+    a.heads = (int)heads;
+    a.kv_heads = (int)kvh;
+    a.head_dim = (int)hd;
+    a.slots = slots->ptr;
+    if (rope) {
+        a.positions = positions->ptr;
+        a.rope = rope->plan;
+    }
+    a.cache = cache->view;
+    return launch(s, "kv_append_qkv", [&] { return vh::launch_cache_rows(s.stream, a); });
+    GUARD_END
+}
+
+extern "C" vh_status vh_kv_cache_gather_f32(const vh_kv_cache *cache, const vh_index *slots, size_t tokens,
+                                            vh_tensor *k, vh_tensor *v) {
+    const char *what = "vh_kv_cache_gather_f32";
+    NEED(cache, what);
+    NEED(slots, what);
+    NEED(k, what);
+    NEED(v, what);
+    const size_t hd = cache->head_dim, kvh = (size_t)cache->view.kv_heads;
+    size_t expected = 0;
+    if (mul_overflows(tokens, kvh * hd, &expected) || k->len != expected) return mismatch(k->len, expected, what);
+    if (v->len != expected) return mismatch(v->len, expected, what);
+    if (slots->len < tokens) return mismatch(slots->len, tokens, what);
+    if (k->rt != cache->rt || v->rt != cache->rt || slots->rt != cache->rt) return other_runtime(what);
+    if (k == v) return aliased(what);
+    GUARD_BEGIN
+    RtState &s = *cache->rt;
+    TRY(set_device(s));
+    if (expected == 0) return VH_OK;
+    return launch(s, "kv_gather", [&] {
+        return vh::launch_cache_gather(s.stream, cache->view, slots->ptr, k->ptr, v->ptr, tokens, hd);
+    });
+    GUARD_END
+}
+
+extern "C" vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const vh_index *added,
+                                        size_t requests, const vh_index *free_pages, const vh_index *free_start,
+                                        size_t page_tokens, vh_index *table, size_t max_pages, vh_index *starts,
+                                        vh_index *lens, vh_index *slots, size_t tokens, vh_index *free_next) {
+    const char *what = "vh_kv_pages_assign";
+    const vh_index *const in[] = {cached, added, free_pages, free_start};
+    vh_index *const written[] = {table, starts, lens, slots, free_next};
+    NEED(rt, what);
+    for (const vh_index *p : in) NEED(p, what);
+    for (const vh_index *p : written) NEED(p, what);
+    if (requests > vh::kMaxRequests)
+        return fail(VH_ERR_KERNEL, "kv pages: at most " + std::to_string(vh::kMaxRequests) + " requests, got " +
+                                       std::to_string(requests));
+    if (page_tokens == 0 || page_tokens > 4096 || (page_tokens & (page_tokens - 1)))
+        return fail(VH_ERR_KERNEL, "kv pages: page_tokens must be a power of two up to 4096, got " +
+                                       std::to_string(page_tokens));
+    size_t entries = 0;
+    if (mul_overflows(requests, max_pages, &entries) || table->len != entries)
+        return mismatch(table->len, entries, what);
+    for (const vh_index *p : {cached, added, (const vh_index *)lens})
+        if (p->len != requests) return mismatch(p->len, requests, what);
+    if (starts->len != requests + 1) return mismatch(starts->len, requests + 1, what);
+    if (slots->len != tokens) return mismatch(slots->len, tokens, what);
+    if (free_start->len != 1) return mismatch(free_start->len, 1, what);
+    if (free_next->len != 1) return mismatch(free_next->len, 1, what);
+    if (tokens > (size_t)INT32_MAX - 1024 || free_pages->len > INT32_MAX)
+        return fail(VH_ERR_KERNEL, "kv pages: tokens or free pages exceed 2^31-1");
+    for (const vh_index *p : in)
+        if (p->rt != rt->s) return other_runtime(what);
+    for (size_t i = 0; i < 5; i++) {
+        if (written[i]->rt != rt->s) return other_runtime(what);
+        for (const vh_index *p : in)
+            if (p == written[i]) return aliased(what);
+        for (size_t j = 0; j < i; j++)
+            if (written[j] == written[i]) return aliased(what);
+    }
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    vh::PagesAssign a{};
+    a.cached = cached->ptr;
+    a.added = added->ptr;
+    a.free_list = free_pages->ptr;
+    a.free_start = free_start->ptr;
+    a.table = table->ptr;
+    a.starts = starts->ptr;
+    a.lens = lens->ptr;
+    a.slots = slots->ptr;
+    a.free_next = free_next->ptr;
+    a.requests = (int)requests;
+    a.free_pages = (int)free_pages->len;
+    a.tokens = (int)tokens;
+    while ((size_t)1 << a.page_shift < page_tokens) a.page_shift++;
+    a.max_pages = (long long)max_pages;
+    return launch(s, "kv_pages_assign", [&] { return vh::launch_pages_assign(s.stream, a); });
+    GUARD_END
 }
 
 // =============================================================================

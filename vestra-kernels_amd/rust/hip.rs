@@ -65,6 +65,18 @@ pub struct VhConv2d {
 pub struct VhConvTranspose2d {
     _p: [u8; 0],
 }
+#[repr(C)]
+pub struct VhIndex {
+    _p: [u8; 0],
+}
+#[repr(C)]
+pub struct VhRope {
+    _p: [u8; 0],
+}
+#[repr(C)]
+pub struct VhKvCache {
+    _p: [u8; 0],
+}
 
 type Status = c_int;
 
@@ -244,6 +256,35 @@ unsafe extern "C" {
     fn vh_bilinear_resize_align_corners_f32(rt: *const VhRuntime, input: *const VhTensor, c: usize, ih: usize,
                                             iw: usize, oh: usize, ow: usize, add: *const VhTensor,
                                             out: *mut *mut VhTensor) -> Status;
+
+    fn vh_upload_i32(rt: *const VhRuntime, values: *const c_int, len: usize, out: *mut *mut VhIndex) -> Status;
+    fn vh_download_i32(rt: *const VhRuntime, index: *const VhIndex, out: *mut c_int, out_len: usize) -> Status;
+    fn vh_index_alloc(rt: *const VhRuntime, len: usize, out: *mut *mut VhIndex) -> Status;
+    fn vh_index_free(index: *mut VhIndex);
+    fn vh_index_len(index: *const VhIndex) -> usize;
+    fn vh_index_device_ptr(index: *const VhIndex) -> *mut c_int;
+
+    fn vh_prepare_rope_axes(rt: *const VhRuntime, head_dim: usize, axes: usize, pairs: *const usize, frequency: f32,
+                            shared_spectrum: c_int, out: *mut *mut VhRope) -> Status;
+    fn vh_rope_free(rope: *mut VhRope);
+    fn vh_rope_axes_run(rope: *const VhRope, x: *const VhTensor, heads: usize, tokens: usize, token_major: c_int,
+                        positions: *const VhIndex, out: *mut VhTensor) -> Status;
+
+    fn vh_kv_cache_new(rt: *const VhRuntime, kind: c_int, pages: usize, page_tokens: usize, kv_heads: usize,
+                       head_dim: usize, out: *mut *mut VhKvCache) -> Status;
+    fn vh_kv_cache_free(cache: *mut VhKvCache);
+    fn vh_kv_cache_slots(cache: *const VhKvCache) -> usize;
+    fn vh_kv_cache_append_f32(cache: *mut VhKvCache, k: *const VhTensor, v: *const VhTensor, tokens: usize,
+                              token_major: c_int, slots: *const VhIndex) -> Status;
+    fn vh_kv_cache_append_qkv_f32(cache: *mut VhKvCache, rope: *const VhRope, qkv: *const VhTensor, heads: usize,
+                                  tokens: usize, positions: *const VhIndex, slots: *const VhIndex,
+                                  q_out: *mut VhTensor) -> Status;
+    fn vh_kv_cache_gather_f32(cache: *const VhKvCache, slots: *const VhIndex, tokens: usize, k: *mut VhTensor,
+                              v: *mut VhTensor) -> Status;
+    fn vh_kv_pages_assign(rt: *const VhRuntime, cached: *const VhIndex, added: *const VhIndex, requests: usize,
+                          free_pages: *const VhIndex, free_start: *const VhIndex, page_tokens: usize,
+                          table: *mut VhIndex, max_pages: usize, starts: *mut VhIndex, lens: *mut VhIndex,
+                          slots: *mut VhIndex, tokens: usize, free_next: *mut VhIndex) -> Status;
 
     fn vh_profile_enable(rt: *mut VhRuntime, enabled: c_int) -> Status;
     fn vh_profile_reset(rt: *mut VhRuntime) -> Status;
@@ -661,6 +702,73 @@ impl HipRuntime {
         Ok(HipLinearF32 { raw: out, runtime: self.clone() })
     }
 
+    // -- streams of frames: positions, paged cache ------------------------------
+
+    pub fn upload_i32(&self, values: &[c_int]) -> Result<HipIndex, HipError> {
+        let mut out = ptr::null_mut();
+        let raw = self.inner.raw;
+        // SAFETY: values holds values.len() integers.
+        self.call(|| unsafe { vh_upload_i32(raw, values.as_ptr(), values.len(), &mut out) })?;
+        Ok(HipIndex { raw: out, runtime: self.clone() })
+    }
+
+    pub fn alloc_i32(&self, len: usize) -> Result<HipIndex, HipError> {
+        let mut out = ptr::null_mut();
+        let raw = self.inner.raw;
+        // SAFETY: live handle.
+        self.call(|| unsafe { vh_index_alloc(raw, len, &mut out) })?;
+        Ok(HipIndex { raw: out, runtime: self.clone() })
+    }
+
+    /// The values of an index (synchronising).
+    pub fn download_i32(&self, index: &HipIndex) -> Result<Vec<c_int>, HipError> {
+        let mut host = vec![0; index.len()];
+        let raw = self.inner.raw;
+        // SAFETY: host holds index.len() integers.
+        self.call(|| unsafe { vh_download_i32(raw, index.raw, host.as_mut_ptr(), host.len()) })?;
+        Ok(host)
+    }
+
+    /// Rotation of pairs.len() position axes; see `vh_prepare_rope_axes`.
+    pub fn prepare_rope_axes(&self, head_dim: usize, pairs: &[usize], frequency: f32, shared_spectrum: bool)
+        -> Result<HipRope, HipError> {
+        let mut out = ptr::null_mut();
+        let raw = self.inner.raw;
+        // SAFETY: pairs holds pairs.len() values.
+        self.call(|| unsafe {
+            vh_prepare_rope_axes(raw, head_dim, pairs.len(), pairs.as_ptr(), frequency,
+                                 c_int::from(shared_spectrum), &mut out)
+        })?;
+        Ok(HipRope { raw: out, runtime: self.clone() })
+    }
+
+    /// A paged cache of keys and values; see `vh_kv_cache_new`.
+    pub fn kv_cache(&self, kind: KvType, pages: usize, page_tokens: usize, kv_heads: usize, head_dim: usize)
+        -> Result<HipKvCache, HipError> {
+        let mut out = ptr::null_mut();
+        let raw = self.inner.raw;
+        // SAFETY: live handle.
+        self.call(|| unsafe {
+            vh_kv_cache_new(raw, kind as c_int, pages, page_tokens, kv_heads, head_dim, &mut out)
+        })?;
+        Ok(HipKvCache { raw: out, runtime: self.clone() })
+    }
+
+    /// Block tables and slot maps of one step; see `vh_kv_pages_assign`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_pages_assign(&self, cached: &HipIndex, added: &HipIndex, free_pages: &HipIndex, free_start: &HipIndex,
+                           page_tokens: usize, table: &mut HipIndex, max_pages: usize, starts: &mut HipIndex,
+                           lens: &mut HipIndex, slots: &mut HipIndex, free_next: &mut HipIndex)
+        -> Result<(), HipError> {
+        let raw = self.inner.raw;
+        let (requests, tokens) = (cached.len(), slots.len());
+        // SAFETY: live handles, the outputs borrowed mutably for the call.
+        self.call(|| unsafe {
+            vh_kv_pages_assign(raw, cached.raw, added.raw, requests, free_pages.raw, free_start.raw, page_tokens,
+                               table.raw, max_pages, starts.raw, lens.raw, slots.raw, tokens, free_next.raw)
+        })
+    }
+
     // -- Q8_0 ------------------------------------------------------------------
 
     /// Rows of BlockQ8_0 (src/lib.rs:33-38) moved to the device.
@@ -996,6 +1104,147 @@ impl HipLinearF32 {
             vh_linear_run_qkv_hnd(raw, input.raw, images, tokens, heads, pos, frequency, &mut q, &mut k, &mut v)
         })?;
         Ok((self.runtime.tensor(q), self.runtime.tensor(k), self.runtime.tensor(v)))
+    }
+}
+
+// ---- streams of frames --------------------------------------------------------
+
+/// Device int32 values: positions, slots, lengths, page tables.
+pub struct HipIndex {
+    raw: *mut VhIndex,
+    runtime: HipRuntime,
+}
+
+// SAFETY: owned device state; every use goes through the runtime's lock.
+unsafe impl Send for HipIndex {}
+unsafe impl Sync for HipIndex {}
+
+impl Drop for HipIndex {
+    fn drop(&mut self) {
+        let _g = self.runtime.guard();
+        // SAFETY: raw came from the library and is freed once.
+        unsafe { vh_index_free(self.raw) }
+    }
+}
+
+impl HipIndex {
+    #[must_use]
+    pub fn len(&self) -> usize {
+        // SAFETY: live handle.
+        unsafe { vh_index_len(self.raw) }
+    }
+
+    #[must_use]
+    pub fn is_empty(&self) -> bool {
+        self.len() == 0
+    }
+
+    /// The raw device address, for interop.
+    #[must_use]
+    pub fn device_ptr(&self) -> *mut c_int {
+        // SAFETY: live handle.
+        unsafe { vh_index_device_ptr(self.raw) }
+    }
+}
+
+/// A prepared rotation of several position axes.
+pub struct HipRope {
+    raw: *mut VhRope,
+    runtime: HipRuntime,
+}
+
+// SAFETY: owned device state; every use goes through the runtime's lock.
+unsafe impl Send for HipRope {}
+unsafe impl Sync for HipRope {}
+
+impl Drop for HipRope {
+    fn drop(&mut self) {
+        let _g = self.runtime.guard();
+        // SAFETY: raw came from the library and is freed once.
+        unsafe { vh_rope_free(self.raw) }
+    }
+}
+
+impl HipRope {
+    pub fn run(&self, x: &HipTensorF32, heads: usize, tokens: usize, token_major: bool, positions: &HipIndex,
+               out: &mut HipTensorF32) -> Result<(), HipError> {
+        let dst = out.raw;
+        // SAFETY: live handles; `out` is borrowed mutably for the call.
+        self.runtime.call(|| unsafe {
+            vh_rope_axes_run(self.raw, x.raw, heads, tokens, c_int::from(token_major), positions.raw, dst)
+        })
+    }
+
+    pub fn run_in_place(&self, x: &mut HipTensorF32, heads: usize, tokens: usize, token_major: bool,
+                        positions: &HipIndex) -> Result<(), HipError> {
+        let raw = x.raw;
+        // SAFETY: live handles; the output may be the input.
+        self.runtime.call(|| unsafe {
+            vh_rope_axes_run(self.raw, raw, heads, tokens, c_int::from(token_major), positions.raw, raw)
+        })
+    }
+}
+
+/// What a cache holds its values in.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+#[repr(i32)]
+pub enum KvType {
+    F32 = 0,
+    Bf16 = 1,
+    Q8_0 = 2,
+}
+
+/// A paged cache of keys and values.
+pub struct HipKvCache {
+    raw: *mut VhKvCache,
+    runtime: HipRuntime,
+}
+
+// SAFETY: owned device state; every use goes through the runtime's lock.
+unsafe impl Send for HipKvCache {}
+unsafe impl Sync for HipKvCache {}
+
+impl Drop for HipKvCache {
+    fn drop(&mut self) {
+        let _g = self.runtime.guard();
+        // SAFETY: raw came from the library and is freed once.
+        unsafe { vh_kv_cache_free(self.raw) }
+    }
+}
+
+impl HipKvCache {
+    #[must_use]
+    pub fn slots(&self) -> usize {
+        // SAFETY: live handle.
+        unsafe { vh_kv_cache_slots(self.raw) }
+    }
+
+    pub fn append(&mut self, k: &HipTensorF32, v: &HipTensorF32, tokens: usize, token_major: bool, slots: &HipIndex)
+        -> Result<(), HipError> {
+        let raw = self.raw;
+        // SAFETY: live handles; the cache is borrowed mutably for the call.
+        self.runtime.call(|| unsafe {
+            vh_kv_cache_append_f32(raw, k.raw, v.raw, tokens, c_int::from(token_major), slots.raw)
+        })
+    }
+
+    /// Rows of a QKV projection: Q (rotated) to `q_out`, K (rotated) and V to their slots.
+    pub fn append_qkv(&mut self, rope: Option<(&HipRope, &HipIndex)>, qkv: &HipTensorF32, heads: usize,
+                      tokens: usize, slots: &HipIndex, q_out: &mut HipTensorF32) -> Result<(), HipError> {
+        let raw = self.raw;
+        let (plan, positions) =
+            rope.map_or((ptr::null(), ptr::null()), |(r, p)| (r.raw.cast_const(), p.raw.cast_const()));
+        // SAFETY: live handles (or null); outputs are borrowed mutably for the call.
+        self.runtime.call(|| unsafe {
+            vh_kv_cache_append_qkv_f32(raw, plan, qkv.raw, heads, tokens, positions, slots.raw, q_out.raw)
+        })
+    }
+
+    /// The stored rows of `tokens` slots as floats.
+    pub fn gather(&self, slots: &HipIndex, tokens: usize, k: &mut HipTensorF32, v: &mut HipTensorF32)
+        -> Result<(), HipError> {
+        // SAFETY: live handles; the outputs are borrowed mutably for the call.
+        self.runtime.call(|| unsafe { vh_kv_cache_gather_f32(self.raw, slots.raw, tokens, k.raw, v.raw) })
     }
 }
 

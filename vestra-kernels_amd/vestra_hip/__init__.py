@@ -27,6 +27,8 @@ _sz = ctypes.c_size_t
 _f32p = ctypes.POINTER(ctypes.c_float)
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _pp = ctypes.POINTER(ctypes.c_void_p)
+_i32p = ctypes.POINTER(ctypes.c_int)
+_szp = ctypes.POINTER(ctypes.c_size_t)
 
 # numpy twin of the reference's #[repr(C)] BlockQ8_0 (src/lib.rs:33-38).
 BLOCK_Q8_0 = np.dtype([("d", "<u2"), ("qs", "i1", (32,))], align=False)
@@ -164,6 +166,22 @@ SIGNATURES = [
     ("vh_vit_block_run", _S, [_p, _p, _p, _sz, _sz, _i64p, ctypes.c_float, ctypes.c_float]),
     ("vh_encoder_run", _S, [_p, _pp, _sz, _p, _sz, _sz, _i64p, ctypes.c_float,
                             ctypes.c_float]),
+    ("vh_upload_i32", _S, [_p, _i32p, _sz, _pp]),
+    ("vh_download_i32", _S, [_p, _p, _i32p, _sz]),
+    ("vh_index_alloc", _S, [_p, _sz, _pp]),
+    ("vh_index_free", None, [_p]),
+    ("vh_index_len", _sz, [_p]),
+    ("vh_index_device_ptr", _p, [_p]),
+    ("vh_prepare_rope_axes", _S, [_p, _sz, _sz, _szp, ctypes.c_float, ctypes.c_int, _pp]),
+    ("vh_rope_free", None, [_p]),
+    ("vh_rope_axes_run", _S, [_p, _p, _sz, _sz, ctypes.c_int, _p, _p]),
+    ("vh_kv_cache_new", _S, [_p, ctypes.c_int, _sz, _sz, _sz, _sz, _pp]),
+    ("vh_kv_cache_free", None, [_p]),
+    ("vh_kv_cache_slots", _sz, [_p]),
+    ("vh_kv_cache_append_f32", _S, [_p, _p, _p, _sz, ctypes.c_int, _p]),
+    ("vh_kv_cache_append_qkv_f32", _S, [_p, _p, _p, _sz, _sz, _p, _p, _p]),
+    ("vh_kv_cache_gather_f32", _S, [_p, _p, _sz, _p, _p]),
+    ("vh_kv_pages_assign", _S, [_p, _p, _p, _sz, _p, _p, _sz, _p, _sz, _p, _p, _p, _sz, _p]),
     ("vh_profile_enable", _S, [_p, ctypes.c_int]),
     ("vh_profile_reset", _S, [_p]),
     ("vh_profile_report", _S, [_p, ctypes.c_char_p, _sz]),
@@ -416,6 +434,100 @@ class ConvTranspose2d:
         try:
             if self._h and self._h.value:
                 lib().vh_conv_transpose2d_free(self._h)
+                self._h = ctypes.c_void_p(None)
+        except Exception:
+            pass
+
+
+class Index:
+    """Device int32 values: positions, slots, lengths, page tables."""
+
+    def __init__(self, runtime: "Runtime", handle: int):
+        self._rt = runtime
+        self._h = ctypes.c_void_p(handle)
+
+    def __len__(self) -> int:
+        return int(lib().vh_index_len(self._h))
+
+    @property
+    def handle(self):
+        return self._h
+
+    @property
+    def device_ptr(self) -> int:
+        return int(lib().vh_index_device_ptr(self._h) or 0)
+
+    def __del__(self):
+        try:
+            if self._h and self._h.value:
+                lib().vh_index_free(self._h)
+                self._h = ctypes.c_void_p(None)
+        except Exception:
+            pass
+
+
+class RopeAxes:
+    """A prepared rotation of several position axes."""
+
+    def __init__(self, runtime: "Runtime", handle: int):
+        self._rt = runtime
+        self._h = ctypes.c_void_p(handle)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def run(self, x: Tensor, heads: int, tokens: int, positions: Index, out: Tensor,
+            token_major: bool = False) -> None:
+        """Rotates x [heads, tokens, head_dim] (or token-major) into out, which may be x."""
+        _check(lib().vh_rope_axes_run(self._h, x.handle, heads, tokens, 1 if token_major else 0,
+                                      positions.handle, out.handle))
+
+    def __del__(self):
+        try:
+            if self._h and self._h.value:
+                lib().vh_rope_free(self._h)
+                self._h = ctypes.c_void_p(None)
+        except Exception:
+            pass
+
+
+class KvCache:
+    """A paged cache of keys and values."""
+
+    TYPES = {"f32": 0, "bf16": 1, "q8_0": 2}
+
+    def __init__(self, runtime: "Runtime", handle: int):
+        self._rt = runtime
+        self._h = ctypes.c_void_p(handle)
+
+    @property
+    def handle(self):
+        return self._h
+
+    @property
+    def slots(self) -> int:
+        return int(lib().vh_kv_cache_slots(self._h))
+
+    def append(self, k: Tensor, v: Tensor, tokens: int, slots: Index, token_major: bool = False) -> None:
+        _check(lib().vh_kv_cache_append_f32(self._h, k.handle, v.handle, tokens,
+                                            1 if token_major else 0, slots.handle))
+
+    def append_qkv(self, qkv: Tensor, heads: int, tokens: int, slots: Index, q_out: Tensor,
+                   rope: RopeAxes | None = None, positions: Index | None = None) -> None:
+        """Rows of a QKV projection: Q (rotated) to q_out, K (rotated) and V to their slots."""
+        _check(lib().vh_kv_cache_append_qkv_f32(
+            self._h, rope.handle if rope is not None else None, qkv.handle, heads, tokens,
+            positions.handle if positions is not None else None, slots.handle, q_out.handle))
+
+    def gather(self, slots: Index, tokens: int, k: Tensor, v: Tensor) -> None:
+        """The stored rows of `slots` as floats, into k and v."""
+        _check(lib().vh_kv_cache_gather_f32(self._h, slots.handle, tokens, k.handle, v.handle))
+
+    def __del__(self):
+        try:
+            if self._h and self._h.value:
+                lib().vh_kv_cache_free(self._h)
                 self._h = ctypes.c_void_p(None)
         except Exception:
             pass
@@ -701,6 +813,47 @@ class Runtime:
         pos = None if pos_yx is None else np.ascontiguousarray(pos_yx, np.int64)
         _check(lib().vh_encoder_run(self._h, ctypes.cast(arr, _pp), len(blocks), x.handle, images,
                                     tokens, _ip(pos), rope_frequency, epsilon))
+
+    # -- streams of frames: positions, paged cache
+    def upload_i32(self, values) -> Index:
+        a = np.ascontiguousarray(values, np.int32).reshape(-1)
+        out = ctypes.c_void_p()
+        _check(lib().vh_upload_i32(self._h, a.ctypes.data_as(_i32p), a.size, ctypes.byref(out)))
+        return Index(self, out.value)
+
+    def download_i32(self, index: Index) -> np.ndarray:
+        out = np.empty(len(index), np.int32)
+        _check(lib().vh_download_i32(self._h, index.handle, out.ctypes.data_as(_i32p), out.size))
+        return out
+
+    def alloc_i32(self, n: int) -> Index:
+        out = ctypes.c_void_p()
+        _check(lib().vh_index_alloc(self._h, n, ctypes.byref(out)))
+        return Index(self, out.value)
+
+    def prepare_rope_axes(self, head_dim: int, pairs, frequency: float, shared: bool = False) -> RopeAxes:
+        """pairs: the rotated pairs of each position axis; shared: one spectrum for all of them."""
+        arr = (_sz * max(1, len(pairs)))(*pairs)
+        out = ctypes.c_void_p()
+        _check(lib().vh_prepare_rope_axes(self._h, head_dim, len(pairs), arr, frequency,
+                                          1 if shared else 0, ctypes.byref(out)))
+        return RopeAxes(self, out.value)
+
+    def kv_cache(self, type: str, pages: int, page_tokens: int, kv_heads: int, head_dim: int) -> KvCache:
+        """type: "f32", "bf16" or "q8_0"."""
+        out = ctypes.c_void_p()
+        _check(lib().vh_kv_cache_new(self._h, KvCache.TYPES.get(type, -1), pages, page_tokens, kv_heads,
+                                     head_dim, ctypes.byref(out)))
+        return KvCache(self, out.value)
+
+    def kv_pages_assign(self, cached: Index, added: Index, free_pages: Index, free_start: Index,
+                        page_tokens: int, table: Index, max_pages: int, starts: Index, lens: Index,
+                        slots: Index, free_next: Index) -> None:
+        """Block tables and slot maps of one step (vh_kv_pages_assign)."""
+        _check(lib().vh_kv_pages_assign(self._h, cached.handle, added.handle, len(cached),
+                                        free_pages.handle, free_start.handle, page_tokens, table.handle,
+                                        max_pages, starts.handle, lens.handle, slots.handle, len(slots),
+                                        free_next.handle))
 
     # -- profiling
     def profile_enable(self, on: bool = True) -> None:
