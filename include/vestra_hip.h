@@ -487,6 +487,29 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
                              size_t page_tokens, vh_index *table, size_t max_pages, vh_index *starts,
                              vh_index *lens, vh_index *slots, size_t tokens, vh_index *free_next);
 
+/* Attention of new tokens over what the cache holds of their requests:
+ *   out[t, h] = sum_j p_j v_j,  p = softmax over j of q[t, h] . k_j / sqrt(head_dim)
+ * with q and out [tokens, heads, head_dim], heads % kv_heads == 0 and query head h
+ * reading head h / (heads / kv_heads) of the cache.  Request r's new tokens are rows
+ * starts[r] .. starts[r + 1] - 1, the last of its lens[r] tokens, which lie in the
+ * pages of its row of table [requests, max_pages] (as vh_kv_pages_assign writes
+ * all three, the new ones already appended).  Token i of n new ones has position
+ * pos = lens[r] - n + i and sees keys lo <= j < hi:
+ *   hi = lens[r] for block = 0 (every key), else min(lens[r], (pos / block + 1) *
+ *        block): block = 1 is causal, block = the tokens of a frame lets a frame see
+ *        itself and the earlier ones;
+ *   lo = max(0, hi - window), or 0 for window = 0.
+ * Keys in a page that is -1 or none of the cache's are not seen, nor is anything that
+ * an unseen key or value holds (infinities and NaN too).  A query that sees no key
+ * gets zeros; one that sees an infinity or NaN in a value has no finite number in
+ * that dim, in a key no defined row.  Rows behind starts[requests] are left as they
+ * were.  Statistics and sums are 32 bits, and products of the stored values keep 24
+ * bits.  At most 4096 requests. */
+vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const vh_tensor *q, size_t heads,
+                                    size_t tokens, size_t requests, const vh_index *table,
+                                    size_t max_pages, const vh_index *starts, const vh_index *lens,
+                                    size_t block, size_t window, vh_tensor *out);
+
 /* ---- profiling (device twin of DA3_FLASH_PROFILE, src/specialized.rs:1324) - */
 /* When enabled, every kernel launch is bracketed by HIP events on the
  * runtime's stream and its duration accumulated under the kernel's name. */

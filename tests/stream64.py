@@ -65,23 +65,41 @@ def pages(cached, added, free, free_start, page, table, tokens):
     return np.array(starts), np.array(lens), slots, table, taken
 
 
-def attention(q, k, v, starts, lens, heads, block=0, window=0):
-    """q [tokens, heads, d]; k, v: per request [len, kv_heads, d]; rows behind the last request are
-    left out.  Keys outside a query's range do not exist for it, whatever they hold."""
-    q = np.asarray(q, np.float64)
-    out = np.zeros(q.shape)
+def seen(length, n, block=0, window=0):
+    """[n, length]: whether a new token sees a key."""
+    pos = np.arange(length - n, length)
+    hi = np.full(n, length) if not block else np.where(pos < 0, 0, np.minimum(length, (pos // block + 1) * block))
+    lo = np.maximum(0, hi - window) if window else np.zeros(n, int)
+    j = np.arange(length)
+    return (j[None] >= lo[:, None]) & (j[None] < hi[:, None])
+
+
+def attention(q, k, v, starts, lens, heads, block=0, window=0, absent=None, dtype=np.float64):
+    """q [tokens, heads, d]; k, v: per request [len, kv_heads, d]; absent: per request [len], keys that are not there.
+    Rows behind the last request are zeros.  An unseen key or value counts for nothing, whatever it holds; a seen
+    value that is not finite makes its dim NaN, a seen key that is not the row infinite (no defined row)."""
+    q = np.asarray(q, dtype)
+    out = np.zeros(q.shape, dtype)
     for r in range(len(lens)):
         n, length = int(starts[r + 1] - starts[r]), int(lens[r])
+        if n <= 0 or length <= 0:
+            continue
         group = heads // k[r].shape[1]
-        for i in range(n):
-            pos = length - n + i
-            hi = length if not block else max(0, min(length, (pos // block + 1) * block))
-            lo = max(0, hi - window) if window else 0
-            if hi <= lo:
-                continue
-            for h in range(heads):
-                kk, vv = k[r][lo:hi, h // group].astype(np.float64), v[r][lo:hi, h // group].astype(np.float64)
-                s = kk @ q[starts[r] + i, h] / np.sqrt(q.shape[-1])
-                p = np.exp(s - s.max())
-                out[starts[r] + i, h] = p @ vv / p.sum()
+        mask = seen(length, n, block, window)
+        if absent is not None:
+            mask &= ~absent[r][None]
+        for h in range(heads):
+            kk, vv = k[r][:, h // group].astype(dtype), v[r][:, h // group].astype(dtype)
+            with np.errstate(invalid="ignore"):
+                s = (q[starts[r]:starts[r + 1], h] @ kk.T) * dtype(1 / np.sqrt(q.shape[-1]))
+            s = np.where(mask, s, -np.inf)
+            bad_key = (mask & ~np.isfinite(kk).all(1)[None]).any(1)
+            s[:, ~np.isfinite(kk).all(1)] = -np.inf
+            top = s.max(1, keepdims=True)
+            p = np.exp(s - np.where(np.isfinite(top), top, 0))
+            total = p.sum(1, keepdims=True)
+            o = p @ np.where(np.isfinite(vv), vv, 0) / np.where(total > 0, total, 1)
+            o[(mask.astype(np.float32) @ (~np.isfinite(vv)).astype(np.float32)) > 0] = np.nan
+            o[bad_key] = np.inf
+            out[starts[r]:starts[r + 1], h] = o
     return out

@@ -365,4 +365,19 @@ struct PagesAssign {
 };
 hipError_t launch_pages_assign(hipStream_t s, const PagesAssign &a);
 
+// ---- attention over the paged cache (k_cache_attn.hip) -----------------------
+struct CacheAttn {
+    const float *q;       // [tokens][heads][head_dim]
+    float *out;
+    const int *table;     // [requests][max_pages]
+    const int *starts, *lens;
+    int tokens, heads, group, head_dim, requests;  // group = heads / kv_heads
+    long long max_pages;
+    unsigned block;       // 0: none, up to 2^31
+    int window;           // 0: none
+    float scale_log2;     // softmax scale times log2(e)
+    CacheView cache;
+};
+hipError_t launch_cache_attn(hipStream_t s, const CacheAttn &a);
+
 }  // namespace vh

@@ -3657,6 +3657,62 @@ extern "C" vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *ca
     GUARD_END
 }
 
+extern "C" vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const vh_tensor *q, size_t heads,
+                                               size_t tokens, size_t requests, const vh_index *table,
+                                               size_t max_pages, const vh_index *starts, const vh_index *lens,
+                                               size_t block, size_t window, vh_tensor *out) {
+    const char *what = "vh_kv_cache_attention_f32";
+    NEED(cache, what);
+    NEED(q, what);
+    NEED(table, what);
+    NEED(starts, what);
+    NEED(lens, what);
+    NEED(out, what);
+    const size_t hd = cache->head_dim, kvh = (size_t)cache->view.kv_heads;
+    if (heads == 0 || heads > 65535 || heads % kvh != 0)
+        return fail(VH_ERR_KERNEL, "kv cache: " + std::to_string(heads) + " query heads over " + std::to_string(kvh) +
+                                       " heads of the cache");
+    if (requests > vh::kMaxRequests)
+        return fail(VH_ERR_KERNEL, "kv cache: at most " + std::to_string(vh::kMaxRequests) + " requests, got " +
+                                       std::to_string(requests));
+    size_t expected = 0, entries = 0;
+    if (mul_overflows(tokens, heads * hd, &expected) || q->len != expected) return mismatch(q->len, expected, what);
+    if (out->len != expected) return mismatch(out->len, expected, what);
+    if (mul_overflows(requests, max_pages, &entries) || table->len != entries)
+        return mismatch(table->len, entries, what);
+    if (starts->len != requests + 1) return mismatch(starts->len, requests + 1, what);
+    if (lens->len != requests) return mismatch(lens->len, requests, what);
+    if (tokens * heads > (size_t)1 << 30)
+        return fail(VH_ERR_KERNEL, "kv cache: more than 2^30 query rows");
+    if (q->rt != cache->rt || table->rt != cache->rt || starts->rt != cache->rt || lens->rt != cache->rt ||
+        out->rt != cache->rt)
+        return other_runtime(what);
+    if (out == q) return aliased(what);
+    GUARD_BEGIN
+    RtState &s = *cache->rt;
+    TRY(set_device(s));
+    if (expected == 0 || requests == 0) return VH_OK;
+    vh::CacheAttn a{};
+    a.q = q->ptr;
+    a.out = out->ptr;
+    a.table = table->ptr;
+    a.starts = starts->ptr;
+    a.lens = lens->ptr;
+    a.tokens = (int)tokens;
+    a.heads = (int)heads;
+    a.group = (int)(heads / kvh);
+    a.head_dim = (int)hd;
+    a.requests = (int)requests;
+    a.max_pages = (long long)max_pages;
+    // Lengths are below 2^31: a larger block or window is no limit.
+    a.block = (unsigned)std::min(block, (size_t)1 << 31);
+    a.window = window < (size_t)INT32_MAX ? (int)window : 0;
+    a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
+    a.cache = cache->view;
+    return launch(s, "kv_attention", [&] { return vh::launch_cache_attn(s.stream, a); });
+    GUARD_END
+}
+
 // =============================================================================
 // profiling
 // =============================================================================

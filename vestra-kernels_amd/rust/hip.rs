@@ -281,6 +281,9 @@ unsafe extern "C" {
                                   q_out: *mut VhTensor) -> Status;
     fn vh_kv_cache_gather_f32(cache: *const VhKvCache, slots: *const VhIndex, tokens: usize, k: *mut VhTensor,
                               v: *mut VhTensor) -> Status;
+    fn vh_kv_cache_attention_f32(cache: *const VhKvCache, q: *const VhTensor, heads: usize, tokens: usize,
+                                 requests: usize, table: *const VhIndex, max_pages: usize, starts: *const VhIndex,
+                                 lens: *const VhIndex, block: usize, window: usize, out: *mut VhTensor) -> Status;
     fn vh_kv_pages_assign(rt: *const VhRuntime, cached: *const VhIndex, added: *const VhIndex, requests: usize,
                           free_pages: *const VhIndex, free_start: *const VhIndex, page_tokens: usize,
                           table: *mut VhIndex, max_pages: usize, starts: *mut VhIndex, lens: *mut VhIndex,
@@ -1245,6 +1248,19 @@ impl HipKvCache {
         -> Result<(), HipError> {
         // SAFETY: live handles; the outputs are borrowed mutably for the call.
         self.runtime.call(|| unsafe { vh_kv_cache_gather_f32(self.raw, slots.raw, tokens, k.raw, v.raw) })
+    }
+
+    /// Attention of new tokens over the cache; see `vh_kv_cache_attention_f32`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention(&self, q: &HipTensorF32, heads: usize, tokens: usize, table: &HipIndex, max_pages: usize,
+                     starts: &HipIndex, lens: &HipIndex, block: usize, window: usize, out: &mut HipTensorF32)
+        -> Result<(), HipError> {
+        let requests = lens.len();
+        // SAFETY: live handles; the output is borrowed mutably for the call.
+        self.runtime.call(|| unsafe {
+            vh_kv_cache_attention_f32(self.raw, q.raw, heads, tokens, requests, table.raw, max_pages, starts.raw,
+                                      lens.raw, block, window, out.raw)
+        })
     }
 }
 

@@ -182,6 +182,7 @@ SIGNATURES = [
     ("vh_kv_cache_append_qkv_f32", _S, [_p, _p, _p, _sz, _sz, _p, _p, _p]),
     ("vh_kv_cache_gather_f32", _S, [_p, _p, _sz, _p, _p]),
     ("vh_kv_pages_assign", _S, [_p, _p, _p, _sz, _p, _p, _sz, _p, _sz, _p, _p, _p, _sz, _p]),
+    ("vh_kv_cache_attention_f32", _S, [_p, _p, _sz, _sz, _sz, _p, _sz, _p, _p, _sz, _sz, _p]),
     ("vh_profile_enable", _S, [_p, ctypes.c_int]),
     ("vh_profile_reset", _S, [_p]),
     ("vh_profile_report", _S, [_p, ctypes.c_char_p, _sz]),
@@ -523,6 +524,14 @@ class KvCache:
     def gather(self, slots: Index, tokens: int, k: Tensor, v: Tensor) -> None:
         """The stored rows of `slots` as floats, into k and v."""
         _check(lib().vh_kv_cache_gather_f32(self._h, slots.handle, tokens, k.handle, v.handle))
+
+    def attention(self, q: Tensor, heads: int, tokens: int, table: Index, max_pages: int, starts: Index,
+                  lens: Index, out: Tensor, block: int = 0, window: int = 0) -> None:
+        """Attention of the new tokens q [tokens, heads, head_dim] over their requests' keys and values
+        (vh_kv_cache_attention_f32): block 0 sees every key, 1 is causal, n causal by frames of n."""
+        _check(lib().vh_kv_cache_attention_f32(self._h, q.handle, heads, tokens, len(lens), table.handle,
+                                               max_pages, starts.handle, lens.handle, block, window,
+                                               out.handle))
 
     def __del__(self):
         try:
