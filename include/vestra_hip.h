@@ -504,7 +504,8 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  * gets zeros; one that sees an infinity or NaN in a value has no finite number in
  * that dim, in a key no defined row.  Rows behind starts[requests] are left as they
  * were.  Statistics and sums are 32 bits, and products of the stored values keep 24
- * bits.  At most 4096 requests. */
+ * bits (less of values below 2^-110: what lies under 2^-126 of them counts as
+ * zero).  At most 4096 requests. */
 vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const vh_tensor *q, size_t heads,
                                     size_t tokens, size_t requests, const vh_index *table,
                                     size_t max_pages, const vh_index *starts, const vh_index *lens,

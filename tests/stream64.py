@@ -29,7 +29,8 @@ def q8_0(x):
         inv = np.where(d != 0, (1.0 / d.astype(np.float64)).astype(np.float32), np.float32(0))
     y = (a * inv).astype(np.float64)
     q = np.clip(np.copysign(np.floor(np.abs(y) + 0.5), y), -127, 127)
-    return (q * d.astype(np.float16).astype(np.float64)).astype(np.float32).reshape(x.shape)
+    with np.errstate(over="ignore", invalid="ignore"):  # scales past binary16 are infinite
+        return (q * d.astype(np.float16).astype(np.float64)).astype(np.float32).reshape(x.shape)
 
 
 def bf16(x):

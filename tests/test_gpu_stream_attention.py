@@ -30,7 +30,7 @@ class Stream:
         self.k, self.v, at = [], [], 0
         # What earlier requests left in the pages.
         if pages * page * kvh * hd <= 1 << 22:
-            junk = rt.upload_f32(np.full(pages * page * kvh * hd, np.nan if kind != "q8_0" else 1e4))
+            junk = rt.upload_f32(np.full(pages * page * kvh * hd, np.nan if kind != "q8_0" else 1e30))
             self.cache.append(junk, junk, pages * page, rt.upload_i32(np.arange(pages * page)))
         for r, n in enumerate(lens):
             self.table[r, :held[r]] = order[at:at + held[r]]
@@ -75,10 +75,13 @@ def close(got, exp, plain):
     norm = np.linalg.norm(exp)
     err, own = np.linalg.norm(got - exp), np.linalg.norm(plain - exp)
     print(f"error {err / max(norm, 1e-300):.2e}, float32 {own / max(norm, 1e-300):.2e}")
-    assert err <= 2 * own + 4 * 2.0 ** -24 * norm, (err, own, norm)
+    # The matrix instructions take a bf16 part below 2^-126 for zero.  A float has two parts behind its first, so each
+    # value is off by less than 2 * 2^-126 there, and an average of values (weights that sum to one) by no more.
+    tiny = 2.0 ** -125
+    assert err <= 2 * own + 4 * 2.0 ** -24 * norm + tiny * np.sqrt(exp.size), (err, own, norm)
     # No single value is far off either: 40 such errors of the root mean square.
     rms = norm / np.sqrt(exp.size)
-    tol = 40 * (2 * own / np.sqrt(exp.size) + 2.0 ** -22 * rms)
+    tol = 40 * (2 * own / np.sqrt(exp.size) + 2.0 ** -22 * rms) + tiny
     worst = np.abs(got - exp) / np.maximum(1.0, np.abs(exp) / rms)
     assert worst.max() <= tol, (worst.max(), tol)
 
@@ -143,12 +146,15 @@ def test_absent_pages_are_not_seen(rt, kind):
     assert (got[s.starts[2]:s.starts[3]] == 0).all()
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("new, lens, block, window", [([1, 1], [100, 70], 1, 20), ([70], [200], 1, 0),
                                                       ([150], [400], 1, 90), ([140], [300], 50, 0)])
 def test_unseen_infinities_and_nan_do_not_show(rt, kind, new, lens, block, window):
     def change(r, k, v):
         n = len(k)
+        if kind == "q8_0":  # blocks whose scale passes binary16
+            v[n - 1, 0, 5], k[n - 2, 1, 7], v[n // 2, 1, 63], k[n // 3, 0, 0], v[3, 0, :], k[5, 1, :] = [1e30] * 6
+            return
         v[n - 1, 0, 5], k[n - 2, 1, 7], v[n // 2, 1, 63] = np.inf, np.nan, np.nan
         k[n // 3, 0, 0], v[3, 0, :], k[5, 1, :] = -np.inf, -np.inf, np.inf
 

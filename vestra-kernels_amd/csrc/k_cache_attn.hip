@@ -1,4 +1,33 @@
-// Attention of new tokens over a paged cache (kernels.h CacheAttn).
+// Attention of new tokens over a paged cache (kernels.h CacheAttn), on the bf16
+// matrix cores with the precision of floats.
+//
+// A float is exactly three bf16 (8 significand bits each, the range of a float), so
+//     q . k = sum over i + j <= 2 of q_i . k_j
+// is six products with what is dropped below 2^-24 of each term, whatever the range
+// of a row; a bf16 key is one part of its own, and so are the values of a Q8_0
+// block (integers up to 127), whose scale joins after the product over its 32
+// dims: three products there.  Probabilities are split the same way against V's
+// parts (a Q8_0 value times its scale has 18 bits: three parts).  The fp32 matrix
+// instructions would take 16 times as long a product, 2.7 times as long as six.
+//
+// Work is cut into tiles of BM query rows (new tokens of one request times the
+// query heads that share a head of the cache, so that a tile reads K and V once for
+// all of them), and the key steps of all tiles, laid end to end, into equal shares
+// of the workgroups: one long stream beside short ones, one query against a long
+// cache and a frame against eight earlier ones all fill the chip.  A tile that
+// ends up with several workgroups is joined from their partial sums by a second
+// launch.  Shares follow from the lengths alone, so the same call gives the same
+// bits.  The lengths are on the device: every workgroup forms the partition itself.
+//
+// Two kernels, by the rows of a request (launch_cache_attn):
+//   few rows:  16 query rows a workgroup, whose four waves take 32 keys each of a
+//     step of 128, on their own: K from global memory straight to the fragments of
+//     S^T = K . Q^T, V through LDS of the wave's own, no barrier in the loop;
+//   many rows: 128 query rows, 32 a wave, which share panels of K and V in LDS.
+// Either way a lane holds its own query's scores, keys 16 t + 4 lh + r of tile t,
+// which is the B operand of O^T += V^T . P^T if the 32 keys of a product are taken in
+// the order (4 lh .. 4 lh + 3 of tile 0, then of tile 1); V^T comes from row-major
+// planes by transposing LDS reads of the same rows.
 #include <algorithm>
 
 #include "common.h"
@@ -7,86 +36,947 @@
 namespace vh {
 namespace {
 
+constexpr float kMaxSlack = 8.0f;  // scores may pass the running maximum by this (base 2)
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// v_mfma_f32_16x16x32_bf16.  Lane l supplies A row l % 16 and B column l % 16 at
+// k = 8 * (l / 16) .. + 7; D[4 * (l / 16) + r][l % 16] lands in register r.
+__device__ __forceinline__ f32x4 mfma16x16x32_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The upper halves of two floats: bf16 by truncation, which never overflows.
+__device__ __forceinline__ uint32_t high_halves(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+// Two floats rounded to bf16 (the empty asm keeps the compiler from converting
+// each again where a half is used).
+__device__ __forceinline__ uint32_t round_halves(float a, float b) {
+    const bf16x2 h = {(__bf16)a, (__bf16)b};
+    uint32_t u = __builtin_bit_cast(uint32_t, h);
+    asm("" : "+v"(u));
+    return u;
+}
+// x = p0 + p1 + p2 exactly (of values above 2^-110): p0 truncated, so that the
+// largest floats stay finite, the others rounded.  An infinity's p1 is NaN.
+__device__ __forceinline__ void split3(float a, float b, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+    p0 = high_halves(a, b);
+    const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+    const float rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    p1 = round_halves(ra, rb);
+    p2 = round_halves(ra - __uint_as_float(p1 << 16), rb - __uint_as_float(p1 & 0xffff0000u));
+}
+__device__ __forceinline__ void split3(f32x4 a, f32x4 b, bf16x8 (&p)[3]) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 u[3];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        uint32_t w0, w1, w2;
+        split3(a[2 * i], a[2 * i + 1], w0, w1, w2);
+        u[0][i] = w0;
+        u[1][i] = w1;
+        u[2][i] = w2;
+        split3(b[2 * i], b[2 * i + 1], w0, w1, w2);
+        u[0][2 + i] = w0;
+        u[1][2 + i] = w1;
+        u[2][2 + i] = w2;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; i++) p[i] = __builtin_bit_cast(bf16x8, u[i]);
+}
+
+// max / sum with the lanes 16 and 32 away, on the VALU: a permlane swap of two
+// copies of v leaves v in one and the partner's v in the other, in either order.
+__device__ __forceinline__ void swap16(float &a, float &b) {
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ void swap32(float &a, float &b) {
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ float max_groups(float v) {
+    float a = v, b = v;
+    swap16(a, b);
+    a = b = fmaxf(a, b);
+    swap32(a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+// Four bf16 of column li of a 4 x 16 tile in LDS, whose row r is in the lanes 4 r
+// .. 4 r + 3 of each 16-lane group (lane i gives the address of row i / 4, columns
+// 4 (i % 4) .. + 3, and receives column i).
+__device__ __forceinline__ bf16x4 read_tr(const char *p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                          (__attribute__((address_space(3))) s16x4 *)p));
+}
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+__device__ __forceinline__ bool finite8(f32x4 a, f32x4 b) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        m = max(m, __float_as_uint(a[e]) & 0x7fffffffu);
+        m = max(m, __float_as_uint(b[e]) & 0x7fffffffu);
+    }
+    return m < 0x7f800000u;
+}
+
+// ---- the partition ----------------------------------------------------------------
+
 // Keys [lo, hi) that a query at position pos of a request of len tokens sees.
 struct Seen {
     int lo, hi;
 };
-__device__ __forceinline__ Seen keys_seen(const CacheAttn &a, int len, long long pos) {
+__device__ __forceinline__ Seen keys_seen(const CacheAttn &a, int len, int pos) {
     long long hi = len;
     if (a.block) hi = pos < 0 ? 0 : min(hi, ((long long)((unsigned)pos / a.block) + 1) * a.block);
     const long long lo = a.window ? max(0ll, hi - a.window) : 0;
     return {(int)lo, (int)hi};
 }
 
-template <int KIND>
-__device__ __forceinline__ float cache_value(const CacheView &c, bool is_v, size_t row, int d) {
-    const void *base = is_v ? c.v : c.k;
-    if constexpr (KIND == kCacheF32) return static_cast<const float *>(base)[row * c.width + d];
-    if constexpr (KIND == kCacheBf16) return (float)static_cast<const __bf16 *>(base)[row * c.width + d];
-    const uint16_t s = (is_v ? c.vd : c.kd)[row * (c.width / 32) + d / 32];
-    return (float)static_cast<const int8_t *>(base)[row * c.width + d] * (float)__builtin_bit_cast(_Float16, s);
+struct Tile {
+    int r, start, len, pos;  // request, its first new token, its tokens, the first new one's position
+    int row, rows;           // query rows (token of the request * group + head of the group)
+    Seen any, all;           // keys that some row sees, that every row sees
+    int step0, cost;         // first key step and their number, 1 where there is none
+};
+
+__device__ __forceinline__ int start_of(const CacheAttn &a, int r) { return min(max(a.starts[r], 0), a.tokens); }
+
+template <int BM, int STEP>
+__device__ __forceinline__ Tile tile_of(const CacheAttn &a, const int *first_tile, int ti) {
+    int lo = 0, hi = a.requests;  // first_tile[lo] <= ti < first_tile[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first_tile[mid] <= ti) lo = mid;
+        else hi = mid;
+    }
+    Tile t;
+    t.r = lo;
+    t.start = start_of(a, lo);
+    const int n = start_of(a, lo + 1) - t.start;
+    // A length that the table's row cannot hold ends with the row, and lengths end
+    // where a step past them still counts in 31 bits.
+    t.len = (int)min((long long)max(a.lens[lo], 0),
+                     min(a.max_pages << a.cache.page_shift, (long long)INT32_MAX - 4095));
+    t.pos = t.len - n;
+    t.row = (ti - first_tile[lo]) * BM;
+    t.rows = min(BM, n * a.group - t.row);
+    const Seen s0 = keys_seen(a, t.len, t.pos + t.row / a.group);
+    const Seen s1 = keys_seen(a, t.len, t.pos + (t.row + t.rows - 1) / a.group);
+    t.any = {s0.lo, s1.hi};
+    t.all = {s1.lo, s0.hi};
+    t.step0 = t.any.lo / STEP;
+    t.cost = max(1, (t.any.hi + STEP - 1) / STEP - t.step0);
+    return t;
 }
 
-// One wave a query and head: a lane takes a key for the scores, then two dims
-// for the sum.
-template <int KIND>
-__global__ __launch_bounds__(64) void cache_attn_kernel(CacheAttn a) {
-    const int lane = threadIdx.x, t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-    const int g = h / a.group;
-    int r = 0;
-    auto start = [&](int i) { return min(max(a.starts[i], 0), a.tokens); };
-    while (r < a.requests && start(r + 1) <= t) r++;
-    if (r == a.requests || start(r) > t) return;
-    const int len = (int)min((long long)max(a.lens[r], 0), a.max_pages << a.cache.page_shift);
-    const long long pos = (long long)len - (start(r + 1) - start(r)) + (t - start(r));
-    const Seen seen = keys_seen(a, len, pos);
-    const float *q = a.q + ((size_t)t * a.heads + h) * a.head_dim;
-    float m = -INFINITY, l = 0.0f, o[2] = {0.0f, 0.0f};
-    const int mask = (1 << a.cache.page_shift) - 1;
-    for (int k0 = seen.lo; k0 < seen.hi; k0 += 64) {
-        const int key = k0 + lane;
-        int page = -1;
-        if (key < seen.hi) page = a.table[(size_t)r * a.max_pages + (key >> a.cache.page_shift)];
-        const bool live = page >= 0 && page < a.cache.slots >> a.cache.page_shift;
-        const size_t row = live ? cache_row(a.cache, (page << a.cache.page_shift) + (key & mask), g) : 0;
-        float s = -INFINITY;
-        if (live) {
-            s = 0.0f;
-            for (int d = 0; d < a.head_dim; d++) s += q[d] * cache_value<KIND>(a.cache, false, row, d);
-            s *= a.scale_log2;
-        }
-        const float mn = fmaxf(m, wave_max(s)), ref = mn == -INFINITY ? 0.0f : mn;
-        const float corr = exp2f(m - ref), p = exp2f(s - ref);
-        m = mn;
-        l = l * corr + wave_sum(p);
-        // 64 keys are summed before they meet the rest: a chain of roundings over a
-        // long context stays short.
-        float some[2] = {0.0f, 0.0f};
-        for (int j = 0; j < 64; j++) {
-            const size_t vrow = (size_t)__shfl((long long)row, j, 64);
-            const float pj = __shfl(p, j, 64);
-            if (!__shfl((int)live, j, 64)) continue;
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                if (lane + 64 * u < a.head_dim) some[u] += pj * cache_value<KIND>(a.cache, true, vrow, lane + 64 * u);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; u++) o[u] = o[u] * corr + some[u];
-    }
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-        if (lane + 64 * u < a.head_dim)
-            a.out[((size_t)t * a.heads + h) * a.head_dim + lane + 64 * u] = l == 0.0f ? 0.0f : o[u] / l;
+// The same in scalar registers (all lanes have formed the same).
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Tile uniform(const Tile &t) {
+    return {uniform(t.r),   uniform(t.start), uniform(t.len),
+            uniform(t.pos), uniform(t.row),   uniform(t.rows),
+            {uniform(t.any.lo), uniform(t.any.hi)}, {uniform(t.all.lo), uniform(t.all.hi)},
+            uniform(t.step0), uniform(t.cost)};
 }
+
+// Inclusive sum over the workgroup's 256 threads, and the sum of all of them.
+__device__ __forceinline__ long long scan256(long long v, long long *tmp, long long *all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long w = __shfl_up(v, o, 64);
+        if (lane >= o) v += w;
+    }
+    if (lane == 63) tmp[wave] = v;
+    __syncthreads();
+    long long before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        if (w < wave) before += tmp[w];
+        sum += tmp[w];
+    }
+    __syncthreads();
+    *all = sum;
+    return v + before;
+}
+
+// What a workgroup knows of the partition: steps of all tiles of one head of the
+// cache (units), the share of a workgroup, and where a given step lies.
+struct Partition {
+    int tiles;
+    long long units, total, share;
+};
+struct Place {
+    int head, tile;
+    long long into;  // steps of the tile before it
+    long long begin; // of the tile, among all steps
+};
+
+template <int BM, int STEP>
+__device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_tile, long long *tmp, int shares) {
+    const int tid = threadIdx.x;
+    Partition p;
+    long long all = 0, base = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += 256) {
+        const int r = r0 + tid;
+        const long long n = r < a.requests ? max(start_of(a, r + 1) - start_of(a, r), 0) : 0;
+        const long long tiles = (n * a.group + BM - 1) / BM;
+        const long long end = base + scan256(tiles, tmp, &all);
+        base += all;
+        // Falling starts may name a token several times: tiles past 2^30 are left out.
+        if (r < a.requests) first_tile[r] = (int)min(end - tiles, 1ll << 30);
+    }
+    if (tid == 0) first_tile[a.requests] = (int)min(base, 1ll << 30);
+    __syncthreads();
+    p.tiles = first_tile[a.requests];
+    p.units = 0;
+    for (int t0 = 0; t0 < p.tiles; t0 += 256) {
+        const int ti = t0 + tid;
+        scan256(ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0, tmp, &all);
+        p.units += all;
+    }
+    p.total = p.units * a.cache.kv_heads;
+    p.share = max((long long)a.min_share, (p.total + shares - 1) / shares);
+    return p;
+}
+
+template <int BM, int STEP>
+__device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, const int *first_tile, long long *tmp,
+                                      long long unit) {
+    __shared__ long long found[2];
+    Place at;
+    at.head = (int)(unit / p.units);
+    const long long x = unit - at.head * p.units;
+    long long all = 0, base = 0;
+    for (int t0 = 0; t0 < p.tiles; t0 += 256) {
+        const int ti = t0 + (int)threadIdx.x;
+        const long long cost = ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0;
+        const long long end = base + scan256(cost, tmp, &all);
+        if (end - cost <= x && x < end) {
+            found[0] = ti;
+            found[1] = end - cost;
+        }
+        base += all;
+        if (x < base) break;
+    }
+    __syncthreads();
+    at.tile = (int)found[0];
+    at.into = x - found[1];
+    at.begin = at.head * p.units + found[1];
+    __syncthreads();
+    return at;
+}
+
+// The slot of a request's key, or -1.
+__device__ __forceinline__ int slot_of(const CacheAttn &a, const Tile &t, int key) {
+    if (key < t.any.lo || key >= t.any.hi) return -1;
+    const int page = a.table[(size_t)t.r * a.max_pages + (key >> a.cache.page_shift)];
+    if (page < 0 || page >= a.cache.slots >> a.cache.page_shift) return -1;
+    return (page << a.cache.page_shift) + (key & ((1 << a.cache.page_shift) - 1));
+}
+// Its row; the row of zeros behind the last one for none.
+__device__ __forceinline__ size_t row_of(const CacheAttn &a, int slot, int g) {
+    return slot < 0 ? (size_t)a.cache.slots * a.cache.kv_heads : cache_row(a.cache, slot, g);
+}
+
+// ---- one wave's arithmetic ---------------------------------------------------------
+
+// QT tiles of 16 queries: their fragments (three parts), running maxima and sums,
+// and O^T: o[df][u][r] = O[query 16 u + li][16 df + 4 lh + r].
+template <int D, int QT>
+struct Queries {
+    static constexpr int C = D / 32, DF = D / 16;
+    bf16x8 q[QT][C][3];
+    f32x4 o[DF][QT];
+    float m[QT], l[QT];
+    Seen seen[QT];
+
+    // Rows first .. first + 16 QT - 1 of the tile (rows past its end: zeros).
+    __device__ __forceinline__ void load(const CacheAttn &a, const Tile &t, int g, int first, int li, int lh) {
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            const int in = first + 16 * u + li;
+            const bool there = in < t.rows;
+            const int row = t.row + (there ? in : 0), token = row / a.group, head = g * a.group + row % a.group;
+            const float *src = a.q + ((size_t)(t.start + token) * a.heads + head) * a.head_dim;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                f32x4 x[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int d = 32 * c + 8 * lh + 4 * e;
+                    x[e] = there && d < a.head_dim ? *reinterpret_cast<const f32x4 *>(src + d)
+                                                   : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                split3(x[0], x[1], q[u][c]);
+            }
+            seen[u] = there ? keys_seen(a, t.len, t.pos + token) : Seen{0, INT32_MAX};
+            m[u] = -INFINITY;
+            l[u] = 0.0f;
+#pragma unroll
+            for (int df = 0; df < DF; df++) o[df][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+
+    // Scores of 32 keys from key on: the unseen ones out.  present: bit 16 t + i.
+    __device__ __forceinline__ void mask(f32x4 (&s)[2][QT], int key, uint32_t present, int lh) const {
+#pragma unroll
+        for (int u = 0; u < QT; u++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int in = 16 * t + 4 * lh + r;
+                    if (key + in < seen[u].lo || key + in >= seen[u].hi || !(present >> in & 1)) s[t][u][r] = -INFINITY;
+                }
+    }
+
+    // The weights of 32 keys as parts, with sums and maxima brought up to date.  The
+    // maximum is only raised where a score passes it by kMaxSlack, so most steps
+    // need no correction.
+    __device__ __forceinline__ void softmax(f32x4 (&s)[2][QT], float scale, bf16x8 (&p)[QT][3]) {
+        float mx[QT];
+        bool raise = false;
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            float v = fmaxf(fmaxf(s[0][u][0], s[0][u][1]), s[0][u][2]);
+            v = fmaxf(fmaxf(v, s[0][u][3]), s[1][u][0]);
+            v = fmaxf(fmaxf(v, s[1][u][1]), s[1][u][2]);
+            mx[u] = fmaxf(v, s[1][u][3]) * scale;
+            raise |= mx[u] > m[u] + kMaxSlack;
+        }
+        // (Before any key was seen the maximum is -inf: any score passes it.)
+        if (__any(raise)) {
+#pragma unroll
+            for (int u = 0; u < QT; u++) {
+                const float mn = fmaxf(m[u], max_groups(mx[u]));
+                const float corr = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
+                m[u] = mn;
+                l[u] *= corr;
+#pragma unroll
+                for (int df = 0; df < DF; df++) o[df][u] *= corr;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            const float off = m[u] == -INFINITY ? 0.0f : -m[u];
+            f32x4 e[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) e[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][u][r], scale, off));
+            l[u] += ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
+            split3(e[0], e[1], p[u]);
+        }
+    }
+
+    // O^T += V^T . P^T for 32 keys; v: this lane's address in the first plane.
+    template <int NP>
+    __device__ __forceinline__ void add(const char *v, int plane, int vx, int vg, const bf16x8 (&p)[QT][3]) {
+#pragma unroll
+        for (int df = 0; df < DF; df++) {
+            bf16x8 f[NP];
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const char *at = v + i * plane + (((2 * df + vg) ^ vx) << 4);
+                const bf16x4 x = read_tr(at), y = read_tr(at + 16 * D * 2);
+                f[i] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            // The small products first.
+#pragma unroll
+            for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+                for (int i = NP - 1; i >= 0; i--)
+                    if (sum - i >= 0)
+#pragma unroll
+                        for (int u = 0; u < QT; u++) o[df][u] = mfma16x16x32_bf16(f[i], p[u][sum - i], o[df][u]);
+        }
+    }
+};
+
+// Swizzle of V's planes: pairs of 16-byte granules by the row, so that the 16
+// rows x 32 bytes of a transposing read spread over the banks.
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+    return D == 64 ? (row & 6) : 2 * (row & 7);
+}
+
+__device__ __forceinline__ float half_value(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+
+// Eight dims of a cache row as it is stored, and as parts.
+template <int KIND>
+struct Octet;
+template <>
+struct Octet<kCacheF32> {
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + row * width + d);
+        a = p[0];
+        b = p[1];
+    }
+    __device__ __forceinline__ void parts(bf16x8 (&p)[3]) const { split3(a, b, p); }
+};
+template <>
+struct Octet<kCacheBf16> {
+    bf16x8 x;
+    __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
+        x = *reinterpret_cast<const bf16x8 *>(static_cast<const __bf16 *>(base) + row * width + d);
+    }
+};
+template <>
+struct Octet<kCacheQ8> {
+    uint2 x;
+    __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
+        x = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(base) + row * width + d);
+    }
+    __device__ __forceinline__ void values(f32x4 &a, f32x4 &b) const {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            a[e] = (float)(int8_t)(x.x >> (8 * e));
+            b[e] = (float)(int8_t)(x.y >> (8 * e));
+        }
+    }
+    // The integers as bf16.
+    __device__ __forceinline__ bf16x8 integers() const {
+        f32x4 a, b;
+        values(a, b);
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(bf16x8, u32x4{high_halves(a[0], a[1]), high_halves(a[2], a[3]),
+                                                high_halves(b[0], b[1]), high_halves(b[2], b[3])});
+    }
+    // (A value is not finite where its block's scale is not.)
+    __device__ __forceinline__ void parts(float d, bf16x8 (&p)[3]) const {
+        f32x4 a, b;
+        values(a, b);
+        split3(a * d, b * d, p);
+    }
+};
+
+// Values that are not finite become zeros; whether there were any.
+__device__ __forceinline__ bool drop(Octet<kCacheF32> &x, uint16_t) {
+    if (finite8(x.a, x.b)) return false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (!(fabsf(x.a[e]) < INFINITY)) x.a[e] = 0.0f;
+        if (!(fabsf(x.b[e]) < INFINITY)) x.b[e] = 0.0f;
+    }
+    return true;
+}
+__device__ __forceinline__ bool drop(Octet<kCacheBf16> &x, uint16_t) {
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (!(fabsf((float)x.x[e]) < INFINITY)) {
+            x.x[e] = (__bf16)0.0f;
+            bad = true;
+        }
+    return bad;
+}
+__device__ __forceinline__ bool drop(Octet<kCacheQ8> &, uint16_t &d) {
+    if ((d & 0x7c00) != 0x7c00) return false;
+    d = 0;
+    return true;
+}
+
+template <int KIND>
+constexpr int kPartsOfK = KIND == kCacheF32 ? 3 : 1;
+template <int KIND>
+constexpr int kPartsOfV = KIND == kCacheBf16 ? 1 : 3;
+
+// A value that is not finite in a step where some query does not see it was
+// staged as zero: the dims of the queries that do see it become NaN here.  32 keys
+// from key on, of which `present` are there; rare, so one by one.
+template <int KIND, int D, int QT>
+__device__ void add_not_finite(const CacheAttn &a, const Tile &t, int g, Queries<D, QT> &w, int key, int lh) {
+    for (int i = 0; i < 32; i++) {
+        const int slot = slot_of(a, t, key + i);
+        if (slot < 0) continue;
+        const size_t row = row_of(a, slot, g);
+#pragma unroll
+        for (int df = 0; df < D / 16; df++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const size_t at = row * D + 16 * df + 4 * lh + r;
+                float v;
+                if constexpr (KIND == kCacheF32) v = static_cast<const float *>(a.cache.v)[at];
+                else if constexpr (KIND == kCacheBf16) v = (float)static_cast<const __bf16 *>(a.cache.v)[at];
+                else v = half_value(a.cache.vd[at / 32]);
+                if (fabsf(v) < INFINITY) continue;
+#pragma unroll
+                for (int u = 0; u < QT; u++)
+                    if (key + i >= w.seen[u].lo && key + i < w.seen[u].hi) w.o[df][u][r] = NAN;
+            }
+    }
+}
+
+// Row `in` of a tile, four dims from d on: the result, or a workgroup's part of it
+// ([2 shares][BM][D] sums, then [2 shares][BM] maxima and sums of weights).
+template <int BM, int D>
+struct Output {
+    const CacheAttn &a;
+    const Tile &t;
+    int g;
+    int part;  // -1: the whole
+    __device__ __forceinline__ void put(int in, int d, f32x4 v, float m, float l) const {
+        if (in >= t.rows) return;
+        if (part < 0) {
+            if (d >= a.head_dim) return;
+            const int row = t.row + in, token = row / a.group, head = g * a.group + row % a.group;
+            const float inv = 1.0f / l;
+            f32x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = l == 0.0f ? 0.0f : v[e] * inv;
+            *reinterpret_cast<f32x4 *>(a.out + ((size_t)(t.start + token) * a.heads + head) * a.head_dim + d) = y;
+        } else {
+            const size_t at = (size_t)part * BM + in;
+            *reinterpret_cast<f32x4 *>(a.parts + at * D + d) = v;
+            if (d == 0) {
+                float *ml = a.parts + (size_t)2 * a.shares * BM * D + 2 * at;
+                ml[0] = m;
+                ml[1] = l;
+            }
+        }
+    }
+};
+
+// Shares in the order of the steps, those of one XCD (workgroups go round-robin over
+// the eight) next to each other: tiles of one head and request share K and V in its
+// L2.
+__device__ __forceinline__ int my_share(const CacheAttn &a) {
+    return (blockIdx.x & 7) * (a.shares >> 3) + (blockIdx.x >> 3);
+}
+
+// Walks this workgroup's steps tile by tile: f(tile, head, first step, steps, part).
+// Without room for parts (a.parts null) every workgroup takes whole tiles.
+template <int BM, int STEP, class F>
+__device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, F f) {
+    __shared__ long long tmp[4];
+    const Partition p = partition<BM, STEP>(a, first_tile, tmp, a.shares);
+    const int w = my_share(a);
+    if (!a.parts) {
+        for (long long id = w; id < (long long)p.tiles * a.cache.kv_heads; id += a.shares) {
+            const int g = uniform((int)(id / p.tiles));
+            const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, (int)(id - (long long)g * p.tiles)));
+            f(t, g, t.step0, t.cost, -1);
+        }
+        return;
+    }
+    long long at = w * p.share;
+    const long long end = min(at + p.share, p.total);
+    if (at >= end) return;
+    Place place = find<BM, STEP>(a, p, first_tile, tmp, at);
+    for (bool first = true; at < end; first = false) {
+        const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, place.tile));
+        const int into = uniform((int)place.into);
+        const int steps = uniform((int)min(end - at, (long long)t.cost - into));
+        const bool whole = into == 0 && steps == t.cost;
+        f(t, uniform(place.head), t.step0 + into, steps, whole ? -1 : 2 * w + (first ? 0 : 1));
+        at += steps;
+        place.into = 0;
+        if (++place.tile == p.tiles) {
+            place.tile = 0;
+            place.head++;
+        }
+    }
+}
+
+// ---- few rows -------------------------------------------------------------------
+
+template <int KIND, int D>
+constexpr int few_wave_bytes() {
+    // V's planes of 32 keys and K's scales, or the wave's O at the end.
+    constexpr int panel = kPartsOfV<KIND> * 32 * D * 2 + (KIND == kCacheQ8 ? 32 * (D / 32) * 4 : 0);
+    constexpr int o = 16 * D * 4 + 128;
+    return panel > o ? panel : o;
+}
+
+template <int KIND, int D>
+__global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
+    constexpr int BM = 16, STEP = 128, C = D / 32, WAVE = few_wave_bytes<KIND, D>();
+    constexpr int NPK = kPartsOfK<KIND>, NPV = kPartsOfV<KIND>, PLANE = 32 * D * 2;
+    constexpr int LPR = D / 8, RPP = 64 / LPR, PASSES = 32 / RPP;  // V: lanes a row, rows a pass
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int *first_tile = reinterpret_cast<int *>(smem + 4 * WAVE);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lh = lane >> 4;
+    char *mine = smem + wave * WAVE;
+    float *k_scale = reinterpret_cast<float *>(mine + NPV * PLANE);  // [C][32]
+
+    walk<BM, STEP>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
+        Queries<D, 1> w;
+        w.load(a, t, g, 0, li, lh);
+        Octet<KIND> kr[2][C], vr[PASSES];
+        uint16_t kd[C] = {}, vd[PASSES] = {};
+        int slot = 0;  // of key `lane & 31` of the step
+        auto load_k = [&] {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const size_t row = row_of(a, __shfl(slot, 16 * j + li, 64), g);
+#pragma unroll
+                for (int c = 0; c < C; c++) kr[j][c].load(a.cache.k, row, D, 32 * c + 8 * lh);
+            }
+            if constexpr (KIND == kCacheQ8) {
+                const size_t row = row_of(a, slot, g);
+#pragma unroll
+                for (int c = 0; c < C; c++) kd[c] = a.cache.kd[row * C + c];
+            }
+        };
+        auto load_v = [&](int from) {
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) {
+                const size_t row = row_of(a, __shfl(from, i * RPP + lane / LPR, 64), g);
+                vr[i].load(a.cache.v, row, D, 8 * (lane % LPR));
+                if constexpr (KIND == kCacheQ8) vd[i] = a.cache.vd[row * C + (lane % LPR) / 4];
+            }
+        };
+        const int keys0 = step0 * STEP + 32 * wave;
+        slot = slot_of(a, t, keys0 + (lane & 31));
+        load_k();
+        load_v(slot);
+        for (int i = 0; i < steps; i++) {
+            const int key = keys0 + i * STEP;
+            const uint32_t present = (uint32_t)__ballot(slot >= 0);
+            const bool partial = key < t.all.lo || key + 32 > t.all.hi || present != 0xffffffffu;
+            const int next = i + 1 < steps ? slot_of(a, t, key + STEP + (lane & 31)) : -1;
+            if (KIND == kCacheQ8 && lane < 32) {
+#pragma unroll
+                for (int c = 0; c < C; c++) k_scale[32 * c + lane] = half_value(kd[c]);
+            }
+            f32x4 s[2][1];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                s[j][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    bf16x8 f[NPK];
+                    if constexpr (KIND == kCacheF32) kr[j][c].parts(f);
+                    else if constexpr (KIND == kCacheBf16) f[0] = kr[j][c].x;
+                    else f[0] = kr[j][c].integers();
+                    f32x4 x = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[j][0];
+#pragma unroll
+                    for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+                        for (int e = NPK - 1; e >= 0; e--)
+                            if (sum - e >= 0) x = mfma16x16x32_bf16(f[e], w.q[0][c][sum - e], x);
+                    if constexpr (KIND == kCacheQ8) {
+                        if (j == 0 && c == 0) wave_fence();
+                        const f32x4 d = *reinterpret_cast<const f32x4 *>(k_scale + 32 * c + 16 * j + 4 * lh);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) s[j][0][r] = __builtin_fmaf(d[r], x[r], s[j][0][r]);
+                    } else {
+                        s[j][0] = x;
+                    }
+                }
+            }
+            slot = next;
+            load_k();
+            if (partial) w.mask(s, key, present, lh);
+            bf16x8 p[1][3];
+            w.softmax(s, a.scale_log2, p);
+            bool dropped = false;
+#pragma unroll
+            for (int j = 0; j < PASSES; j++) {
+                if (partial) dropped |= drop(vr[j], vd[j]);
+                const int row = j * RPP + lane / LPR;
+                char *at = mine + row * (D * 2) + (((lane % LPR) ^ v_swizzle<D>(row)) << 4);
+                if constexpr (KIND == kCacheBf16) {
+                    *reinterpret_cast<bf16x8 *>(at) = vr[j].x;
+                } else {
+                    bf16x8 f[3];
+                    if constexpr (KIND == kCacheF32) vr[j].parts(f);
+                    else vr[j].parts(half_value(vd[j]), f);
+#pragma unroll
+                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(at + e * PLANE) = f[e];
+                }
+            }
+            load_v(next);
+            wave_fence();
+            const int vrow = 4 * lh + (li >> 2);
+            w.template add<NPV>(mine + vrow * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow), (li & 3) >> 1, p);
+            wave_fence();
+            if (__any(dropped)) add_not_finite<KIND>(a, t, g, w, key, lh);
+        }
+        // The four waves' sums, each on its own maximum, joined by all threads.
+        float *o = reinterpret_cast<float *>(mine);
+#pragma unroll
+        for (int df = 0; df < D / 16; df++) *reinterpret_cast<f32x4 *>(o + li * D + 16 * df + 4 * lh) = w.o[df][0];
+        const float l = sum_groups(w.l[0]);
+        if (lh == 0) {
+            o[16 * D + 2 * li] = w.m[0];
+            o[16 * D + 2 * li + 1] = l;
+        }
+        __syncthreads();
+        const Output<BM, D> out{a, t, g, part};
+        const int row = tid >> 4;
+        float m = -INFINITY, sum = 0.0f, f[4];
+#pragma unroll
+        for (int v = 0; v < 4; v++) m = fmaxf(m, reinterpret_cast<float *>(smem + v * WAVE)[16 * D + 2 * row]);
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const float *x = reinterpret_cast<float *>(smem + v * WAVE) + 16 * D + 2 * row;
+            f[v] = x[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[0] - m);
+            sum += x[1] * f[v];
+        }
+#pragma unroll
+        for (int d = 4 * (tid & 15); d < D; d += 64) {
+            f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                y += *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(smem + v * WAVE) + row * D + d) * f[v];
+            out.put(row, d, y, m, sum);
+        }
+        __syncthreads();
+    });
+}
+
+// ---- many rows --------------------------------------------------------------------
+
+template <int KIND, int D>
+constexpr int many_step() {
+    return KIND == kCacheF32 && D == 128 ? 32 : 64;
+}
+template <int KIND, int D>
+constexpr int many_bytes() {
+    constexpr int step = many_step<KIND, D>();
+    return (kPartsOfK<KIND> + kPartsOfV<KIND>)*step * D * 2 + (KIND == kCacheQ8 ? step * (D / 32) * 4 : 0) + 2 * step +
+           64;
+}
+
+template <int KIND, int D>
+__global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
+    constexpr int QT = 2, BM = 4 * QT * 16, STEP = many_step<KIND, D>(), C = D / 32;
+    constexpr int NPK = kPartsOfK<KIND>, NPV = kPartsOfV<KIND>, PLANE = STEP * D * 2;
+    constexpr int LPR = D / 8, RPP = 256 / LPR, PASSES = STEP / RPP;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char *kp = smem, *vp = smem + NPK * PLANE;
+    float *k_scale = reinterpret_cast<float *>(smem + (NPK + NPV) * PLANE);  // [C][STEP]
+    uint8_t *there = reinterpret_cast<uint8_t *>(k_scale) + (KIND == kCacheQ8 ? STEP * C * 4 : 0);  // [2][STEP]
+    int *flags = reinterpret_cast<int *>(there + 2 * STEP);  // [2] a key is absent, [2] a value was dropped
+    int *first_tile = reinterpret_cast<int *>(smem + many_bytes<KIND, D>());
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lh = lane >> 4;
+    const int srow = tid / LPR, sg = tid % LPR;  // staged row of a pass, and granule
+    auto k_swizzle = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
+
+    walk<BM, STEP>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
+        const int first = 16 * QT * wave;
+        const bool works = first < t.rows;
+        Queries<D, QT> w;
+        w.load(a, t, g, first, li, lh);
+        Octet<KIND> kr[PASSES], vr[PASSES];
+        uint16_t kd[PASSES] = {}, vd[PASSES] = {};
+        int slot[PASSES], next[PASSES];
+        auto look_up = [&](int step) {
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) next[i] = slot_of(a, t, step * STEP + i * RPP + srow);
+        };
+        auto load = [&] {
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) {
+                slot[i] = next[i];
+                const size_t row = row_of(a, slot[i], g);
+                kr[i].load(a.cache.k, row, D, 8 * sg);
+                vr[i].load(a.cache.v, row, D, 8 * sg);
+                if constexpr (KIND == kCacheQ8) {
+                    kd[i] = a.cache.kd[row * C + sg / 4];
+                    vd[i] = a.cache.vd[row * C + sg / 4];
+                }
+            }
+        };
+        look_up(step0);
+        load();
+        look_up(step0 + 1);
+        if (tid < 4) flags[tid] = 0;
+        for (int i = 0; i < steps; i++) {
+            const int key = (step0 + i) * STEP;
+            const bool edge = key < t.all.lo || key + STEP > t.all.hi;
+            __syncthreads();  // the panels' last readers are done
+            bool absent = false, dropped = false;
+#pragma unroll
+            for (int j = 0; j < PASSES; j++) {
+                const int row = j * RPP + srow;
+                absent |= slot[j] < 0;
+                if (sg == 0) there[(i & 1) * STEP + row] = slot[j] >= 0;
+                char *kat = kp + row * (D * 2) + ((sg ^ k_swizzle(row)) << 4);
+                char *vat = vp + row * (D * 2) + ((sg ^ v_swizzle<D>(row)) << 4);
+                if (edge) dropped |= drop(vr[j], vd[j]);
+                bf16x8 f[3];
+                if constexpr (KIND == kCacheF32) {
+                    kr[j].parts(f);
+#pragma unroll
+                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(kat + e * PLANE) = f[e];
+                    vr[j].parts(f);
+#pragma unroll
+                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(vat + e * PLANE) = f[e];
+                } else if constexpr (KIND == kCacheBf16) {
+                    *reinterpret_cast<bf16x8 *>(kat) = kr[j].x;
+                    *reinterpret_cast<bf16x8 *>(vat) = vr[j].x;
+                } else {
+                    *reinterpret_cast<bf16x8 *>(kat) = kr[j].integers();
+                    if (sg % 4 == 0) k_scale[(sg / 4) * STEP + row] = half_value(kd[j]);
+                    vr[j].parts(half_value(vd[j]), f);
+#pragma unroll
+                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(vat + e * PLANE) = f[e];
+                }
+            }
+            if (absent) flags[i & 1] = 1;
+            if (dropped) flags[2 + (i & 1)] = 1;
+            if (i + 1 < steps) {
+                load();
+                look_up(step0 + i + 2);
+            }
+            __syncthreads();
+            if (tid == 0) flags[(i + 1) & 1] = flags[2 + ((i + 1) & 1)] = 0;
+            if (!works) continue;
+            const bool partial = edge || flags[i & 1];
+            const bool fix = flags[2 + (i & 1)];
+#pragma unroll
+            for (int h = 0; h < STEP / 32; h++) {
+                f32x4 s[2][QT];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+#pragma unroll
+                    for (int u = 0; u < QT; u++) s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    const int row = 32 * h + 16 * j + li;
+#pragma unroll
+                    for (int c = 0; c < C; c++) {
+                        bf16x8 f[NPK];
+#pragma unroll
+                        for (int e = 0; e < NPK; e++)
+                            f[e] = *reinterpret_cast<const bf16x8 *>(kp + e * PLANE + row * (D * 2) +
+                                                                     (((4 * c + lh) ^ k_swizzle(row)) << 4));
+                        f32x4 x[QT];
+#pragma unroll
+                        for (int u = 0; u < QT; u++)
+                            x[u] = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[j][u];
+#pragma unroll
+                        for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+                            for (int e = NPK - 1; e >= 0; e--)
+                                if (sum - e >= 0)
+#pragma unroll
+                                    for (int u = 0; u < QT; u++)
+                                        x[u] = mfma16x16x32_bf16(f[e], w.q[u][c][sum - e], x[u]);
+                        if constexpr (KIND == kCacheQ8) {
+                            const f32x4 d =
+                                *reinterpret_cast<const f32x4 *>(k_scale + c * STEP + 32 * h + 16 * j + 4 * lh);
+#pragma unroll
+                            for (int u = 0; u < QT; u++)
+#pragma unroll
+                                for (int r = 0; r < 4; r++) s[j][u][r] = __builtin_fmaf(d[r], x[u][r], s[j][u][r]);
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < QT; u++) s[j][u] = x[u];
+                        }
+                    }
+                }
+                if (partial) {
+                    const uint32_t present = (uint32_t)__ballot(there[(i & 1) * STEP + 32 * h + (lane & 31)] != 0);
+                    w.mask(s, key + 32 * h, present, lh);
+                }
+                bf16x8 p[QT][3];
+                w.softmax(s, a.scale_log2, p);
+                const int vrow = 4 * lh + (li >> 2);
+                w.template add<NPV>(vp + (32 * h + vrow) * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow),
+                                    (li & 3) >> 1, p);
+                if (fix) add_not_finite<KIND>(a, t, g, w, key + 32 * h, lh);
+            }
+        }
+        const Output<BM, D> out{a, t, g, part};
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            const float l = sum_groups(w.l[u]);
+#pragma unroll
+            for (int df = 0; df < D / 16; df++)
+                out.put(first + 16 * u + li, 16 * df + 4 * lh, w.o[df][u], w.m[u], l);
+        }
+        __syncthreads();
+    });
+}
+
+// ---- tiles that several workgroups share ---------------------------------------------
+
+// Every border between two shares that lies inside a tile names it; the first
+// such border's workgroup joins its parts.
+template <int BM, int STEP, int D>
+__global__ __launch_bounds__(256) void join_kernel(CacheAttn a) {
+    extern __shared__ int first_tile[];
+    __shared__ long long tmp[4];
+    const Partition p = partition<BM, STEP>(a, first_tile, tmp, a.shares);
+    const long long border = (blockIdx.x + 1) * p.share;
+    if (border >= p.total) return;
+    const Place at = find<BM, STEP>(a, p, first_tile, tmp, border);
+    if (at.into == 0 || at.begin < border - p.share) return;  // between two tiles, or not the first
+    const Tile t = tile_of<BM, STEP>(a, first_tile, at.tile);
+    const int w0 = blockIdx.x, w1 = (int)((at.begin + t.cost - 1) / p.share);
+    const Output<BM, D> out{a, t, at.head, -1};
+    const float *ml = a.parts + (size_t)2 * a.shares * BM * D;
+    constexpr int LANES = D / 4;
+    for (int i = threadIdx.x; i < t.rows * LANES; i += 256) {
+        const int in = i / LANES, d = 4 * (i % LANES);
+        float m = -INFINITY, l = 0.0f;
+        f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = w0; w <= w1; w++) {
+            const size_t x = (size_t)(2 * w + (w == w0 && at.begin > w * p.share ? 1 : 0)) * BM + in;
+            const float mw = ml[2 * x], mn = fmaxf(m, mw);
+            const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float f1 = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mn);
+            m = mn;
+            l = l * f0 + ml[2 * x + 1] * f1;
+            y = y * f0 + *reinterpret_cast<const f32x4 *>(a.parts + x * D + d) * f1;
+        }
+        out.put(in, d, y, m, l);
+    }
+}
+
+template <int KIND, int D>
+hipError_t run_kind(hipStream_t s, const CacheAttn &a, bool few) {
+    const size_t lds = few ? 4 * few_wave_bytes<KIND, D>() : many_bytes<KIND, D>();
+    const size_t index = ((size_t)a.requests + 1) * sizeof(int);
+    static std::atomic<uint64_t> done_few{0}, done_many{0};
+    constexpr size_t most = (kMaxRequests + 1) * sizeof(int);
+    hipError_t e = few ? ensure_dynamic_lds(few_rows_kernel<KIND, D>, 4 * few_wave_bytes<KIND, D>() + most, done_few)
+                       : ensure_dynamic_lds(many_rows_kernel<KIND, D>, many_bytes<KIND, D>() + most, done_many);
+    if (e != hipSuccess) return e;
+    if (few) few_rows_kernel<KIND, D><<<a.shares, 256, lds + index, s>>>(a);
+    else many_rows_kernel<KIND, D><<<a.shares, 256, lds + index, s>>>(a);
+    e = hipGetLastError();
+    if (e != hipSuccess || !a.parts) return e;
+    if (few) join_kernel<16, 128, D><<<a.shares - 1, 256, index, s>>>(a);
+    else join_kernel<128, many_step<KIND, D>(), D><<<a.shares - 1, 256, index, s>>>(a);
+    return hipGetLastError();
+}
+
+constexpr int kShares = 512;  // two workgroups a CU
+
+// Tiles of 16 rows where the requests have few on average.
+bool few_rows(size_t rows, size_t requests) { return rows <= 32 * requests; }
 
 }  // namespace
 
-hipError_t launch_cache_attn(hipStream_t s, const CacheAttn &a) {
-    const unsigned grid = (unsigned)((size_t)a.tokens * a.heads);
-    if (a.cache.kind == kCacheF32) cache_attn_kernel<kCacheF32><<<grid, 64, 0, s>>>(a);
-    else if (a.cache.kind == kCacheBf16) cache_attn_kernel<kCacheBf16><<<grid, 64, 0, s>>>(a);
-    else cache_attn_kernel<kCacheQ8><<<grid, 64, 0, s>>>(a);
-    return hipGetLastError();
+size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t width) {
+    return (size_t)2 * kShares * (few_rows(tokens * group, requests) ? 16 : 128) * (width + 2);
+}
+
+hipError_t launch_cache_attn(hipStream_t s, CacheAttn a) {
+    a.shares = kShares;
+    a.min_share = 1;
+    const bool few = few_rows((size_t)a.tokens * a.group, (size_t)a.requests);
+    const bool wide = a.cache.width == 128;
+    switch (a.cache.kind) {
+        case kCacheF32: return wide ? run_kind<kCacheF32, 128>(s, a, few) : run_kind<kCacheF32, 64>(s, a, few);
+        case kCacheBf16: return wide ? run_kind<kCacheBf16, 128>(s, a, few) : run_kind<kCacheBf16, 64>(s, a, few);
+        default: return wide ? run_kind<kCacheQ8, 128>(s, a, few) : run_kind<kCacheQ8, 64>(s, a, few);
+    }
 }
 
 }  // namespace vh

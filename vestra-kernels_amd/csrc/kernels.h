@@ -318,6 +318,7 @@ hipError_t launch_gemm_q8_0_qkv(hipStream_t s, const int8_t *a_qs, const uint16_
 constexpr int kCacheF32 = 0, kCacheBf16 = 1, kCacheQ8 = 2;
 // K and V rows [page][kv_head][token of the page][width], width = 64 or 128
 // (columns past head_dim are zeros): rows of one head and page are consecutive.
+// One row of zeros follows the last.
 // Q8_0: the values as int8, the scales of their blocks of 32 as kd and vd
 // [row][width / 32] (binary16 bits).
 struct CacheView {
@@ -377,7 +378,12 @@ struct CacheAttn {
     int window;           // 0: none
     float scale_log2;     // softmax scale times log2(e)
     CacheView cache;
+    // Room for the parts of tiles that several workgroups share
+    // (cache_attn_floats()), or null: every tile is one workgroup's.
+    float *parts;
+    int shares, min_share;  // set by the launcher
 };
-hipError_t launch_cache_attn(hipStream_t s, const CacheAttn &a);
+size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t width);
+hipError_t launch_cache_attn(hipStream_t s, CacheAttn a);
 
 }  // namespace vh

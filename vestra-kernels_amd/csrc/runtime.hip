@@ -128,6 +128,7 @@ struct RtState {
     Workspace fcnt;                             // and the in-kernel merge's arrival counters
     Workspace aq;                               // Q8_0 activation blocks
     Workspace sx;                               // split rows of a projection's input
+    Workspace pa;                               // parts of the paged attention's tiles
     std::vector<void *> recorded;               // outgrown blocks that a graph may hold
     float *tw = nullptr;                        // balanced-tail GEMM partials
     unsigned *tcnt = nullptr;                   // and arrival counters (zeroed once)
@@ -152,7 +153,7 @@ struct RtState {
         give_back();
         hipStreamSynchronize(stream);
         for (auto &kv : rope_cache) hipFree(kv.second);
-        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx})
+        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx, &pa})
             if (w->p) hipFree(w->p);
         for (void *p : recorded) hipFree(p);
         if (tw) hipFree(tw);
@@ -3467,18 +3468,19 @@ extern "C" vh_status vh_kv_cache_new(const vh_runtime *rt, int type, size_t page
     w.width = head_dim <= 64 ? 64 : 128;
     while ((size_t)1 << w.page_shift < page_tokens) w.page_shift++;
     w.slots = (int)slots;
+    rows++;  // of zeros
     const size_t value = type == vh::kCacheF32 ? 4 : type == vh::kCacheBf16 ? 2 : 1;
     for (void **p : {&w.k, &w.v}) {
         char *q = nullptr;
         TRY(dalloc(s, rows * w.width * value, &q, "kv cache allocation"));
         *p = q;
-        if (rows && hipMemsetAsync(q, 0, rows * w.width * value, s.stream) != hipSuccess)
+        if (hipMemsetAsync(q, 0, rows * w.width * value, s.stream) != hipSuccess)
             return fail(VH_ERR_UPLOAD, hip_msg(what, hipGetLastError()));
     }
     if (type == vh::kCacheQ8)
         for (uint16_t **p : {&w.kd, &w.vd}) {
             TRY(dalloc(s, rows * (w.width / 32), p, "kv cache allocation"));
-            if (rows && hipMemsetAsync(*p, 0, rows * (w.width / 32) * 2, s.stream) != hipSuccess)
+            if (hipMemsetAsync(*p, 0, rows * (w.width / 32) * 2, s.stream) != hipSuccess)
                 return fail(VH_ERR_UPLOAD, hip_msg(what, hipGetLastError()));
         }
     *out = c.release();
@@ -3709,6 +3711,10 @@ extern "C" vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const v
     a.window = window < (size_t)INT32_MAX ? (int)window : 0;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.cache = cache->view;
+    // Without room for parts (a capture before this size ran) a tile's keys stay
+    // with one workgroup.
+    a.parts = static_cast<float *>(
+        grow_workspace(s, s.pa, vh::cache_attn_floats(tokens, heads / kvh, requests, a.cache.width) * sizeof(float)));
     return launch(s, "kv_attention", [&] { return vh::launch_cache_attn(s.stream, a); });
     GUARD_END
 }
