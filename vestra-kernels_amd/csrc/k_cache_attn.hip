@@ -186,19 +186,30 @@ __device__ __forceinline__ Tile uniform(const Tile &t) {
             uniform(t.step0), uniform(t.cost)};
 }
 
-// Inclusive sum over the workgroup's 256 threads, and the sum of all of them.
-__device__ __forceinline__ long long scan256(long long v, long long *tmp, long long *all) {
+// v of the lane that a DPP control names, zero where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long long dpp_or_zero(long long v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
+// Inclusive sum over the workgroup's threads, and the sum of all of them.  Within a
+// wave by DPP (row_shr 1, 2, 4, 8, then the last lane of a row to the next row and
+// of the lower half to the upper).
+template <int THREADS>
+__device__ __forceinline__ long long scan_all(long long v, long long *tmp, long long *all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const long long w = __shfl_up(v, o, 64);
-        if (lane >= o) v += w;
-    }
+    v += dpp_or_zero<0x111, 0xf>(v);
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);
+    v += dpp_or_zero<0x143, 0xc>(v);
     if (lane == 63) tmp[wave] = v;
     __syncthreads();
     long long before = 0, sum = 0;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < THREADS / 64; w++) {
         if (w < wave) before += tmp[w];
         sum += tmp[w];
     }
@@ -219,16 +230,16 @@ struct Place {
     long long begin; // of the tile, among all steps
 };
 
-template <int BM, int STEP>
+template <int BM, int STEP, int THREADS>
 __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_tile, long long *tmp, int shares) {
     const int tid = threadIdx.x;
     Partition p;
     long long all = 0, base = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += 256) {
+    for (int r0 = 0; r0 < a.requests; r0 += THREADS) {
         const int r = r0 + tid;
         const long long n = r < a.requests ? max(start_of(a, r + 1) - start_of(a, r), 0) : 0;
         const long long tiles = (n * a.group + BM - 1) / BM;
-        const long long end = base + scan256(tiles, tmp, &all);
+        const long long end = base + scan_all<THREADS>(tiles, tmp, &all);
         base += all;
         // Falling starts may name a token several times: tiles past 2^30 are left out.
         if (r < a.requests) first_tile[r] = (int)min(end - tiles, 1ll << 30);
@@ -237,9 +248,9 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
     __syncthreads();
     p.tiles = first_tile[a.requests];
     p.units = 0;
-    for (int t0 = 0; t0 < p.tiles; t0 += 256) {
+    for (int t0 = 0; t0 < p.tiles; t0 += THREADS) {
         const int ti = t0 + tid;
-        scan256(ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0, tmp, &all);
+        scan_all<THREADS>(ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0, tmp, &all);
         p.units += all;
     }
     p.total = p.units * a.cache.kv_heads;
@@ -247,7 +258,7 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
     return p;
 }
 
-template <int BM, int STEP>
+template <int BM, int STEP, int THREADS>
 __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, const int *first_tile, long long *tmp,
                                       long long unit) {
     __shared__ long long found[2];
@@ -255,10 +266,10 @@ __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, co
     at.head = (int)(unit / p.units);
     const long long x = unit - at.head * p.units;
     long long all = 0, base = 0;
-    for (int t0 = 0; t0 < p.tiles; t0 += 256) {
+    for (int t0 = 0; t0 < p.tiles; t0 += THREADS) {
         const int ti = t0 + (int)threadIdx.x;
         const long long cost = ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0;
-        const long long end = base + scan256(cost, tmp, &all);
+        const long long end = base + scan_all<THREADS>(cost, tmp, &all);
         if (end - cost <= x && x < end) {
             found[0] = ti;
             found[1] = end - cost;
@@ -274,16 +285,14 @@ __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, co
     return at;
 }
 
-// The slot of a request's key, or -1.
+// The slot of a key of a tile that sees some; one of the page of zeros behind the
+// last where the key is not there.  No branch: the table is read for the nearest
+// key of the tile.
 __device__ __forceinline__ int slot_of(const CacheAttn &a, const Tile &t, int key) {
-    if (key < t.any.lo || key >= t.any.hi) return -1;
-    const int page = a.table[(size_t)t.r * a.max_pages + (key >> a.cache.page_shift)];
-    if (page < 0 || page >= a.cache.slots >> a.cache.page_shift) return -1;
+    const int near = min(max(key, t.any.lo), t.any.hi - 1), pages = a.cache.slots >> a.cache.page_shift;
+    int page = a.table[(size_t)t.r * a.max_pages + (near >> a.cache.page_shift)];
+    if (near != key || (unsigned)page >= (unsigned)pages) page = pages;
     return (page << a.cache.page_shift) + (key & ((1 << a.cache.page_shift) - 1));
-}
-// Its row; the row of zeros behind the last one for none.
-__device__ __forceinline__ size_t row_of(const CacheAttn &a, int slot, int g) {
-    return slot < 0 ? (size_t)a.cache.slots * a.cache.kv_heads : cache_row(a.cache, slot, g);
 }
 
 // ---- one wave's arithmetic ---------------------------------------------------------
@@ -327,33 +336,42 @@ struct Queries {
 
     // Scores of 32 keys from key on: the unseen ones out.  present: bit 16 t + i.
     __device__ __forceinline__ void mask(f32x4 (&s)[2][QT], int key, uint32_t present, int lh) const {
+        asm volatile("" : "+s"(key));  // keeps what follows out of the steps that need none
 #pragma unroll
-        for (int u = 0; u < QT; u++)
+        for (int u = 0; u < QT; u++) {
+            // Bits [lo, hi) - key of 32, this lane's four of each tile lowest.
+            const int lo = min(max(seen[u].lo - key, 0), 32), hi = min(max(seen[u].hi - key, 0), 32);
+            const uint32_t bits =
+                (present & (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1)) >> (4 * lh);
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int in = 16 * t + 4 * lh + r;
-                    if (key + in < seen[u].lo || key + in >= seen[u].hi || !(present >> in & 1)) s[t][u][r] = -INFINITY;
-                }
+                for (int r = 0; r < 4; r++)
+                    if (!(bits & (1u << (16 * t + r)))) s[t][u][r] = -INFINITY;
+        }
     }
 
-    // The weights of 32 keys as parts, with sums and maxima brought up to date.  The
-    // maximum is only raised where a score passes it by kMaxSlack, so most steps
-    // need no correction.
-    __device__ __forceinline__ void softmax(f32x4 (&s)[2][QT], float scale, bf16x8 (&p)[QT][3]) {
+    // Brings the maxima up to those of H times 32 keys' scores.  They are only raised
+    // where a score passes one by kMaxSlack, so most steps need no correction.
+    // (Before any key was seen the maximum is -inf: any score passes it.)
+    template <int H>
+    __device__ __forceinline__ void raise(const f32x4 (&s)[H][2][QT], float scale) {
         float mx[QT];
-        bool raise = false;
+        bool over = false;
 #pragma unroll
         for (int u = 0; u < QT; u++) {
-            float v = fmaxf(fmaxf(s[0][u][0], s[0][u][1]), s[0][u][2]);
-            v = fmaxf(fmaxf(v, s[0][u][3]), s[1][u][0]);
-            v = fmaxf(fmaxf(v, s[1][u][1]), s[1][u][2]);
-            mx[u] = fmaxf(v, s[1][u][3]) * scale;
-            raise |= mx[u] > m[u] + kMaxSlack;
+            float v = s[0][0][u][0];
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                v = fmaxf(fmaxf(v, s[h][0][u][0]), s[h][0][u][1]);
+                v = fmaxf(fmaxf(v, s[h][0][u][2]), s[h][0][u][3]);
+                v = fmaxf(fmaxf(v, s[h][1][u][0]), s[h][1][u][1]);
+                v = fmaxf(fmaxf(v, s[h][1][u][2]), s[h][1][u][3]);
+            }
+            mx[u] = v * scale;
+            over |= mx[u] > m[u] + kMaxSlack;
         }
-        // (Before any key was seen the maximum is -inf: any score passes it.)
-        if (__any(raise)) {
+        if (__any(over)) {
 #pragma unroll
             for (int u = 0; u < QT; u++) {
                 const float mn = fmaxf(m[u], max_groups(mx[u]));
@@ -364,6 +382,10 @@ struct Queries {
                 for (int df = 0; df < DF; df++) o[df][u] *= corr;
             }
         }
+    }
+
+    // The weights of 32 keys as parts, and their sums.
+    __device__ __forceinline__ void weights(const f32x4 (&s)[2][QT], float scale, bf16x8 (&p)[QT][3]) {
 #pragma unroll
         for (int u = 0; u < QT; u++) {
             const float off = m[u] == -INFINITY ? 0.0f : -m[u];
@@ -380,23 +402,29 @@ struct Queries {
     // O^T += V^T . P^T for 32 keys; v: this lane's address in the first plane.
     template <int NP>
     __device__ __forceinline__ void add(const char *v, int plane, int vx, int vg, const bf16x8 (&p)[QT][3]) {
+        // Two tiles of dims at a time, the small products first: 2 QT sums that do
+        // not wait for each other.
 #pragma unroll
-        for (int df = 0; df < DF; df++) {
-            bf16x8 f[NP];
+        for (int d0 = 0; d0 < DF; d0 += 2) {
+            bf16x8 f[2][NP];
 #pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const char *at = v + i * plane + (((2 * df + vg) ^ vx) << 4);
-                const bf16x4 x = read_tr(at), y = read_tr(at + 16 * D * 2);
-                f[i] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-            // The small products first.
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    const char *at = v + i * plane + (((2 * (d0 + k) + vg) ^ vx) << 4);
+                    const bf16x4 x = read_tr(at), y = read_tr(at + 16 * D * 2);
+                    f[k][i] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
 #pragma unroll
             for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
                 for (int i = NP - 1; i >= 0; i--)
                     if (sum - i >= 0)
 #pragma unroll
-                        for (int u = 0; u < QT; u++) o[df][u] = mfma16x16x32_bf16(f[i], p[u][sum - i], o[df][u]);
+                        for (int k = 0; k < 2; k++)
+#pragma unroll
+                            for (int u = 0; u < QT; u++)
+                                o[d0 + k][u] = mfma16x16x32_bf16(f[k][i], p[u][sum - i], o[d0 + k][u]);
         }
     }
 };
@@ -497,8 +525,8 @@ template <int KIND, int D, int QT>
 __device__ void add_not_finite(const CacheAttn &a, const Tile &t, int g, Queries<D, QT> &w, int key, int lh) {
     for (int i = 0; i < 32; i++) {
         const int slot = slot_of(a, t, key + i);
-        if (slot < 0) continue;
-        const size_t row = row_of(a, slot, g);
+        if (slot >= a.cache.slots) continue;
+        const size_t row = cache_row(a.cache, slot, g);
 #pragma unroll
         for (int df = 0; df < D / 16; df++)
 #pragma unroll
@@ -553,32 +581,33 @@ __device__ __forceinline__ int my_share(const CacheAttn &a) {
     return (blockIdx.x & 7) * (a.shares >> 3) + (blockIdx.x >> 3);
 }
 
-// Walks this workgroup's steps tile by tile: f(tile, head, first step, steps, part).
-// Without room for parts (a.parts null) every workgroup takes whole tiles.
-template <int BM, int STEP, class F>
+// Walks this workgroup's steps tile by tile: f(tile, head, first step, steps, part),
+// no steps where a tile sees no key.  Without room for parts (a.parts null) every
+// workgroup takes whole tiles.
+template <int BM, int STEP, int THREADS, class F>
 __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, F f) {
-    __shared__ long long tmp[4];
-    const Partition p = partition<BM, STEP>(a, first_tile, tmp, a.shares);
+    __shared__ long long tmp[THREADS / 64];
+    const Partition p = partition<BM, STEP, THREADS>(a, first_tile, tmp, a.shares);
     const int w = my_share(a);
-    if (!a.parts) {
-        for (long long id = w; id < (long long)p.tiles * a.cache.kv_heads; id += a.shares) {
-            const int g = uniform((int)(id / p.tiles));
-            const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, (int)(id - (long long)g * p.tiles)));
-            f(t, g, t.step0, t.cost, -1);
-        }
-        return;
-    }
-    long long at = w * p.share;
-    const long long end = min(at + p.share, p.total);
+    const bool share = a.parts != nullptr;
+    // Steps of this workgroup, or the numbers of its tiles.
+    long long at = share ? w * p.share : w;
+    const long long end = share ? min(at + p.share, p.total) : (long long)p.tiles * a.cache.kv_heads;
     if (at >= end) return;
-    Place place = find<BM, STEP>(a, p, first_tile, tmp, at);
+    Place place = {0, 0, 0, 0};
+    if (share) place = find<BM, STEP, THREADS>(a, p, first_tile, tmp, at);
     for (bool first = true; at < end; first = false) {
+        if (!share) {
+            place.head = (int)(at / p.tiles);
+            place.tile = (int)(at - (long long)place.head * p.tiles);
+        }
         const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, place.tile));
         const int into = uniform((int)place.into);
-        const int steps = uniform((int)min(end - at, (long long)t.cost - into));
+        const int steps = share ? uniform((int)min(end - at, (long long)t.cost - into)) : t.cost;
         const bool whole = into == 0 && steps == t.cost;
-        f(t, uniform(place.head), t.step0 + into, steps, whole ? -1 : 2 * w + (first ? 0 : 1));
-        at += steps;
+        f(t, uniform(place.head), t.step0 + into, t.any.lo < t.any.hi ? steps : 0,
+          whole ? -1 : 2 * w + (first ? 0 : 1));
+        at += share ? steps : a.shares;
         place.into = 0;
         if (++place.tile == p.tiles) {
             place.tile = 0;
@@ -610,77 +639,87 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
     char *mine = smem + wave * WAVE;
     float *k_scale = reinterpret_cast<float *>(mine + NPV * PLANE);  // [C][32]
 
-    walk<BM, STEP>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
+    walk<BM, STEP, 256>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
         Queries<D, 1> w;
         w.load(a, t, g, 0, li, lh);
         Octet<KIND> kr[2][C], vr[PASSES];
         uint16_t kd[C] = {}, vd[PASSES] = {};
-        int slot = 0;  // of key `lane & 31` of the step
-        auto load_k = [&] {
+        // Of key `lane & 31` of a step, looked up two steps ahead.
+        auto look_up = [&](int i) { return slot_of(a, t, (step0 + i) * STEP + 32 * wave + (lane & 31)); };
+        auto load_k = [&](int slot) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const size_t row = row_of(a, __shfl(slot, 16 * j + li, 64), g);
+                const size_t row = cache_row(a.cache, __shfl(slot, 16 * j + li, 64), g);
 #pragma unroll
                 for (int c = 0; c < C; c++) kr[j][c].load(a.cache.k, row, D, 32 * c + 8 * lh);
             }
             if constexpr (KIND == kCacheQ8) {
-                const size_t row = row_of(a, slot, g);
+                const size_t row = cache_row(a.cache, slot, g);
 #pragma unroll
                 for (int c = 0; c < C; c++) kd[c] = a.cache.kd[row * C + c];
             }
         };
-        auto load_v = [&](int from) {
+        auto load_v = [&](int slot) {
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
-                const size_t row = row_of(a, __shfl(from, i * RPP + lane / LPR, 64), g);
+                const size_t row = cache_row(a.cache, __shfl(slot, i * RPP + lane / LPR, 64), g);
                 vr[i].load(a.cache.v, row, D, 8 * (lane % LPR));
                 if constexpr (KIND == kCacheQ8) vd[i] = a.cache.vd[row * C + (lane % LPR) / 4];
             }
         };
-        const int keys0 = step0 * STEP + 32 * wave;
-        slot = slot_of(a, t, keys0 + (lane & 31));
-        load_k();
-        load_v(slot);
+        int slot = 0, next = 0;
+        if (steps) {
+            slot = look_up(0);
+            next = look_up(1);
+            load_k(slot);
+            load_v(slot);
+        }
         for (int i = 0; i < steps; i++) {
-            const int key = keys0 + i * STEP;
-            const uint32_t present = (uint32_t)__ballot(slot >= 0);
+            const int key = (step0 + i) * STEP + 32 * wave;
+            const uint32_t present = (uint32_t)__ballot(slot < a.cache.slots);
             const bool partial = key < t.all.lo || key + 32 > t.all.hi || present != 0xffffffffu;
-            const int next = i + 1 < steps ? slot_of(a, t, key + STEP + (lane & 31)) : -1;
+            const int after = look_up(i + 2);
             if (KIND == kCacheQ8 && lane < 32) {
 #pragma unroll
                 for (int c = 0; c < C; c++) k_scale[32 * c + lane] = half_value(kd[c]);
             }
-            f32x4 s[2][1];
+            f32x4 sx[1][2][1];
+            f32x4(&s)[2][1] = sx[0];
+            s[0][0] = s[1][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (KIND == kCacheQ8) wave_fence();
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                s[j][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c = 0; c < C; c++) {
+                bf16x8 f[2][NPK];
+                f32x4 x[2];
 #pragma unroll
-                for (int c = 0; c < C; c++) {
-                    bf16x8 f[NPK];
-                    if constexpr (KIND == kCacheF32) kr[j][c].parts(f);
-                    else if constexpr (KIND == kCacheBf16) f[0] = kr[j][c].x;
-                    else f[0] = kr[j][c].integers();
-                    f32x4 x = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[j][0];
+                for (int j = 0; j < 2; j++) {
+                    if constexpr (KIND == kCacheF32) kr[j][c].parts(f[j]);
+                    else if constexpr (KIND == kCacheBf16) f[j][0] = kr[j][c].x;
+                    else f[j][0] = kr[j][c].integers();
+                    x[j] = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[j][0];
+                }
 #pragma unroll
-                    for (int sum = 2; sum >= 0; sum--)
+                for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
-                        for (int e = NPK - 1; e >= 0; e--)
-                            if (sum - e >= 0) x = mfma16x16x32_bf16(f[e], w.q[0][c][sum - e], x);
+                    for (int e = NPK - 1; e >= 0; e--)
+                        if (sum - e >= 0)
+#pragma unroll
+                            for (int j = 0; j < 2; j++) x[j] = mfma16x16x32_bf16(f[j][e], w.q[0][c][sum - e], x[j]);
+#pragma unroll
+                for (int j = 0; j < 2; j++)
                     if constexpr (KIND == kCacheQ8) {
-                        if (j == 0 && c == 0) wave_fence();
                         const f32x4 d = *reinterpret_cast<const f32x4 *>(k_scale + 32 * c + 16 * j + 4 * lh);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) s[j][0][r] = __builtin_fmaf(d[r], x[r], s[j][0][r]);
+                        for (int r = 0; r < 4; r++) s[j][0][r] = __builtin_fmaf(d[r], x[j][r], s[j][0][r]);
                     } else {
-                        s[j][0] = x;
+                        s[j][0] = x[j];
                     }
-                }
             }
-            slot = next;
-            load_k();
+            load_k(next);
             if (partial) w.mask(s, key, present, lh);
             bf16x8 p[1][3];
-            w.softmax(s, a.scale_log2, p);
+            w.raise(sx, a.scale_log2);
+            w.weights(s, a.scale_log2, p);
             bool dropped = false;
 #pragma unroll
             for (int j = 0; j < PASSES; j++) {
@@ -698,6 +737,8 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
                 }
             }
             load_v(next);
+            slot = next;
+            next = after;
             wave_fence();
             const int vrow = 4 * lh + (li >> 2);
             w.template add<NPV>(mine + vrow * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow), (li & 3) >> 1, p);
@@ -743,6 +784,8 @@ template <int KIND, int D>
 constexpr int many_step() {
     return KIND == kCacheF32 && D == 128 ? 32 : 64;
 }
+template <int D>
+constexpr int kManyThreads = D == 64 ? 256 : 512;
 template <int KIND, int D>
 constexpr int many_bytes() {
     constexpr int step = many_step<KIND, D>();
@@ -751,10 +794,10 @@ constexpr int many_bytes() {
 }
 
 template <int KIND, int D>
-__global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
-    constexpr int QT = 2, BM = 4 * QT * 16, STEP = many_step<KIND, D>(), C = D / 32;
+__global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) void many_rows_kernel(CacheAttn a) {
+    constexpr int THREADS = kManyThreads<D>, QT = 512 / THREADS, BM = 128, STEP = many_step<KIND, D>(), C = D / 32;
     constexpr int NPK = kPartsOfK<KIND>, NPV = kPartsOfV<KIND>, PLANE = STEP * D * 2;
-    constexpr int LPR = D / 8, RPP = 256 / LPR, PASSES = STEP / RPP;
+    constexpr int LPR = D / 8, RPP = THREADS / LPR, PASSES = STEP / RPP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     char *kp = smem, *vp = smem + NPK * PLANE;
     float *k_scale = reinterpret_cast<float *>(smem + (NPK + NPV) * PLANE);  // [C][STEP]
@@ -767,7 +810,7 @@ __global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
     const int srow = tid / LPR, sg = tid % LPR;  // staged row of a pass, and granule
     auto k_swizzle = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
 
-    walk<BM, STEP>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
+    walk<BM, STEP, THREADS>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
         const int first = 16 * QT * wave;
         const bool works = first < t.rows;
         Queries<D, QT> w;
@@ -783,7 +826,7 @@ __global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
                 slot[i] = next[i];
-                const size_t row = row_of(a, slot[i], g);
+                const size_t row = cache_row(a.cache, slot[i], g);
                 kr[i].load(a.cache.k, row, D, 8 * sg);
                 vr[i].load(a.cache.v, row, D, 8 * sg);
                 if constexpr (KIND == kCacheQ8) {
@@ -792,9 +835,11 @@ __global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
                 }
             }
         };
-        look_up(step0);
-        load();
-        look_up(step0 + 1);
+        if (steps) {
+            look_up(step0);
+            load();
+            look_up(step0 + 1);
+        }
         if (tid < 4) flags[tid] = 0;
         for (int i = 0; i < steps; i++) {
             const int key = (step0 + i) * STEP;
@@ -804,8 +849,8 @@ __global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
 #pragma unroll
             for (int j = 0; j < PASSES; j++) {
                 const int row = j * RPP + srow;
-                absent |= slot[j] < 0;
-                if (sg == 0) there[(i & 1) * STEP + row] = slot[j] >= 0;
+                absent |= slot[j] >= a.cache.slots;
+                if (sg == 0) there[(i & 1) * STEP + row] = slot[j] < a.cache.slots;
                 char *kat = kp + row * (D * 2) + ((sg ^ k_swizzle(row)) << 4);
                 char *vat = vp + row * (D * 2) + ((sg ^ v_swizzle<D>(row)) << 4);
                 if (edge) dropped |= drop(vr[j], vd[j]);
@@ -839,57 +884,72 @@ __global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
             if (!works) continue;
             const bool partial = edge || flags[i & 1];
             const bool fix = flags[2 + (i & 1)];
+            constexpr int H = STEP / 32;
+            f32x4 s[H][2][QT];
 #pragma unroll
-            for (int h = 0; h < STEP / 32; h++) {
-                f32x4 s[2][QT];
+            for (int h = 0; h < H; h++) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int u = 0; u < QT; u++) s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    const int row = 32 * h + 16 * j + li;
+                    for (int u = 0; u < QT; u++) s[h][j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int c = 0; c < C; c++) {
-                        bf16x8 f[NPK];
+                for (int c = 0; c < C; c++) {
+                    bf16x8 f[2][NPK];
+                    f32x4 x[2][QT];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int row = 32 * h + 16 * j + li;
 #pragma unroll
                         for (int e = 0; e < NPK; e++)
-                            f[e] = *reinterpret_cast<const bf16x8 *>(kp + e * PLANE + row * (D * 2) +
-                                                                     (((4 * c + lh) ^ k_swizzle(row)) << 4));
-                        f32x4 x[QT];
+                            f[j][e] = *reinterpret_cast<const bf16x8 *>(kp + e * PLANE + row * (D * 2) +
+                                                                        (((4 * c + lh) ^ k_swizzle(row)) << 4));
 #pragma unroll
                         for (int u = 0; u < QT; u++)
-                            x[u] = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[j][u];
+                            x[j][u] = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[h][j][u];
+                    }
 #pragma unroll
-                        for (int sum = 2; sum >= 0; sum--)
+                    for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
-                            for (int e = NPK - 1; e >= 0; e--)
-                                if (sum - e >= 0)
+                        for (int e = NPK - 1; e >= 0; e--)
+                            if (sum - e >= 0)
+#pragma unroll
+                                for (int j = 0; j < 2; j++)
 #pragma unroll
                                     for (int u = 0; u < QT; u++)
-                                        x[u] = mfma16x16x32_bf16(f[e], w.q[u][c][sum - e], x[u]);
+                                        x[j][u] = mfma16x16x32_bf16(f[j][e], w.q[u][c][sum - e], x[j][u]);
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
                         if constexpr (KIND == kCacheQ8) {
                             const f32x4 d =
                                 *reinterpret_cast<const f32x4 *>(k_scale + c * STEP + 32 * h + 16 * j + 4 * lh);
 #pragma unroll
                             for (int u = 0; u < QT; u++)
 #pragma unroll
-                                for (int r = 0; r < 4; r++) s[j][u][r] = __builtin_fmaf(d[r], x[u][r], s[j][u][r]);
+                                for (int r = 0; r < 4; r++)
+                                    s[h][j][u][r] = __builtin_fmaf(d[r], x[j][u][r], s[h][j][u][r]);
                         } else {
 #pragma unroll
-                            for (int u = 0; u < QT; u++) s[j][u] = x[u];
+                            for (int u = 0; u < QT; u++) s[h][j][u] = x[j][u];
                         }
-                    }
                 }
-                if (partial) {
+            }
+            if (partial)
+#pragma unroll
+                for (int h = 0; h < H; h++) {
                     const uint32_t present = (uint32_t)__ballot(there[(i & 1) * STEP + 32 * h + (lane & 31)] != 0);
-                    w.mask(s, key + 32 * h, present, lh);
+                    w.mask(s[h], key + 32 * h, present, lh);
                 }
+            w.raise(s, a.scale_log2);
+            const int vrow = 4 * lh + (li >> 2);
+#pragma unroll
+            for (int h = 0; h < H; h++) {
                 bf16x8 p[QT][3];
-                w.softmax(s, a.scale_log2, p);
-                const int vrow = 4 * lh + (li >> 2);
+                w.weights(s[h], a.scale_log2, p);
                 w.template add<NPV>(vp + (32 * h + vrow) * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow),
                                     (li & 3) >> 1, p);
-                if (fix) add_not_finite<KIND>(a, t, g, w, key + 32 * h, lh);
             }
+            if (fix)
+                for (int h = 0; h < H; h++) add_not_finite<KIND>(a, t, g, w, key + 32 * h, lh);
         }
         const Output<BM, D> out{a, t, g, part};
 #pragma unroll
@@ -907,34 +967,65 @@ __global__ __launch_bounds__(256, 2) void many_rows_kernel(CacheAttn a) {
 
 // Every border between two shares that lies inside a tile names it; the first
 // such border's workgroup joins its parts.
+// A row's four dims of a part, or of several: O on the maximum m, and the sum of
+// weights.
+struct Sums {
+    float m, l;
+    f32x4 y;
+    __device__ __forceinline__ void join(const Sums &b) {
+        const float mn = fmaxf(m, b.m);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        const float fb = b.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(b.m - mn);
+        m = mn;
+        l = l * f + b.l * fb;
+        y = y * f + b.y * fb;
+    }
+};
+
+// Of the workgroup's 1024 / D groups of lanes (a group holds a row) as many share a
+// row as the rows leave: a single query's parts are summed by all of them.
 template <int BM, int STEP, int D>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttn a) {
-    extern __shared__ int first_tile[];
+    extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ long long tmp[4];
-    const Partition p = partition<BM, STEP>(a, first_tile, tmp, a.shares);
+    __shared__ Sums some[256];
+    int *first_tile = reinterpret_cast<int *>(smem);
+    const Partition p = partition<BM, STEP, 256>(a, first_tile, tmp, a.shares);
     const long long border = (blockIdx.x + 1) * p.share;
     if (border >= p.total) return;
-    const Place at = find<BM, STEP>(a, p, first_tile, tmp, border);
+    const Place at = find<BM, STEP, 256>(a, p, first_tile, tmp, border);
     if (at.into == 0 || at.begin < border - p.share) return;  // between two tiles, or not the first
-    const Tile t = tile_of<BM, STEP>(a, first_tile, at.tile);
-    const int w0 = blockIdx.x, w1 = (int)((at.begin + t.cost - 1) / p.share);
-    const Output<BM, D> out{a, t, at.head, -1};
+    const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, at.tile));
+    const int w0 = blockIdx.x, w1 = uniform((int)((at.begin + t.cost - 1) / p.share));
+    const int part0 = 2 * w0 + (at.begin > w0 * p.share ? 1 : 0);
+    const Output<BM, D> out{a, t, uniform(at.head), -1};
     const float *ml = a.parts + (size_t)2 * a.shares * BM * D;
-    constexpr int LANES = D / 4;
-    for (int i = threadIdx.x; i < t.rows * LANES; i += 256) {
-        const int in = i / LANES, d = 4 * (i % LANES);
-        float m = -INFINITY, l = 0.0f;
-        f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int w = w0; w <= w1; w++) {
-            const size_t x = (size_t)(2 * w + (w == w0 && at.begin > w * p.share ? 1 : 0)) * BM + in;
-            const float mw = ml[2 * x], mn = fmaxf(m, mw);
-            const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            const float f1 = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mn);
-            m = mn;
-            l = l * f0 + ml[2 * x + 1] * f1;
-            y = y * f0 + *reinterpret_cast<const f32x4 *>(a.parts + x * D + d) * f1;
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+    int rows = 1;  // at once
+    while (rows < GROUPS && rows < t.rows) rows *= 2;
+    const int sharers = GROUPS / rows;
+    const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+    for (int in = group % rows; in < (t.rows + rows - 1) / rows * rows; in += rows) {
+        auto part = [&](int w) {
+            const size_t x = (size_t)(w == w0 ? part0 : 2 * w) * BM + min(in, t.rows - 1);
+            return Sums{ml[2 * x], ml[2 * x + 1], *reinterpret_cast<const f32x4 *>(a.parts + x * D + d)};
+        };
+        Sums sum{-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int w = w0 + group / rows; w <= w1; w += 4 * sharers) {
+            Sums x[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = part(min(w + u * sharers, w1));
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (w + u * sharers <= w1) sum.join(x[u]);
         }
-        out.put(in, d, y, m, l);
+        if (sharers > 1) {  // one pass: all rows at once
+            some[threadIdx.x] = sum;
+            __syncthreads();
+            if (group >= rows) return;
+            for (int i = 1; i < sharers; i++) sum.join(some[threadIdx.x + i * rows * LANES]);
+        }
+        out.put(in, d, sum.y, sum.m, sum.l);
     }
 }
 
@@ -948,7 +1039,7 @@ hipError_t run_kind(hipStream_t s, const CacheAttn &a, bool few) {
                        : ensure_dynamic_lds(many_rows_kernel<KIND, D>, many_bytes<KIND, D>() + most, done_many);
     if (e != hipSuccess) return e;
     if (few) few_rows_kernel<KIND, D><<<a.shares, 256, lds + index, s>>>(a);
-    else many_rows_kernel<KIND, D><<<a.shares, 256, lds + index, s>>>(a);
+    else many_rows_kernel<KIND, D><<<a.shares, kManyThreads<D>, lds + index, s>>>(a);
     e = hipGetLastError();
     if (e != hipSuccess || !a.parts) return e;
     if (few) join_kernel<16, 128, D><<<a.shares - 1, 256, index, s>>>(a);

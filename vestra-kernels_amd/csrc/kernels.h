@@ -318,7 +318,7 @@ hipError_t launch_gemm_q8_0_qkv(hipStream_t s, const int8_t *a_qs, const uint16_
 constexpr int kCacheF32 = 0, kCacheBf16 = 1, kCacheQ8 = 2;
 // K and V rows [page][kv_head][token of the page][width], width = 64 or 128
 // (columns past head_dim are zeros): rows of one head and page are consecutive.
-// One row of zeros follows the last.
+// One page of zeros follows the last.
 // Q8_0: the values as int8, the scales of their blocks of 32 as kd and vd
 // [row][width / 32] (binary16 bits).
 struct CacheView {

@@ -3468,7 +3468,7 @@ extern "C" vh_status vh_kv_cache_new(const vh_runtime *rt, int type, size_t page
     w.width = head_dim <= 64 ? 64 : 128;
     while ((size_t)1 << w.page_shift < page_tokens) w.page_shift++;
     w.slots = (int)slots;
-    rows++;  // of zeros
+    rows += page_tokens * kv_heads;  // a page of zeros
     const size_t value = type == vh::kCacheF32 ? 4 : type == vh::kCacheBf16 ? 2 : 1;
     for (void **p : {&w.k, &w.v}) {
         char *q = nullptr;
