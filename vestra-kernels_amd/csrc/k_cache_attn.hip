@@ -285,13 +285,17 @@ __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, co
     return at;
 }
 
-// The slot of a key of a tile that sees some; one of the page of zeros behind the
-// last where the key is not there.  No branch: the table is read for the nearest
-// key of the tile.
-__device__ __forceinline__ int slot_of(const CacheAttn &a, const Tile &t, int key) {
-    const int near = min(max(key, t.any.lo), t.any.hi - 1), pages = a.cache.slots >> a.cache.page_shift;
-    int page = a.table[(size_t)t.r * a.max_pages + (near >> a.cache.page_shift)];
-    if (near != key || (unsigned)page >= (unsigned)pages) page = pages;
+// The page of a key of a tile that sees some (of the nearest such key: no branch),
+// and the key's slot, one of the page of zeros behind the last where it is not
+// there.  Apart, so that a loop can load the page a step before it looks at it:
+// looking waits for every load issued before.
+__device__ __forceinline__ int page_of(const CacheAttn &a, const Tile &t, int key) {
+    const int near = min(max(key, t.any.lo), t.any.hi - 1);
+    return a.table[(size_t)t.r * a.max_pages + (near >> a.cache.page_shift)];
+}
+__device__ __forceinline__ int slot_of(const CacheAttn &a, const Tile &t, int key, int page) {
+    const int pages = a.cache.slots >> a.cache.page_shift;
+    if (key < t.any.lo || key >= t.any.hi || (unsigned)page >= (unsigned)pages) page = pages;
     return (page << a.cache.page_shift) + (key & ((1 << a.cache.page_shift) - 1));
 }
 
@@ -438,31 +442,42 @@ __device__ __forceinline__ int v_swizzle(int row) {
 
 __device__ __forceinline__ float half_value(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
 
+// Loads that pass by the caches, where nothing is read twice.
+template <bool NT, class T>
+__device__ __forceinline__ T ld(const T *p) {
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 // Eight dims of a cache row as it is stored, and as parts.
 template <int KIND>
 struct Octet;
 template <>
 struct Octet<kCacheF32> {
     f32x4 a, b;
+    template <bool NT>
     __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
         const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + row * width + d);
-        a = p[0];
-        b = p[1];
+        a = ld<NT>(p);
+        b = ld<NT>(p + 1);
     }
     __device__ __forceinline__ void parts(bf16x8 (&p)[3]) const { split3(a, b, p); }
 };
 template <>
 struct Octet<kCacheBf16> {
     bf16x8 x;
+    template <bool NT>
     __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
-        x = *reinterpret_cast<const bf16x8 *>(static_cast<const __bf16 *>(base) + row * width + d);
+        x = ld<NT>(reinterpret_cast<const bf16x8 *>(static_cast<const __bf16 *>(base) + row * width + d));
     }
 };
 template <>
 struct Octet<kCacheQ8> {
-    uint2 x;
+    u32x2 x;
+    template <bool NT>
     __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
-        x = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(base) + row * width + d);
+        x = ld<NT>(reinterpret_cast<const u32x2 *>(static_cast<const int8_t *>(base) + row * width + d));
     }
     __device__ __forceinline__ void values(f32x4 &a, f32x4 &b) const {
 #pragma unroll
@@ -524,7 +539,7 @@ constexpr int kPartsOfV = KIND == kCacheBf16 ? 1 : 3;
 template <int KIND, int D, int QT>
 __device__ void add_not_finite(const CacheAttn &a, const Tile &t, int g, Queries<D, QT> &w, int key, int lh) {
     for (int i = 0; i < 32; i++) {
-        const int slot = slot_of(a, t, key + i);
+        const int slot = slot_of(a, t, key + i, page_of(a, t, key + i));
         if (slot >= a.cache.slots) continue;
         const size_t row = cache_row(a.cache, slot, g);
 #pragma unroll
@@ -644,14 +659,14 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
         w.load(a, t, g, 0, li, lh);
         Octet<KIND> kr[2][C], vr[PASSES];
         uint16_t kd[C] = {}, vd[PASSES] = {};
-        // Of key `lane & 31` of a step, looked up two steps ahead.
-        auto look_up = [&](int i) { return slot_of(a, t, (step0 + i) * STEP + 32 * wave + (lane & 31)); };
+        // Of key `lane & 31` of a step.
+        auto key_of = [&](int i) { return (step0 + i) * STEP + 32 * wave + (lane & 31); };
         auto load_k = [&](int slot) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const size_t row = cache_row(a.cache, __shfl(slot, 16 * j + li, 64), g);
 #pragma unroll
-                for (int c = 0; c < C; c++) kr[j][c].load(a.cache.k, row, D, 32 * c + 8 * lh);
+                for (int c = 0; c < C; c++) kr[j][c].template load<true>(a.cache.k, row, D, 32 * c + 8 * lh);
             }
             if constexpr (KIND == kCacheQ8) {
                 const size_t row = cache_row(a.cache, slot, g);
@@ -663,14 +678,15 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
                 const size_t row = cache_row(a.cache, __shfl(slot, i * RPP + lane / LPR, 64), g);
-                vr[i].load(a.cache.v, row, D, 8 * (lane % LPR));
+                vr[i].template load<true>(a.cache.v, row, D, 8 * (lane % LPR));
                 if constexpr (KIND == kCacheQ8) vd[i] = a.cache.vd[row * C + (lane % LPR) / 4];
             }
         };
-        int slot = 0, next = 0;
+        int slot = 0, next_page = 0;
         if (steps) {
-            slot = look_up(0);
-            next = look_up(1);
+            const int page = page_of(a, t, key_of(0));
+            next_page = page_of(a, t, key_of(1));
+            slot = slot_of(a, t, key_of(0), page);
             load_k(slot);
             load_v(slot);
         }
@@ -678,7 +694,8 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
             const int key = (step0 + i) * STEP + 32 * wave;
             const uint32_t present = (uint32_t)__ballot(slot < a.cache.slots);
             const bool partial = key < t.all.lo || key + 32 > t.all.hi || present != 0xffffffffu;
-            const int after = look_up(i + 2);
+            const int next = slot_of(a, t, key_of(i + 1), next_page);
+            next_page = page_of(a, t, key_of(i + 2));
             if (KIND == kCacheQ8 && lane < 32) {
 #pragma unroll
                 for (int c = 0; c < C; c++) k_scale[32 * c + lane] = half_value(kd[c]);
@@ -738,7 +755,6 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
             }
             load_v(next);
             slot = next;
-            next = after;
             wave_fence();
             const int vrow = 4 * lh + (li >> 2);
             w.template add<NPV>(mine + vrow * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow), (li & 3) >> 1, p);
@@ -817,18 +833,18 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
         w.load(a, t, g, first, li, lh);
         Octet<KIND> kr[PASSES], vr[PASSES];
         uint16_t kd[PASSES] = {}, vd[PASSES] = {};
-        int slot[PASSES], next[PASSES];
+        int slot[PASSES], page[PASSES];
         auto look_up = [&](int step) {
 #pragma unroll
-            for (int i = 0; i < PASSES; i++) next[i] = slot_of(a, t, step * STEP + i * RPP + srow);
+            for (int i = 0; i < PASSES; i++) page[i] = page_of(a, t, step * STEP + i * RPP + srow);
         };
-        auto load = [&] {
+        auto load = [&](int step) {
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
-                slot[i] = next[i];
+                slot[i] = slot_of(a, t, step * STEP + i * RPP + srow, page[i]);
                 const size_t row = cache_row(a.cache, slot[i], g);
-                kr[i].load(a.cache.k, row, D, 8 * sg);
-                vr[i].load(a.cache.v, row, D, 8 * sg);
+                kr[i].template load<false>(a.cache.k, row, D, 8 * sg);
+                vr[i].template load<false>(a.cache.v, row, D, 8 * sg);
                 if constexpr (KIND == kCacheQ8) {
                     kd[i] = a.cache.kd[row * C + sg / 4];
                     vd[i] = a.cache.vd[row * C + sg / 4];
@@ -837,7 +853,7 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
         };
         if (steps) {
             look_up(step0);
-            load();
+            load(step0);
             look_up(step0 + 1);
         }
         if (tid < 4) flags[tid] = 0;
@@ -876,7 +892,7 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
             if (absent) flags[i & 1] = 1;
             if (dropped) flags[2 + (i & 1)] = 1;
             if (i + 1 < steps) {
-                load();
+                load(step0 + i + 1);
                 look_up(step0 + i + 2);
             }
             __syncthreads();
@@ -1059,7 +1075,7 @@ size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t wi
 }
 
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a) {
-    a.shares = kShares;
+    a.shares = getenv("SH") ? atoi(getenv("SH")) : kShares;
     a.min_share = 1;
     const bool few = few_rows((size_t)a.tokens * a.group, (size_t)a.requests);
     const bool wide = a.cache.width == 128;
