@@ -21,14 +21,15 @@
 //
 // Two kernels, by the rows of a request (launch_cache_attn):
 //   few rows:  16 query rows a workgroup, whose four waves take 32 keys each of a
-//     step of 128, on their own: K from global memory straight to the fragments of
-//     S^T = K . Q^T, V through LDS of the wave's own, no barrier in the loop;
+//     step of 128, on their own: K and then V through LDS of the
+//     wave's own, no barrier in the loop;
 //   many rows: 128 query rows, 32 a wave, which share panels of K and V in LDS.
 // Either way a lane holds its own query's scores, keys 16 t + 4 lh + r of tile t,
 // which is the B operand of O^T += V^T . P^T if the 32 keys of a product are taken in
 // the order (4 lh .. 4 lh + 3 of tile 0, then of tile 1); V^T comes from row-major
 // planes by transposing LDS reads of the same rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
@@ -39,6 +40,8 @@ namespace {
 constexpr float kMaxSlack = 8.0f;  // scores may pass the running maximum by this (base 2)
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // v_mfma_f32_16x16x32_bf16.  Lane l supplies A row l % 16 and B column l % 16 at
 // k = 8 * (l / 16) .. + 7; D[4 * (l / 16) + r][l % 16] lands in register r.
@@ -68,7 +71,6 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t &p0, uint32_t 
     p2 = round_halves(ra - __uint_as_float(p1 << 16), rb - __uint_as_float(p1 & 0xffff0000u));
 }
 __device__ __forceinline__ void split3(f32x4 a, f32x4 b, bf16x8 (&p)[3]) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     u32x4 u[3];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -84,6 +86,14 @@ __device__ __forceinline__ void split3(f32x4 a, f32x4 b, bf16x8 (&p)[3]) {
     }
 #pragma unroll
     for (int i = 0; i < 3; i++) p[i] = __builtin_bit_cast(bf16x8, u[i]);
+}
+
+__device__ __forceinline__ void split3(f32x4 a, bf16x4 (&p)[3]) {
+    uint32_t u[3][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) split3(a[2 * i], a[2 * i + 1], u[0][i], u[1][i], u[2][i]);
+#pragma unroll
+    for (int i = 0; i < 3; i++) p[i] = __builtin_bit_cast(bf16x4, u32x2{u[i][0], u[i][1]});
 }
 
 // max / sum with the lanes 16 and 32 away, on the VALU: a permlane swap of two
@@ -388,28 +398,29 @@ struct Queries {
         }
     }
 
-    // The weights of 32 keys as parts, and their sums.
-    __device__ __forceinline__ void weights(const f32x4 (&s)[2][QT], float scale, bf16x8 (&p)[QT][3]) {
+    // The scores of 32 keys become their weights, which are summed.
+    __device__ __forceinline__ void weights(f32x4 (&s)[2][QT], float scale) {
 #pragma unroll
         for (int u = 0; u < QT; u++) {
             const float off = m[u] == -INFINITY ? 0.0f : -m[u];
-            f32x4 e[2];
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) e[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][u][r], scale, off));
-            l[u] += ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
-            split3(e[0], e[1], p[u]);
+                for (int r = 0; r < 4; r++)
+                    s[t][u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][u][r], scale, off));
+            l[u] += ((s[0][u][0] + s[0][u][1]) + (s[0][u][2] + s[0][u][3])) +
+                    ((s[1][u][0] + s[1][u][1]) + (s[1][u][2] + s[1][u][3]));
         }
     }
 
-    // O^T += V^T . P^T for 32 keys; v: this lane's address in the first plane.
-    template <int NP>
+    // O^T += V^T . P^T for 32 keys, of dims 16 d0 .. 16 (d0 + n) - 1; v: this lane's
+    // address in the first plane.
+    template <int NP, int D0, int N>
     __device__ __forceinline__ void add(const char *v, int plane, int vx, int vg, const bf16x8 (&p)[QT][3]) {
         // Two tiles of dims at a time, the small products first: 2 QT sums that do
         // not wait for each other.
 #pragma unroll
-        for (int d0 = 0; d0 < DF; d0 += 2) {
+        for (int d0 = D0; d0 < D0 + N; d0 += 2) {
             bf16x8 f[2][NP];
 #pragma unroll
             for (int k = 0; k < 2; k++)
@@ -433,8 +444,13 @@ struct Queries {
     }
 };
 
-// Swizzle of V's planes: pairs of 16-byte granules by the row, so that the 16
-// rows x 32 bytes of a transposing read spread over the banks.
+// Swizzles of the planes in LDS ([key][D] bf16, in granules of 16 bytes).  K: a
+// fragment read takes one granule of 16 rows.  V: a transposing read takes a pair of
+// granules of 16 rows.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+    return D == 64 ? (row >> 1) & 7 : row & 15;
+}
 template <int D>
 __device__ __forceinline__ int v_swizzle(int row) {
     return D == 64 ? (row & 6) : 2 * (row & 7);
@@ -448,62 +464,79 @@ __device__ __forceinline__ T ld(const T *p) {
     if constexpr (NT) return __builtin_nontemporal_load(p);
     else return *p;
 }
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// Eight dims of a cache row as it is stored, and as parts.
-template <int KIND>
+// Eight dims of a cache row as it is stored, of lane sg of the D / 8 that share the
+// row, and their way to the planes.  Every load covers whole lines, so that none is
+// asked for twice.
+template <int KIND, int D>
 struct Octet;
-template <>
-struct Octet<kCacheF32> {
-    f32x4 a, b;
+template <int D>
+struct Octet<kCacheF32, D> {
+    f32x4 a, b;  // dims 4 sg .. + 3, and D / 2 further
     template <bool NT>
-    __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + row * width + d);
-        a = ld<NT>(p);
-        b = ld<NT>(p + 1);
+    __device__ __forceinline__ void load(const void *base, size_t row, int sg) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + row * D);
+        a = ld<NT>(p + sg);
+        b = ld<NT>(p + D / 8 + sg);
     }
-    __device__ __forceinline__ void parts(bf16x8 (&p)[3]) const { split3(a, b, p); }
+    // To the row at `at` of the first plane.
+    template <bool SCALED>
+    __device__ __forceinline__ void stage(char *at, int plane, int sg, int swizzle, float) const {
+        bf16x4 p[3];
+        char *x = at + (((sg >> 1) ^ swizzle) << 4) + (sg & 1) * 8;
+        split3(a, p);
+#pragma unroll
+        for (int i = 0; i < 3; i++) *reinterpret_cast<bf16x4 *>(x + i * plane) = p[i];
+        x = at + (((D / 16 + (sg >> 1)) ^ swizzle) << 4) + (sg & 1) * 8;
+        split3(b, p);
+#pragma unroll
+        for (int i = 0; i < 3; i++) *reinterpret_cast<bf16x4 *>(x + i * plane) = p[i];
+    }
 };
-template <>
-struct Octet<kCacheBf16> {
-    bf16x8 x;
+template <int D>
+struct Octet<kCacheBf16, D> {
+    bf16x8 x;  // dims 8 sg .. + 7
     template <bool NT>
-    __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
-        x = ld<NT>(reinterpret_cast<const bf16x8 *>(static_cast<const __bf16 *>(base) + row * width + d));
+    __device__ __forceinline__ void load(const void *base, size_t row, int sg) {
+        x = ld<NT>(reinterpret_cast<const bf16x8 *>(static_cast<const __bf16 *>(base) + row * D) + sg);
+    }
+    template <bool SCALED>
+    __device__ __forceinline__ void stage(char *at, int, int sg, int swizzle, float) const {
+        *reinterpret_cast<bf16x8 *>(at + ((sg ^ swizzle) << 4)) = x;
     }
 };
-template <>
-struct Octet<kCacheQ8> {
-    u32x2 x;
+template <int D>
+struct Octet<kCacheQ8, D> {
+    u32x2 x;  // dims 8 sg .. + 7
     template <bool NT>
-    __device__ __forceinline__ void load(const void *base, size_t row, int width, int d) {
-        x = ld<NT>(reinterpret_cast<const u32x2 *>(static_cast<const int8_t *>(base) + row * width + d));
+    __device__ __forceinline__ void load(const void *base, size_t row, int sg) {
+        x = ld<NT>(reinterpret_cast<const u32x2 *>(static_cast<const int8_t *>(base) + row * D) + sg);
     }
-    __device__ __forceinline__ void values(f32x4 &a, f32x4 &b) const {
+    // As integers, or times the scale d (18 bits: three parts).
+    template <bool SCALED>
+    __device__ __forceinline__ void stage(char *at, int plane, int sg, int swizzle, float d) const {
+        f32x4 a, b;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            a[e] = (float)(int8_t)(x.x >> (8 * e));
-            b[e] = (float)(int8_t)(x.y >> (8 * e));
+            a[e] = (float)(int8_t)(x[0] >> (8 * e));
+            b[e] = (float)(int8_t)(x[1] >> (8 * e));
         }
-    }
-    // The integers as bf16.
-    __device__ __forceinline__ bf16x8 integers() const {
-        f32x4 a, b;
-        values(a, b);
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        return __builtin_bit_cast(bf16x8, u32x4{high_halves(a[0], a[1]), high_halves(a[2], a[3]),
-                                                high_halves(b[0], b[1]), high_halves(b[2], b[3])});
-    }
-    // (A value is not finite where its block's scale is not.)
-    __device__ __forceinline__ void parts(float d, bf16x8 (&p)[3]) const {
-        f32x4 a, b;
-        values(a, b);
-        split3(a * d, b * d, p);
+        at += (sg ^ swizzle) << 4;
+        if constexpr (SCALED) {
+            bf16x8 p[3];
+            split3(a * d, b * d, p);
+#pragma unroll
+            for (int i = 0; i < 3; i++) *reinterpret_cast<bf16x8 *>(at + i * plane) = p[i];
+        } else {
+            *reinterpret_cast<u32x4 *>(at) = u32x4{high_halves(a[0], a[1]), high_halves(a[2], a[3]),
+                                                   high_halves(b[0], b[1]), high_halves(b[2], b[3])};
+        }
     }
 };
 
 // Values that are not finite become zeros; whether there were any.
-__device__ __forceinline__ bool drop(Octet<kCacheF32> &x, uint16_t) {
+template <int D>
+__device__ __forceinline__ bool drop(Octet<kCacheF32, D> &x, uint16_t) {
     if (finite8(x.a, x.b)) return false;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -512,7 +545,8 @@ __device__ __forceinline__ bool drop(Octet<kCacheF32> &x, uint16_t) {
     }
     return true;
 }
-__device__ __forceinline__ bool drop(Octet<kCacheBf16> &x, uint16_t) {
+template <int D>
+__device__ __forceinline__ bool drop(Octet<kCacheBf16, D> &x, uint16_t) {
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 8; e++)
@@ -522,7 +556,9 @@ __device__ __forceinline__ bool drop(Octet<kCacheBf16> &x, uint16_t) {
         }
     return bad;
 }
-__device__ __forceinline__ bool drop(Octet<kCacheQ8> &, uint16_t &d) {
+// (Of a block whose scale is not.)
+template <int D>
+__device__ __forceinline__ bool drop(Octet<kCacheQ8, D> &, uint16_t &d) {
     if ((d & 0x7c00) != 0x7c00) return false;
     d = 0;
     return true;
@@ -633,10 +669,20 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, F f) {
 
 // ---- few rows -------------------------------------------------------------------
 
+// A wave holds the rows of K or of V of one step in flight, never both: 64 KB to a CU
+// at a row of 256 bytes.  Twice that lowers what the memory delivers (reading
+// scattered pages of 16 KB and nothing else: 64 KB in flight a CU 6.8 TB/s, 128 KB
+// 6.3, 256 KB 5.4), and the registers are the same for both.  A Q8_0 value stays the
+// integer it is; its scale joins its weight, once for each block of 32 dims (few
+// weights, where the values of a step are many).
+
+template <int KIND>
+constexpr int kFewParts = KIND == kCacheF32 ? 3 : 1;
 template <int KIND, int D>
 constexpr int few_wave_bytes() {
-    // V's planes of 32 keys and K's scales, or the wave's O at the end.
-    constexpr int panel = kPartsOfV<KIND> * 32 * D * 2 + (KIND == kCacheQ8 ? 32 * (D / 32) * 4 : 0);
+    // The planes of 32 keys, K's and then V's, and the scales of both, or the wave's O
+    // at the end.
+    constexpr int panel = kFewParts<KIND> * 32 * D * 2 + (KIND == kCacheQ8 ? 2 * 32 * (D / 32) * 4 : 0);
     constexpr int o = 16 * D * 4 + 128;
     return panel > o ? panel : o;
 }
@@ -644,120 +690,135 @@ constexpr int few_wave_bytes() {
 template <int KIND, int D>
 __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
     constexpr int BM = 16, STEP = 128, C = D / 32, WAVE = few_wave_bytes<KIND, D>();
-    constexpr int NPK = kPartsOfK<KIND>, NPV = kPartsOfV<KIND>, PLANE = 32 * D * 2;
-    constexpr int LPR = D / 8, RPP = 64 / LPR, PASSES = 32 / RPP;  // V: lanes a row, rows a pass
+    constexpr int NP = kFewParts<KIND>, PLANE = 32 * D * 2;
+    constexpr int LPR = D / 8, RPP = 64 / LPR, PASSES = 32 / RPP;  // lanes a row, rows a pass
     extern __shared__ __attribute__((aligned(16))) char smem[];
     int *first_tile = reinterpret_cast<int *>(smem + 4 * WAVE);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lh = lane >> 4;
     char *mine = smem + wave * WAVE;
-    float *k_scale = reinterpret_cast<float *>(mine + NPV * PLANE);  // [C][32]
+    float *scales = reinterpret_cast<float *>(mine + NP * PLANE);  // [k, v][C][32]
+    const int srow = lane / LPR, sg = lane % LPR;  // row of a pass and granule that this lane moves
 
     walk<BM, STEP, 256>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
         Queries<D, 1> w;
         w.load(a, t, g, 0, li, lh);
-        Octet<KIND> kr[2][C], vr[PASSES];
-        uint16_t kd[C] = {}, vd[PASSES] = {};
-        // Of key `lane & 31` of a step.
-        auto key_of = [&](int i) { return (step0 + i) * STEP + 32 * wave + (lane & 31); };
-        auto load_k = [&](int slot) {
+        Octet<KIND, D> x[PASSES];
+        uint16_t d[C] = {};  // scales of key `lane & 31`
+        auto load = [&](const void *base, const uint16_t *scale, int slot) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const size_t row = cache_row(a.cache, __shfl(slot, 16 * j + li, 64), g);
-#pragma unroll
-                for (int c = 0; c < C; c++) kr[j][c].template load<true>(a.cache.k, row, D, 32 * c + 8 * lh);
-            }
+            for (int i = 0; i < PASSES; i++)
+                x[i].template load<true>(base, cache_row(a.cache, __shfl(slot, i * RPP + srow, 64), g), sg);
             if constexpr (KIND == kCacheQ8) {
                 const size_t row = cache_row(a.cache, slot, g);
 #pragma unroll
-                for (int c = 0; c < C; c++) kd[c] = a.cache.kd[row * C + c];
+                for (int c = 0; c < C; c++) d[c] = scale[row * C + c];
             }
         };
-        auto load_v = [&](int slot) {
-#pragma unroll
-            for (int i = 0; i < PASSES; i++) {
-                const size_t row = cache_row(a.cache, __shfl(slot, i * RPP + lane / LPR, 64), g);
-                vr[i].template load<true>(a.cache.v, row, D, 8 * (lane % LPR));
-                if constexpr (KIND == kCacheQ8) vd[i] = a.cache.vd[row * C + (lane % LPR) / 4];
-            }
-        };
+        // Of key `lane & 31` of a step.
+        auto key_of = [&](int i) { return (step0 + i) * STEP + 32 * wave + (lane & 31); };
         int slot = 0, next_page = 0;
         if (steps) {
             const int page = page_of(a, t, key_of(0));
             next_page = page_of(a, t, key_of(1));
             slot = slot_of(a, t, key_of(0), page);
-            load_k(slot);
-            load_v(slot);
+            load(a.cache.k, a.cache.kd, slot);
         }
         for (int i = 0; i < steps; i++) {
             const int key = (step0 + i) * STEP + 32 * wave;
             const uint32_t present = (uint32_t)__ballot(slot < a.cache.slots);
             const bool partial = key < t.all.lo || key + 32 > t.all.hi || present != 0xffffffffu;
+            auto put_scales = [&](float *to) {
+                if (KIND == kCacheQ8 && lane < 32) {
+#pragma unroll
+                    for (int c = 0; c < C; c++) to[32 * c + lane] = half_value(d[c]);
+                }
+            };
+            put_scales(scales);
+#pragma unroll
+            for (int j = 0; j < PASSES; j++) {
+                const int row = j * RPP + srow;
+                x[j].template stage<false>(mine + row * (D * 2), PLANE, sg, k_swizzle<D>(row), 0.0f);
+            }
+            load(a.cache.v, a.cache.vd, slot);
             const int next = slot_of(a, t, key_of(i + 1), next_page);
             next_page = page_of(a, t, key_of(i + 2));
-            if (KIND == kCacheQ8 && lane < 32) {
-#pragma unroll
-                for (int c = 0; c < C; c++) k_scale[32 * c + lane] = half_value(kd[c]);
-            }
+            wave_fence();
             f32x4 sx[1][2][1];
             f32x4(&s)[2][1] = sx[0];
             s[0][0] = s[1][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (KIND == kCacheQ8) wave_fence();
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                bf16x8 f[2][NPK];
-                f32x4 x[2];
+                bf16x8 f[2][NP];
+                f32x4 y[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    if constexpr (KIND == kCacheF32) kr[j][c].parts(f[j]);
-                    else if constexpr (KIND == kCacheBf16) f[j][0] = kr[j][c].x;
-                    else f[j][0] = kr[j][c].integers();
-                    x[j] = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[j][0];
+                    const int row = 16 * j + li;
+#pragma unroll
+                    for (int e = 0; e < NP; e++)
+                        f[j][e] = *reinterpret_cast<const bf16x8 *>(mine + e * PLANE + row * (D * 2) +
+                                                                    (((4 * c + lh) ^ k_swizzle<D>(row)) << 4));
+                    y[j] = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[j][0];
                 }
 #pragma unroll
                 for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
-                    for (int e = NPK - 1; e >= 0; e--)
+                    for (int e = NP - 1; e >= 0; e--)
                         if (sum - e >= 0)
 #pragma unroll
-                            for (int j = 0; j < 2; j++) x[j] = mfma16x16x32_bf16(f[j][e], w.q[0][c][sum - e], x[j]);
+                            for (int j = 0; j < 2; j++) y[j] = mfma16x16x32_bf16(f[j][e], w.q[0][c][sum - e], y[j]);
 #pragma unroll
                 for (int j = 0; j < 2; j++)
                     if constexpr (KIND == kCacheQ8) {
-                        const f32x4 d = *reinterpret_cast<const f32x4 *>(k_scale + 32 * c + 16 * j + 4 * lh);
+                        const f32x4 z = *reinterpret_cast<const f32x4 *>(scales + 32 * c + 16 * j + 4 * lh);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) s[j][0][r] = __builtin_fmaf(d[r], x[j][r], s[j][0][r]);
+                        for (int r = 0; r < 4; r++) s[j][0][r] = __builtin_fmaf(z[r], y[j][r], s[j][0][r]);
                     } else {
-                        s[j][0] = x[j];
+                        s[j][0] = y[j];
                     }
             }
-            load_k(next);
+            wave_fence();
             if (partial) w.mask(s, key, present, lh);
-            bf16x8 p[1][3];
             w.raise(sx, a.scale_log2);
-            w.weights(s, a.scale_log2, p);
+            w.weights(s, a.scale_log2);
             bool dropped = false;
+            if (KIND == kCacheQ8 && partial) {
+#pragma unroll
+                for (int c = 0; c < C; c++) dropped |= drop(x[0], d[c]);
+            }
+            put_scales(scales + 32 * C);
 #pragma unroll
             for (int j = 0; j < PASSES; j++) {
-                if (partial) dropped |= drop(vr[j], vd[j]);
-                const int row = j * RPP + lane / LPR;
-                char *at = mine + row * (D * 2) + (((lane % LPR) ^ v_swizzle<D>(row)) << 4);
-                if constexpr (KIND == kCacheBf16) {
-                    *reinterpret_cast<bf16x8 *>(at) = vr[j].x;
-                } else {
-                    bf16x8 f[3];
-                    if constexpr (KIND == kCacheF32) vr[j].parts(f);
-                    else vr[j].parts(half_value(vd[j]), f);
-#pragma unroll
-                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(at + e * PLANE) = f[e];
-                }
+                uint16_t none = 0;
+                if (KIND != kCacheQ8 && partial) dropped |= drop(x[j], none);
+                const int row = j * RPP + srow;
+                x[j].template stage<false>(mine + row * (D * 2), PLANE, sg, v_swizzle<D>(row), 0.0f);
             }
-            load_v(next);
             slot = next;
+            load(a.cache.k, a.cache.kd, slot);
             wave_fence();
             const int vrow = 4 * lh + (li >> 2);
-            w.template add<NPV>(mine + vrow * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow), (li & 3) >> 1, p);
+            const char *v = mine + vrow * (D * 2) + (li & 1) * 8;
+            const int vx = v_swizzle<D>(vrow), vg = (li & 3) >> 1;
+            bf16x8 p[1][3];
+            if constexpr (KIND == kCacheQ8) {
+                auto block = [&](auto cc) {
+                    constexpr int c = decltype(cc)::value;
+                    const f32x4 *z = reinterpret_cast<const f32x4 *>(scales + 32 * (C + c) + 4 * lh);
+                    split3(s[0][0] * z[0], s[1][0] * z[4], p[0]);
+                    w.template add<1, 2 * c, 2>(v, PLANE, vx, vg, p);
+                };
+                block(std::integral_constant<int, 0>{});
+                block(std::integral_constant<int, 1>{});
+                if constexpr (C == 4) {
+                    block(std::integral_constant<int, 2>{});
+                    block(std::integral_constant<int, 3>{});
+                }
+            } else {
+                split3(s[0][0], s[1][0], p[0]);
+                w.template add<NP, 0, D / 16>(v, PLANE, vx, vg, p);
+            }
             wave_fence();
             if (__any(dropped)) add_not_finite<KIND>(a, t, g, w, key, lh);
         }
@@ -824,14 +885,13 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lh = lane >> 4;
     const int srow = tid / LPR, sg = tid % LPR;  // staged row of a pass, and granule
-    auto k_swizzle = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
 
     walk<BM, STEP, THREADS>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
         const int first = 16 * QT * wave;
         const bool works = first < t.rows;
         Queries<D, QT> w;
         w.load(a, t, g, first, li, lh);
-        Octet<KIND> kr[PASSES], vr[PASSES];
+        Octet<KIND, D> kr[PASSES], vr[PASSES];
         uint16_t kd[PASSES] = {}, vd[PASSES] = {};
         int slot[PASSES], page[PASSES];
         auto look_up = [&](int step) {
@@ -843,8 +903,8 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
             for (int i = 0; i < PASSES; i++) {
                 slot[i] = slot_of(a, t, step * STEP + i * RPP + srow, page[i]);
                 const size_t row = cache_row(a.cache, slot[i], g);
-                kr[i].template load<false>(a.cache.k, row, D, 8 * sg);
-                vr[i].template load<false>(a.cache.v, row, D, 8 * sg);
+                kr[i].template load<false>(a.cache.k, row, sg);
+                vr[i].template load<false>(a.cache.v, row, sg);
                 if constexpr (KIND == kCacheQ8) {
                     kd[i] = a.cache.kd[row * C + sg / 4];
                     vd[i] = a.cache.vd[row * C + sg / 4];
@@ -867,27 +927,10 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
                 const int row = j * RPP + srow;
                 absent |= slot[j] >= a.cache.slots;
                 if (sg == 0) there[(i & 1) * STEP + row] = slot[j] < a.cache.slots;
-                char *kat = kp + row * (D * 2) + ((sg ^ k_swizzle(row)) << 4);
-                char *vat = vp + row * (D * 2) + ((sg ^ v_swizzle<D>(row)) << 4);
                 if (edge) dropped |= drop(vr[j], vd[j]);
-                bf16x8 f[3];
-                if constexpr (KIND == kCacheF32) {
-                    kr[j].parts(f);
-#pragma unroll
-                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(kat + e * PLANE) = f[e];
-                    vr[j].parts(f);
-#pragma unroll
-                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(vat + e * PLANE) = f[e];
-                } else if constexpr (KIND == kCacheBf16) {
-                    *reinterpret_cast<bf16x8 *>(kat) = kr[j].x;
-                    *reinterpret_cast<bf16x8 *>(vat) = vr[j].x;
-                } else {
-                    *reinterpret_cast<bf16x8 *>(kat) = kr[j].integers();
-                    if (sg % 4 == 0) k_scale[(sg / 4) * STEP + row] = half_value(kd[j]);
-                    vr[j].parts(half_value(vd[j]), f);
-#pragma unroll
-                    for (int e = 0; e < 3; e++) *reinterpret_cast<bf16x8 *>(vat + e * PLANE) = f[e];
-                }
+                kr[j].template stage<false>(kp + row * (D * 2), PLANE, sg, k_swizzle<D>(row), 0.0f);
+                if (KIND == kCacheQ8 && sg % 4 == 0) k_scale[(sg / 4) * STEP + row] = half_value(kd[j]);
+                vr[j].template stage<true>(vp + row * (D * 2), PLANE, sg, v_swizzle<D>(row), half_value(vd[j]));
             }
             if (absent) flags[i & 1] = 1;
             if (dropped) flags[2 + (i & 1)] = 1;
@@ -918,7 +961,7 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
 #pragma unroll
                         for (int e = 0; e < NPK; e++)
                             f[j][e] = *reinterpret_cast<const bf16x8 *>(kp + e * PLANE + row * (D * 2) +
-                                                                        (((4 * c + lh) ^ k_swizzle(row)) << 4));
+                                                                        (((4 * c + lh) ^ k_swizzle<D>(row)) << 4));
 #pragma unroll
                         for (int u = 0; u < QT; u++)
                             x[j][u] = KIND == kCacheQ8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[h][j][u];
@@ -960,8 +1003,10 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
 #pragma unroll
             for (int h = 0; h < H; h++) {
                 bf16x8 p[QT][3];
-                w.weights(s[h], a.scale_log2, p);
-                w.template add<NPV>(vp + (32 * h + vrow) * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow),
+                w.weights(s[h], a.scale_log2);
+#pragma unroll
+                for (int u = 0; u < QT; u++) split3(s[h][0][u], s[h][1][u], p[u]);
+                w.template add<NPV, 0, D / 16>(vp + (32 * h + vrow) * (D * 2) + (li & 1) * 8, PLANE, v_swizzle<D>(vrow),
                                     (li & 3) >> 1, p);
             }
             if (fix)
@@ -1075,7 +1120,7 @@ size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t wi
 }
 
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a) {
-    a.shares = getenv("SH") ? atoi(getenv("SH")) : kShares;
+    a.shares = kShares;
     a.min_share = 1;
     const bool few = few_rows((size_t)a.tokens * a.group, (size_t)a.requests);
     const bool wide = a.cache.width == 128;
