@@ -296,16 +296,16 @@ __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, co
 }
 
 // The page of a key of a tile that sees some (of the nearest such key: no branch),
-// and the key's slot, one of the page of zeros behind the last where it is not
+// and the key's slot, in the page of zeros behind the last where its page is not
 // there.  Apart, so that a loop can load the page a step before it looks at it:
 // looking waits for every load issued before.
 __device__ __forceinline__ int page_of(const CacheAttn &a, const Tile &t, int key) {
     const int near = min(max(key, t.any.lo), t.any.hi - 1);
     return a.table[(size_t)t.r * a.max_pages + (near >> a.cache.page_shift)];
 }
-__device__ __forceinline__ int slot_of(const CacheAttn &a, const Tile &t, int key, int page) {
+__device__ __forceinline__ int slot_of(const CacheAttn &a, int key, int page) {
     const int pages = a.cache.slots >> a.cache.page_shift;
-    if (key < t.any.lo || key >= t.any.hi || (unsigned)page >= (unsigned)pages) page = pages;
+    if ((unsigned)page >= (unsigned)pages) page = pages;
     return (page << a.cache.page_shift) + (key & ((1 << a.cache.page_shift) - 1));
 }
 
@@ -467,17 +467,19 @@ __device__ __forceinline__ T ld(const T *p) {
 
 // Eight dims of a cache row as it is stored, of lane sg of the D / 8 that share the
 // row, and their way to the planes.  Every load covers whole lines, so that none is
-// asked for twice.
+// asked for twice.  A load is at a base, wherever it can one that the wave shares (its
+// rows in one page), plus 32 bits of a lane's own: the 64-bit products of a row's
+// address are scalar then.
 template <int KIND, int D>
 struct Octet;
 template <int D>
 struct Octet<kCacheF32, D> {
     f32x4 a, b;  // dims 4 sg .. + 3, and D / 2 further
+    static constexpr int kRow = 4 * D, kLane = 16;  // bytes
     template <bool NT>
-    __device__ __forceinline__ void load(const void *base, size_t row, int sg) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + row * D);
-        a = ld<NT>(p + sg);
-        b = ld<NT>(p + D / 8 + sg);
+    __device__ __forceinline__ void load(const char *base, uint32_t at) {
+        a = ld<NT>(reinterpret_cast<const f32x4 *>(base + at));
+        b = ld<NT>(reinterpret_cast<const f32x4 *>(base + at + 2 * D));
     }
     // To the row at `at` of the first plane.
     template <bool SCALED>
@@ -496,9 +498,10 @@ struct Octet<kCacheF32, D> {
 template <int D>
 struct Octet<kCacheBf16, D> {
     bf16x8 x;  // dims 8 sg .. + 7
+    static constexpr int kRow = 2 * D, kLane = 16;
     template <bool NT>
-    __device__ __forceinline__ void load(const void *base, size_t row, int sg) {
-        x = ld<NT>(reinterpret_cast<const bf16x8 *>(static_cast<const __bf16 *>(base) + row * D) + sg);
+    __device__ __forceinline__ void load(const char *base, uint32_t at) {
+        x = ld<NT>(reinterpret_cast<const bf16x8 *>(base + at));
     }
     template <bool SCALED>
     __device__ __forceinline__ void stage(char *at, int, int sg, int swizzle, float) const {
@@ -508,9 +511,10 @@ struct Octet<kCacheBf16, D> {
 template <int D>
 struct Octet<kCacheQ8, D> {
     u32x2 x;  // dims 8 sg .. + 7
+    static constexpr int kRow = D, kLane = 8;
     template <bool NT>
-    __device__ __forceinline__ void load(const void *base, size_t row, int sg) {
-        x = ld<NT>(reinterpret_cast<const u32x2 *>(static_cast<const int8_t *>(base) + row * D) + sg);
+    __device__ __forceinline__ void load(const char *base, uint32_t at) {
+        x = ld<NT>(reinterpret_cast<const u32x2 *>(base + at));
     }
     // As integers, or times the scale d (18 bits: three parts).
     template <bool SCALED>
@@ -575,7 +579,7 @@ constexpr int kPartsOfV = KIND == kCacheBf16 ? 1 : 3;
 template <int KIND, int D, int QT>
 __device__ void add_not_finite(const CacheAttn &a, const Tile &t, int g, Queries<D, QT> &w, int key, int lh) {
     for (int i = 0; i < 32; i++) {
-        const int slot = slot_of(a, t, key + i, page_of(a, t, key + i));
+        const int slot = slot_of(a, key + i, page_of(a, t, key + i));
         if (slot >= a.cache.slots) continue;
         const size_t row = cache_row(a.cache, slot, g);
 #pragma unroll
@@ -707,9 +711,23 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
         Octet<KIND, D> x[PASSES];
         uint16_t d[C] = {};  // scales of key `lane & 31`
         auto load = [&](const void *base, const uint16_t *scale, int slot) {
+            using O = Octet<KIND, D>;
+            if (a.cache.page_shift >= 4) {  // the halves of a step are in one page each
 #pragma unroll
-            for (int i = 0; i < PASSES; i++)
-                x[i].template load<true>(base, cache_row(a.cache, __shfl(slot, i * RPP + srow, 64), g), sg);
+                for (int h = 0; h < 2; h++) {
+                    const char *rows = static_cast<const char *>(base) +
+                                       cache_row(a.cache, __builtin_amdgcn_readlane(slot, 16 * h), g) * O::kRow;
+#pragma unroll
+                    for (int i = 0; i < PASSES / 2; i++)
+                        x[h * (PASSES / 2) + i].template load<true>(rows, (i * RPP + srow) * O::kRow + sg * O::kLane);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PASSES; i++)
+                    x[i].template load<true>(static_cast<const char *>(base) +
+                                                 cache_row(a.cache, __shfl(slot, i * RPP + srow, 64), g) * O::kRow,
+                                             sg * O::kLane);
+            }
             if constexpr (KIND == kCacheQ8) {
                 const size_t row = cache_row(a.cache, slot, g);
 #pragma unroll
@@ -722,7 +740,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
         if (steps) {
             const int page = page_of(a, t, key_of(0));
             next_page = page_of(a, t, key_of(1));
-            slot = slot_of(a, t, key_of(0), page);
+            slot = slot_of(a, key_of(0), page);
             load(a.cache.k, a.cache.kd, slot);
         }
         for (int i = 0; i < steps; i++) {
@@ -742,7 +760,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
                 x[j].template stage<false>(mine + row * (D * 2), PLANE, sg, k_swizzle<D>(row), 0.0f);
             }
             load(a.cache.v, a.cache.vd, slot);
-            const int next = slot_of(a, t, key_of(i + 1), next_page);
+            const int next = slot_of(a, key_of(i + 1), next_page);
             next_page = page_of(a, t, key_of(i + 2));
             wave_fence();
             f32x4 sx[1][2][1];
@@ -899,15 +917,28 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
             for (int i = 0; i < PASSES; i++) page[i] = page_of(a, t, step * STEP + i * RPP + srow);
         };
         auto load = [&](int step) {
+            using O = Octet<KIND, D>;
+            const char *k = static_cast<const char *>(a.cache.k), *v = static_cast<const char *>(a.cache.v);
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
-                slot[i] = slot_of(a, t, step * STEP + i * RPP + srow, page[i]);
-                const size_t row = cache_row(a.cache, slot[i], g);
-                kr[i].template load<false>(a.cache.k, row, sg);
-                vr[i].template load<false>(a.cache.v, row, sg);
+                slot[i] = slot_of(a, step * STEP + i * RPP + srow, page[i]);
+                // A wave's rows of a pass (four or eight) are in one page, or each has its own.
+                size_t row;
+                uint32_t at = sg * O::kLane;
+                if (a.cache.page_shift >= 3) {
+                    row = cache_row(a.cache, uniform(slot[i]), g);
+                    at += (lane / LPR) * O::kRow;
+                    kr[i].template load<false>(k + row * O::kRow, at);
+                    vr[i].template load<false>(v + row * O::kRow, at);
+                } else {
+                    row = cache_row(a.cache, slot[i], g);
+                    kr[i].template load<false>(k + row * O::kRow, at);
+                    vr[i].template load<false>(v + row * O::kRow, at);
+                }
                 if constexpr (KIND == kCacheQ8) {
-                    kd[i] = a.cache.kd[row * C + sg / 4];
-                    vd[i] = a.cache.vd[row * C + sg / 4];
+                    row = cache_row(a.cache, slot[i], g) * C + sg / 4;
+                    kd[i] = a.cache.kd[row];
+                    vd[i] = a.cache.vd[row];
                 }
             }
         };
