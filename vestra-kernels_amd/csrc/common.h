@@ -126,6 +126,38 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// v of the lane that a DPP control names, zero where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long long dpp_or_zero(long long v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
+// Inclusive sum over the workgroup's threads, and the sum of all of them.  Within a
+// wave by DPP (row_shr 1, 2, 4, 8, then the last lane of a row to the next row and
+// of the lower half to the upper).
+template <int THREADS>
+__device__ __forceinline__ long long scan_all(long long v, long long *tmp, long long *all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v += dpp_or_zero<0x111, 0xf>(v);
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);
+    v += dpp_or_zero<0x143, 0xc>(v);
+    if (lane == 63) tmp[wave] = v;
+    __syncthreads();
+    long long before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+        if (w < wave) before += tmp[w];
+        sum += tmp[w];
+    }
+    __syncthreads();
+    *all = sum;
+    return v + before;
+}
+
 // LayerNorm of one row held by one wave in registers: r[j] = the float4
 // chunk lane + 64 j of the row (n4 = cols / 4 <= 256 chunks; absent chunks
 // are zero).  Mean, then the variance about the mean (two passes over the

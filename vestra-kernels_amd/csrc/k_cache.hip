@@ -12,11 +12,42 @@ namespace vh {
 namespace {
 
 constexpr int kU = 4;  // row groups that a wave has in flight
+constexpr size_t kStreamBytes = (size_t)64 << 20;
 
 // quantize_row_q8_0's value (src/q8_0_dot.rs:38-44): half away from zero, NaN to 0.
 __device__ __forceinline__ int q8_of(float v, float inv) {
     const float q = roundf(mul_rn(v, inv));
     return isnan(q) ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+// Sine and cosine of a number of turns, to floats.  Whole quarters go off exactly;
+// what is left, at most an eighth of a turn, is an angle below pi / 4, where the power
+// series to the 15th and 16th power are exact to 2^-54: the results are the
+// correctly rounded ones but where a value lies within that of the middle between two
+// floats.
+__device__ __forceinline__ void turn_sincos(double turns, float &sn, float &cs) {
+    const double r = turns - rint(turns), quarters = rint(4.0 * r);
+    const double x = (r - 0.25 * quarters) * 6.283185307179586476925286766559, z = x * x;
+    double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;  // 15!, 16!
+    s = __builtin_fma(s, z, 1.0 / 6227020800.0);
+    c = __builtin_fma(c, z, -1.0 / 87178291200.0);
+    s = __builtin_fma(s, z, -1.0 / 39916800.0);
+    c = __builtin_fma(c, z, 1.0 / 479001600.0);
+    s = __builtin_fma(s, z, 1.0 / 362880.0);
+    c = __builtin_fma(c, z, -1.0 / 3628800.0);
+    s = __builtin_fma(s, z, -1.0 / 5040.0);
+    c = __builtin_fma(c, z, 1.0 / 40320.0);
+    s = __builtin_fma(s, z, 1.0 / 120.0);
+    c = __builtin_fma(c, z, -1.0 / 720.0);
+    s = __builtin_fma(s, z, -1.0 / 6.0);
+    c = __builtin_fma(c, z, 1.0 / 24.0);
+    s = __builtin_fma(s * z, x, x);
+    c = __builtin_fma(c, z, -0.5);
+    c = __builtin_fma(c, z, 1.0);
+    const int q = (int)quarters & 3;
+    const float fs = (float)(q & 1 ? c : s), fc = (float)(q & 1 ? s : c);
+    sn = q & 2 ? -fs : fs;
+    cs = q == 1 || q == 2 ? -fc : fc;
 }
 
 // Rows of one token, head_dim floats each, of which Q and K are rotated on the
@@ -31,8 +62,12 @@ __device__ __forceinline__ int q8_of(float v, float inv) {
 // 10^6 leaves nothing of a 32-bit angle), as sine and cosine in LDS.
 //
 // x0' = x0 c - x1 s, x1' = x1 c + x0 s, products and sums rounded one by one, as
-// rope2d's.  KIND: what the cache holds, or -1 for rotation alone.
-template <int KIND>
+// rope2d's.  KIND: what the cache holds, or -1 for rotation alone.  NT: loads and
+// stores that pass by the caches, for calls beyond what those hold.
+//
+// A small call is a chain of latencies, so the first rows and slots are asked for
+// before the angles are formed.
+template <int KIND, bool NT>
 __global__ __launch_bounds__(256) void cache_rows_kernel(CacheRows a) {
     extern __shared__ __attribute__((aligned(16))) float angles[];  // [tokens][pairs][sin, cos]
     __shared__ __attribute__((aligned(16))) float exchange[4][kU][256];
@@ -41,89 +76,91 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(CacheRows a) {
     const int t0 = blockIdx.x * a.per_group;
     const int nt = min(a.per_group, a.tokens - t0);
     const RopePlan &rope = a.rope;
-    if (rope.pairs) {
-        for (int i = tid; i < nt * rope.pairs; i += 256) {
-            const int t = i / rope.pairs, p = i - t * rope.pairs;
-            const double turns = (double)a.positions[(size_t)(t0 + t) * rope.axes + rope.axis[p]] * rope.turns[p];
-            double sn, cs;
-            sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
-            angles[2 * i] = (float)sn;
-            angles[2 * i + 1] = (float)cs;
-        }
-        __syncthreads();
-    }
     const int lanes = a.head_dim >> 2;        // of a row
     const int rows = 64 / lanes;              // of a group
     const int sub = lane / lanes, c = lane - sub * lanes;
     const bool used = sub < rows;
+    const int total_rows = a.heads + 2 * a.kv_heads;
+    const int groups = (total_rows + rows - 1) / rows;
+    const int n = nt * groups;
+
+    f32x4 x[kU];
+    int slot[kU];
+    auto token_of = [&](int idx) { return min(idx, n - 1) / groups; };
+    auto row_of = [&](int idx) {
+        idx = min(idx, n - 1);
+        return (idx - idx / groups * groups) * rows + sub;
+    };
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+            const size_t t = t0 + token_of(base + 4 * u);
+            const int h = min(row_of(base + 4 * u), total_rows - 1);
+            const float *src;
+            if (h < a.heads) src = a.q + t * a.q_token + (size_t)h * a.q_head;
+            else if (h < a.heads + a.kv_heads) src = a.k + t * a.kv_token + (size_t)(h - a.heads) * a.kv_head;
+            else src = a.v + t * a.kv_token + (size_t)(h - a.heads - a.kv_heads) * a.kv_head;
+            const f32x4 *p = reinterpret_cast<const f32x4 *>(src) + (used ? c : 0);
+            x[u] = NT ? __builtin_nontemporal_load(p) : *p;
+            if constexpr (KIND >= 0) slot[u] = a.slots[t];
+        }
+    };
+    // Few tokens of many rows are shared by gridDim.y workgroups.
+    const int base0 = blockIdx.y * 4 * kU + wave, stride = gridDim.y * 4 * kU;
+    if (base0 < n) load(base0);
+
     // Of this lane's four dims: the pair (or -1), the other dim, and whether it
     // is the first of the two.
     int pair[4], other[4];
     bool first[4];
+    const i32x4 codes = rope.pairs ? reinterpret_cast<const i32x4 *>(rope.dims)[used ? c : 0] : i32x4{-1, -1, -1, -1};
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        pair[e] = -1;
-        other[e] = 4 * c + e;
-        first[e] = false;
-        if (rope.pairs && used) {
-            const int code = rope.dims[4 * c + e];
-            if (code >= 0) {
-                pair[e] = code >> 9;
-                first[e] = (code >> 8) & 1;
-                other[e] = code & 255;
-            }
-        }
+        pair[e] = codes[e] >> 9;  // -1 stays
+        first[e] = (codes[e] >> 8) & 1;
+        other[e] = codes[e] < 0 ? 4 * c + e : codes[e] & 255;
     }
-    const int total_rows = a.heads + 2 * a.kv_heads;
-    const int groups = (total_rows + rows - 1) / rows;
-    const int n = nt * groups;
-    for (int base = wave; base < n; base += 4 * kU) {
-        f32x4 x[kU];
-        int row[kU], tok[kU];
-#pragma unroll
-        for (int u = 0; u < kU; u++) {
-            const int idx = min(base + 4 * u, n - 1);
-            tok[u] = idx / groups;
-            row[u] = (idx - tok[u] * groups) * rows + sub;
-            const int h = min(row[u], total_rows - 1);
-            const float *src;
-            if (h < a.heads) src = a.q + (size_t)(t0 + tok[u]) * a.q_token + (size_t)h * a.q_head;
-            else if (h < a.heads + a.kv_heads)
-                src = a.k + (size_t)(t0 + tok[u]) * a.kv_token + (size_t)(h - a.heads) * a.kv_head;
-            else src = a.v + (size_t)(t0 + tok[u]) * a.kv_token + (size_t)(h - a.heads - a.kv_heads) * a.kv_head;
-            x[u] = reinterpret_cast<const f32x4 *>(src)[used ? c : 0];
+    if (rope.pairs) {
+        for (int i = tid; i < nt * rope.pairs; i += 256) {
+            const int t = i / rope.pairs, p = i - t * rope.pairs;
+            const int axis = (p >= rope.ends[0]) + (p >= rope.ends[1]) + (p >= rope.ends[2]);
+            const double position = a.positions[(size_t)(t0 + t) * rope.axes + axis];
+            turn_sincos(position * rope.turns[p], angles[2 * i], angles[2 * i + 1]);
         }
+        __syncthreads();
+    }
+    for (int base = base0; base < n; base += stride) {
 #pragma unroll
         for (int u = 0; u < kU; u++) {
             if (base + 4 * u >= n) break;
+            const int tok = token_of(base + 4 * u), row = row_of(base + 4 * u);
             f32x4 y = x[u];
             if (rope.pairs) {
                 float *buf = exchange[wave][u];
                 reinterpret_cast<f32x4 *>(buf)[lane] = y;
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 const float *mine = buf + sub * a.head_dim;
-                const bool turned = row[u] < a.heads + a.kv_heads;
+                const bool turned = row < a.heads + a.kv_heads;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float *sc = angles + 2 * (tok[u] * rope.pairs + max(pair[e], 0));
+                    const float *sc = angles + 2 * (tok * rope.pairs + max(pair[e], 0));
                     const float w = used ? mine[other[e]] : 0.0f;
                     const float s = first[e] ? -sc[0] : sc[0];
                     const float r = add_rn(mul_rn(y[e], sc[1]), mul_rn(w, s));
                     if (turned && pair[e] >= 0) y[e] = r;
                 }
             }
-            const bool live = used && row[u] < total_rows;
-            if (row[u] < a.heads) {
-                if (live)
-                    reinterpret_cast<f32x4 *>(a.q_out + (size_t)(t0 + tok[u]) * a.o_token +
-                                              (size_t)row[u] * a.o_head)[c] = y;
+            const bool live = used && row < total_rows;
+            if (row < a.heads && live) {
+                f32x4 *p = reinterpret_cast<f32x4 *>(a.q_out + (size_t)(t0 + tok) * a.o_token + (size_t)row * a.o_head) + c;
+                if constexpr (NT) __builtin_nontemporal_store(y, p);
+                else *p = y;
             }
             if constexpr (KIND >= 0) {
-                const int slot = a.slots[t0 + tok[u]];
-                const bool write = live && row[u] >= a.heads && slot >= 0 && slot < a.cache.slots;
-                const bool is_v = row[u] >= a.heads + a.kv_heads;
-                const int g = row[u] - a.heads - (is_v ? a.kv_heads : 0);
-                const size_t at = cache_row(a.cache, slot, g);
+                const bool write = live && row >= a.heads && slot[u] >= 0 && slot[u] < a.cache.slots;
+                const bool is_v = row >= a.heads + a.kv_heads;
+                const int g = row - a.heads - (is_v ? a.kv_heads : 0);
+                const size_t at = cache_row(a.cache, slot[u], g);
                 if constexpr (KIND == kCacheF32) {
                     if (write)
                         reinterpret_cast<f32x4 *>(static_cast<float *>(is_v ? a.cache.v : a.cache.k) +
@@ -156,67 +193,47 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(CacheRows a) {
                 }
             }
         }
+        if (base + stride < n) load(base + stride);
     }
 }
 
 // The rows of n slots as floats, [n][kv_heads][head_dim]; zeros where a slot is
 // none of the cache's.
-template <int KIND>
+template <int KIND, bool NT>
 __global__ __launch_bounds__(256) void cache_gather_kernel(CacheView cache, const int *__restrict__ slots,
                                                            float *__restrict__ k_out, float *__restrict__ v_out,
-                                                           size_t quads, int head_dim) {
+                                                           int tokens, int head_dim) {
     const int lanes = head_dim >> 2, per_token = 2 * cache.kv_heads * lanes;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += (size_t)gridDim.x * 256) {
-        const size_t t = i / per_token;
-        const int in = (int)(i - t * per_token);
-        const int row = in / lanes, c = in - row * lanes;
-        const bool is_v = row >= cache.kv_heads;
-        const int g = is_v ? row - cache.kv_heads : row;
+    for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
         const int slot = slots[t];
-        f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
-        if (slot >= 0 && slot < cache.slots) {
-            const size_t at = cache_row(cache, slot, g);
-            const void *base = is_v ? cache.v : cache.k;
-            if constexpr (KIND == kCacheF32) {
-                y = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at * cache.width)[c];
-            } else if constexpr (KIND == kCacheBf16) {
-                const bf16x4 b =
-                    reinterpret_cast<const bf16x4 *>(static_cast<const __bf16 *>(base) + at * cache.width)[c];
+        for (int in = threadIdx.x; in < per_token; in += 256) {
+            const int row = in / lanes, c = in - row * lanes;
+            const bool is_v = row >= cache.kv_heads;
+            const int g = is_v ? row - cache.kv_heads : row;
+            f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
+            if (slot >= 0 && slot < cache.slots) {
+                const size_t at = cache_row(cache, slot, g) * cache.width;
+                const void *base = is_v ? cache.v : cache.k;
+                if constexpr (KIND == kCacheF32) {
+                    y = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at)[c];
+                } else if constexpr (KIND == kCacheBf16) {
+                    const bf16x4 b = reinterpret_cast<const bf16x4 *>(static_cast<const __bf16 *>(base) + at)[c];
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (float)b[e];
-            } else {
-                const uint32_t p =
-                    reinterpret_cast<const uint32_t *>(static_cast<const int8_t *>(base) + at * cache.width)[c];
-                const float d = (float)__builtin_bit_cast(
-                    _Float16, (is_v ? cache.vd : cache.kd)[at * (cache.width / 32) + (c >> 3)]);
+                    for (int e = 0; e < 4; e++) y[e] = (float)b[e];
+                } else {
+                    const uint32_t p = reinterpret_cast<const uint32_t *>(static_cast<const int8_t *>(base) + at)[c];
+                    const float d =
+                        (float)__builtin_bit_cast(_Float16, (is_v ? cache.vd : cache.kd)[at / 32 + (c >> 3)]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(p >> (8 * e)) * d;
+                    for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(p >> (8 * e)) * d;
+                }
             }
+            f32x4 *out = reinterpret_cast<f32x4 *>(is_v ? v_out : k_out) +
+                         ((size_t)t * cache.kv_heads + g) * lanes + c;
+            if constexpr (NT) __builtin_nontemporal_store(y, out);
+            else *out = y;
         }
-        reinterpret_cast<f32x4 *>(is_v ? v_out : k_out)[(t * cache.kv_heads + g) * lanes + c] = y;
     }
-}
-
-// Inclusive sum over the workgroup's 256 threads (tmp: 4 values of LDS, free on
-// return), and the sum of all of them.
-__device__ __forceinline__ long long scan256(long long v, long long *tmp, long long *all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const long long w = __shfl_up(v, o, 64);
-        if (lane >= o) v += w;
-    }
-    if (lane == 63) tmp[wave] = v;
-    __syncthreads();
-    long long before = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        if (w < wave) before += tmp[w];
-        sum += tmp[w];
-    }
-    __syncthreads();
-    *all = sum;
-    return v + before;
 }
 
 // Block tables and slot maps from the requests' lengths.
@@ -238,24 +255,41 @@ __global__ __launch_bounds__(256) void pages_assign_kernel(PagesAssign a) {
     const int tid = threadIdx.x;
     const int mask = (1 << a.page_shift) - 1;
     long long tokens = 0, pages = 0, all = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += 256) {
-        const int r = r0 + tid;
-        const bool in = r < a.requests;
-        const long long c = in ? max(a.cached[r], 0) : 0, n = in ? max(a.added[r], 0) : 0;
-        const long long end = tokens + scan256(n, tmp, &all);
+    for (int r0 = 0; r0 < a.requests; r0 += 1024) {  // four in a row a thread
+        long long c[4], n[4], s[4], fresh[4], sum = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int r = r0 + 4 * tid + u;
+            c[u] = r < a.requests ? max(a.cached[r], 0) : 0;
+            n[u] = r < a.requests ? max(a.added[r], 0) : 0;
+            sum += n[u];
+        }
+        long long at = tokens + scan_all<256>(sum, tmp, &all) - sum;
         tokens += all;
-        // Tokens past the slot map's end are not placed.
-        const long long s = min(end - n, (long long)a.tokens), placed = min(end, (long long)a.tokens) - s;
-        const long long held = (c + mask) >> a.page_shift, need = (c + placed + mask) >> a.page_shift;
-        const long long upto = pages + scan256(need - held, tmp, &all);
+        sum = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            // Tokens past the slot map's end are not placed.
+            s[u] = min(at, (long long)a.tokens);
+            at += n[u];
+            n[u] = min(at, (long long)a.tokens) - s[u];
+            fresh[u] = ((c[u] + n[u] + mask) >> a.page_shift) - ((c[u] + mask) >> a.page_shift);
+            sum += fresh[u];
+        }
+        at = pages + scan_all<256>(sum, tmp, &all) - sum;
         pages += all;
-        if (in) {
-            start[r] = (int)s;
-            first[r] = (int)min(upto - (need - held), (long long)INT32_MAX);
-            if (blockIdx.x == 0) {
-                a.starts[r] = (int)s;
-                a.lens[r] = (int)min(c + placed, (long long)INT32_MAX);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int r = r0 + 4 * tid + u;
+            if (r < a.requests) {
+                start[r] = (int)s[u];
+                first[r] = (int)min(at, (long long)INT32_MAX);
+                if (blockIdx.x == 0) {
+                    a.starts[r] = (int)s[u];
+                    a.lens[r] = (int)min(c[u] + n[u], (long long)INT32_MAX);
+                }
             }
+            at += fresh[u];
         }
     }
     const int last = (int)min(tokens, (long long)a.tokens);
@@ -268,27 +302,39 @@ __global__ __launch_bounds__(256) void pages_assign_kernel(PagesAssign a) {
         }
     }
     __syncthreads();
+    // Four tokens in a row a thread: one bisection, and then steps to the next
+    // request that has any.
+    const int from = blockIdx.x * 1024 + 4 * tid;
+    int r = 0;
+    if (from < last) {
+        int hi = a.requests;  // start[r] <= from < start[hi]
+        while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if (start[mid] <= from) r = mid;
+            else hi = mid;
+        }
+    }
+    int c = 0, begin = -1;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-        const int t = blockIdx.x * 1024 + u * 256 + tid;
+        const int t = from + u;
         if (t >= a.tokens) break;
         int slot = -1;
         if (t < last) {
-            int lo = 0, hi = a.requests;  // start[lo] <= t < start[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start[mid] <= t) lo = mid;
-                else hi = mid;
+            while (start[r + 1] <= t) r++;
+            if (begin != start[r] || u == 0) {
+                begin = start[r];
+                c = max(a.cached[r], 0);
             }
-            const long long c = max(a.cached[lo], 0), pos = c + (t - start[lo]);
-            const long long col = pos >> a.page_shift, held = (c + mask) >> a.page_shift;
+            const long long pos = (long long)c + (t - begin);
+            const long long col = pos >> a.page_shift, held = ((long long)c + mask) >> a.page_shift;
             if (col < a.max_pages) {
-                int *entry = a.table + (size_t)lo * a.max_pages + col;
+                int *entry = a.table + (size_t)r * a.max_pages + col;
                 int page;
                 if (col < held) {
                     page = *entry;
                 } else {
-                    const long long at = (long long)free_start + first[lo] + (col - held);
+                    const long long at = (long long)free_start + first[r] + (col - held);
                     page = at >= 0 && at < a.free_pages ? a.free_list[at] : -1;
                     if ((pos & mask) == 0) *entry = page;
                 }
@@ -307,24 +353,34 @@ hipError_t launch_cache_rows(hipStream_t s, CacheRows a) {
     // Tokens of a workgroup: as many as leave eight workgroups to a CU, so that
     // few share the forming of angles and the small calls still spread.
     a.per_group = std::min(16, std::max(1, a.tokens / 2048));
-    const unsigned grid = (unsigned)((a.tokens + a.per_group - 1) / a.per_group);
+    const int groups = (a.heads + 2 * a.kv_heads + 256 / a.head_dim - 1) / (256 / a.head_dim);
+    const dim3 grid((unsigned)((a.tokens + a.per_group - 1) / a.per_group),
+                    a.tokens < 256 ? (groups + 4 * kU - 1) / (4 * kU) : 1);
     const size_t lds = (size_t)a.per_group * a.rope.pairs * 2 * sizeof(float);
-    if (a.kv_heads == 0) cache_rows_kernel<-1><<<grid, 256, lds, s>>>(a);
-    else if (a.cache.kind == kCacheF32) cache_rows_kernel<kCacheF32><<<grid, 256, lds, s>>>(a);
-    else if (a.cache.kind == kCacheBf16) cache_rows_kernel<kCacheBf16><<<grid, 256, lds, s>>>(a);
-    else cache_rows_kernel<kCacheQ8><<<grid, 256, lds, s>>>(a);
+    const bool nt = (size_t)a.tokens * (a.heads + 2 * a.kv_heads) * a.head_dim * sizeof(float) >= kStreamBytes;
+    auto run = [&](auto kernel, auto streaming) {
+        if (nt) streaming<<<grid, 256, lds, s>>>(a);
+        else kernel<<<grid, 256, lds, s>>>(a);
+    };
+    if (a.kv_heads == 0) run(cache_rows_kernel<-1, false>, cache_rows_kernel<-1, true>);
+    else if (a.cache.kind == kCacheF32) run(cache_rows_kernel<kCacheF32, false>, cache_rows_kernel<kCacheF32, true>);
+    else if (a.cache.kind == kCacheBf16) run(cache_rows_kernel<kCacheBf16, false>, cache_rows_kernel<kCacheBf16, true>);
+    else run(cache_rows_kernel<kCacheQ8, false>, cache_rows_kernel<kCacheQ8, true>);
     return hipGetLastError();
 }
 
 hipError_t launch_cache_gather(hipStream_t s, const CacheView &cache, const int *slots, float *k, float *v,
                                size_t n, size_t head_dim) {
-    const size_t quads = n * 2 * cache.kv_heads * (head_dim / 4);
-    if (quads == 0) return hipSuccess;
-    const unsigned grid = (unsigned)std::min<size_t>((quads + 255) / 256, 16384);
-    auto run = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(cache, slots, k, v, quads, (int)head_dim); };
-    if (cache.kind == kCacheF32) run(cache_gather_kernel<kCacheF32>);
-    else if (cache.kind == kCacheBf16) run(cache_gather_kernel<kCacheBf16>);
-    else run(cache_gather_kernel<kCacheQ8>);
+    if (n == 0) return hipSuccess;
+    const unsigned grid = (unsigned)std::min<size_t>(n, 1 << 16);
+    const bool nt = n * 2 * cache.kv_heads * head_dim * sizeof(float) >= kStreamBytes;
+    auto run = [&](auto kernel, auto streaming) {
+        if (nt) streaming<<<grid, 256, 0, s>>>(cache, slots, k, v, (int)n, (int)head_dim);
+        else kernel<<<grid, 256, 0, s>>>(cache, slots, k, v, (int)n, (int)head_dim);
+    };
+    if (cache.kind == kCacheF32) run(cache_gather_kernel<kCacheF32, false>, cache_gather_kernel<kCacheF32, true>);
+    else if (cache.kind == kCacheBf16) run(cache_gather_kernel<kCacheBf16, false>, cache_gather_kernel<kCacheBf16, true>);
+    else run(cache_gather_kernel<kCacheQ8, false>, cache_gather_kernel<kCacheQ8, true>);
     return hipGetLastError();
 }
 

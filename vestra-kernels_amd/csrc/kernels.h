@@ -335,8 +335,8 @@ __host__ __device__ inline size_t cache_row(const CacheView &c, int slot, int g)
 // Rotation pairs on the device; pairs == 0: no rotation.
 struct RopePlan {
     int axes, pairs;
+    int ends[3];          // pairs of the first axis, the first two, the first three
     const double *turns;  // [pairs] turns per unit of position
-    const int *axis;      // [pairs]
     const int *dims;      // [head_dim] pair << 9 | first << 8 | the other dim, or -1
 };
 struct CacheRows {

@@ -3368,32 +3368,33 @@ extern "C" vh_status vh_prepare_rope_axes(const vh_runtime *rt, size_t head_dim,
     RtState &s = *rt->s;
     TRY(set_device(s));
     std::vector<double> turns(n);
-    std::vector<int> ints(n + head_dim, -1);  // axis of each pair, then the dims
-    int *dims = ints.data() + n;
+    std::vector<int> dims(head_dim, -1);
     size_t i = 0, o = 0;
     for (size_t a = 0; a < axes; a++) {
         for (size_t j = 0; j < pairs[a]; j++, i++) {
             const double e = shared_spectrum ? (double)i / (double)n : (double)j / (double)pairs[a];
             const size_t first = shared_spectrum ? i : o + j, second = shared_spectrum ? n + i : o + pairs[a] + j;
             turns[i] = std::pow((double)frequency, -e) / 6.283185307179586476925286766559;
-            ints[i] = (int)a;
             dims[first] = (int)(i << 9 | 1 << 8 | second);
             dims[second] = (int)(i << 9 | first);
         }
         o += 2 * pairs[a];
     }
     auto r = std::make_unique<vh_rope>();
-    const size_t tb = n * sizeof(double), ib = ints.size() * sizeof(int);
-    TRY(dalloc(s, tb + ib, &r->block, "rope plan allocation"));
+    const size_t tb = n * sizeof(double), db = head_dim * sizeof(int);
+    TRY(dalloc(s, db + tb, &r->block, "rope plan allocation"));
     r->rt = rt->s;
-    TRY(h2d(s, r->block, turns.data(), tb, "rope plan upload"));
-    TRY(h2d(s, r->block + tb, ints.data(), ib, "rope plan upload"));
+    TRY(h2d(s, r->block, dims.data(), db, "rope plan upload"));
+    TRY(h2d(s, r->block + db, turns.data(), tb, "rope plan upload"));
     r->head_dim = head_dim;
     r->plan.axes = (int)axes;
     r->plan.pairs = (int)n;
-    r->plan.turns = reinterpret_cast<const double *>(r->block);
-    r->plan.axis = reinterpret_cast<const int *>(r->block + tb);
-    r->plan.dims = r->plan.axis + n;
+    for (size_t a = 0, end = 0; a < 3; a++) {
+        if (a < axes) end += pairs[a];
+        r->plan.ends[a] = (int)end;
+    }
+    r->plan.dims = reinterpret_cast<const int *>(r->block);
+    r->plan.turns = reinterpret_cast<const double *>(r->block + db);
     *out = r.release();
     return VH_OK;
     GUARD_END
