@@ -15,9 +15,9 @@
 // all of them), and the key steps of all tiles, laid end to end, into equal shares
 // of the workgroups: one long stream beside short ones, one query against a long
 // cache and a frame against eight earlier ones all fill the chip.  A tile that
-// ends up with several workgroups is joined from their partial sums by a second
-// launch.  Shares follow from the lengths alone, so the same call gives the same
-// bits.  The lengths are on the device: every workgroup forms the partition itself.
+// ends up with several workgroups is joined from their partial sums.  Shares follow from the lengths alone and parts are joined in order, so the same
+// call gives the same bits.  The lengths are on the device: every workgroup forms the
+// partition itself.
 //
 // Two kernels, by the rows of a request (launch_cache_attn):
 //   few rows:  16 query rows a workgroup, whose four waves take 32 keys each of a
@@ -201,11 +201,11 @@ __device__ __forceinline__ Tile uniform(const Tile &t) {
 struct Partition {
     int tiles;
     long long units, total, share;
+    long long end, cost;  // of the tile of this thread's number: steps up to its end, and its own
 };
 struct Place {
     int head, tile;
     long long into;  // steps of the tile before it
-    long long begin; // of the tile, among all steps
 };
 
 template <int BM, int STEP, int THREADS>
@@ -225,8 +225,9 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
     if (tid == 0) first_tile[a.requests] = (int)min(base, 1ll << 30);
     __syncthreads();
     p.tiles = first_tile[a.requests];
-    p.units = 0;
-    for (int t0 = 0; t0 < p.tiles; t0 += THREADS) {
+    p.cost = tid < p.tiles ? tile_of<BM, STEP>(a, first_tile, tid).cost : 0;
+    p.end = scan_all<THREADS>(p.cost, tmp, &p.units);
+    for (int t0 = THREADS; t0 < p.tiles; t0 += THREADS) {
         const int ti = t0 + tid;
         scan_all<THREADS>(ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0, tmp, &all);
         p.units += all;
@@ -236,6 +237,16 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
     return p;
 }
 
+// Steps of the first THREADS tiles.
+template <int THREADS>
+__device__ __forceinline__ long long first_units(const Partition &p, long long *tmp) {
+    if (threadIdx.x == THREADS - 1) tmp[0] = p.end;
+    __syncthreads();
+    const long long n = tmp[0];
+    __syncthreads();
+    return n;
+}
+
 template <int BM, int STEP, int THREADS>
 __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, const int *first_tile, long long *tmp,
                                       long long unit) {
@@ -243,22 +254,24 @@ __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, co
     Place at;
     at.head = (int)(unit / p.units);
     const long long x = unit - at.head * p.units;
-    long long all = 0, base = 0;
-    for (int t0 = 0; t0 < p.tiles; t0 += THREADS) {
-        const int ti = t0 + (int)threadIdx.x;
-        const long long cost = ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0;
-        const long long end = base + scan_all<THREADS>(cost, tmp, &all);
+    long long cost = p.cost, end = p.end, all = 0;
+    for (int t0 = 0;;) {
         if (end - cost <= x && x < end) {
-            found[0] = ti;
+            found[0] = t0 + (int)threadIdx.x;
             found[1] = end - cost;
         }
-        base += all;
-        if (x < base) break;
+        t0 += THREADS;
+        if (t0 >= p.tiles) break;
+        const int ti = t0 + (int)threadIdx.x;
+        const long long before = t0 == THREADS ? first_units<THREADS>(p, tmp) : all;
+        cost = ti < p.tiles ? tile_of<BM, STEP>(a, first_tile, ti).cost : 0;
+        long long some = 0;
+        end = before + scan_all<THREADS>(cost, tmp, &some);
+        all = before + some;
     }
     __syncthreads();
     at.tile = (int)found[0];
     at.into = x - found[1];
-    at.begin = at.head * p.units + found[1];
     __syncthreads();
     return at;
 }
@@ -567,9 +580,41 @@ __device__ void add_not_finite(const CacheAttn &a, const Tile &t, int g, Queries
     }
 }
 
-// Row `in` of a tile, four dims from d on: the result, or a workgroup's part of it
-// ([2 shares][BM][D] sums, then [2 shares][BM] maxima and sums of weights).
+// The parts.  Where the last workgroup of a tile joins them (HERE) they are read and
+// written past the L2 of an XCD (sc1), as the workgroups of a tile may be on several;
+// a launch of its own sees them anyway.
+template <bool HERE>
+struct Parts {
+    __amdgpu_buffer_rsrc_t base;
+    __device__ __forceinline__ explicit Parts(const CacheAttn &a)
+        : base(__builtin_amdgcn_make_buffer_rsrc(a.parts, 0, 0xffffffff, 0x00027000)) {}
+    static constexpr int kAgent = HERE ? 16 : 0;
+    __device__ __forceinline__ void put(uint32_t at, f32x4 v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), base, at, 0, kAgent);
+    }
+    __device__ __forceinline__ void put(uint32_t at, float x, float y) const {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(x), __float_as_uint(y)}, base, at, 0, kAgent);
+    }
+    __device__ __forceinline__ f32x4 four(uint32_t at) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(base, at, 0, kAgent));
+    }
+    __device__ __forceinline__ u32x2 two(uint32_t at) const {
+        return __builtin_amdgcn_raw_buffer_load_b64(base, at, 0, kAgent);
+    }
+};
+// Offsets in bytes of row `in` of part x: [2 shares][BM][D] sums, then [2 shares][BM]
+// maxima and sums of weights.
 template <int BM, int D>
+__device__ __forceinline__ uint32_t sums_at(uint32_t x, int in) {
+    return (x * BM + in) * (D * 4);
+}
+template <int BM, int D>
+__device__ __forceinline__ uint32_t weights_at(const CacheAttn &a, uint32_t x, int in) {
+    return 2u * a.shares * BM * D * 4 + (x * BM + in) * 8;
+}
+
+// Row `in` of a tile, four dims from d on: the result, or a workgroup's part of it.
+template <int BM, int D, bool HERE>
 struct Output {
     const CacheAttn &a;
     const Tile &t;
@@ -586,13 +631,9 @@ struct Output {
             for (int e = 0; e < 4; e++) y[e] = l == 0.0f ? 0.0f : v[e] * inv;
             *reinterpret_cast<f32x4 *>(a.out + ((size_t)(t.start + token) * a.heads + head) * a.head_dim + d) = y;
         } else {
-            const size_t at = (size_t)part * BM + in;
-            *reinterpret_cast<f32x4 *>(a.parts + at * D + d) = v;
-            if (d == 0) {
-                float *ml = a.parts + (size_t)2 * a.shares * BM * D + 2 * at;
-                ml[0] = m;
-                ml[1] = l;
-            }
+            const Parts<HERE> parts(a);
+            parts.put(sums_at<BM, D>(part, in) + 4 * d, v);
+            if (d == 0) parts.put(weights_at<BM, D>(a, part, in), m, l);
         }
     }
 };
@@ -604,12 +645,70 @@ __device__ __forceinline__ int my_share(const CacheAttn &a) {
     return (blockIdx.x & 7) * (a.shares >> 3) + (blockIdx.x >> 3);
 }
 
+// A row's four dims of a part, or of several: O on the maximum m, and the sum of
+// weights.
+struct Sums {
+    float m, l;
+    f32x4 y;
+    __device__ __forceinline__ void join(const Sums &b) {
+        const float mn = fmaxf(m, b.m);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        const float fb = b.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(b.m - mn);
+        m = mn;
+        l = l * f + b.l * fb;
+        y = y * f + b.y * fb;
+    }
+};
+
+// The parts of shares w0 .. w1 (of w0 the one at part0) become the tile's output.  Of
+// the workgroup's groups of D / 4 lanes (a group holds a row) as many share a row as the
+// rows leave: a single query's parts are summed by all of them.
+template <int BM, int D, int THREADS, bool HERE>
+__device__ void join_parts(const CacheAttn &a, const Tile &t, int g, int w0, int w1, int part0, char *smem) {
+    Sums *some = reinterpret_cast<Sums *>(smem);
+    const Output<BM, D, HERE> out{a, t, g, -1};
+    const Parts<HERE> parts(a);
+    constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
+    int rows = 1;  // at once
+    while (rows < GROUPS && rows < t.rows) rows *= 2;
+    const int sharers = GROUPS / rows;
+    const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+    for (int in = group % rows; in < (t.rows + rows - 1) / rows * rows; in += rows) {
+        auto part = [&](int w) {
+            const int x = w == w0 ? part0 : 2 * w, row = min(in, t.rows - 1);
+            const u32x2 ml = parts.two(weights_at<BM, D>(a, x, row));
+            return Sums{__uint_as_float(ml[0]), __uint_as_float(ml[1]), parts.four(sums_at<BM, D>(x, row) + 4 * d)};
+        };
+        Sums sum{-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int w = w0 + group / rows; w <= w1; w += 4 * sharers) {
+            Sums x[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = part(min(w + u * sharers, w1));
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (w + u * sharers <= w1) sum.join(x[u]);
+        }
+        if (sharers > 1) {  // all rows at once
+            some[threadIdx.x] = sum;
+            __syncthreads();
+            if (group < rows)
+                for (int i = 1; i < sharers; i++) sum.join(some[threadIdx.x + i * rows * LANES]);
+        }
+        if (group < rows) out.put(in, d, sum.y, sum.m, sum.l);
+    }
+}
+
 // Walks this workgroup's steps tile by tile: f(tile, head, first step, steps, part),
 // no steps where a tile sees no key.  Without room for parts (a.parts null) every
 // workgroup takes whole tiles.
-template <int BM, int STEP, int THREADS, class F>
-__device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, F f) {
+//
+// HERE: of the workgroups that hold a part of a tile the one that is done last joins
+// them, in the order of the shares.  They count in the counter of the tile's first share
+// (of which it is the last tile, so no other counts there), zero before and after.
+template <int BM, int STEP, int THREADS, int D, bool HERE, class F>
+__device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *smem, F f) {
     __shared__ long long tmp[THREADS / 64];
+    __shared__ int is_last;
     const Partition p = partition<BM, STEP, THREADS>(a, first_tile, tmp, a.shares);
     const int w = my_share(a);
     const bool share = a.parts != nullptr;
@@ -617,7 +716,7 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, F f) {
     long long at = share ? w * p.share : w;
     const long long end = share ? min(at + p.share, p.total) : (long long)p.tiles * a.cache.kv_heads;
     if (at >= end) return;
-    Place place = {0, 0, 0, 0};
+    Place place = {0, 0, 0};
     if (share) place = find<BM, STEP, THREADS>(a, p, first_tile, tmp, at);
     for (bool first = true; at < end; first = false) {
         if (!share) {
@@ -625,11 +724,27 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, F f) {
             place.tile = (int)(at - (long long)place.head * p.tiles);
         }
         const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, place.tile));
-        const int into = uniform((int)place.into);
+        const int into = uniform((int)place.into), g = uniform(place.head);
         const int steps = share ? uniform((int)min(end - at, (long long)t.cost - into)) : t.cost;
         const bool whole = into == 0 && steps == t.cost;
-        f(t, uniform(place.head), t.step0 + into, t.any.lo < t.any.hi ? steps : 0,
-          whole ? -1 : 2 * w + (first ? 0 : 1));
+        f(t, g, t.step0 + into, t.any.lo < t.any.hi ? steps : 0, whole ? -1 : 2 * w + (first ? 0 : 1));
+        if (HERE && !whole) {
+            const long long begin = at - into;
+            const int w0 = uniform((int)(begin / p.share)), w1 = uniform((int)((begin + t.cost - 1) / p.share));
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's parts are out
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                unsigned *counter = a.counters + w0;
+                is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                          (unsigned)(w1 - w0);
+                if (is_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (is_last) {
+                join_parts<BM, D, THREADS, true>(a, t, g, w0, w1, 2 * w0 + (begin > w0 * p.share ? 1 : 0), smem);
+                __syncthreads();
+            }
+        }
         at += share ? steps : a.shares;
         place.into = 0;
         if (++place.tile == p.tiles) {
@@ -673,7 +788,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
     float *scales = reinterpret_cast<float *>(mine + NP * PLANE);  // [k, v][C][32]
     const int srow = lane / LPR, sg = lane % LPR;  // row of a pass and granule that this lane moves
 
-    walk<BM, STEP, 256>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
+    walk<BM, STEP, 256, D, true>(a, first_tile, smem, [&](const Tile &t, int g, int step0, int steps, int part) {
         Queries<D, 1> w;
         w.load(a, t, g, 0, li, lh);
         Octet<KIND, D> x[PASSES];
@@ -818,7 +933,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
             o[16 * D + 2 * li + 1] = l;
         }
         __syncthreads();
-        const Output<BM, D> out{a, t, g, part};
+        const Output<BM, D, true> out{a, t, g, part};
         const int row = tid >> 4;
         float m = -INFINITY, sum = 0.0f, f[4];
 #pragma unroll
@@ -872,7 +987,7 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
     const int li = lane & 15, lh = lane >> 4;
     const int srow = tid / LPR, sg = tid % LPR;  // staged row of a pass, and granule
 
-    walk<BM, STEP, THREADS>(a, first_tile, [&](const Tile &t, int g, int step0, int steps, int part) {
+    walk<BM, STEP, THREADS, D, false>(a, first_tile, smem, [&](const Tile &t, int g, int step0, int steps, int part) {
         const int first = 16 * QT * wave;
         const bool works = first < t.rows;
         Queries<D, QT> w;
@@ -1011,7 +1126,7 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
             if (fix)
                 for (int h = 0; h < H; h++) add_not_finite<KIND>(a, t, g, w, key + 32 * h, lh);
         }
-        const Output<BM, D> out{a, t, g, part};
+        const Output<BM, D, false> out{a, t, g, part};
 #pragma unroll
         for (int u = 0; u < QT; u++) {
             const float l = sum_groups(w.l[u]);
@@ -1023,70 +1138,25 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
     });
 }
 
-// ---- tiles that several workgroups share ---------------------------------------------
-
-// Every border between two shares that lies inside a tile names it; the first
-// such border's workgroup joins its parts.
-// A row's four dims of a part, or of several: O on the maximum m, and the sum of
-// weights.
-struct Sums {
-    float m, l;
-    f32x4 y;
-    __device__ __forceinline__ void join(const Sums &b) {
-        const float mn = fmaxf(m, b.m);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float fb = b.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(b.m - mn);
-        m = mn;
-        l = l * f + b.l * fb;
-        y = y * f + b.y * fb;
-    }
-};
-
-// Of the workgroup's 1024 / D groups of lanes (a group holds a row) as many share a
-// row as the rows leave: a single query's parts are summed by all of them.
+// Joins the parts of many_rows_kernel, whose tiles would keep the last workgroup of
+// each busy for long (a frame against eight 126 us this way, 138 the other; the few
+// rows of the other kernel are joined there: one token 15.2 us against 18.2).  Every
+// border between two shares that lies inside a tile names it; the first such border's
+// workgroup joins its parts.
 template <int BM, int STEP, int D>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttn a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ long long tmp[4];
-    __shared__ Sums some[256];
-    int *first_tile = reinterpret_cast<int *>(smem);
+    int *first_tile = reinterpret_cast<int *>(smem + 256 * sizeof(Sums));
     const Partition p = partition<BM, STEP, 256>(a, first_tile, tmp, a.shares);
     const long long border = (blockIdx.x + 1) * p.share;
     if (border >= p.total) return;
     const Place at = find<BM, STEP, 256>(a, p, first_tile, tmp, border);
-    if (at.into == 0 || at.begin < border - p.share) return;  // between two tiles, or not the first
+    const long long begin = border - at.into, before = border - p.share;
+    if (at.into == 0 || begin < before) return;  // between two tiles, or not the first
     const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, at.tile));
-    const int w0 = blockIdx.x, w1 = uniform((int)((at.begin + t.cost - 1) / p.share));
-    const int part0 = 2 * w0 + (at.begin > w0 * p.share ? 1 : 0);
-    const Output<BM, D> out{a, t, uniform(at.head), -1};
-    const float *ml = a.parts + (size_t)2 * a.shares * BM * D;
-    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-    int rows = 1;  // at once
-    while (rows < GROUPS && rows < t.rows) rows *= 2;
-    const int sharers = GROUPS / rows;
-    const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
-    for (int in = group % rows; in < (t.rows + rows - 1) / rows * rows; in += rows) {
-        auto part = [&](int w) {
-            const size_t x = (size_t)(w == w0 ? part0 : 2 * w) * BM + min(in, t.rows - 1);
-            return Sums{ml[2 * x], ml[2 * x + 1], *reinterpret_cast<const f32x4 *>(a.parts + x * D + d)};
-        };
-        Sums sum{-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
-        for (int w = w0 + group / rows; w <= w1; w += 4 * sharers) {
-            Sums x[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) x[u] = part(min(w + u * sharers, w1));
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (w + u * sharers <= w1) sum.join(x[u]);
-        }
-        if (sharers > 1) {  // one pass: all rows at once
-            some[threadIdx.x] = sum;
-            __syncthreads();
-            if (group >= rows) return;
-            for (int i = 1; i < sharers; i++) sum.join(some[threadIdx.x + i * rows * LANES]);
-        }
-        out.put(in, d, sum.y, sum.m, sum.l);
-    }
+    const int w0 = blockIdx.x, w1 = uniform((int)((begin + t.cost - 1) / p.share));
+    join_parts<BM, D, 256, false>(a, t, uniform(at.head), w0, w1, 2 * w0 + (begin > before ? 1 : 0), smem);
 }
 
 template <int KIND, int D>
@@ -1101,9 +1171,8 @@ hipError_t run_kind(hipStream_t s, const CacheAttn &a, bool few) {
     if (few) few_rows_kernel<KIND, D><<<a.shares, 256, lds + index, s>>>(a);
     else many_rows_kernel<KIND, D><<<a.shares, kManyThreads<D>, lds + index, s>>>(a);
     e = hipGetLastError();
-    if (e != hipSuccess || !a.parts) return e;
-    if (few) join_kernel<16, 128, D><<<a.shares - 1, 256, index, s>>>(a);
-    else join_kernel<128, many_step<KIND, D>(), D><<<a.shares - 1, 256, index, s>>>(a);
+    if (e != hipSuccess || few || !a.parts) return e;
+    join_kernel<128, many_step<KIND, D>(), D><<<a.shares - 1, 256, 256 * sizeof(Sums) + index, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1114,15 +1183,18 @@ bool few_rows(size_t rows, size_t requests) { return rows <= 32 * requests; }
 
 }  // namespace
 
+static_assert(kShares <= kAttnCounters, "a counter for each share");
+
 size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t width) {
     return (size_t)2 * kShares * (few_rows(tokens * group, requests) ? 16 : 128) * (width + 2);
 }
 
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a) {
-    a.shares = kShares;
-    a.min_share = 1;
     const bool few = few_rows((size_t)a.tokens * a.group, (size_t)a.requests);
     const bool wide = a.cache.width == 128;
+    // As many as run at once: two a CU, one of eight waves.
+    a.shares = !few && wide ? kShares / 2 : kShares;
+    a.min_share = 1;
     switch (a.cache.kind) {
         case kCacheF32: return wide ? run_kind<kCacheF32, 128>(s, a, few) : run_kind<kCacheF32, 64>(s, a, few);
         case kCacheBf16: return wide ? run_kind<kCacheBf16, 128>(s, a, few) : run_kind<kCacheBf16, 64>(s, a, few);

@@ -379,10 +379,14 @@ struct CacheAttn {
     float scale_log2;     // softmax scale times log2(e)
     CacheView cache;
     // Room for the parts of tiles that several workgroups share
-    // (cache_attn_floats()), or null: every tile is one workgroup's.
+    // (cache_attn_floats()) and kAttnCounters counters, zero before and after, or
+    // null: every tile is one workgroup's.  Launches sharing them must not overlap in
+    // time.
     float *parts;
+    unsigned *counters;
     int shares, min_share;  // set by the launcher
 };
+constexpr size_t kAttnCounters = 1024;
 size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t width);
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a);
 

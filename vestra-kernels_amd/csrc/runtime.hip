@@ -128,7 +128,8 @@ struct RtState {
     Workspace fcnt;                             // and the in-kernel merge's arrival counters
     Workspace aq;                               // Q8_0 activation blocks
     Workspace sx;                               // split rows of a projection's input
-    Workspace pa;                               // parts of the paged attention's tiles
+    Workspace pa;                               // counters and parts of the paged attention's tiles
+    unsigned long long pa_capture = 0;          // the capture that took it, where it is recorded
     std::vector<void *> recorded;               // outgrown blocks that a graph may hold
     float *tw = nullptr;                        // balanced-tail GEMM partials
     unsigned *tcnt = nullptr;                   // and arrival counters (zeroed once)
@@ -3660,6 +3661,38 @@ extern "C" vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *ca
     GUARD_END
 }
 
+// Room for the parts of the paged attention's tiles, counters first (zeroed here;
+// every launch leaves them zero).  A capture takes the runtime's block for its graph
+// alone: the next call outside gets another, so replays of the graph, on whatever
+// stream, and other graphs never meet in it.  Without room (a capture of a size that
+// has not run since the last capture) a tile's keys stay with one workgroup.
+static void attn_workspace(RtState &s, size_t floats, vh::CacheAttn *a) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(s.stream, &st, &id) != hipSuccess) {
+        hipGetLastError();
+        return;
+    }
+    const bool captured = st != hipStreamCaptureStatusNone;
+    if (!captured && s.pa.recorded) {
+        s.recorded.push_back(s.pa.p);
+        s.pa = Workspace{};
+    }
+    if (captured && s.pa.recorded && s.pa_capture != id) return;
+    const size_t head = vh::kAttnCounters * sizeof(unsigned), had = s.pa.bytes;
+    char *p = static_cast<char *>(grow_workspace(s, s.pa, head + floats * sizeof(float)));
+    if (!p) return;
+    if (s.pa.bytes != had && hipMemsetAsync(p, 0, head, s.stream) != hipSuccess) {
+        hipGetLastError();
+        hipFree(p);
+        s.pa = Workspace{};
+        return;
+    }
+    if (captured) s.pa_capture = id;
+    a->counters = reinterpret_cast<unsigned *>(p);
+    a->parts = reinterpret_cast<float *>(p + head);
+}
+
 extern "C" vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const vh_tensor *q, size_t heads,
                                                size_t tokens, size_t requests, const vh_index *table,
                                                size_t max_pages, const vh_index *starts, const vh_index *lens,
@@ -3712,10 +3745,7 @@ extern "C" vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const v
     a.window = window < (size_t)INT32_MAX ? (int)window : 0;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.cache = cache->view;
-    // Without room for parts (a capture before this size ran) a tile's keys stay
-    // with one workgroup.
-    a.parts = static_cast<float *>(
-        grow_workspace(s, s.pa, vh::cache_attn_floats(tokens, heads / kvh, requests, a.cache.width) * sizeof(float)));
+    attn_workspace(s, vh::cache_attn_floats(tokens, heads / kvh, requests, a.cache.width), &a);
     return launch(s, "kv_attention", [&] { return vh::launch_cache_attn(s.stream, a); });
     GUARD_END
 }
