@@ -154,8 +154,13 @@ struct Tile {
     int r, start, len, pos;  // request, its first new token, its tokens, the first new one's position
     int row, rows;           // query rows (token of the request * group + head of the group)
     Seen any, all;           // keys that some row sees, that every row sees
-    int step0, cost;         // first key step and their number, 1 where there is none
+    int step0, cost;         // first key step; their number, 1 where there is none, and kTileCost
 };
+
+// What a tile costs besides its key steps, in steps: queries fetched, first loads
+// waited for, output written.  Without it a share of many short tiles takes twice as
+// long as one of a long tile.
+constexpr int kTileCost = 2;
 
 __device__ __forceinline__ int start_of(const CacheAttn &a, int r) { return min(max(a.starts[r], 0), a.tokens); }
 
@@ -183,7 +188,7 @@ __device__ __forceinline__ Tile tile_of(const CacheAttn &a, const int *first_til
     t.any = {s0.lo, s1.hi};
     t.all = {s1.lo, s0.hi};
     t.step0 = t.any.lo / STEP;
-    t.cost = max(1, (t.any.hi + STEP - 1) / STEP - t.step0);
+    t.cost = max(1, (t.any.hi + STEP - 1) / STEP - t.step0) + kTileCost;
     return t;
 }
 
@@ -727,7 +732,8 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
         const int into = uniform((int)place.into), g = uniform(place.head);
         const int steps = share ? uniform((int)min(end - at, (long long)t.cost - into)) : t.cost;
         const bool whole = into == 0 && steps == t.cost;
-        f(t, g, t.step0 + into, t.any.lo < t.any.hi ? steps : 0, whole ? -1 : 2 * w + (first ? 0 : 1));
+        const int from = max(into - kTileCost, 0), to = max(into + steps - kTileCost, 0);
+        f(t, g, t.step0 + from, t.any.lo < t.any.hi ? to - from : 0, whole ? -1 : 2 * w + (first ? 0 : 1));
         if (HERE && !whole) {
             const long long begin = at - into;
             const int w0 = uniform((int)(begin / p.share)), w1 = uniform((int)((begin + t.cost - 1) / p.share));
@@ -789,8 +795,6 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
     const int srow = lane / LPR, sg = lane % LPR;  // row of a pass and granule that this lane moves
 
     walk<BM, STEP, 256, D, true>(a, first_tile, smem, [&](const Tile &t, int g, int step0, int steps, int part) {
-        Queries<D, 1> w;
-        w.load(a, t, g, 0, li, lh);
         Octet<KIND, D> x[PASSES];
         uint16_t d[C] = {};  // scales of key `lane & 31`
         auto load = [&](const void *base, const uint16_t *scale, int slot) {
@@ -826,6 +830,8 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
             slot = slot_of(a, key_of(0), page);
             load(a.cache.k, a.cache.kd, slot);
         }
+        Queries<D, 1> w;  // (read behind the first keys)
+        w.load(a, t, g, 0, li, lh);
         for (int i = 0; i < steps; i++) {
             const int key = (step0 + i) * STEP + 32 * wave;
             const uint32_t present = (uint32_t)__ballot(slot < a.cache.slots);
@@ -990,8 +996,6 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
     walk<BM, STEP, THREADS, D, false>(a, first_tile, smem, [&](const Tile &t, int g, int step0, int steps, int part) {
         const int first = 16 * QT * wave;
         const bool works = first < t.rows;
-        Queries<D, QT> w;
-        w.load(a, t, g, first, li, lh);
         Octet<KIND, D> kr[PASSES], vr[PASSES];
         uint16_t kd[PASSES] = {}, vd[PASSES] = {};
         int slot[PASSES], page[PASSES];
@@ -1031,6 +1035,8 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
             look_up(step0 + 1);
         }
         if (tid < 4) flags[tid] = 0;
+        Queries<D, QT> w;
+        w.load(a, t, g, first, li, lh);
         for (int i = 0; i < steps; i++) {
             const int key = (step0 + i) * STEP;
             const bool edge = key < t.all.lo || key + STEP > t.all.hi;
