@@ -238,7 +238,7 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
         p.units += all;
     }
     p.total = p.units * a.cache.kv_heads;
-    p.share = max((long long)a.min_share, (p.total + shares - 1) / shares);
+    p.share = max(1ll, (p.total + shares - 1) / shares);
     return p;
 }
 
@@ -665,22 +665,23 @@ struct Sums {
     }
 };
 
-// The parts of shares w0 .. w1 (of w0 the one at part0) become the tile's output.  Of
-// the workgroup's groups of D / 4 lanes (a group holds a row) as many share a row as the
-// rows leave: a single query's parts are summed by all of them.
+// The parts of shares w0 .. w1 (of w0 the one at part0) become the tile's output: rows
+// from .. to - 1.  Of the workgroup's groups of D / 4 lanes (a group holds a row) as many
+// share a row as the rows leave: a single query's parts are summed by all of them.
 template <int BM, int D, int THREADS, bool HERE>
-__device__ void join_parts(const CacheAttn &a, const Tile &t, int g, int w0, int w1, int part0, char *smem) {
+__device__ void join_parts(const CacheAttn &a, const Tile &t, int g, int w0, int w1, int part0, int from, int to,
+                           char *smem) {
     Sums *some = reinterpret_cast<Sums *>(smem);
     const Output<BM, D, HERE> out{a, t, g, -1};
     const Parts<HERE> parts(a);
     constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
     int rows = 1;  // at once
-    while (rows < GROUPS && rows < t.rows) rows *= 2;
+    while (rows < GROUPS && rows < to - from) rows *= 2;
     const int sharers = GROUPS / rows;
     const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
-    for (int in = group % rows; in < (t.rows + rows - 1) / rows * rows; in += rows) {
+    for (int in = from + group % rows; in < from + (to - from + rows - 1) / rows * rows; in += rows) {
         auto part = [&](int w) {
-            const int x = w == w0 ? part0 : 2 * w, row = min(in, t.rows - 1);
+            const int x = w == w0 ? part0 : 2 * w, row = min(in, to - 1);
             const u32x2 ml = parts.two(weights_at<BM, D>(a, x, row));
             return Sums{__uint_as_float(ml[0]), __uint_as_float(ml[1]), parts.four(sums_at<BM, D>(x, row) + 4 * d)};
         };
@@ -699,7 +700,7 @@ __device__ void join_parts(const CacheAttn &a, const Tile &t, int g, int w0, int
             if (group < rows)
                 for (int i = 1; i < sharers; i++) sum.join(some[threadIdx.x + i * rows * LANES]);
         }
-        if (group < rows) out.put(in, d, sum.y, sum.m, sum.l);
+        if (group < rows && in < to) out.put(in, d, sum.y, sum.m, sum.l);
     }
 }
 
@@ -747,7 +748,8 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
             }
             __syncthreads();
             if (is_last) {
-                join_parts<BM, D, THREADS, true>(a, t, g, w0, w1, 2 * w0 + (begin > w0 * p.share ? 1 : 0), smem);
+                join_parts<BM, D, THREADS, true>(a, t, g, w0, w1, 2 * w0 + (begin > w0 * p.share ? 1 : 0), 0,
+                                                   t.rows, smem);
                 __syncthreads();
             }
         }
@@ -1148,7 +1150,8 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
 // each busy for long (a frame against eight 126 us this way, 138 the other; the few
 // rows of the other kernel are joined there: one token 15.2 us against 18.2).  Every
 // border between two shares that lies inside a tile names it; the first such border's
-// workgroup joins its parts.
+// workgroups join its parts, kJoinRows rows each.
+constexpr int kJoinRows = 16;
 template <int BM, int STEP, int D>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttn a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1162,7 +1165,10 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttn a) {
     if (at.into == 0 || begin < before) return;  // between two tiles, or not the first
     const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, at.tile));
     const int w0 = blockIdx.x, w1 = uniform((int)((begin + t.cost - 1) / p.share));
-    join_parts<BM, D, 256, false>(a, t, uniform(at.head), w0, w1, 2 * w0 + (begin > before ? 1 : 0), smem);
+    const int from = blockIdx.y * kJoinRows;
+    if (from >= t.rows) return;
+    join_parts<BM, D, 256, false>(a, t, uniform(at.head), w0, w1, 2 * w0 + (begin > before ? 1 : 0), from,
+                                  min(from + kJoinRows, t.rows), smem);
 }
 
 template <int KIND, int D>
@@ -1178,29 +1184,43 @@ hipError_t run_kind(hipStream_t s, const CacheAttn &a, bool few) {
     else many_rows_kernel<KIND, D><<<a.shares, kManyThreads<D>, lds + index, s>>>(a);
     e = hipGetLastError();
     if (e != hipSuccess || few || !a.parts) return e;
-    join_kernel<128, many_step<KIND, D>(), D><<<a.shares - 1, 256, 256 * sizeof(Sums) + index, s>>>(a);
+    join_kernel<128, many_step<KIND, D>(), D><<<dim3(a.shares - 1, 128 / kJoinRows), 256, 256 * sizeof(Sums) + index, s>>>(a);
     return hipGetLastError();
 }
 
 constexpr int kShares = 512;  // two workgroups a CU
 
-// Tiles of 16 rows where the requests have few on average.
-bool few_rows(size_t rows, size_t requests) { return rows <= 32 * requests; }
+// Whether requests of these query rows (new tokens times the heads that share a head
+// of the cache) go to tiles of 16, by their average.  More rows read K and V once
+// for each 16; tiles of 128 do the arithmetic of 128 whatever they hold.  Measured in
+// us, tiles of 16 / of 128, for 16, 32, 64 and 128 rows against 65536 keys of one request
+// and 4096 of sixteen (f32 and bf16 heads: 12 of 64; wide: 8 of 128 for 32):
+//   f32        79/118 132/119 224/144 464/174    74/117 133/119 217/142 376/173
+//   f32 wide  137/154 211/158 379/163 691/223   120/144 160/147 260/157 523/219
+//   bf16       49/72   76/73  109/90  254/98     43/72   71/74  108/90  169/98
+//   bf16 wide  77/89  102/90  177/92  330/118    59/79   66/81   90/83  193/113
+//   Q8_0       46/118  67/119 114/136 216/143    40/116  66/118 115/134 209/141
+//   Q8_0 wide  68/160  84/162 137/163 259/193    49/149  73/151 120/154 236/184
+// (wide floats: LDS holds one workgroup of the few-row kernel a CU.)
+bool few_rows(const CacheView &c, size_t rows, size_t requests) {
+    const size_t most = c.kind == kCacheQ8 ? 64 : c.kind == kCacheF32 && c.width == 128 ? 16 : 32;
+    return rows <= most * requests;
+}
 
 }  // namespace
 
 static_assert(kShares <= kAttnCounters, "a counter for each share");
 
-size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t width) {
-    return (size_t)2 * kShares * (few_rows(tokens * group, requests) ? 16 : 128) * (width + 2);
+size_t cache_attn_floats(const CacheView &cache, size_t tokens, size_t group, size_t requests) {
+    return (size_t)2 * kShares * (few_rows(cache, tokens * group, requests) ? 16 : 128) * (cache.width + 2);
 }
 
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a) {
-    const bool few = few_rows((size_t)a.tokens * a.group, (size_t)a.requests);
+    const bool few = few_rows(a.cache, (size_t)a.tokens * a.group, (size_t)a.requests);
     const bool wide = a.cache.width == 128;
-    // As many as run at once: two a CU, one of eight waves.
-    a.shares = !few && wide ? kShares / 2 : kShares;
-    a.min_share = 1;
+    // As many as run at once: two a CU, one of eight waves (Q8_0 chunks of 32 / 8 heads
+    // of 128: 368 us, with two 388) or of the LDS of wide floats.
+    a.shares = wide && (!few || a.cache.kind == kCacheF32) ? kShares / 2 : kShares;
     switch (a.cache.kind) {
         case kCacheF32: return wide ? run_kind<kCacheF32, 128>(s, a, few) : run_kind<kCacheF32, 64>(s, a, few);
         case kCacheBf16: return wide ? run_kind<kCacheBf16, 128>(s, a, few) : run_kind<kCacheBf16, 64>(s, a, few);

@@ -384,10 +384,10 @@ struct CacheAttn {
     // time.
     float *parts;
     unsigned *counters;
-    int shares, min_share;  // set by the launcher
+    int shares;  // set by the launcher
 };
 constexpr size_t kAttnCounters = 1024;
-size_t cache_attn_floats(size_t tokens, size_t group, size_t requests, size_t width);
+size_t cache_attn_floats(const CacheView &cache, size_t tokens, size_t group, size_t requests);
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a);
 
 }  // namespace vh

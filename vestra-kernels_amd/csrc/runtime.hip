@@ -3745,7 +3745,7 @@ extern "C" vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const v
     a.window = window < (size_t)INT32_MAX ? (int)window : 0;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.cache = cache->view;
-    attn_workspace(s, vh::cache_attn_floats(tokens, heads / kvh, requests, a.cache.width), &a);
+    attn_workspace(s, vh::cache_attn_floats(a.cache, tokens, heads / kvh, requests), &a);
     return launch(s, "kv_attention", [&] { return vh::launch_cache_attn(s.stream, a); });
     GUARD_END
 }
