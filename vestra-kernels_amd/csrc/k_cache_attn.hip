@@ -15,9 +15,9 @@
 // all of them), and the key steps of all tiles, laid end to end, into equal shares
 // of the workgroups: one long stream beside short ones, one query against a long
 // cache and a frame against eight earlier ones all fill the chip.  A tile that
-// ends up with several workgroups is joined from their partial sums.  Shares follow from the lengths alone and parts are joined in order, so the same
-// call gives the same bits.  The lengths are on the device: every workgroup forms the
-// partition itself.
+// ends up with several workgroups is joined from their partial sums.  Shares follow
+// from the lengths alone and parts are joined in order, so the same call gives the same
+// bits.  The lengths are on the device: every workgroup forms the partition itself.
 //
 // Two kernels, by the rows of a request (launch_cache_attn):
 //   few rows:  16 query rows a workgroup, whose four waves take 32 keys each of a
@@ -561,7 +561,7 @@ constexpr int kPartsOfV = KIND == kCacheBf16 ? 1 : 3;
 
 // A value that is not finite in a step where some query does not see it was
 // staged as zero: the dims of the queries that do see it become NaN here.  32 keys
-// from key on, of which `present` are there; rare, so one by one.
+// from key on; rare, so one by one.
 template <int KIND, int D, int QT>
 __device__ void add_not_finite(const CacheAttn &a, const Tile &t, int g, Queries<D, QT> &w, int key, int lh) {
     for (int i = 0; i < 32; i++) {
@@ -781,9 +781,15 @@ constexpr int few_wave_bytes() {
     constexpr int o = 16 * D * 4 + 128;
     return panel > o ? panel : o;
 }
-
 template <int KIND, int D>
-__global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
+constexpr int few_workgroups() {  // a CU
+    return 4 * few_wave_bytes<KIND, D>() > 80 * 1024 ? 1 : 2;
+}
+
+// (Of wide floats LDS holds one workgroup a CU, which so may use every register: 64
+// tokens against 3000 keys of 8 heads of 128 242 us, with half of them 267.)
+template <int KIND, int D>
+__global__ __launch_bounds__(256, (few_workgroups<KIND, D>())) void few_rows_kernel(CacheAttn a) {
     constexpr int BM = 16, STEP = 128, C = D / 32, WAVE = few_wave_bytes<KIND, D>();
     constexpr int NP = kFewParts<KIND>, PLANE = 32 * D * 2;
     constexpr int LPR = D / 8, RPP = 64 / LPR, PASSES = 32 / RPP;  // lanes a row, rows a pass
@@ -966,6 +972,8 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(CacheAttn a) {
 
 // ---- many rows --------------------------------------------------------------------
 
+// Keys of a step.  (Wide floats, of six planes: 128 query rows of 8 heads against 65536 keys
+// 214 us, with 64 keys 230; 2000 tokens of 32 / 8 heads against 20000 3230 and 3180.)
 template <int KIND, int D>
 constexpr int many_step() {
     return KIND == kCacheF32 && D == 128 ? 32 : 64;
@@ -1195,16 +1203,16 @@ constexpr int kShares = 512;  // two workgroups a CU
 // for each 16; tiles of 128 do the arithmetic of 128 whatever they hold.  Measured in
 // us, tiles of 16 / of 128, for 16, 32, 64 and 128 rows against 65536 keys of one request
 // and 4096 of sixteen (f32 and bf16 heads: 12 of 64; wide: 8 of 128 for 32):
-//   f32        79/118 132/119 224/144 464/174    74/117 133/119 217/142 376/173
-//   f32 wide  137/154 211/158 379/163 691/223   120/144 160/147 260/157 523/219
-//   bf16       49/72   76/73  109/90  254/98     43/72   71/74  108/90  169/98
-//   bf16 wide  77/89  102/90  177/92  330/118    59/79   66/81   90/83  193/113
-//   Q8_0       46/118  67/119 114/136 216/143    40/116  66/118 115/134 209/141
-//   Q8_0 wide  68/160  84/162 137/163 259/193    49/149  73/151 120/154 236/184
-// (wide floats: LDS holds one workgroup of the few-row kernel a CU.)
+//   f32        78/117 133/118 220/143 472/169    74/116 133/119 214/141 367/169
+//   f32 wide  102/155 169/158 314/162 602/215    91/144 145/147 283/154 572/215
+//   bf16       49/71   71/73  103/89  226/96     42/71   69/73  108/89  179/96
+//   bf16 wide  76/88  102/90  170/91  315/116    58/79   63/80   92/82  198/110
+//   Q8_0       47/117  67/119 114/135 215/142    41/116  67/117 114/133 209/139
+//   Q8_0 wide  68/161  84/164 135/165 253/194    48/152  72/154 118/156 233/185
+// Fewer keys, whose number the host does not know, favour the tiles of 16 more: 64 rows
+// against 4096 of one request f32 24/33, bf16 18/29, Q8_0 19/33.
 bool few_rows(const CacheView &c, size_t rows, size_t requests) {
-    const size_t most = c.kind == kCacheQ8 ? 64 : c.kind == kCacheF32 && c.width == 128 ? 16 : 32;
-    return rows <= most * requests;
+    return rows <= (c.kind == kCacheQ8 ? 64 : 32) * requests;
 }
 
 }  // namespace
