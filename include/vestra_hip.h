@@ -505,7 +505,14 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  * that dim, in a key no defined row.  Rows behind starts[requests] are left as they
  * were.  Statistics and sums are 32 bits, and products of the stored values keep 24
  * bits (less of values below 2^-110: what lies under 2^-126 of them counts as
- * zero).  At most 4096 requests. */
+ * zero).  The same call gives the same bits.  At most 4096 requests, 65535 heads and
+ * 2^30 query rows (tokens * heads).
+ * The parts of rows whose keys several workgroups share lie in a workspace of the
+ * runtime (35 MB at most).  A call inside a stream capture takes it for its graph
+ * alone, until the runtime ends, and the next call outside gets another: replays may
+ * overlap with other graphs and calls.  Where none is left (nothing as large ran since
+ * the last capture) the graph goes without: slower where there are few rows, its last
+ * bits other than an eager call's. */
 vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const vh_tensor *q, size_t heads,
                                     size_t tokens, size_t requests, const vh_index *table,
                                     size_t max_pages, const vh_index *starts, const vh_index *lens,

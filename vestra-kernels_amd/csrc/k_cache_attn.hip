@@ -618,6 +618,18 @@ __device__ __forceinline__ uint32_t weights_at(const CacheAttn &a, uint32_t x, i
     return 2u * a.shares * BM * D * 4 + (x * BM + in) * 8;
 }
 
+// Of a tile that is joined by a launch of its own, left by the workgroup of its first
+// share behind the parts: a record for each share.
+struct Joint {
+    int start, row, rows;  // of the tile
+    int head, last, part;  // its last share (-1: no tile goes on from this share), its first part
+    int unused[2];
+};
+template <int BM, int D>
+__device__ __forceinline__ Joint *joint_of(const CacheAttn &a, int w) {
+    return reinterpret_cast<Joint *>(reinterpret_cast<char *>(a.parts) + weights_at<BM, D>(a, 2 * a.shares, 0)) + w;
+}
+
 // Row `in` of a tile, four dims from d on: the result, or a workgroup's part of it.
 template <int BM, int D, bool HERE>
 struct Output {
@@ -721,7 +733,11 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
     // Steps of this workgroup, or the numbers of its tiles.
     long long at = share ? w * p.share : w;
     const long long end = share ? min(at + p.share, p.total) : (long long)p.tiles * a.cache.kv_heads;
-    if (at >= end) return;
+    int goes_on = -1;  // the last share of a tile that begins here and ends in a later one
+    const auto leave = [&](const Joint &j) {
+        if (!HERE && share && threadIdx.x == 0) *joint_of<BM, D>(a, w) = j;
+    };
+    if (at >= end) return leave(Joint{0, 0, 0, 0, -1});
     Place place = {0, 0, 0};
     if (share) place = find<BM, STEP, THREADS>(a, p, first_tile, tmp, at);
     for (bool first = true; at < end; first = false) {
@@ -735,6 +751,10 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
         const bool whole = into == 0 && steps == t.cost;
         const int from = max(into - kTileCost, 0), to = max(into + steps - kTileCost, 0);
         f(t, g, t.step0 + from, t.any.lo < t.any.hi ? to - from : 0, whole ? -1 : 2 * w + (first ? 0 : 1));
+        if (!HERE && !whole && into == 0) {
+            goes_on = uniform((int)((at + t.cost - 1) / p.share));
+            leave(Joint{t.start, t.row, t.rows, g, goes_on, 2 * w + (first ? 0 : 1)});
+        }
         if (HERE && !whole) {
             const long long begin = at - into;
             const int w0 = uniform((int)(begin / p.share)), w1 = uniform((int)((begin + t.cost - 1) / p.share));
@@ -760,6 +780,7 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
             place.head++;
         }
     }
+    if (goes_on < 0) leave(Joint{0, 0, 0, 0, -1});
 }
 
 // ---- few rows -------------------------------------------------------------------
@@ -770,6 +791,12 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
 // 6.3, 256 KB 5.4), and the registers are the same for both.  A Q8_0 value stays the
 // integer it is; its scale joins its weight, once for each block of 32 dims (few
 // weights, where the values of a step are many).
+//
+// Bound by the reads of K and V: a token each of 64 requests of 130 to 16384 keys, 32 / 8
+// heads of 128 in bf16 (846 MB), takes 144 us, 5.9 TB/s; requests of one length
+// 6.3 to 6.5 (reading alone: 6.4, past the caches 7.2).  Small calls are a chain of
+// latencies (lengths, table, K, V, parts, counter, parts): one token against 3461 keys
+// of 12 heads of 64 in floats 14.7 us.
 
 template <int KIND>
 constexpr int kFewParts = KIND == kCacheF32 ? 3 : 1;
@@ -972,6 +999,13 @@ __global__ __launch_bounds__(256, (few_workgroups<KIND, D>())) void few_rows_ker
 
 // ---- many rows --------------------------------------------------------------------
 
+// Bound by the matrix instructions and what does not hide under them (an 8-cycle issue
+// of each, the softmax and the splits on the VALU).  12 heads of 64, 3457 tokens against
+// 20742 keys in bf16 (three products of 220 GFLOP): 610 us, 1.08 PFLOP/s, where a large
+// library product in bf16 reaches 1.31; 865 against 6920 floats (six of 18): 115 us,
+// 0.96; 6 ragged causal chunks in Q8_0 with a window, 32 / 8 heads of 128 (three and six
+// of 65 in all): 360 us, 0.81.
+
 // Keys of a step.  (Wide floats, of six planes: 128 query rows of 8 heads against 65536 keys
 // 214 us, with 64 keys 230; 2000 tokens of 32 / 8 heads against 20000 3230 and 3180.)
 template <int KIND, int D>
@@ -1155,28 +1189,25 @@ __global__ __launch_bounds__(kManyThreads<D>, kManyThreads<D> == 256 ? 2 : 1) vo
 }
 
 // Joins the parts of many_rows_kernel, whose tiles would keep the last workgroup of
-// each busy for long (a frame against eight 126 us this way, 138 the other; the few
-// rows of the other kernel are joined there: one token 15.2 us against 18.2).  Every
-// border between two shares that lies inside a tile names it; the first such border's
-// workgroups join its parts, kJoinRows rows each.
-constexpr int kJoinRows = 16;
-template <int BM, int STEP, int D>
+// each busy for long (a frame against eight 115 us this way, 138 the other; the few
+// rows of the other kernel are joined there: one token 15.2 us against 18.2).  A
+// workgroup takes so few rows that each has two of its groups of lanes: the parts of a
+// row are a chain of loads (128 tokens against 4096 keys of 12 heads of 64 in floats 33.0
+// us, with twice the rows 36.7, with half 30.5, but three chunks of 900 57.2, 55.6, 61.0).
+template <int D>
+constexpr int kJoinRows = 512 / D;
+template <int BM, int D>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttn a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ long long tmp[4];
-    int *first_tile = reinterpret_cast<int *>(smem + 256 * sizeof(Sums));
-    const Partition p = partition<BM, STEP, 256>(a, first_tile, tmp, a.shares);
-    const long long border = (blockIdx.x + 1) * p.share;
-    if (border >= p.total) return;
-    const Place at = find<BM, STEP, 256>(a, p, first_tile, tmp, border);
-    const long long begin = border - at.into, before = border - p.share;
-    if (at.into == 0 || begin < before) return;  // between two tiles, or not the first
-    const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, at.tile));
-    const int w0 = blockIdx.x, w1 = uniform((int)((begin + t.cost - 1) / p.share));
-    const int from = blockIdx.y * kJoinRows;
-    if (from >= t.rows) return;
-    join_parts<BM, D, 256, false>(a, t, uniform(at.head), w0, w1, 2 * w0 + (begin > before ? 1 : 0), from,
-                                  min(from + kJoinRows, t.rows), smem);
+    __shared__ __attribute__((aligned(16))) char smem[256 * sizeof(Sums)];
+    const Joint j = *joint_of<BM, D>(a, blockIdx.x);
+    const int from = blockIdx.y * kJoinRows<D>;
+    if (j.last < 0 || from >= j.rows) return;
+    Tile t{};
+    t.start = uniform(j.start);
+    t.row = uniform(j.row);
+    t.rows = uniform(j.rows);
+    join_parts<BM, D, 256, false>(a, t, uniform(j.head), blockIdx.x, uniform(j.last), uniform(j.part), from,
+                                  min(from + kJoinRows<D>, t.rows), smem);
 }
 
 template <int KIND, int D>
@@ -1192,11 +1223,11 @@ hipError_t run_kind(hipStream_t s, const CacheAttn &a, bool few) {
     else many_rows_kernel<KIND, D><<<a.shares, kManyThreads<D>, lds + index, s>>>(a);
     e = hipGetLastError();
     if (e != hipSuccess || few || !a.parts) return e;
-    join_kernel<128, many_step<KIND, D>(), D><<<dim3(a.shares - 1, 128 / kJoinRows), 256, 256 * sizeof(Sums) + index, s>>>(a);
+    join_kernel<128, D><<<dim3(a.shares, 128 / kJoinRows<D>), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
-constexpr int kShares = 512;  // two workgroups a CU
+constexpr int kShares = 512;
 
 // Whether requests of these query rows (new tokens times the heads that share a head
 // of the cache) go to tiles of 16, by their average.  More rows read K and V once
@@ -1215,20 +1246,26 @@ bool few_rows(const CacheView &c, size_t rows, size_t requests) {
     return rows <= (c.kind == kCacheQ8 ? 64 : 32) * requests;
 }
 
+// As many workgroups as run at once: two a CU, one of eight waves (Q8_0 chunks of 32 /
+// 8 heads of 128: 368 us, with two 388) or of the LDS of wide floats.
+int shares_of(const CacheView &c, bool few) {
+    return c.width == 128 && (!few || c.kind == kCacheF32) ? kShares / 2 : kShares;
+}
+
 }  // namespace
 
 static_assert(kShares <= kAttnCounters, "a counter for each share");
 
 size_t cache_attn_floats(const CacheView &cache, size_t tokens, size_t group, size_t requests) {
-    return (size_t)2 * kShares * (few_rows(cache, tokens * group, requests) ? 16 : 128) * (cache.width + 2);
+    const bool few = few_rows(cache, tokens * group, requests);
+    const size_t shares = shares_of(cache, few);
+    return 2 * shares * (few ? 16 : 128) * (cache.width + 2) + (few ? 0 : shares * sizeof(Joint) / sizeof(float));
 }
 
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a) {
     const bool few = few_rows(a.cache, (size_t)a.tokens * a.group, (size_t)a.requests);
     const bool wide = a.cache.width == 128;
-    // As many as run at once: two a CU, one of eight waves (Q8_0 chunks of 32 / 8 heads
-    // of 128: 368 us, with two 388) or of the LDS of wide floats.
-    a.shares = wide && (!few || a.cache.kind == kCacheF32) ? kShares / 2 : kShares;
+    a.shares = shares_of(a.cache, few);
     switch (a.cache.kind) {
         case kCacheF32: return wide ? run_kind<kCacheF32, 128>(s, a, few) : run_kind<kCacheF32, 64>(s, a, few);
         case kCacheBf16: return wide ? run_kind<kCacheBf16, 128>(s, a, few) : run_kind<kCacheBf16, 64>(s, a, few);
