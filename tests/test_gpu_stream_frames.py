@@ -330,3 +330,17 @@ def test_as_many_requests_as_a_call_takes(rt, kind):
     Stream(rt, kind, [1] * n, lens, 2, 1, 64, 8).check(1)
     new = [int(3 * u) for u in seeded.uniform01(6, n)]
     Stream(rt, kind, new, [a + b for a, b in zip(lens, new)], 2, 1, 64, 8).check(1)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 70, 70]])
+def test_requests_that_share_pages(rt, kind, new):
+    """The same pages in the rows of several requests, which are only read: a prefix kept once."""
+    s = Stream(rt, kind, new, [200, 200, 200], 4, 2, 64, 16)
+    s.table[1, :8] = s.table[0, :8]
+    s.table[2] = s.table[0]
+    for kv in (s.k, s.v):
+        kv[1][:128], kv[2] = kv[0][:128], kv[0]
+    s.q[s.starts[2]:] = s.q[:new[0]]
+    got = s.check(1)
+    assert_bits_equal(got[s.starts[2]:].ravel(), got[:new[0]].ravel(), "the same request again")

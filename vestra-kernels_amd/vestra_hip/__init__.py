@@ -224,6 +224,16 @@ def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32)
 
 
+def _i32(values) -> np.ndarray:
+    """As int32; values that are none are refused, not wrapped or cut."""
+    a = np.asarray(values).reshape(-1)
+    with np.errstate(invalid="ignore"):
+        out = np.ascontiguousarray(a, np.int32)
+    if not np.array_equal(a, out):
+        raise InvalidArgument("upload_i32: values outside int32")
+    return out
+
+
 def _fp(a: np.ndarray):
     return a.ctypes.data_as(_f32p)
 
@@ -825,7 +835,7 @@ class Runtime:
 
     # -- streams of frames: positions, paged cache
     def upload_i32(self, values) -> Index:
-        a = np.ascontiguousarray(values, np.int32).reshape(-1)
+        a = _i32(values)
         out = ctypes.c_void_p()
         _check(lib().vh_upload_i32(self._h, a.ctypes.data_as(_i32p), a.size, ctypes.byref(out)))
         return Index(self, out.value)
