@@ -207,13 +207,14 @@ struct Partition {
     int tiles;
     long long units, total, share;
     long long end, cost;  // of the tile of this thread's number: steps up to its end, and its own
+    Tile mine;            // and the tile itself (TILE)
 };
 struct Place {
     int head, tile;
     long long into;  // steps of the tile before it
 };
 
-template <int BM, int STEP, int THREADS>
+template <int BM, int STEP, int THREADS, bool TILE>
 __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_tile, long long *tmp, int shares) {
     const int tid = threadIdx.x;
     Partition p;
@@ -230,7 +231,12 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
     if (tid == 0) first_tile[a.requests] = (int)min(base, 1ll << 30);
     __syncthreads();
     p.tiles = first_tile[a.requests];
-    p.cost = tid < p.tiles ? tile_of<BM, STEP>(a, first_tile, tid).cost : 0;
+    if constexpr (TILE) {
+        p.mine = tid < p.tiles ? tile_of<BM, STEP>(a, first_tile, tid) : Tile{};
+        p.cost = p.mine.cost;
+    } else {
+        p.cost = tid < p.tiles ? tile_of<BM, STEP>(a, first_tile, tid).cost : 0;
+    }
     p.end = scan_all<THREADS>(p.cost, tmp, &p.units);
     for (int t0 = THREADS; t0 < p.tiles; t0 += THREADS) {
         const int ti = t0 + tid;
@@ -252,9 +258,10 @@ __device__ __forceinline__ long long first_units(const Partition &p, long long *
     return n;
 }
 
-template <int BM, int STEP, int THREADS>
+// The tile itself is left in `found_tile`, if that is asked for (TILE).
+template <int BM, int STEP, int THREADS, bool TILE>
 __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, const int *first_tile, long long *tmp,
-                                      long long unit) {
+                                      long long unit, Tile *found_tile) {
     __shared__ long long found[2];
     Place at;
     at.head = (int)(unit / p.units);
@@ -264,6 +271,7 @@ __device__ __forceinline__ Place find(const CacheAttn &a, const Partition &p, co
         if (end - cost <= x && x < end) {
             found[0] = t0 + (int)threadIdx.x;
             found[1] = end - cost;
+            if constexpr (TILE) *found_tile = t0 ? tile_of<BM, STEP>(a, first_tile, (int)found[0]) : p.mine;
         }
         t0 += THREADS;
         if (t0 >= p.tiles) break;
@@ -727,7 +735,7 @@ template <int BM, int STEP, int THREADS, int D, bool HERE, class F>
 __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *smem, F f) {
     __shared__ long long tmp[THREADS / 64];
     __shared__ int is_last;
-    const Partition p = partition<BM, STEP, THREADS>(a, first_tile, tmp, a.shares);
+    const Partition p = partition<BM, STEP, THREADS, HERE>(a, first_tile, tmp, a.shares);
     const int w = my_share(a);
     const bool share = a.parts != nullptr;
     // Steps of this workgroup, or the numbers of its tiles.
@@ -739,13 +747,16 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
     };
     if (at >= end) return leave(Joint{0, 0, 0, 0, -1});
     Place place = {0, 0, 0};
-    if (share) place = find<BM, STEP, THREADS>(a, p, first_tile, tmp, at);
+    __shared__ Tile found_tile;
+    if (share) place = find<BM, STEP, THREADS, HERE>(a, p, first_tile, tmp, at, &found_tile);
     for (bool first = true; at < end; first = false) {
         if (!share) {
             place.head = (int)(at / p.tiles);
             place.tile = (int)(at - (long long)place.head * p.tiles);
         }
-        const Tile t = uniform(tile_of<BM, STEP>(a, first_tile, place.tile));
+        // Few rows: the first tile as it was found (one token against 3461 keys 14.4 us,
+        // formed again 14.6; many rows have no registers for it).
+        const Tile t = uniform(HERE && share && first ? found_tile : tile_of<BM, STEP>(a, first_tile, place.tile));
         const int into = uniform((int)place.into), g = uniform(place.head);
         const int steps = share ? uniform((int)min(end - at, (long long)t.cost - into)) : t.cost;
         const bool whole = into == 0 && steps == t.cost;
@@ -796,7 +807,7 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
 // heads of 128 in bf16 (846 MB), takes 144 us, 5.9 TB/s; requests of one length
 // 6.3 to 6.5 (reading alone: 6.4, past the caches 7.2).  Small calls are a chain of
 // latencies (lengths, table, K, V, parts, counter, parts): one token against 3461 keys
-// of 12 heads of 64 in floats 14.7 us.
+// of 12 heads of 64 in floats 14.4 us.
 
 template <int KIND>
 constexpr int kFewParts = KIND == kCacheF32 ? 3 : 1;
