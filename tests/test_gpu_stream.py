@@ -207,6 +207,47 @@ def test_append_qkv_equals_its_parts(rt, kind, tokens, heads, kvh, hd, pairs, sh
     assert_bits_equal(rt.download_f32(a.got[1]) + 0.0, exp.ravel() + 0.0, "v against numpy")
 
 
+def _tiled(rt, n, piece):
+    """n floats on the device that repeat `piece`."""
+    t, p = rt.alloc_f32(n), rt.upload_f32(piece)
+    for at in range(0, n, piece.size):
+        rt.copy_segment_into_f32(t, at, p, 0, min(piece.size, n - at))
+    return t
+
+
+def test_rows_past_4_gib(rt):
+    """Tensors whose bytes pass 2^32: the last tokens of a rotation in place, and of an append from QKV rows."""
+    hd, tokens, tail = 64, (1 << 24) + 35, 700
+    rope = rt.prepare_rope_axes(hd, [30], 10000.0, shared=True)
+    piece = seeded.normal(21, (1 << 20) * hd)
+    x = _tiled(rt, tokens * hd, piece)
+    pos = np.arange(tokens) % 5000
+    rope.run(x, 1, tokens, rt.upload_i32(pos), x)
+    rows = np.arange(tokens - tail, tokens)
+    src = piece.reshape(-1, 1, hd)[rows % (1 << 20)]
+    exp = ref.rotate(src, pos[rows, None], [30], 10000.0, True)
+    got = rt.download_f32(rt.copy_segment_f32(x, (tokens - tail) * hd, tail * hd)).reshape(exp.shape)
+    assert (np.abs(got - exp) <= ROPE_TOL * 2 * np.abs(src).max(-1, keepdims=True)).all()
+    del x
+
+    heads, kvh, tokens = 12, 2, (1 << 20) + 35
+    width = (heads + 2 * kvh) * hd
+    piece = seeded.normal(22, (1 << 15) * width)
+    qkv, q = _tiled(rt, tokens * width, piece), rt.alloc_f32(tokens * heads * hd)
+    cache = rt.kv_cache("f32", 8, 128, kvh, hd)
+    slots = np.full(tokens, -1)
+    slots[-tail:] = _slots(3, tail, 1024)
+    cache.append_qkv(qkv, heads, tokens, rt.upload_i32(slots), q)
+    rows = np.arange(tokens - tail, tokens)
+    exp = piece.reshape(-1, heads + 2 * kvh, hd)[rows % (1 << 15)]
+    got = rt.download_f32(rt.copy_segment_f32(q, (tokens - tail) * heads * hd, tail * heads * hd))
+    assert_bits_equal(got, exp[:, :heads].ravel(), "q")
+    k, v = rt.alloc_f32(tail * kvh * hd), rt.alloc_f32(tail * kvh * hd)
+    cache.gather(rt.upload_i32(slots[-tail:]), tail, k, v)
+    assert_bits_equal(rt.download_f32(k), exp[:, heads:heads + kvh].ravel(), "k")
+    assert_bits_equal(rt.download_f32(v), exp[:, heads + kvh:].ravel(), "v")
+
+
 # ---- page tables ---------------------------------------------------------------------
 
 

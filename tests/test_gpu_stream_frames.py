@@ -11,7 +11,7 @@ import stream64 as ref
 import vestra_hip as vh
 from conftest import assert_bits_equal
 from test_gpu_graph import _capture, _hip
-from test_gpu_stream import ROPE_TOL
+from test_gpu_stream import ROPE_TOL, _tiled
 from test_gpu_stream_attention import KINDS, Stream, close
 from vestra_hip import da3, seeded
 
@@ -344,3 +344,18 @@ def test_requests_that_share_pages(rt, kind, new):
     s.q[s.starts[2]:] = s.q[:new[0]]
     got = s.check(1)
     assert_bits_equal(got[s.starts[2]:].ravel(), got[:new[0]].ravel(), "the same request again")
+
+
+def test_queries_past_4_gib(rt):
+    """Queries and outputs whose bytes pass 2^32, against few keys: the last tokens."""
+    heads, kvh, hd, tokens, tail, n = 2, 1, 64, (1 << 23) + 50, 500, 10
+    piece = seeded.normal(31, (1 << 16) * heads * hd)
+    q, out = _tiled(rt, tokens * heads * hd, piece), rt.alloc_f32(tokens * heads * hd)
+    cache = rt.kv_cache("f32", 1, 16, kvh, hd)
+    k, v = (seeded.normal(s, n * hd).reshape(n, 1, hd) for s in (32, 33))
+    cache.append(rt.upload_f32(k), rt.upload_f32(v), n, rt.upload_i32(np.arange(n)), token_major=True)
+    cache.attention(q, heads, tokens, rt.upload_i32([0]), 1, rt.upload_i32([0, tokens]), rt.upload_i32([n]), out)
+    got = rt.download_f32(rt.copy_segment_f32(out, (tokens - tail) * heads * hd, tail * heads * hd))
+    last = piece.reshape(-1, heads, hd)[np.arange(tokens - tail, tokens) % (1 << 16)]
+    args = (last, [k], [v], [0, tail], [n], heads)
+    close(got.reshape(last.shape), ref.attention(*args), ref.attention(*args, dtype=np.float32))

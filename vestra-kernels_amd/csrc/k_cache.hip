@@ -367,6 +367,8 @@ hipError_t launch_cache_rows(hipStream_t s, CacheRows a) {
     // spread as well (865 tokens of 48 heads of 128: 10.4 us against 11.2).
     const int per = 256 / a.head_dim, groups = (a.heads + 2 * a.kv_heads + per - 1) / per;
     a.per_group = std::min((16 + groups - 1) / groups, std::max(1, a.tokens / 2048));
+    // (No more workgroups than a launch has threads for; 16 tokens then, at 2^27.)
+    a.per_group = std::max(a.per_group, (a.tokens + (1 << 23) - 1) >> 23);
     const dim3 grid((unsigned)((a.tokens + a.per_group - 1) / a.per_group),
                     a.tokens < 2048 ? (groups + 4 * kU - 1) / (4 * kU) : 1);
     const size_t lds = (size_t)a.per_group * a.rope.pairs * 2 * sizeof(float);
