@@ -503,7 +503,8 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  * an unseen key or value holds (infinities and NaN too).  A query that sees no key
  * gets zeros; one that sees an infinity or NaN in a value has no finite number in
  * that dim, in a key no defined row.  Rows behind starts[requests] are left as they
- * were.  Statistics and sums are 32 bits, and products of the stored values keep 24
+ * were; a request whose starts fall has none, and rows that two requests name hold
+ * what either gives.  Statistics and sums are 32 bits, and products of the stored values keep 24
  * bits (less of values below 2^-110: what lies under 2^-126 of them counts as
  * zero).  The same call gives the same bits.  At most 4096 requests, 65535 heads and
  * 2^30 query rows (tokens * heads).

@@ -359,3 +359,19 @@ def test_queries_past_4_gib(rt):
     last = piece.reshape(-1, heads, hd)[np.arange(tokens - tail, tokens) % (1 << 16)]
     args = (last, [k], [v], [0, tail], [n], heads)
     close(got.reshape(last.shape), ref.attention(*args), ref.attention(*args, dtype=np.float32))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [100, 90]])
+def test_starts_that_fall_cost_no_more_than_a_batch(rt, new):
+    """Starts that name every token for every second request: the call takes no longer than its batch allows, writes
+    nothing behind the batch, and the runtime's next call is as ever."""
+    s = Stream(rt, "bf16", new, [300, 500], 4, 2, 64, 16)
+    good = s.run(1)
+    n, t = 3000, s.tokens
+    starts = np.tile([0, t], n // 2 + 1)[:n + 1]
+    table, lens = np.tile(s.table[:1], (n, 1)), np.full(n, 300)
+    out = rt.upload_f32(np.full(s.q.size, 5.0))
+    s.cache.attention(rt.upload_f32(s.q), 4, t, rt.upload_i32(table), s.width, rt.upload_i32(starts),
+                      rt.upload_i32(lens), out, block=1)
+    assert rt.download_f32(out).shape == (s.q.size,)
+    assert_bits_equal(s.run(1).ravel(), good.ravel(), "the next call")

@@ -219,16 +219,18 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
     const int tid = threadIdx.x;
     Partition p;
     long long all = 0, base = 0;
+    // Falling starts would name tokens several times: tiles past what a batch of so many
+    // tokens and requests can have are left out.
+    const long long most = (long long)a.tokens * a.group / BM + a.requests;
     for (int r0 = 0; r0 < a.requests; r0 += THREADS) {
         const int r = r0 + tid;
         const long long n = r < a.requests ? max(start_of(a, r + 1) - start_of(a, r), 0) : 0;
         const long long tiles = (n * a.group + BM - 1) / BM;
         const long long end = base + scan_all<THREADS>(tiles, tmp, &all);
         base += all;
-        // Falling starts may name a token several times: tiles past 2^30 are left out.
-        if (r < a.requests) first_tile[r] = (int)min(end - tiles, 1ll << 30);
+        if (r < a.requests) first_tile[r] = (int)min(end - tiles, most);
     }
-    if (tid == 0) first_tile[a.requests] = (int)min(base, 1ll << 30);
+    if (tid == 0) first_tile[a.requests] = (int)min(base, most);
     __syncthreads();
     p.tiles = first_tile[a.requests];
     if constexpr (TILE) {
