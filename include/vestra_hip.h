@@ -499,7 +499,8 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  *        block): block = 1 is causal, block = the tokens of a frame lets a frame see
  *        itself and the earlier ones;
  *   lo = max(0, hi - window), or 0 for window = 0.
- * Keys in a page that is -1 or none of the cache's are not seen, nor is anything that
+ * Keys past the max_pages * page_tokens that a row of the table holds (lens may count
+ * them), or in a page that is -1 or none of the cache's, are not seen, nor is anything that
  * an unseen key or value holds (infinities and NaN too).  A query that sees no key
  * gets zeros; one that sees an infinity or NaN in a value has no finite number in
  * that dim, in a key no defined row.  Rows behind starts[requests] are left as they

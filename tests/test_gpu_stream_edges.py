@@ -1,0 +1,72 @@
+"""The operators of a stream at their edges, where a call is legal and its values unusual: against float64 numpy
+(tests/stream64.py)."""
+import numpy as np
+import pytest
+
+import stream64 as ref
+import vestra_hip as vh
+from conftest import assert_bits_equal
+from test_gpu_stream_attention import KINDS, Stream, close
+from vestra_hip import seeded
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- requests that outgrow their row of the table ------------------------------------
+
+
+def _cut(s, columns):
+    """The table's first columns; which keys lie behind them."""
+    s.width, s.table = columns, np.ascontiguousarray(s.table[:, :columns])
+    return [np.arange(n) >= columns * s.page for n in s.lens]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new, lens, columns, heads, kvh, hd", [
+    ([4, 1, 2], [50, 49, 20], 3, 4, 2, 64), ([10, 1], [70, 300], 4, 2, 2, 128),
+    ([200, 90], [260, 100], 12, 4, 2, 64), ([150, 140], [700, 300], 20, 4, 1, 128)])
+@pytest.mark.parametrize("block, window", [(1, 0), (50, 0), (1, 20), (0, 30), (16, 100)])
+def test_a_request_past_its_row_keeps_its_positions(rt, kind, new, lens, columns, heads, kvh, hd, block, window):
+    """Positions, blocks and windows follow from lens; only the keys that the row cannot hold are missing."""
+    s = Stream(rt, kind, new, lens, heads, kvh, hd, 16, spare_rows=1)
+    s.check(block, window, absent=_cut(s, columns))
+
+
+@pytest.mark.parametrize("new", [3, 300])
+def test_the_longest_length_of_a_short_row(rt, new):
+    """A length of 2^31 - 1 over a row of 64 tokens: every key for a late position, none in a window at its end."""
+    s = Stream(rt, "f32", [new], [64], 2, 1, 64, 16)
+    _cut(s, 4)
+    exp = s.run(0)
+    s.lens = np.array([2**31 - 1])
+    for block in (0, 1, 865, 2**31, 2**40):
+        assert_bits_equal(s.run(block).ravel(), exp.ravel(), f"block {block}")
+    for block in (0, 1, 865):
+        assert (s.run(block, window=1000) == 0).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("block", [1, 10])
+def test_a_step_past_the_row_of_a_table(rt, kind, block):
+    """Tables, appends and attention of a step whose first request outgrows its row of 64 tokens and whose second does
+    not: the tokens that found a place see themselves."""
+    heads, kvh, hd, page, width, had, new = 4, 2, 64, 16, 4, [60, 5], [10, 3]
+    cache = rt.kv_cache(kind, 12, page, kvh, hd)
+    table = rt.upload_i32(np.full(2 * width, -1))
+    free, cached, start = rt.upload_i32([7, 3, 9, 0, 11, 5, 2]), rt.upload_i32([0, 0]), rt.upload_i32([0])
+    ks, vs = ([seeded.normal(s + r, (a + b) * kvh * hd).reshape(-1, kvh, hd) for r, (a, b) in enumerate(zip(had, new))]
+              for s in (1, 11))
+    q = seeded.normal(5, sum(new) * heads * hd).reshape(-1, heads, hd)
+    for step, n in enumerate((had, new)):
+        starts, lens, slots, nxt = rt.alloc_i32(3), rt.alloc_i32(2), rt.alloc_i32(sum(n)), rt.alloc_i32(1)
+        rt.kv_pages_assign(cached, rt.upload_i32(n), free, start, page, table, width, starts, lens, slots, nxt)
+        rows = [np.concatenate([x[a * step:a * step + b] for x, a, b in zip(xs, had, n)]) for xs in (ks, vs)]
+        cache.append(rt.upload_f32(rows[0]), rt.upload_f32(rows[1]), sum(n), slots, token_major=True)
+        cached, start = lens, nxt
+    assert list(rt.download_i32(slots)[:10] >= 0) == [True] * 4 + [False] * 6
+    out = rt.alloc_f32(q.size)
+    cache.attention(rt.upload_f32(q), heads, sum(new), table, width, starts, lens, out, block=block)
+    lens = rt.download_i32(lens)
+    args = (q, [ref.stored(k, kind) for k in ks], [ref.stored(v, kind) for v in vs], rt.download_i32(starts), lens,
+            heads, block, 0, [np.arange(n) >= width * page for n in lens])
+    close(rt.download_f32(out).reshape(q.shape), ref.attention(*args), ref.attention(*args, dtype=np.float32))

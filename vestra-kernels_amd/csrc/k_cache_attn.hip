@@ -139,7 +139,8 @@ __device__ __forceinline__ bool finite8(f32x4 a, f32x4 b) {
 
 // ---- the partition ----------------------------------------------------------------
 
-// Keys [lo, hi) that a query at position pos of a request of len tokens sees.
+// Keys [lo, hi) that a query at position pos of a request of len tokens sees: of those that
+// its row of the table holds, however long the request is.
 struct Seen {
     int lo, hi;
 };
@@ -147,7 +148,7 @@ __device__ __forceinline__ Seen keys_seen(const CacheAttn &a, int len, int pos) 
     long long hi = len;
     if (a.block) hi = pos < 0 ? 0 : min(hi, ((long long)((unsigned)pos / a.block) + 1) * a.block);
     const long long lo = a.window ? max(0ll, hi - a.window) : 0;
-    return {(int)lo, (int)hi};
+    return {min((int)lo, a.row_keys), min((int)hi, a.row_keys)};
 }
 
 struct Tile {
@@ -176,10 +177,7 @@ __device__ __forceinline__ Tile tile_of(const CacheAttn &a, const int *first_til
     t.r = lo;
     t.start = start_of(a, lo);
     const int n = start_of(a, lo + 1) - t.start;
-    // A length that the table's row cannot hold ends with the row, and lengths end
-    // where a step past them still counts in 31 bits.
-    t.len = (int)min((long long)max(a.lens[lo], 0),
-                     min(a.max_pages << a.cache.page_shift, (long long)INT32_MAX - 4095));
+    t.len = max(a.lens[lo], 0);
     t.pos = t.len - n;
     t.row = (ti - first_tile[lo]) * BM;
     t.rows = min(BM, n * a.group - t.row);
@@ -1279,6 +1277,8 @@ hipError_t launch_cache_attn(hipStream_t s, CacheAttn a) {
     const bool few = few_rows(a.cache, (size_t)a.tokens * a.group, (size_t)a.requests);
     const bool wide = a.cache.width == 128;
     a.shares = shares_of(a.cache, few);
+    // What a row of the table holds, short of where a step past it no longer counts in 31 bits.
+    a.row_keys = (int)std::min(a.max_pages << a.cache.page_shift, (long long)INT32_MAX - 4095);
     switch (a.cache.kind) {
         case kCacheF32: return wide ? run_kind<kCacheF32, 128>(s, a, few) : run_kind<kCacheF32, 64>(s, a, few);
         case kCacheBf16: return wide ? run_kind<kCacheBf16, 128>(s, a, few) : run_kind<kCacheBf16, 64>(s, a, few);

@@ -384,7 +384,7 @@ struct CacheAttn {
     // time.
     float *parts;
     unsigned *counters;
-    int shares;  // set by the launcher
+    int shares, row_keys;  // set by the launcher
 };
 constexpr size_t kAttnCounters = 1024;
 size_t cache_attn_floats(const CacheView &cache, size_t tokens, size_t group, size_t requests);
