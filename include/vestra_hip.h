@@ -500,15 +500,16 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  *        itself and the earlier ones;
  *   lo = max(0, hi - window), or 0 for window = 0.
  * Keys past the max_pages * page_tokens that a row of the table holds (lens may count
- * them), or in a page that is -1 or none of the cache's, are not seen, nor is anything that
- * an unseen key or value holds (infinities and NaN too).  A query that sees no key
- * gets zeros; one that sees an infinity or NaN in a value has no finite number in
- * that dim, in a key no defined row.  Rows behind starts[requests] are left as they
- * were; a request whose starts fall has none, and rows that two requests name hold
- * what either gives.  Statistics and sums are 32 bits, and products of the stored values keep 24
- * bits (less of values below 2^-110: what lies under 2^-126 of them counts as
- * zero).  The same call gives the same bits.  At most 4096 requests, 65535 heads and
- * 2^30 query rows (tokens * heads).
+ * them), or in a page that is -1 or none of the cache's, are not seen, nor is anything
+ * that an unseen key or value holds (infinities and NaN too).  A query that sees no key
+ * gets zeros; one that sees an infinity or NaN in a value has no finite number in that
+ * dim, in a key no defined row.  Rows before starts[0] and behind the last request are
+ * left as they were.  A start below an earlier one counts as the highest before it, so
+ * that a row is one request's; its position follows from the rows up to its request's
+ * end.  Statistics and sums are 32 bits, and products of the stored values keep 24 bits
+ * (less of values below 2^-110: what lies under 2^-126 of them counts as zero).  The same
+ * call gives the same bits.  At most 4096 requests, 65535 heads and 2^30 query rows
+ * (tokens * heads).
  * The parts of rows whose keys several workgroups share lie in a workspace of the
  * runtime (35 MB at most).  A call inside a stream capture takes it for its graph
  * alone, until the runtime ends, and the next call outside gets another: replays may

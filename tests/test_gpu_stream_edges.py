@@ -70,3 +70,39 @@ def test_a_step_past_the_row_of_a_table(rt, kind, block):
     args = (q, [ref.stored(k, kind) for k in ks], [ref.stored(v, kind) for v in vs], rt.download_i32(starts), lens,
             heads, block, 0, [np.arange(n) >= width * page for n in lens])
     close(rt.download_f32(out).reshape(q.shape), ref.attention(*args), ref.attention(*args, dtype=np.float32))
+
+
+# ---- starts that fall ---------------------------------------------------------------
+
+
+def _walk_of_starts(case, requests, tokens):
+    u = seeded.uniform01(requests + tokens, requests + 1)
+    if case == "up and down":
+        return (u * (tokens + 1)).astype(int)
+    if case == "all of it again":
+        return np.tile([0, tokens], requests)[:requests + 1]
+    # Rising, with a fall in one place of every hundred.
+    rise = np.linspace(0, tokens, requests + 1).astype(int)
+    return np.where(u < 0.01, (rise * u * 100).astype(int), rise)
+
+
+@pytest.mark.parametrize("kind, heads, kvh", [("f32", 2, 2), ("bf16", 8, 1), ("q8_0", 4, 2)])
+@pytest.mark.parametrize("case, requests, tokens", [
+    ([50, 100, 50, 100, 50, 100, 0, 50], 7, 100), ([0, 90, 0, 90, 0, 100], 5, 100), ([0, 400, 100, 390, 200, 900], 5, 900),
+    ([-7, 3, 2**31 - 1, -2**31, 50], 4, 60), ([60, 40, 20, 0], 3, 60), ("up and down", 40, 700),
+    ("all of it again", 301, 64), ("rising", 600, 700), ("rising", 1200, 9000)])
+def test_a_start_that_falls_counts_as_the_highest_before_it(rt, kind, heads, kvh, case, requests, tokens):
+    """Each row is one request's, or none's: of the rows that two requests name the first one's, at the position that
+    its distance from the request's end gives; rows before the first start and behind the last stay as they were."""
+    starts = np.array(case) if isinstance(case, list) else _walk_of_starts(case, requests, tokens)
+    lens = [20 + int(60 * u) for u in seeded.uniform01(requests, requests)]
+    s = Stream(rt, kind, [0] * requests, lens, heads, kvh, 64, 16, spare_rows=tokens)
+    s.starts = starts
+    high = np.maximum.accumulate(np.clip(starts, 0, tokens))
+    for block, window in ((1, 0), (0, 17)):
+        got = s.run(block, window, fill=7.0)
+        args = (s.q, s.k, s.v, high, s.lens, heads, block, window)
+        lo, hi = high[0], high[-1]
+        close(got[lo:hi], ref.attention(*args)[lo:hi], ref.attention(*args, dtype=np.float32)[lo:hi])
+        assert (got[:lo] == 7.0).all() and (got[hi:] == 7.0).all()
+        assert_bits_equal(s.run(block, window, fill=7.0).ravel(), got.ravel(), "again")

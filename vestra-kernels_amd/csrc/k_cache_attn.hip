@@ -164,22 +164,34 @@ struct Tile {
 constexpr int kTileCost = 2;
 
 __device__ __forceinline__ int start_of(const CacheAttn &a, int r) { return min(max(a.starts[r], 0), a.tokens); }
+// The highest of the starts up to r, which is where request r begins: a row is one request's,
+// whatever the starts, and the tiles are no more than a batch of so many tokens and requests has.
+__device__ int highest_start(const CacheAttn &a, int r) {
+    int h = 0;
+#pragma unroll 1
+    for (int i = 0; i <= r; i++) h = max(h, start_of(a, i));
+    return h;
+}
+// In first_tile: the request's own start is not that one.  (Tiles stay below 2^26 + 2^12.)
+constexpr int kFell = 1 << 30;
 
 template <int BM, int STEP>
 __device__ __forceinline__ Tile tile_of(const CacheAttn &a, const int *first_tile, int ti) {
     int lo = 0, hi = a.requests;  // first_tile[lo] <= ti < first_tile[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (first_tile[mid] <= ti) lo = mid;
+        if ((first_tile[mid] & ~kFell) <= ti) lo = mid;
         else hi = mid;
     }
     Tile t;
     t.r = lo;
+    const int first = first_tile[lo];
     t.start = start_of(a, lo);
+    if (__builtin_expect(first & kFell, 0)) t.start = highest_start(a, lo);
     const int n = start_of(a, lo + 1) - t.start;
     t.len = max(a.lens[lo], 0);
     t.pos = t.len - n;
-    t.row = (ti - first_tile[lo]) * BM;
+    t.row = (ti - (first & ~kFell)) * BM;
     t.rows = min(BM, n * a.group - t.row);
     const Seen s0 = keys_seen(a, t.len, t.pos + t.row / a.group);
     const Seen s1 = keys_seen(a, t.len, t.pos + (t.row + t.rows - 1) / a.group);
@@ -217,18 +229,27 @@ __device__ __forceinline__ Partition partition(const CacheAttn &a, int *first_ti
     const int tid = threadIdx.x;
     Partition p;
     long long all = 0, base = 0;
-    // Falling starts would name tokens several times: tiles past what a batch of so many
-    // tokens and requests can have are left out.
-    const long long most = (long long)a.tokens * a.group / BM + a.requests;
+    long long falls = 0;  // so far
     for (int r0 = 0; r0 < a.requests; r0 += THREADS) {
         const int r = r0 + tid;
-        const long long n = r < a.requests ? max(start_of(a, r + 1) - start_of(a, r), 0) : 0;
-        const long long tiles = (n * a.group + BM - 1) / BM;
-        const long long end = base + scan_all<THREADS>(tiles, tmp, &all);
+        const bool there = r < a.requests;
+        const int own = there ? start_of(a, r) : 0;
+        int start = own, next = there ? start_of(a, r + 1) : 0;
+        const long long fell = next < start;
+        auto tiles_of = [&] { return ((long long)max(next - start, 0) * a.group + BM - 1) / BM; };
+        long long tiles = tiles_of();
+        // Falls are counted above the tiles.
+        long long end = base + scan_all<THREADS>(tiles + (fell << 48), tmp, &all);
+        falls += all >> 48;
+        if (__builtin_expect(falls != 0, 0)) {
+            start = there ? highest_start(a, r) : 0;
+            tiles = tiles_of();
+            end = base + scan_all<THREADS>(tiles, tmp, &all);
+        }
         base += all;
-        if (r < a.requests) first_tile[r] = (int)min(end - tiles, most);
+        if (there) first_tile[r] = (int)(end - tiles) | (start != own ? kFell : 0);
     }
-    if (tid == 0) first_tile[a.requests] = (int)min(base, most);
+    if (tid == 0) first_tile[a.requests] = (int)base;
     __syncthreads();
     p.tiles = first_tile[a.requests];
     if constexpr (TILE) {
