@@ -507,8 +507,10 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  * left as they were.  A start below an earlier one counts as the highest before it, so
  * that a row is one request's; its position follows from the rows up to its request's
  * end.  Statistics and sums are 32 bits, and products of the stored values keep 24 bits
- * (less of values below 2^-110: what lies under 2^-126 of them counts as zero).  The same
- * call gives the same bits.  At most 4096 requests, 65535 heads and 2^30 query rows
+ * (less of values below 2^-110: what lies under 2^-126 of them counts as zero).  Weights
+ * are up to 2^8 before they are divided by their sum, so n keys' values below 2^120 / n
+ * give finite rows; larger ones may pass the floats on the way.  The same call gives the
+ * same bits.  At most 4096 requests, 65535 heads and 2^30 query rows
  * (tokens * heads).
  * The parts of rows whose keys several workgroups share lie in a workspace of the
  * runtime (35 MB at most).  A call inside a stream capture takes it for its graph

@@ -106,3 +106,44 @@ def test_a_start_that_falls_counts_as_the_highest_before_it(rt, kind, heads, kvh
         close(got[lo:hi], ref.attention(*args)[lo:hi], ref.attention(*args, dtype=np.float32)[lo:hi])
         assert (got[:lo] == 7.0).all() and (got[hi:] == 7.0).all()
         assert_bits_equal(s.run(block, window, fill=7.0).ravel(), got.ravel(), "again")
+
+
+# ---- values near the largest ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("requests, new, heads, hd", [(128, 1, 8, 64), (128, 1, 8, 128), (32, 40, 16, 64),
+                                                      (32, 40, 16, 128)])
+@pytest.mark.parametrize("rise", [7.9, 8.1])
+def test_large_values_of_a_score_that_rises_late(rt, kind, requests, new, heads, hd, rise):
+    """Flat scores and, steps later, one key whose score passes them by about 8 (base 2), all values at the size up to
+    which rows are finite.  Enough tiles that a workgroup has several steps of each."""
+    n = 300
+    size = 2.0 ** 120 / n
+
+    def change(r, k, v):
+        k[:] = 0
+        k[280, :, 0] = rise * np.log(2.0) * np.sqrt(hd)
+        v[:] = np.clip(v, -1, 1) * np.float32(size) * np.float32(0.99)  # (of what bf16 makes of it)
+        v[280] = np.float32(size * 0.99)
+
+    s = Stream(rt, kind, [new] * requests, [n] * requests, heads, heads, hd, 16, change=change)
+    s.q[:] = 0
+    s.q[..., 0] = 1
+    got = s.run(0)
+    args = (s.q, s.k, s.v, s.starts, s.lens, heads)
+    exp, plain = ref.attention(*args), ref.attention(*args, dtype=np.float32)
+    assert np.isfinite(plain).all()
+    close(got, exp, plain)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 200])
+@pytest.mark.parametrize("exponent", [-100, -110, -118, -126])
+def test_small_values_keep_what_they_have(rt, kind, new, exponent):
+    """Values near the smallest: off by no more than the parts below 2^-126 that count as zero."""
+
+    def change(r, k, v):
+        v *= np.float32(2.0) ** np.float32(exponent)
+
+    Stream(rt, kind, [new], [333], 4, 2, 64, 16, change=change).check(1)

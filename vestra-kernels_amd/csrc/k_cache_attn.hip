@@ -37,7 +37,12 @@
 namespace vh {
 namespace {
 
-constexpr float kMaxSlack = 8.0f;  // scores may pass the running maximum by this (base 2)
+// Scores may pass the running maximum by this (base 2).  Weights then reach 2^8, and n weighted
+// values of a row sum to a finite number below 2^120 / n.  (Eight taken off every exponent, so that
+// weights end at one, costs an instruction a score: a 3457-token frame against 20742 keys in
+// bf16 634 us against 619.  Taken off the maximum instead, one key's value no longer returns as
+// it is.)
+constexpr float kMaxSlack = 8.0f;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
