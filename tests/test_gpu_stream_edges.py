@@ -147,3 +147,17 @@ def test_small_values_keep_what_they_have(rt, kind, new, exponent):
         v *= np.float32(2.0) ** np.float32(exponent)
 
     Stream(rt, kind, [new], [333], 4, 2, 64, 16, change=change).check(1)
+
+
+# ---- limits -------------------------------------------------------------------------------
+
+
+def test_calls_of_more_than_2_27_tokens_are_refused(rt):
+    n = (1 << 27) + 1
+    cache, slots = rt.kv_cache("bf16", 1, 16, 1, 4), rt.alloc_i32(n)
+    k, v = rt.alloc_f32(4 * n), rt.alloc_f32(4 * n)
+    rope = rt.prepare_rope_axes(4, [1], 100.0)
+    for call in (lambda: cache.gather(slots, n, k, v), lambda: cache.append(k, v, n, slots),
+                 lambda: rope.run(k, 1, n, slots, v)):
+        with pytest.raises(vh.KernelError, match="2\\^27 tokens"):
+            call()

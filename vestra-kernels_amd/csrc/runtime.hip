@@ -3591,6 +3591,7 @@ extern "C" vh_status vh_kv_cache_gather_f32(const vh_kv_cache *cache, const vh_i
     if (mul_overflows(tokens, kvh * hd, &expected) || k->len != expected) return mismatch(k->len, expected, what);
     if (v->len != expected) return mismatch(v->len, expected, what);
     if (slots->len < tokens) return mismatch(slots->len, tokens, what);
+    if (tokens > kMaxCacheTokens) return fail(VH_ERR_KERNEL, "kv cache: more than 2^27 tokens");
     if (k->rt != cache->rt || v->rt != cache->rt || slots->rt != cache->rt) return other_runtime(what);
     if (k == v) return aliased(what);
     GUARD_BEGIN
