@@ -161,3 +161,11 @@ def test_calls_of_more_than_2_27_tokens_are_refused(rt):
                  lambda: rope.run(k, 1, n, slots, v)):
         with pytest.raises(vh.KernelError, match="2\\^27 tokens"):
             call()
+
+
+def test_page_tables_say_how_many_tokens_they_take(rt):
+    """2^31 - 1025 tokens; one more is refused, with that number."""
+    one, two, slots = rt.upload_i32([0]), rt.alloc_i32(2), rt.alloc_i32(2**31 - 1024)
+    with pytest.raises(vh.KernelError, match="2\\^31 - 1025 tokens"):
+        rt.kv_pages_assign(one, rt.upload_i32([1]), rt.upload_i32([0]), rt.upload_i32([0]), 16, rt.alloc_i32(4), 4, two,
+                           rt.alloc_i32(1), slots, rt.alloc_i32(1))

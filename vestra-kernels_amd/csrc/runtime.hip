@@ -3630,7 +3630,8 @@ extern "C" vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *ca
     if (free_start->len != 1) return mismatch(free_start->len, 1, what);
     if (free_next->len != 1) return mismatch(free_next->len, 1, what);
     if (tokens > (size_t)INT32_MAX - 1024 || free_pages->len > INT32_MAX)
-        return fail(VH_ERR_KERNEL, "kv pages: tokens or free pages exceed 2^31-1");
+        return fail(VH_ERR_KERNEL, "kv pages: at most 2^31 - 1025 tokens and 2^31 - 1 free pages, got " +
+                                       std::to_string(tokens) + " and " + std::to_string(free_pages->len));
     for (const vh_index *p : in)
         if (p->rt != rt->s) return other_runtime(what);
     for (size_t i = 0; i < 5; i++) {
