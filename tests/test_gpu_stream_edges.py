@@ -169,3 +169,23 @@ def test_page_tables_say_how_many_tokens_they_take(rt):
     with pytest.raises(vh.KernelError, match="2\\^31 - 1025 tokens"):
         rt.kv_pages_assign(one, rt.upload_i32([1]), rt.upload_i32([0]), rt.upload_i32([0]), 16, rt.alloc_i32(4), 4, two,
                            rt.alloc_i32(1), slots, rt.alloc_i32(1))
+
+
+# ---- appends that pass by the caches ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("token_major", [False, True])
+def test_appends_past_the_caches_are_exact(rt, kind, token_major):
+    tokens, kvh, hd, page = 16501, 24, 64, 32  # 203 MB
+    k, v = (seeded.normal(s, tokens * kvh * hd).reshape(tokens, kvh, hd) for s in (1, 2))
+    pages = -(-tokens // page)
+    slots = np.argsort(seeded.uniform01(3, pages * page), kind="stable")[:tokens]
+    cache = rt.kv_cache(kind, pages, page, kvh, hd)
+    given = [rt.upload_f32(x if token_major else np.ascontiguousarray(x.transpose(1, 0, 2))) for x in (k, v)]
+    at = rt.upload_i32(slots)
+    cache.append(*given, tokens, at, token_major=token_major)
+    out = [rt.alloc_f32(tokens * kvh * hd) for _ in range(2)]
+    cache.gather(at, tokens, *out)
+    for x, t in zip((k, v), out):
+        assert_bits_equal(rt.download_f32(t) + 0.0, ref.stored(x, kind).ravel() + 0.0, kind)

@@ -13,12 +13,6 @@ namespace {
 
 constexpr int kU = 4;  // row groups that a wave has in flight
 
-// Calls that read this much pass by the caches (13828 rows of 36 heads of 64 and
-// their way back as floats: 70.4 us from memory, 76.3 through the caches; 35.8 against
-// 39.2 where the rows are still cached); in place, where what was read is
-// written at once, calls of four times as much (226 MB 64 us against 86).
-constexpr size_t kStreamBytes = (size_t)64 << 20;
-
 // quantize_row_q8_0's value (src/q8_0_dot.rs:38-44): half away from zero, NaN to 0.
 __device__ __forceinline__ int q8_of(float v, float inv) {
     const float q = roundf(mul_rn(v, inv));
@@ -372,8 +366,7 @@ hipError_t launch_cache_rows(hipStream_t s, CacheRows a) {
     const dim3 grid((unsigned)((a.tokens + a.per_group - 1) / a.per_group),
                     a.tokens < 2048 ? (groups + 4 * kU - 1) / (4 * kU) : 1);
     const size_t lds = (size_t)a.per_group * a.rope.pairs * 2 * sizeof(float);
-    const size_t bytes = (size_t)a.tokens * (a.heads + 2 * a.kv_heads) * a.head_dim * sizeof(float);
-    const bool nt = bytes >= (a.q == a.q_out ? 4 * kStreamBytes : kStreamBytes);
+    const bool nt = rows_pass_caches(a);
     auto run = [&](auto kernel, auto streaming) {
         if (nt) streaming<<<grid, 256, lds, s>>>(a);
         else kernel<<<grid, 256, lds, s>>>(a);

@@ -351,6 +351,20 @@ struct CacheRows {
     CacheView cache;
     int per_group;           // set by the launcher
 };
+// Whether a call's loads and stores pass by the caches: where it reads this much (13828
+// rows of 36 heads of 64 and their way back as floats: 70.4 us from memory, 76.3 through
+// the caches; 35.8 against 39.2 where the rows are still cached).
+// K and V alone: three times as much.  (Past the caches and through them, from memory and where
+// the rows are still cached, us: 13828 rows of 24 heads of 64, 170 MB, to bfloat16 50/51 and
+// 46/40, to floats 68/68 and 56/66; 27000 of 8 heads of 128, 221 MB, to bfloat16 62/63 and
+// 57/62, to floats 77/80 and 65/79, to Q8_0 69/69 and 70/67.)
+// A rotation in place, where what was read is written at once: four times (226 MB 64 us against
+// 86).
+constexpr size_t kRowsStreamBytes = (size_t)64 << 20;
+inline bool rows_pass_caches(const CacheRows &a) {
+    const size_t bytes = ((size_t)a.heads + 2 * (size_t)a.kv_heads) * a.tokens * a.head_dim * sizeof(float);
+    return bytes >= kRowsStreamBytes * (a.heads == 0 ? 3 : a.q == a.q_out ? 4 : 1);
+}
 hipError_t launch_cache_rows(hipStream_t s, CacheRows a);
 hipError_t launch_cache_gather(hipStream_t s, const CacheView &cache, const int *slots, float *k, float *v,
                                size_t n, size_t head_dim);
