@@ -480,7 +480,9 @@ vh_status vh_kv_cache_gather_f32(const vh_kv_cache *cache, const vh_index *slots
  * Pages come from free_pages[free_start ..] in the order of the requests.  Where the
  * list ends, page -1 is entered and the tokens get slot -1 (free_next past the list's
  * length says so), as tokens past the table's row and past `tokens` (which then do not
- * count in starts and lens) do.  The next step passes lens as cached and free_next as
+ * count in starts and lens) do.  Tokens past the row count in lens and take their pages,
+ * which nothing names: of free_pages[free_start .. free_next) those that no row has, to be
+ * given back by the caller, as all pages are.  The next step passes lens as cached and free_next as
  * free_start.  At most 4096 requests, 2^31 - 1025 tokens and 2^31 - 1 free pages. */
 vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const vh_index *added,
                              size_t requests, const vh_index *free_pages, const vh_index *free_start,

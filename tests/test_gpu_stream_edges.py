@@ -189,3 +189,24 @@ def test_appends_past_the_caches_are_exact(rt, kind, token_major):
     cache.gather(at, tokens, *out)
     for x, t in zip((k, v), out):
         assert_bits_equal(rt.download_f32(t) + 0.0, ref.stored(x, kind).ravel() + 0.0, kind)
+
+
+# ---- pages past a row -----------------------------------------------------------------------
+
+
+def test_pages_past_a_row_are_those_that_no_row_has(rt):
+    """A request past its row takes pages that the table cannot hold.  They are what the step took less what the rows
+    have; given back they serve the next request."""
+    page, width, free = 8, 3, np.array([40, 41, 42, 43, 44, 45, 46, 47])
+    table = np.full((3, width), -1)
+    table[0, :3], table[1, :1] = [1, 2, 3], [4]
+    cached, added = [20, 8, 0], [25, 6, 9]
+    t, starts, lens = rt.upload_i32(table), rt.alloc_i32(4), rt.alloc_i32(3)
+    slots, nxt = rt.alloc_i32(sum(added)), rt.alloc_i32(1)
+    rt.kv_pages_assign(rt.upload_i32(cached), rt.upload_i32(added), rt.upload_i32(free), rt.upload_i32([1]), page, t,
+                       width, starts, lens, slots, nxt)
+    got, taken = rt.download_i32(t).reshape(3, width), free[1:int(rt.download_i32(nxt)[0])]
+    assert list(taken) == [41, 42, 43, 44, 45, 46] and got.tolist() == [[1, 2, 3], [4, 44, -1], [45, 46, -1]]
+    assert list(np.setdiff1d(taken, got)) == [41, 42, 43]
+    s = rt.download_i32(slots)
+    assert (s[4:25] == -1).all() and list(s[:4]) == [28, 29, 30, 31] and (s[25:] >= 0).all()
