@@ -210,3 +210,29 @@ def test_pages_past_a_row_are_those_that_no_row_has(rt):
     assert list(np.setdiff1d(taken, got)) == [41, 42, 43]
     s = rt.download_i32(slots)
     assert (s[4:25] == -1).all() and list(s[:4]) == [28, 29, 30, 31] and (s[25:] >= 0).all()
+
+
+# ---- a batch in two calls -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_batch_in_two_calls(rt, kind):
+    """A chunk and single tokens over the same queries and output, each call with its own requests: they are those of
+    the batch, and neither call writes the other's rows."""
+    s = Stream(rt, kind, [300] + [1] * 20, [500] + list(range(40, 60)), 8, 2, 64, 16, spare_rows=3)
+    q, both = rt.upload_f32(s.q), rt.upload_f32(np.full(s.q.size, 7.0))
+    got = []
+    for requests in (slice(0, 1), slice(1, 21)):
+        starts = s.starts[requests.start:requests.stop + 1]
+        args = (q, 8, s.tokens, rt.upload_i32(s.table[requests]), s.width, rt.upload_i32(starts),
+                rt.upload_i32(s.lens[requests]))
+        out = rt.upload_f32(np.full(s.q.size, 7.0))
+        for t in (out, both):
+            s.cache.attention(*args, t, block=1)
+        got.append(rt.download_f32(out).reshape(s.q.shape))
+        rows = np.r_[0:starts[0], starts[-1]:s.tokens]
+        assert (got[-1][rows] == 7.0).all()
+    assert_bits_equal(rt.download_f32(both)[:-3 * 512], np.concatenate([got[0][:300], got[1][300:320]]).ravel(), "both")
+    args = (s.q, s.k, s.v, s.starts, s.lens, 8, 1)
+    close(rt.download_f32(both).reshape(s.q.shape)[:320], ref.attention(*args)[:320],
+          ref.attention(*args, dtype=np.float32)[:320])

@@ -478,7 +478,10 @@ __device__ __forceinline__ int v_swizzle(int row) {
 
 __device__ __forceinline__ float half_value(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
 
-// Loads that pass by the caches, where nothing is read twice.
+// Loads that pass by the caches: those of the few rows, whose tiles mostly read a row of the
+// cache once (64 requests of 4 rows against 4096 keys each, 8 heads of 128 in bf16, 164 us,
+// through the caches 184).  The second tile of 17 to 32 rows reads it again: of 64 requests no
+// slower (342 and 381), of 16 up to 1.2 times (69 and 57).
 template <bool NT, class T>
 __device__ __forceinline__ T ld(const T *p) {
     if constexpr (NT) return __builtin_nontemporal_load(p);
@@ -825,7 +828,9 @@ __device__ __forceinline__ void walk(const CacheAttn &a, int *first_tile, char *
 // A wave holds the rows of K or of V of one step in flight, never both: 64 KB to a CU
 // at a row of 256 bytes.  Twice that lowers what the memory delivers (reading
 // scattered pages of 16 KB and nothing else: 64 KB in flight a CU 6.8 TB/s, 128 KB
-// 6.3, 256 KB 5.4), and the registers are the same for both.  A Q8_0 value stays the
+// 6.3, 256 KB 5.4), and the registers are the same for both.  (Shorter rows have less in flight,
+// and reach less: 65536 keys in sixteen requests, 12 heads of 64 in bf16 42 us, 4.8 TB/s, 8 of
+// 128 in Q8_0 52, 2.7, where the conversion of its bytes counts too.)  A Q8_0 value stays the
 // integer it is; its scale joins its weight, once for each block of 32 dims (few
 // weights, where the values of a step are many).
 //
@@ -1278,7 +1283,12 @@ constexpr int kShares = 512;
 //   Q8_0       47/117  67/119 114/135 215/142    41/116  67/117 114/133 209/139
 //   Q8_0 wide  68/161  84/164 135/165 253/194    48/152  72/154 118/156 233/185
 // Fewer keys, whose number the host does not know, favour the tiles of 16 more: 64 rows
-// against 4096 of one request f32 24/33, bf16 18/29, Q8_0 19/33.
+// against 4096 of one request f32 24/33, bf16 18/29, Q8_0 19/33.  So floats keep 32 rows, where
+// the table has the tiles of 128 ahead: against 300, 1000 and 4096 keys of one request f32 14/17
+// 15/20 21/26, wide 18/18 20/21 30/30; of sixteen 26/27 48/43 136/114, wide 24/28 50/51 159/147.
+// The average is the call's: a chunk beside single tokens sends all to one form.  A chunk of 2000
+// with 63 tokens, 4096 keys each, 32 / 8 heads of 128: bf16 621 us in one call, 448 in two, Q8_0
+// 1113 and 611; a chunk of 449: 316 and 271, 339 and 285.
 bool few_rows(const CacheView &c, size_t rows, size_t requests) {
     return rows <= (c.kind == kCacheQ8 ? 64 : 32) * requests;
 }
