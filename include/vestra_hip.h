@@ -482,8 +482,9 @@ vh_status vh_kv_cache_gather_f32(const vh_kv_cache *cache, const vh_index *slots
  * length says so), as tokens past the table's row and past `tokens` (which then do not
  * count in starts and lens) do.  Tokens past the row count in lens and take their pages,
  * which nothing names: of free_pages[free_start .. free_next) those that no row has, to be
- * given back by the caller, as all pages are.  The next step passes lens as cached and free_next as
- * free_start.  At most 4096 requests, 2^31 - 1025 tokens and 2^31 - 1 free pages. */
+ * given back by the caller, as all pages are.  The next step passes lens as cached and
+ * free_next as free_start.  At most 4096 requests, 2^31 - 1025 tokens and 2^31 - 1 free
+ * pages. */
 vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const vh_index *added,
                              size_t requests, const vh_index *free_pages, const vh_index *free_start,
                              size_t page_tokens, vh_index *table, size_t max_pages, vh_index *starts,
@@ -512,8 +513,7 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  * (less of values below 2^-110: what lies under 2^-126 of them counts as zero).  Weights
  * are up to 2^8 before they are divided by their sum, so n keys' values below 2^120 / n
  * give finite rows; larger ones may pass the floats on the way.  The same call gives the
- * same bits.  At most 4096 requests, 65535 heads and 2^30 query rows
- * (tokens * heads).
+ * same bits.  At most 4096 requests, 65535 heads and 2^30 query rows (tokens * heads).
  * The parts of rows whose keys several workgroups share lie in a workspace of the
  * runtime (35 MB at most).  A call inside a stream capture takes it for its graph
  * alone, until the runtime ends, and the next call outside gets another: replays may
