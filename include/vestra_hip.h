@@ -50,6 +50,8 @@ typedef struct vh_block vh_block;         /* prepared DA3-BASE encoder block */
 typedef struct vh_linear_q8 vh_linear_q8; /* projection with BlockQ8_0 weights */
 typedef struct vh_conv2d vh_conv2d;       /* prepared 2-D convolution (DPT head) */
 typedef struct vh_conv_transpose2d vh_conv_transpose2d; /* prepared transposed convolution */
+typedef struct vh_fp8_tensor vh_fp8_tensor; /* device rows of e4m3 values */
+typedef struct vh_linear_fp8 vh_linear_fp8; /* projection with e4m3 weights */
 typedef struct vh_index vh_index;         /* device int32 values */
 typedef struct vh_rope vh_rope;           /* prepared rotation of several position axes */
 typedef struct vh_kv_cache vh_kv_cache;   /* paged cache of keys and values */
@@ -524,6 +526,65 @@ vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const vh_tensor *q
                                     size_t tokens, size_t requests, const vh_index *table,
                                     size_t max_pages, const vh_index *starts, const vh_index *lens,
                                     size_t block, size_t window, vh_tensor *out);
+
+/* ---- rows in 8-bit floating point --------------------------------------------- */
+/* No counterpart in the reference.  Rows of e4m3 codes (1 sign, 4 exponent, 3 mantissa
+ * bits, the largest 448, 0x7f and 0xff NaN, no infinity) with a power-of-two scale for
+ * each 128 values of a row: code * 2^(exponent - 127), the exponent a byte up to 254.
+ * The last block of a row may be shorter.  Every handle of a call has to belong to one
+ * runtime (clones count as one); others are refused with VH_ERR_INVALID_ARGUMENT.
+ * At most 2^27 rows, and values of a row; at least one value. */
+/* Uninitialised. */
+vh_status vh_fp8_alloc(const vh_runtime *rt, size_t rows, size_t k, vh_fp8_tensor **out);
+/* codes [rows * k] bytes, exponents [rows * ceil(k / 128)] bytes. */
+vh_status vh_fp8_upload(const vh_runtime *rt, const void *codes, const void *exponents, size_t rows, size_t k,
+                        vh_fp8_tensor **out);
+/* Synchronising; either may be NULL. */
+vh_status vh_fp8_download(const vh_runtime *rt, const vh_fp8_tensor *tensor, void *codes, void *exponents);
+void vh_fp8_free(vh_fp8_tensor *tensor);
+size_t vh_fp8_rows(const vh_fp8_tensor *tensor);
+size_t vh_fp8_k(const vh_fp8_tensor *tensor);
+/* Rows of floats [rows, k] in e4m3: of each block the least exponent e >= -127 with all
+ * of its finite values within 448 * 2^e, and each value times 2^-e rounded to nearest
+ * even.  NaN and infinities become NaN. */
+vh_status vh_quantize_fp8(const vh_runtime *rt, const vh_tensor *x, size_t rows, size_t k, vh_fp8_tensor **out);
+vh_status vh_quantize_fp8_into(const vh_runtime *rt, const vh_tensor *x, size_t rows, size_t k,
+                               vh_fp8_tensor *out);
+/* The values that the codes stand for, out [rows, k]. */
+vh_status vh_dequantize_fp8_into(const vh_runtime *rt, const vh_fp8_tensor *tensor, vh_tensor *out);
+/* c [a.rows, b.rows] = a . b^T of the values, in 32-bit sums.  A value counts to within
+ * 2^-25 of 2^E, E the largest exponent of its row: exactly, unless exponents of a
+ * row differ by more than 15. */
+vh_status vh_gemm_fp8_into(const vh_runtime *rt, const vh_fp8_tensor *a, const vh_fp8_tensor *b, vh_tensor *c);
+
+/* A projection with e4m3 weights, as vh_linear_q8_0 is one with Q8_0's: weight row-major
+ * [K, N] floats, the rows of its transpose quantised as vh_quantize_fp8 does; bias and
+ * gamma ([N]) may be NULL. */
+vh_status vh_prepare_linear_fp8(const vh_runtime *rt, size_t input_features, size_t output_features,
+                                const float *weight, const float *bias, const float *gamma, vh_linear_fp8 **out);
+/* The same from a checkpoint's e4m3 codes of the transpose, [N, K] bytes, with a finite
+ * float scale for each 128 x 128 of them, [ceil(N / 128), ceil(K / 128)]. */
+vh_status vh_prepare_linear_fp8_blocks(const vh_runtime *rt, size_t input_features, size_t output_features,
+                                       const void *codes, const float *scales, const float *bias,
+                                       const float *gamma, vh_linear_fp8 **out);
+void vh_linear_fp8_free(vh_linear_fp8 *linear);
+size_t vh_linear_fp8_input_features(const vh_linear_fp8 *linear);
+size_t vh_linear_fp8_output_features(const vh_linear_fp8 *linear);
+/* out [rows, N] = (quantize(input) . W + bias) * gamma, input rows of floats quantised as
+ * vh_quantize_fp8 does; gelu(quantize(input) . W + bias), without a gamma; residual +=
+ * (quantize(input) . W + bias) * gamma.  The quantised rows lie in a workspace of the
+ * runtime.  A call inside a stream capture takes it for its graph alone, until the
+ * runtime ends; where none is left (nothing as large ran since the last capture) it is
+ * refused with VH_ERR_UPLOAD. */
+vh_status vh_linear_fp8_run(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows, vh_tensor *out);
+vh_status vh_linear_fp8_run_gelu(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows, vh_tensor *out);
+vh_status vh_linear_fp8_run_residual(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows,
+                                     vh_tensor *residual);
+/* The same from rows quantised before, once for every projection that reads them. */
+vh_status vh_linear_fp8_run_rows(const vh_linear_fp8 *linear, const vh_fp8_tensor *input, vh_tensor *out);
+vh_status vh_linear_fp8_run_rows_gelu(const vh_linear_fp8 *linear, const vh_fp8_tensor *input, vh_tensor *out);
+vh_status vh_linear_fp8_run_rows_residual(const vh_linear_fp8 *linear, const vh_fp8_tensor *input,
+                                          vh_tensor *residual);
 
 /* ---- profiling (device twin of DA3_FLASH_PROFILE, src/specialized.rs:1324) - */
 /* When enabled, every kernel launch is bracketed by HIP events on the

@@ -313,6 +313,36 @@ hipError_t launch_gemm_q8_0_qkv(hipStream_t s, const int8_t *a_qs, const uint16_
                                 const float *bias, float *q, float *kk, float *v, size_t tokens,
                                 size_t heads, const float *rot);
 
+// ---- rows in 8-bit floating point (k_fp8.hip) ---------------------------------
+// Rows of e4m3 codes with a power-of-two scale for each 128 values, on the device.
+// Rows are padded to 16 and k to 128, with zeros.
+struct Fp8Rows {
+    size_t rows, k;
+    uint8_t *codes;  // [rows16 / 16][blocks] panels of 2048 bytes (k_fp8.hip)
+    uint8_t *exps;   // [blocks][rows16] exponent + 127
+    uint16_t *rel;   // [blocks][rows16] 2^(exponent - row_e), at least 2^-126, as the upper half of a float
+    int *row_e;      // [rows16] largest exponent of the row
+};
+__host__ __device__ inline size_t fp8_rows16(size_t rows) { return (rows + 15) & ~(size_t)15; }
+__host__ __device__ inline size_t fp8_blocks(size_t k) { return (k + 127) / 128; }
+__host__ __device__ inline uint16_t fp8_relative(int exp_code, int row_e) {
+    const int e = exp_code - row_e;  // + 127
+    return (uint16_t)((e > 1 ? e : 1) << 7);
+}
+hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out);
+hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out);
+// c [m][n] = a . b^T, then the epilogue (Store: (v + bias) * gamma; Gelu: gelu(v +
+// bias); Residual: c += (v + bias) * gamma); bias and gamma may be null.  With b_scales
+// [ceil(n / 128)][blocks] these are the scales of b's codes, for 128 x 128 values.
+struct Fp8Gemm {
+    Fp8Rows a, b;
+    const float *b_scales, *bias, *gamma;
+    float *c;
+    size_t m, n;
+    int m_tiles, n_tiles, tiles;  // set by the launcher
+};
+hipError_t launch_gemm_fp8(hipStream_t s, const Fp8Gemm &g, Epi epi);
+
 // ---- paged cache of keys and values (k_cache.hip) ---------------------------
 // What a cache holds a value in.
 constexpr int kCacheF32 = 0, kCacheBf16 = 1, kCacheQ8 = 2;

@@ -128,6 +128,8 @@ struct RtState {
     Workspace fcnt;                             // and the in-kernel merge's arrival counters
     Workspace aq;                               // Q8_0 activation blocks
     Workspace sx;                               // split rows of a projection's input
+    Workspace f8;                               // e4m3 rows of a projection's input
+    unsigned long long f8_capture = 0;          // the capture that took it, where it is recorded
     Workspace pa;                               // counters and parts of the paged attention's tiles
     unsigned long long pa_capture = 0;          // the capture that took it, where it is recorded
     std::vector<void *> recorded;               // outgrown blocks that a graph may hold
@@ -154,7 +156,7 @@ struct RtState {
         give_back();
         hipStreamSynchronize(stream);
         for (auto &kv : rope_cache) hipFree(kv.second);
-        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx, &pa})
+        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx, &f8, &pa})
             if (w->p) hipFree(w->p);
         for (void *p : recorded) hipFree(p);
         if (tw) hipFree(tw);
@@ -302,6 +304,50 @@ struct vh_linear_q8 {
         if (!rt) return;
         hipSetDevice(rt->device);
         L.release(rt->stream);
+    }
+};
+
+namespace {
+
+// Rows in e4m3 in one block of device memory (kernels.h Fp8Rows).
+size_t fp8_bytes(size_t rows, size_t k) {
+    const size_t r = vh::fp8_rows16(rows), b = vh::fp8_blocks(k);
+    return r * b * (128 + 1 + 2) + r * sizeof(int);
+}
+vh::Fp8Rows fp8_view(void *block, size_t rows, size_t k) {
+    const size_t r = vh::fp8_rows16(rows), b = vh::fp8_blocks(k);
+    vh::Fp8Rows w{};
+    w.rows = rows;
+    w.k = k;
+    w.codes = static_cast<uint8_t *>(block);
+    w.exps = w.codes + r * b * 128;
+    w.rel = reinterpret_cast<uint16_t *>(w.exps + r * b);
+    w.row_e = reinterpret_cast<int *>(w.rel + r * b);
+    return w;
+}
+
+}  // namespace
+
+struct vh_fp8_tensor {
+    Rt rt;
+    vh::Fp8Rows view{};
+    ~vh_fp8_tensor() {
+        if (!rt || !view.codes) return;
+        hipSetDevice(rt->device);
+        hipFreeAsync(view.codes, rt->stream);
+    }
+};
+
+struct vh_linear_fp8 {
+    Rt rt;
+    vh::Fp8Rows w{};
+    float *scales = nullptr;  // for 128 x 128 codes, or null
+    float *bias = nullptr, *gamma = nullptr;
+    ~vh_linear_fp8() {
+        if (!rt) return;
+        hipSetDevice(rt->device);
+        for (void *p : {(void *)w.codes, (void *)scales, (void *)bias, (void *)gamma})
+            if (p) hipFreeAsync(p, rt->stream);
     }
 };
 
@@ -520,6 +566,27 @@ vh_status no_workspace(RtState &s, const char *what) {
     if (capturing(s.stream))
         return fail(VH_ERR_UPLOAD, std::string(what) + ": a stream capture cannot grow it; run the size once before");
     return fail(VH_ERR_UPLOAD, hip_msg(what, hipErrorOutOfMemory));
+}
+
+// The workspace w for a call that may be captured, or null.  A capture takes the block for
+// its graph alone: the next call outside gets another, so replays of the graph, on
+// whatever stream, and other graphs never meet in it.
+void *graph_workspace(RtState &s, Workspace &w, unsigned long long &owner, size_t bytes) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(s.stream, &st, &id) != hipSuccess) {
+        hipGetLastError();
+        return nullptr;
+    }
+    const bool captured = st != hipStreamCaptureStatusNone;
+    if (!captured && w.recorded) {
+        s.recorded.push_back(w.p);
+        w = Workspace{};
+    }
+    if (captured && w.recorded && owner != id) return nullptr;
+    void *p = grow_workspace(s, w, bytes);
+    if (captured && p) owner = id;
+    return p;
 }
 
 vh_status workspace(RtState &s, size_t floats, float **out) {
@@ -3750,6 +3817,384 @@ extern "C" vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const v
     attn_workspace(s, vh::cache_attn_floats(a.cache, tokens, heads / kvh, requests), &a);
     return launch(s, "kv_attention", [&] { return vh::launch_cache_attn(s.stream, a); });
     GUARD_END
+}
+
+// =============================================================================
+// rows in 8-bit floating point
+// =============================================================================
+
+// Of one call: so that every launch stays below 2^32 threads.
+constexpr size_t kMaxFp8 = (size_t)1 << 27;
+
+static vh_status check_fp8_shape(size_t rows, size_t k, const char *what) {
+    if (k == 0 || rows > kMaxFp8 || k > kMaxFp8)
+        return fail(VH_ERR_KERNEL, std::string(what) + ": rows=" + std::to_string(rows) + ", k=" + std::to_string(k) +
+                                       " are not 0 to 2^27 rows of 1 to 2^27 values");
+    return VH_OK;
+}
+
+static vh_status new_fp8(const Rt &rt, size_t rows, size_t k, vh_fp8_tensor **out, const char *what) {
+    auto t = std::make_unique<vh_fp8_tensor>();
+    char *p = nullptr;
+    TRY(dalloc(*rt, fp8_bytes(rows, k), &p, what));
+    t->rt = rt;
+    t->view = fp8_view(p, rows, k);
+    *out = t.release();
+    return VH_OK;
+}
+
+// Where a code is in its rows' panels (k_fp8.hip).
+static size_t fp8_at(const vh::Fp8Rows &w, size_t row, size_t d) {
+    const size_t in = d % 128;
+    return ((row / 16 * vh::fp8_blocks(w.k) + d / 128) * 2 + in / 16 % 2) * 1024 +
+           (in / 32 * 16 + row % 16) * 16 + in % 16;
+}
+
+// Row-major codes [rows][k] and exponents [rows][blocks] (null: 127) to the device block of w.
+static vh_status upload_fp8(RtState &s, const vh::Fp8Rows &w, const uint8_t *codes, const uint8_t *exponents,
+                            const char *what) {
+    const size_t r16 = vh::fp8_rows16(w.rows), blocks = vh::fp8_blocks(w.k);
+    std::vector<uint8_t> host(fp8_bytes(w.rows, w.k));
+    const vh::Fp8Rows h = fp8_view(host.data(), w.rows, w.k);
+    for (size_t r = 0; r < r16; r++) {
+        int most = -127;
+        for (size_t b = 0; b < blocks; b++) {
+            const int e = r < w.rows ? (exponents ? exponents[r * blocks + b] : 127) : 0;
+            h.exps[b * r16 + r] = (uint8_t)e;
+            most = std::max(most, e - 127);
+        }
+        h.row_e[r] = most;
+        for (size_t b = 0; b < blocks; b++) h.rel[b * r16 + r] = vh::fp8_relative(h.exps[b * r16 + r], most);
+        if (r >= w.rows) continue;
+        for (size_t d = 0; d < w.k; d += 16) {
+            const size_t n = std::min((size_t)16, w.k - d);
+            std::memcpy(h.codes + fp8_at(w, r, d), codes + r * w.k + d, n);
+        }
+    }
+    return h2d(s, w.codes, host.data(), host.size(), what);
+}
+
+extern "C" vh_status vh_fp8_alloc(const vh_runtime *rt, size_t rows, size_t k, vh_fp8_tensor **out) {
+    const char *what = "vh_fp8_alloc";
+    NEED(rt, what);
+    NEED(out, what);
+    TRY(check_fp8_shape(rows, k, what));
+    GUARD_BEGIN
+    TRY(set_device(*rt->s));
+    return new_fp8(rt->s, rows, k, out, what);
+    GUARD_END
+}
+
+extern "C" vh_status vh_fp8_upload(const vh_runtime *rt, const void *codes, const void *exponents, size_t rows,
+                                   size_t k, vh_fp8_tensor **out) {
+    const char *what = "vh_fp8_upload";
+    NEED(rt, what);
+    NEED(out, what);
+    TRY(check_fp8_shape(rows, k, what));
+    if (rows && (!codes || !exponents)) return null_arg("vh_fp8_upload codes");
+    const uint8_t *e = static_cast<const uint8_t *>(exponents);
+    for (size_t i = 0; i < rows * vh::fp8_blocks(k); i++)
+        if (e[i] == 255) return fail(VH_ERR_KERNEL, "vh_fp8_upload: an exponent is 255, which is no scale");
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    vh_fp8_tensor *t = nullptr;
+    TRY(new_fp8(rt->s, rows, k, &t, what));
+    vh_status st = upload_fp8(s, t->view, static_cast<const uint8_t *>(codes), e, what);
+    if (st) {
+        delete t;
+        return st;
+    }
+    *out = t;
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" vh_status vh_fp8_download(const vh_runtime *rt, const vh_fp8_tensor *tensor, void *codes,
+                                     void *exponents) {
+    const char *what = "vh_fp8_download";
+    NEED(rt, what);
+    NEED(tensor, what);
+    if (tensor->rt != rt->s) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    const vh::Fp8Rows &w = tensor->view;
+    if (w.rows == 0) return VH_OK;
+    const size_t r16 = vh::fp8_rows16(w.rows), blocks = vh::fp8_blocks(w.k);
+    std::vector<uint8_t> host(r16 * blocks * 129);
+    hipError_t e = hipMemcpyAsync(host.data(), w.codes, host.size(), hipMemcpyDeviceToHost, s.stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(s.stream);
+    if (e != hipSuccess) return fail(VH_ERR_DOWNLOAD, hip_msg("device-to-host transfer", e));
+    for (size_t r = 0; r < w.rows; r++) {
+        for (size_t d = 0; codes && d < w.k; d += 16)
+            std::memcpy(static_cast<uint8_t *>(codes) + r * w.k + d, &host[fp8_at(w, r, d)],
+                        std::min((size_t)16, w.k - d));
+        for (size_t b = 0; exponents && b < blocks; b++)
+            static_cast<uint8_t *>(exponents)[r * blocks + b] = host[r16 * blocks * 128 + b * r16 + r];
+    }
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" void vh_fp8_free(vh_fp8_tensor *tensor) { delete tensor; }
+extern "C" size_t vh_fp8_rows(const vh_fp8_tensor *tensor) { return tensor ? tensor->view.rows : 0; }
+extern "C" size_t vh_fp8_k(const vh_fp8_tensor *tensor) { return tensor ? tensor->view.k : 0; }
+
+static vh_status quantize_fp8(RtState &s, const float *x, const vh::Fp8Rows &out) {
+    if (out.rows == 0) return VH_OK;
+    return launch(s, "quantize_fp8", [&] { return vh::launch_quantize_fp8(s.stream, x, out); });
+}
+
+extern "C" vh_status vh_quantize_fp8(const vh_runtime *rt, const vh_tensor *x, size_t rows, size_t k,
+                                     vh_fp8_tensor **out) {
+    const char *what = "vh_quantize_fp8";
+    NEED(rt, what);
+    NEED(x, what);
+    NEED(out, what);
+    TRY(check_fp8_shape(rows, k, what));
+    if (x->len != rows * k) return mismatch(rows * k, x->len, what);
+    if (x->rt != rt->s) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    vh_fp8_tensor *t = nullptr;
+    TRY(new_fp8(rt->s, rows, k, &t, what));
+    vh_status st = quantize_fp8(s, x->ptr, t->view);
+    if (st) {
+        delete t;
+        return st;
+    }
+    *out = t;
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" vh_status vh_quantize_fp8_into(const vh_runtime *rt, const vh_tensor *x, size_t rows, size_t k,
+                                          vh_fp8_tensor *out) {
+    const char *what = "vh_quantize_fp8_into";
+    NEED(rt, what);
+    NEED(x, what);
+    NEED(out, what);
+    TRY(check_fp8_shape(rows, k, what));
+    if (out->view.rows != rows || out->view.k != k) return mismatch(out->view.rows * out->view.k, rows * k, what);
+    if (x->len != rows * k) return mismatch(rows * k, x->len, what);
+    if (x->rt != rt->s || out->rt != rt->s) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    return quantize_fp8(s, x->ptr, out->view);
+    GUARD_END
+}
+
+extern "C" vh_status vh_dequantize_fp8_into(const vh_runtime *rt, const vh_fp8_tensor *tensor, vh_tensor *out) {
+    const char *what = "vh_dequantize_fp8_into";
+    NEED(rt, what);
+    NEED(tensor, what);
+    NEED(out, what);
+    const vh::Fp8Rows &w = tensor->view;
+    if (out->len != w.rows * w.k) return mismatch(out->len, w.rows * w.k, what);
+    if (tensor->rt != rt->s || out->rt != rt->s) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    if (w.rows == 0) return VH_OK;
+    return launch(s, "dequantize_fp8", [&] { return vh::launch_dequantize_fp8(s.stream, w, out->ptr); });
+    GUARD_END
+}
+
+extern "C" vh_status vh_gemm_fp8_into(const vh_runtime *rt, const vh_fp8_tensor *a, const vh_fp8_tensor *b,
+                                      vh_tensor *c) {
+    const char *what = "vh_gemm_fp8_into";
+    NEED(rt, what);
+    NEED(a, what);
+    NEED(b, what);
+    NEED(c, what);
+    if (a->view.k != b->view.k) return mismatch(a->view.k, b->view.k, what);
+    if (c->len != a->view.rows * b->view.rows) return mismatch(c->len, a->view.rows * b->view.rows, what);
+    if (a->rt != rt->s || b->rt != rt->s || c->rt != rt->s) return other_runtime(what);
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    if (c->len == 0) return VH_OK;
+    vh::Fp8Gemm g{};
+    g.a = a->view;
+    g.b = b->view;
+    g.c = c->ptr;
+    g.m = a->view.rows;
+    g.n = b->view.rows;
+    return launch(s, "gemm_fp8", [&] { return vh::launch_gemm_fp8(s.stream, g, vh::Epi::Store); });
+    GUARD_END
+}
+
+static vh_status check_linear_fp8(size_t k, size_t n, bool given, const char *what) {
+    if (k == 0 || n == 0 || k > kMaxFp8 || n > kMaxFp8 || !given)
+        return fail(VH_ERR_BLAS, std::string(what) + ": linear parameter shape K=" + std::to_string(k) + ", N=" +
+                                     std::to_string(n) + " is out of range (1 to 2^27) or without its buffers");
+    return VH_OK;
+}
+
+static vh_status linear_fp8_vectors(RtState &s, const float *bias, const float *gamma, vh_linear_fp8 *l) {
+    if (bias) TRY(upload_array(s, bias, l->w.rows, &l->bias, "linear bias upload"));
+    if (gamma) TRY(upload_array(s, gamma, l->w.rows, &l->gamma, "linear gamma upload"));
+    return VH_OK;
+}
+
+extern "C" vh_status vh_prepare_linear_fp8(const vh_runtime *rt, size_t input_features, size_t output_features,
+                                           const float *weight, const float *bias, const float *gamma,
+                                           vh_linear_fp8 **out) {
+    const char *what = "vh_prepare_linear_fp8";
+    NEED(rt, what);
+    NEED(out, what);
+    const size_t k = input_features, n = output_features;
+    TRY(check_linear_fp8(k, n, weight != nullptr, what));
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    auto l = std::make_unique<vh_linear_fp8>();
+    l->rt = rt->s;
+    char *block = nullptr;
+    TRY(dalloc(s, fp8_bytes(n, k), &block, "fp8 weight allocation"));
+    l->w = fp8_view(block, n, k);
+    float *w = nullptr, *wt = nullptr;
+    TRY(upload_array(s, weight, k * n, &w, "linear weight upload"));
+    vh_status st = dalloc(s, k * n, &wt, "linear weight allocation");
+    if (!st) st = launch(s, "transpose_weight", [&] { return vh::launch_transpose(s.stream, w, wt, k, n); });
+    if (!st) st = quantize_fp8(s, wt, l->w);
+    hipFreeAsync(w, s.stream);
+    if (wt) hipFreeAsync(wt, s.stream);
+    if (!st) st = linear_fp8_vectors(s, bias, gamma, l.get());
+    if (st) return st;
+    *out = l.release();
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" vh_status vh_prepare_linear_fp8_blocks(const vh_runtime *rt, size_t input_features,
+                                                  size_t output_features, const void *codes, const float *scales,
+                                                  const float *bias, const float *gamma, vh_linear_fp8 **out) {
+    const char *what = "vh_prepare_linear_fp8_blocks";
+    NEED(rt, what);
+    NEED(out, what);
+    const size_t k = input_features, n = output_features;
+    TRY(check_linear_fp8(k, n, codes && scales, what));
+    const size_t blocks = (n + 127) / 128 * vh::fp8_blocks(k);
+    for (size_t i = 0; i < blocks; i++)
+        if (!std::isfinite(scales[i]))
+            return fail(VH_ERR_BLAS, std::string(what) + ": scale " + std::to_string(i) + " is not finite");
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    auto l = std::make_unique<vh_linear_fp8>();
+    l->rt = rt->s;
+    char *block = nullptr;
+    TRY(dalloc(s, fp8_bytes(n, k), &block, "fp8 weight allocation"));
+    l->w = fp8_view(block, n, k);
+    TRY(upload_fp8(s, l->w, static_cast<const uint8_t *>(codes), nullptr, "fp8 weight upload"));
+    TRY(upload_array(s, scales, blocks, &l->scales, "fp8 scale upload"));
+    TRY(linear_fp8_vectors(s, bias, gamma, l.get()));
+    *out = l.release();
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" void vh_linear_fp8_free(vh_linear_fp8 *linear) { delete linear; }
+extern "C" size_t vh_linear_fp8_input_features(const vh_linear_fp8 *linear) { return linear ? linear->w.k : 0; }
+extern "C" size_t vh_linear_fp8_output_features(const vh_linear_fp8 *linear) { return linear ? linear->w.rows : 0; }
+
+// One run, from floats (x) or from rows quantised before (q).
+static vh_status run_fp8(const vh_linear_fp8 *l, const vh_tensor *x, const vh_fp8_tensor *q, size_t rows,
+                         vh::Epi epi, vh_tensor *out, const char *what) {
+    const size_t k = l->w.k, n = l->w.rows;
+    size_t expected = 0;
+    if (x && (rows > kMaxFp8 || mul_overflows(rows, k, &expected) || x->len != expected))
+        return fail(VH_ERR_BLAS, std::string(what) + ": linear input rows=" + std::to_string(rows) + ", K=" +
+                                     std::to_string(k) + " does not match device input length " +
+                                     std::to_string(x->len));
+    if (q && q->view.k != k)
+        return fail(VH_ERR_BLAS, std::string(what) + ": rows of " + std::to_string(q->view.k) +
+                                     " values, the linear has K=" + std::to_string(k));
+    if (epi == vh::Epi::Gelu && l->gamma)
+        return fail(VH_ERR_BLAS, std::string(what) + ": the linear carries a LayerScale gamma");
+    if (out->len != rows * n) return mismatch(out->len, rows * n, what);
+    if ((x ? x->rt : q->rt) != l->rt || out->rt != l->rt) return other_runtime(what);
+    if (out == x) return aliased(what);
+    GUARD_BEGIN
+    RtState &s = *l->rt;
+    TRY(set_device(s));
+    if (rows == 0) return VH_OK;
+    vh::Fp8Gemm g{};
+    if (q) {
+        g.a = q->view;
+    } else {
+        void *p = graph_workspace(s, s.f8, s.f8_capture, fp8_bytes(rows, k));
+        if (!p) return no_workspace(s, "fp8 activation workspace");
+        g.a = fp8_view(p, rows, k);
+        TRY(quantize_fp8(s, x->ptr, g.a));
+    }
+    g.b = l->w;
+    g.b_scales = l->scales;
+    g.bias = l->bias;
+    g.gamma = l->gamma;
+    g.c = out->ptr;
+    g.m = rows;
+    g.n = n;
+    return launch(s, "gemm_fp8", [&] { return vh::launch_gemm_fp8(s.stream, g, epi); });
+    GUARD_END
+}
+
+extern "C" vh_status vh_linear_fp8_run(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows,
+                                    vh_tensor *out) {
+    const char *what = "vh_linear_fp8_run";
+    NEED(linear, what);
+    NEED(input, what);
+    NEED(out, what);
+    return run_fp8(linear, input, nullptr, rows, vh::Epi::Store, out, what);
+}
+
+extern "C" vh_status vh_linear_fp8_run_gelu(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows,
+                                    vh_tensor *out) {
+    const char *what = "vh_linear_fp8_run_gelu";
+    NEED(linear, what);
+    NEED(input, what);
+    NEED(out, what);
+    return run_fp8(linear, input, nullptr, rows, vh::Epi::Gelu, out, what);
+}
+
+extern "C" vh_status vh_linear_fp8_run_residual(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows,
+                                    vh_tensor *residual) {
+    const char *what = "vh_linear_fp8_run_residual";
+    NEED(linear, what);
+    NEED(input, what);
+    NEED(residual, what);
+    return run_fp8(linear, input, nullptr, rows, vh::Epi::Residual, residual, what);
+}
+
+extern "C" vh_status vh_linear_fp8_run_rows(const vh_linear_fp8 *linear, const vh_fp8_tensor *input,
+                                         vh_tensor *out) {
+    const char *what = "vh_linear_fp8_run_rows";
+    NEED(linear, what);
+    NEED(input, what);
+    NEED(out, what);
+    return run_fp8(linear, nullptr, input, input->view.rows, vh::Epi::Store, out, what);
+}
+
+extern "C" vh_status vh_linear_fp8_run_rows_gelu(const vh_linear_fp8 *linear, const vh_fp8_tensor *input,
+                                         vh_tensor *out) {
+    const char *what = "vh_linear_fp8_run_rows_gelu";
+    NEED(linear, what);
+    NEED(input, what);
+    NEED(out, what);
+    return run_fp8(linear, nullptr, input, input->view.rows, vh::Epi::Gelu, out, what);
+}
+
+extern "C" vh_status vh_linear_fp8_run_rows_residual(const vh_linear_fp8 *linear, const vh_fp8_tensor *input,
+                                         vh_tensor *residual) {
+    const char *what = "vh_linear_fp8_run_rows_residual";
+    NEED(linear, what);
+    NEED(input, what);
+    NEED(residual, what);
+    return run_fp8(linear, nullptr, input, input->view.rows, vh::Epi::Residual, residual, what);
 }
 
 // =============================================================================

@@ -77,6 +77,14 @@ pub struct VhRope {
 pub struct VhKvCache {
     _p: [u8; 0],
 }
+#[repr(C)]
+pub struct VhFp8Tensor {
+    _p: [u8; 0],
+}
+#[repr(C)]
+pub struct VhLinearFp8 {
+    _p: [u8; 0],
+}
 
 type Status = c_int;
 
@@ -288,6 +296,42 @@ unsafe extern "C" {
                           free_pages: *const VhIndex, free_start: *const VhIndex, page_tokens: usize,
                           table: *mut VhIndex, max_pages: usize, starts: *mut VhIndex, lens: *mut VhIndex,
                           slots: *mut VhIndex, tokens: usize, free_next: *mut VhIndex) -> Status;
+
+    fn vh_fp8_alloc(rt: *const VhRuntime, rows: usize, k: usize, out: *mut *mut VhFp8Tensor) -> Status;
+    fn vh_fp8_upload(rt: *const VhRuntime, codes: *const c_void, exponents: *const c_void, rows: usize, k: usize,
+                     out: *mut *mut VhFp8Tensor) -> Status;
+    fn vh_fp8_download(rt: *const VhRuntime, tensor: *const VhFp8Tensor, codes: *mut c_void,
+                       exponents: *mut c_void) -> Status;
+    fn vh_fp8_free(tensor: *mut VhFp8Tensor);
+    fn vh_fp8_rows(tensor: *const VhFp8Tensor) -> usize;
+    fn vh_fp8_k(tensor: *const VhFp8Tensor) -> usize;
+    fn vh_quantize_fp8(rt: *const VhRuntime, x: *const VhTensor, rows: usize, k: usize,
+                       out: *mut *mut VhFp8Tensor) -> Status;
+    fn vh_quantize_fp8_into(rt: *const VhRuntime, x: *const VhTensor, rows: usize, k: usize,
+                            out: *mut VhFp8Tensor) -> Status;
+    fn vh_dequantize_fp8_into(rt: *const VhRuntime, tensor: *const VhFp8Tensor, out: *mut VhTensor) -> Status;
+    fn vh_gemm_fp8_into(rt: *const VhRuntime, a: *const VhFp8Tensor, b: *const VhFp8Tensor,
+                        c: *mut VhTensor) -> Status;
+    fn vh_prepare_linear_fp8(rt: *const VhRuntime, input_features: usize, output_features: usize,
+                             weight: *const f32, bias: *const f32, gamma: *const f32,
+                             out: *mut *mut VhLinearFp8) -> Status;
+    fn vh_prepare_linear_fp8_blocks(rt: *const VhRuntime, input_features: usize, output_features: usize,
+                                    codes: *const c_void, scales: *const f32, bias: *const f32, gamma: *const f32,
+                                    out: *mut *mut VhLinearFp8) -> Status;
+    fn vh_linear_fp8_free(linear: *mut VhLinearFp8);
+    fn vh_linear_fp8_input_features(linear: *const VhLinearFp8) -> usize;
+    fn vh_linear_fp8_output_features(linear: *const VhLinearFp8) -> usize;
+    fn vh_linear_fp8_run(linear: *const VhLinearFp8, input: *const VhTensor, rows: usize,
+                         out: *mut VhTensor) -> Status;
+    fn vh_linear_fp8_run_gelu(linear: *const VhLinearFp8, input: *const VhTensor, rows: usize,
+                              out: *mut VhTensor) -> Status;
+    fn vh_linear_fp8_run_residual(linear: *const VhLinearFp8, input: *const VhTensor, rows: usize,
+                                  residual: *mut VhTensor) -> Status;
+    fn vh_linear_fp8_run_rows(linear: *const VhLinearFp8, input: *const VhFp8Tensor, out: *mut VhTensor) -> Status;
+    fn vh_linear_fp8_run_rows_gelu(linear: *const VhLinearFp8, input: *const VhFp8Tensor,
+                                   out: *mut VhTensor) -> Status;
+    fn vh_linear_fp8_run_rows_residual(linear: *const VhLinearFp8, input: *const VhFp8Tensor,
+                                       residual: *mut VhTensor) -> Status;
 
     fn vh_profile_enable(rt: *mut VhRuntime, enabled: c_int) -> Status;
     fn vh_profile_reset(rt: *mut VhRuntime) -> Status;
@@ -981,6 +1025,109 @@ impl HipRuntime {
         self.make(|out| unsafe { vh_bilinear_resize_align_corners_f32(raw, input.raw, c, ih, iw, oh, ow, add, out) })
     }
 
+    // -- rows in 8-bit floating point ---------------------------------------------
+
+    /// Uninitialised rows.
+    pub fn fp8_alloc(&self, rows: usize, k: usize) -> Result<HipFp8Tensor, HipError> {
+        let raw = self.inner.raw;
+        let mut out = ptr::null_mut();
+        // SAFETY: live runtime.
+        self.call(|| unsafe { vh_fp8_alloc(raw, rows, k, &mut out) })?;
+        Ok(HipFp8Tensor { raw: out, runtime: self.clone() })
+    }
+
+    /// Row-major e4m3 codes and the exponent (+ 127) of each 128 values of a row.
+    pub fn fp8_upload(&self, codes: &[u8], exponents: &[u8], rows: usize, k: usize)
+        -> Result<HipFp8Tensor, HipError> {
+        if codes.len() != rows.saturating_mul(k) || exponents.len() != rows.saturating_mul(k.div_ceil(128)) {
+            return Err(HipError::LengthMismatch { destination: rows.saturating_mul(k), source_len: codes.len() });
+        }
+        let raw = self.inner.raw;
+        let mut out = ptr::null_mut();
+        // SAFETY: lengths checked above.
+        self.call(|| unsafe {
+            vh_fp8_upload(raw, codes.as_ptr().cast(), exponents.as_ptr().cast(), rows, k, &mut out)
+        })?;
+        Ok(HipFp8Tensor { raw: out, runtime: self.clone() })
+    }
+
+    /// The codes and exponents of `tensor` (synchronising).
+    pub fn fp8_download(&self, tensor: &HipFp8Tensor) -> Result<(Vec<u8>, Vec<u8>), HipError> {
+        let (rows, k) = (tensor.rows(), tensor.k());
+        let (mut codes, mut exponents) = (vec![0u8; rows * k], vec![0u8; rows * k.div_ceil(128)]);
+        let raw = self.inner.raw;
+        // SAFETY: the buffers have the tensor's sizes.
+        self.call(|| unsafe {
+            vh_fp8_download(raw, tensor.raw, codes.as_mut_ptr().cast(), exponents.as_mut_ptr().cast())
+        })?;
+        Ok((codes, exponents))
+    }
+
+    pub fn quantize_fp8(&self, x: &HipTensorF32, rows: usize, k: usize) -> Result<HipFp8Tensor, HipError> {
+        let raw = self.inner.raw;
+        let mut out = ptr::null_mut();
+        // SAFETY: live handles.
+        self.call(|| unsafe { vh_quantize_fp8(raw, x.raw, rows, k, &mut out) })?;
+        Ok(HipFp8Tensor { raw: out, runtime: self.clone() })
+    }
+
+    pub fn quantize_fp8_into(&self, x: &HipTensorF32, rows: usize, k: usize, out: &mut HipFp8Tensor)
+        -> Result<(), HipError> {
+        let (raw, dst) = (self.inner.raw, out.raw);
+        // SAFETY: live handles; the output is borrowed mutably for the call.
+        self.call(|| unsafe { vh_quantize_fp8_into(raw, x.raw, rows, k, dst) })
+    }
+
+    /// The values that the codes stand for.
+    pub fn dequantize_fp8_into(&self, tensor: &HipFp8Tensor, out: &mut HipTensorF32) -> Result<(), HipError> {
+        let (raw, dst) = (self.inner.raw, out.raw);
+        // SAFETY: live handles; the output is borrowed mutably for the call.
+        self.call(|| unsafe { vh_dequantize_fp8_into(raw, tensor.raw, dst) })
+    }
+
+    /// c [a.rows, b.rows] = a . b^T.
+    pub fn gemm_fp8_into(&self, a: &HipFp8Tensor, b: &HipFp8Tensor, c: &mut HipTensorF32) -> Result<(), HipError> {
+        let (raw, dst) = (self.inner.raw, c.raw);
+        // SAFETY: live handles; the output is borrowed mutably for the call.
+        self.call(|| unsafe { vh_gemm_fp8_into(raw, a.raw, b.raw, dst) })
+    }
+
+    /// A projection with e4m3 weights from floats [K, N].
+    pub fn prepare_linear_fp8(&self, input_features: usize, output_features: usize, weight: &[f32],
+                              bias: Option<&[f32]>, gamma: Option<&[f32]>) -> Result<HipLinearFp8, HipError> {
+        let wanted = input_features.saturating_mul(output_features);
+        if weight.len() != wanted || [bias, gamma].iter().flatten().any(|v| v.len() != output_features) {
+            return Err(HipError::LengthMismatch { destination: wanted, source_len: weight.len() });
+        }
+        let raw = self.inner.raw;
+        let mut out = ptr::null_mut();
+        // SAFETY: lengths checked above.
+        self.call(|| unsafe {
+            vh_prepare_linear_fp8(raw, input_features, output_features, weight.as_ptr(), opt_ptr(bias),
+                                  opt_ptr(gamma), &mut out)
+        })?;
+        Ok(HipLinearFp8 { raw: out, runtime: self.clone() })
+    }
+
+    /// The same from e4m3 codes [N, K] with a float scale for each 128 x 128 of them.
+    pub fn prepare_linear_fp8_blocks(&self, input_features: usize, output_features: usize, codes: &[u8],
+                                     scales: &[f32], bias: Option<&[f32]>, gamma: Option<&[f32]>)
+        -> Result<HipLinearFp8, HipError> {
+        let wanted = input_features.saturating_mul(output_features);
+        if codes.len() != wanted || scales.len() != input_features.div_ceil(128) * output_features.div_ceil(128)
+            || [bias, gamma].iter().flatten().any(|v| v.len() != output_features) {
+            return Err(HipError::LengthMismatch { destination: wanted, source_len: codes.len() });
+        }
+        let raw = self.inner.raw;
+        let mut out = ptr::null_mut();
+        // SAFETY: lengths checked above.
+        self.call(|| unsafe {
+            vh_prepare_linear_fp8_blocks(raw, input_features, output_features, codes.as_ptr().cast(),
+                                         scales.as_ptr(), opt_ptr(bias), opt_ptr(gamma), &mut out)
+        })?;
+        Ok(HipLinearFp8 { raw: out, runtime: self.clone() })
+    }
+
     // -- profiling (device twin of DA3_FLASH_PROFILE, src/specialized.rs:1324) ----
 
     pub fn profile_enable(&self, enabled: bool) -> Result<(), HipError> {
@@ -1349,6 +1496,115 @@ impl HipLinearQ8 {
         let raw = self.raw;
         // SAFETY: live handles.
         self.runtime.call(|| unsafe { vh_linear_q8_0_run_residual(raw, input.raw, rows, residual.raw) })
+    }
+}
+
+// ---- rows in 8-bit floating point ----------------------------------------------
+
+/// Device rows of e4m3 values with a power-of-two scale for each 128 of a row.
+pub struct HipFp8Tensor {
+    raw: *mut VhFp8Tensor,
+    runtime: HipRuntime,
+}
+
+// SAFETY: owned device state; every use goes through the runtime's lock.
+unsafe impl Send for HipFp8Tensor {}
+unsafe impl Sync for HipFp8Tensor {}
+
+impl Drop for HipFp8Tensor {
+    fn drop(&mut self) {
+        let _g = self.runtime.guard();
+        // SAFETY: raw came from the library and is freed once.
+        unsafe { vh_fp8_free(self.raw) }
+    }
+}
+
+impl HipFp8Tensor {
+    #[must_use]
+    pub fn rows(&self) -> usize {
+        // SAFETY: live handle.
+        unsafe { vh_fp8_rows(self.raw) }
+    }
+
+    #[must_use]
+    pub fn k(&self) -> usize {
+        // SAFETY: live handle.
+        unsafe { vh_fp8_k(self.raw) }
+    }
+}
+
+/// A projection with e4m3 weights.
+pub struct HipLinearFp8 {
+    raw: *mut VhLinearFp8,
+    runtime: HipRuntime,
+}
+
+// SAFETY: owned device state; every use goes through the runtime's lock.
+unsafe impl Send for HipLinearFp8 {}
+unsafe impl Sync for HipLinearFp8 {}
+
+impl Drop for HipLinearFp8 {
+    fn drop(&mut self) {
+        let _g = self.runtime.guard();
+        // SAFETY: raw came from the library and is freed once.
+        unsafe { vh_linear_fp8_free(self.raw) }
+    }
+}
+
+impl HipLinearFp8 {
+    #[must_use]
+    pub fn input_features(&self) -> usize {
+        // SAFETY: live handle.
+        unsafe { vh_linear_fp8_input_features(self.raw) }
+    }
+
+    #[must_use]
+    pub fn output_features(&self) -> usize {
+        // SAFETY: live handle.
+        unsafe { vh_linear_fp8_output_features(self.raw) }
+    }
+
+    /// (quantize(input) . W + bias) * gamma
+    pub fn run(&self, input: &HipTensorF32, rows: usize, out: &mut HipTensorF32) -> Result<(), HipError> {
+        let dst = out.raw;
+        // SAFETY: live handles; the output is borrowed mutably for the call.
+        self.runtime.call(|| unsafe { vh_linear_fp8_run(self.raw, input.raw, rows, dst) })
+    }
+
+    /// gelu(quantize(input) . W + bias)
+    pub fn run_gelu(&self, input: &HipTensorF32, rows: usize, out: &mut HipTensorF32) -> Result<(), HipError> {
+        let dst = out.raw;
+        // SAFETY: as above.
+        self.runtime.call(|| unsafe { vh_linear_fp8_run_gelu(self.raw, input.raw, rows, dst) })
+    }
+
+    /// residual += (quantize(input) . W + bias) * gamma
+    pub fn run_residual(&self, input: &HipTensorF32, rows: usize, residual: &mut HipTensorF32)
+        -> Result<(), HipError> {
+        let dst = residual.raw;
+        // SAFETY: as above.
+        self.runtime.call(|| unsafe { vh_linear_fp8_run_residual(self.raw, input.raw, rows, dst) })
+    }
+
+    /// `run` on rows quantised before, once for every projection that reads them.
+    pub fn run_rows(&self, input: &HipFp8Tensor, out: &mut HipTensorF32) -> Result<(), HipError> {
+        let dst = out.raw;
+        // SAFETY: as above.
+        self.runtime.call(|| unsafe { vh_linear_fp8_run_rows(self.raw, input.raw, dst) })
+    }
+
+    /// `run_gelu` on rows quantised before.
+    pub fn run_rows_gelu(&self, input: &HipFp8Tensor, out: &mut HipTensorF32) -> Result<(), HipError> {
+        let dst = out.raw;
+        // SAFETY: as above.
+        self.runtime.call(|| unsafe { vh_linear_fp8_run_rows_gelu(self.raw, input.raw, dst) })
+    }
+
+    /// `run_residual` on rows quantised before.
+    pub fn run_rows_residual(&self, input: &HipFp8Tensor, residual: &mut HipTensorF32) -> Result<(), HipError> {
+        let dst = residual.raw;
+        // SAFETY: as above.
+        self.runtime.call(|| unsafe { vh_linear_fp8_run_rows_residual(self.raw, input.raw, dst) })
     }
 }
 

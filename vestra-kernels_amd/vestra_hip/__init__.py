@@ -183,6 +183,27 @@ SIGNATURES = [
     ("vh_kv_cache_gather_f32", _S, [_p, _p, _sz, _p, _p]),
     ("vh_kv_pages_assign", _S, [_p, _p, _p, _sz, _p, _p, _sz, _p, _sz, _p, _p, _p, _sz, _p]),
     ("vh_kv_cache_attention_f32", _S, [_p, _p, _sz, _sz, _sz, _p, _sz, _p, _p, _sz, _sz, _p]),
+    ("vh_fp8_alloc", _S, [_p, _sz, _sz, _pp]),
+    ("vh_fp8_upload", _S, [_p, _p, _p, _sz, _sz, _pp]),
+    ("vh_fp8_download", _S, [_p, _p, _p, _p]),
+    ("vh_fp8_free", None, [_p]),
+    ("vh_fp8_rows", _sz, [_p]),
+    ("vh_fp8_k", _sz, [_p]),
+    ("vh_quantize_fp8", _S, [_p, _p, _sz, _sz, _pp]),
+    ("vh_quantize_fp8_into", _S, [_p, _p, _sz, _sz, _p]),
+    ("vh_dequantize_fp8_into", _S, [_p, _p, _p]),
+    ("vh_gemm_fp8_into", _S, [_p, _p, _p, _p]),
+    ("vh_prepare_linear_fp8", _S, [_p, _sz, _sz, _f32p, _f32p, _f32p, _pp]),
+    ("vh_prepare_linear_fp8_blocks", _S, [_p, _sz, _sz, _p, _f32p, _f32p, _f32p, _pp]),
+    ("vh_linear_fp8_free", None, [_p]),
+    ("vh_linear_fp8_input_features", _sz, [_p]),
+    ("vh_linear_fp8_output_features", _sz, [_p]),
+    ("vh_linear_fp8_run", _S, [_p, _p, _sz, _p]),
+    ("vh_linear_fp8_run_gelu", _S, [_p, _p, _sz, _p]),
+    ("vh_linear_fp8_run_residual", _S, [_p, _p, _sz, _p]),
+    ("vh_linear_fp8_run_rows", _S, [_p, _p, _p]),
+    ("vh_linear_fp8_run_rows_gelu", _S, [_p, _p, _p]),
+    ("vh_linear_fp8_run_rows_residual", _S, [_p, _p, _p]),
     ("vh_profile_enable", _S, [_p, ctypes.c_int]),
     ("vh_profile_reset", _S, [_p]),
     ("vh_profile_report", _S, [_p, ctypes.c_char_p, _sz]),
@@ -232,6 +253,21 @@ def _i32(values) -> np.ndarray:
     if not np.array_equal(a, out):
         raise InvalidArgument("upload_i32: values outside int32")
     return out
+
+
+def _vector(values, n: int) -> np.ndarray:
+    """n floats; another number of them is refused, as the C side cannot see how many there are."""
+    a = _f32(values).reshape(-1)
+    if a.size != n:
+        raise InvalidArgument(f"{a.size} values where {n} are wanted")
+    return a
+
+
+def _bytes(values, n: int) -> np.ndarray:
+    a = np.asarray(values)
+    if a.dtype.itemsize != 1 or a.size != n:
+        raise InvalidArgument(f"{a.size} values of {a.dtype} where {n} bytes are wanted")
+    return np.ascontiguousarray(a).reshape(-1).view(np.uint8)
 
 
 def _fp(a: np.ndarray):
@@ -547,6 +583,75 @@ class KvCache:
         try:
             if self._h and self._h.value:
                 lib().vh_kv_cache_free(self._h)
+                self._h = ctypes.c_void_p(None)
+        except Exception:
+            pass
+
+
+class Fp8Tensor:
+    """Device rows of e4m3 values with a power-of-two scale for each 128 of a row."""
+
+    def __init__(self, runtime: "Runtime", handle: int):
+        self._rt = runtime
+        self._h = ctypes.c_void_p(handle)
+
+    @property
+    def handle(self):
+        return self._h
+
+    @property
+    def rows(self) -> int:
+        return int(lib().vh_fp8_rows(self._h))
+
+    @property
+    def k(self) -> int:
+        return int(lib().vh_fp8_k(self._h))
+
+    def __del__(self):
+        try:
+            if self._h and self._h.value:
+                lib().vh_fp8_free(self._h)
+                self._h = ctypes.c_void_p(None)
+        except Exception:
+            pass
+
+
+class LinearFp8:
+    """A projection with e4m3 weights; float input rows are quantised per run."""
+
+    def __init__(self, runtime: "Runtime", handle: int):
+        self._rt = runtime
+        self._h = ctypes.c_void_p(handle)
+
+    def input_features(self) -> int:
+        return int(lib().vh_linear_fp8_input_features(self._h))
+
+    def output_features(self) -> int:
+        return int(lib().vh_linear_fp8_output_features(self._h))
+
+    def run(self, x: Tensor, rows: int, out: Tensor) -> None:
+        _check(lib().vh_linear_fp8_run(self._h, x.handle, rows, out.handle))
+
+    def run_gelu(self, x: Tensor, rows: int, out: Tensor) -> None:
+        _check(lib().vh_linear_fp8_run_gelu(self._h, x.handle, rows, out.handle))
+
+    def run_residual(self, x: Tensor, rows: int, residual: Tensor) -> None:
+        _check(lib().vh_linear_fp8_run_residual(self._h, x.handle, rows, residual.handle))
+
+    def run_rows(self, x: Fp8Tensor, out: Tensor) -> None:
+        """The same from rows quantised before, once for every projection that reads them."""
+        _check(lib().vh_linear_fp8_run_rows(self._h, x.handle, out.handle))
+
+    def run_rows_gelu(self, x: Fp8Tensor, out: Tensor) -> None:
+        _check(lib().vh_linear_fp8_run_rows_gelu(self._h, x.handle, out.handle))
+
+    def run_rows_residual(self, x: Fp8Tensor, residual: Tensor) -> None:
+        _check(lib().vh_linear_fp8_run_rows_residual(self._h, x.handle, residual.handle))
+
+    def __del__(self):
+        try:
+            if self._h and self._h.value:
+                lib().vh_linear_fp8_free(self._h)
                 self._h = ctypes.c_void_p(None)
         except Exception:
             pass
@@ -873,6 +978,63 @@ class Runtime:
                                         free_pages.handle, free_start.handle, page_tokens, table.handle,
                                         max_pages, starts.handle, lens.handle, slots.handle, len(slots),
                                         free_next.handle))
+
+    # -- rows in 8-bit floating point
+    def _fp8(self, fn, *args) -> Fp8Tensor:
+        out = ctypes.c_void_p()
+        _check(fn(self._h, *args, ctypes.byref(out)))
+        return Fp8Tensor(self, out.value)
+
+    def alloc_fp8(self, rows: int, k: int) -> Fp8Tensor:
+        return self._fp8(lib().vh_fp8_alloc, rows, k)
+
+    def fp8_upload(self, codes, exponents, rows: int, k: int) -> Fp8Tensor:
+        """codes: rows x k bytes; exponents: rows x ceil(k / 128) bytes, 127 for a scale of one."""
+        c, e = _bytes(codes, rows * k), _bytes(exponents, rows * -(-k // 128))
+        return self._fp8(lib().vh_fp8_upload, c.ctypes.data, e.ctypes.data, rows, k)
+
+    def fp8_download(self, t: Fp8Tensor):
+        """(codes [rows, k], exponents [rows, ceil(k / 128)])."""
+        c, e = np.zeros((t.rows, t.k), np.uint8), np.zeros((t.rows, -(-t.k // 128)), np.uint8)
+        _check(lib().vh_fp8_download(self._h, t.handle, c.ctypes.data, e.ctypes.data))
+        return c, e
+
+    def quantize_fp8(self, x: Tensor, rows: int, k: int) -> Fp8Tensor:
+        return self._fp8(lib().vh_quantize_fp8, x.handle, rows, k)
+
+    def quantize_fp8_into(self, x: Tensor, rows: int, k: int, out: Fp8Tensor) -> None:
+        _check(lib().vh_quantize_fp8_into(self._h, x.handle, rows, k, out.handle))
+
+    def dequantize_fp8_into(self, t: Fp8Tensor, out: Tensor) -> None:
+        """The values that the codes stand for."""
+        _check(lib().vh_dequantize_fp8_into(self._h, t.handle, out.handle))
+
+    def gemm_fp8_into(self, a: Fp8Tensor, b: Fp8Tensor, c: Tensor) -> None:
+        """c [a.rows, b.rows] = a . b^T."""
+        _check(lib().vh_gemm_fp8_into(self._h, a.handle, b.handle, c.handle))
+
+    def _linear_fp8(self, fn, *args) -> LinearFp8:
+        out = ctypes.c_void_p()
+        _check(fn(self._h, *args, ctypes.byref(out)))
+        return LinearFp8(self, out.value)
+
+    def prepare_linear_fp8(self, input_features: int, output_features: int, weight, bias=None,
+                           gamma=None) -> LinearFp8:
+        """weight: floats [K, N], quantised on the device."""
+        n = output_features
+        w = _vector(weight, input_features * n)
+        b, g = (None if v is None else _vector(v, n) for v in (bias, gamma))
+        return self._linear_fp8(lib().vh_prepare_linear_fp8, input_features, n, _fp(w),
+                                _fp(b) if b is not None else None, _fp(g) if g is not None else None)
+
+    def prepare_linear_fp8_blocks(self, input_features: int, output_features: int, codes, scales, bias=None,
+                                  gamma=None) -> LinearFp8:
+        """codes: e4m3 bytes [N, K]; scales: a float for each 128 x 128 of them."""
+        k, n = input_features, output_features
+        c, s = _bytes(codes, n * k), _vector(scales, -(-n // 128) * -(-k // 128))
+        b, g = (None if v is None else _vector(v, n) for v in (bias, gamma))
+        return self._linear_fp8(lib().vh_prepare_linear_fp8_blocks, k, n, c.ctypes.data, _fp(s),
+                                _fp(b) if b is not None else None, _fp(g) if g is not None else None)
 
     # -- profiling
     def profile_enable(self, on: bool = True) -> None:
