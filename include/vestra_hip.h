@@ -52,6 +52,7 @@ typedef struct vh_conv2d vh_conv2d;       /* prepared 2-D convolution (DPT head)
 typedef struct vh_conv_transpose2d vh_conv_transpose2d; /* prepared transposed convolution */
 typedef struct vh_fp8_tensor vh_fp8_tensor; /* device rows of e4m3 values */
 typedef struct vh_linear_fp8 vh_linear_fp8; /* projection with e4m3 weights */
+typedef struct vh_cross_kv vh_cross_kv;   /* keys and values of an encoder's states */
 typedef struct vh_index vh_index;         /* device int32 values */
 typedef struct vh_rope vh_rope;           /* prepared rotation of several position axes */
 typedef struct vh_kv_cache vh_kv_cache;   /* paged cache of keys and values */
@@ -585,6 +586,49 @@ vh_status vh_linear_fp8_run_rows(const vh_linear_fp8 *linear, const vh_fp8_tenso
 vh_status vh_linear_fp8_run_rows_gelu(const vh_linear_fp8 *linear, const vh_fp8_tensor *input, vh_tensor *out);
 vh_status vh_linear_fp8_run_rows_residual(const vh_linear_fp8 *linear, const vh_fp8_tensor *input,
                                           vh_tensor *residual);
+
+/* ---- attention over an encoder's states ------------------------------------------ */
+/* No counterpart in the reference.  Keys and values of `images` images of up to `tokens`
+ * tokens each, kv_heads heads of head_dim (a multiple of 4 up to 128), formed once and read
+ * by every query that comes after: no tokens at first.  Values are scaled by a power of
+ * two so that the largest magnitude lies in [2^14, 2^15), of K over each head of an
+ * image, of V over each dim of a head of an image, and held
+ *   type 0: in two binary16 halves: 22 bits of a value down to 2^-18 of the largest, and
+ *           2^-40 of the largest below that;
+ *   type 1: in one, rounded to nearest even: 11 bits down to 2^-28 of the largest.
+ * 1 to 65535 images and heads, 1 to 2^30 tokens.  Not to be made inside a stream
+ * capture.  Every handle of a call has to belong to one runtime (clones count as one). */
+vh_status vh_cross_kv_new(const vh_runtime *rt, int type, size_t images, size_t tokens, size_t kv_heads,
+                          size_t head_dim, vh_cross_kv **out);
+void vh_cross_kv_free(vh_cross_kv *kv);
+/* Replaces what every image has by the K and V rows of `tokens` tokens (no more than it
+ * was made for): [images, kv_heads, tokens, head_dim], or [images, tokens, kv_heads,
+ * head_dim] when token_major.  seen [images * tokens] or NULL: a token with a 0 there is
+ * left out, as is anything that it holds (infinities and NaN too); an image may have none
+ * that is seen. */
+vh_status vh_cross_kv_write_f32(vh_cross_kv *kv, const vh_tensor *k, const vh_tensor *v, size_t tokens,
+                                int token_major, const vh_index *seen);
+/* The same from rows of a KV projection, [images * tokens, 2 * kv_heads * head_dim] as
+ * vh_linear_run writes them: K, then V, heads in order. */
+vh_status vh_cross_kv_write_rows_f32(vh_cross_kv *kv, const vh_tensor *rows, size_t tokens, const vh_index *seen);
+/* What is stored, as floats: k and v [images, tokens it was made for, kv_heads, head_dim],
+ * the seen tokens in order and zeros behind them; lens [images], their numbers, or NULL. */
+vh_status vh_cross_kv_read_f32(const vh_cross_kv *kv, vh_tensor *k, vh_tensor *v, vh_index *lens);
+/* out[i, t, h] = sum_j p_j v_j, p = softmax over the seen tokens j of image i of
+ * q[i, t, h] . k_j / sqrt(head_dim), with q and out [images, heads, tokens, head_dim], or
+ * [images, tokens, heads, head_dim] when token_major; heads % kv_heads == 0 and query head
+ * h reads head h / (heads / kv_heads).  The number of queries has nothing to do with
+ * that of the states.  Zeros where an image has no token to see.  A query row is scaled and
+ * held in two halves as type 0 is; statistics and sums are 32 bits.  A key that is not
+ * finite leaves no defined row of its image and head, a value none in its dim.  The same
+ * call gives the same bits.  At most 2^30 query rows (tokens * heads) of an image.
+ * The parts of rows whose keys several workgroups share lie in a workspace of the
+ * runtime (140 MB at most).  A call inside a stream capture takes it for its graph alone, until
+ * the runtime ends; where none is left (nothing as large ran since the last capture)
+ * the graph goes without: slower where there are few rows, its last bits other than an
+ * eager call's. */
+vh_status vh_cross_attention_f32(const vh_cross_kv *kv, const vh_tensor *q, size_t heads, size_t tokens,
+                                 int token_major, vh_tensor *out);
 
 /* ---- profiling (device twin of DA3_FLASH_PROFILE, src/specialized.rs:1324) - */
 /* When enabled, every kernel launch is bracketed by HIP events on the

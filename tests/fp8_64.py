@@ -66,3 +66,39 @@ def block_values(codes, scales):
 
 def gelu(x):
     return x * 0.5 * np.vectorize(math.erfc)(-x * math.sqrt(0.5))
+
+
+# ---- an encoder's states --------------------------------------------------------------
+
+
+def halves(x, amax, parts):
+    """x as `parts` binary16 halves of x 2^-e hold it, amax 2^-e in [2^14, 2^15)."""
+    _, e = np.frexp(amax.astype(np.float64))
+    e = np.where(amax == 0, 0, e - 15)
+    s = np.ldexp(np.asarray(x, np.float64), -e)
+    hi = s.astype(np.float16).astype(np.float64)
+    lo = (s - hi).astype(np.float32).astype(np.float16).astype(np.float64) if parts == 2 else 0.0
+    return np.ldexp(hi + lo, e)
+
+
+def stored(k, v, kind, seen=None):
+    """K and V [tokens, heads, dim] of one image as its states hold them: the seen tokens."""
+    if seen is not None:
+        k, v = k[seen != 0], v[seen != 0]
+    if not len(k):
+        return k.astype(np.float64), v.astype(np.float64)
+    parts = 2 if kind == "f32" else 1
+    top = lambda x, axis: np.max(np.where(np.isfinite(x), np.abs(x), 0), axis, keepdims=True)  # noqa: E731
+    return halves(k, top(k, (0, 2)), parts), halves(v, top(v, 0), parts)
+
+
+def attention(q, k, v):
+    """One image: q [n, heads, d], k and v [tokens, kv_heads, d] -> [n, heads, d]."""
+    n, heads, d = q.shape
+    out = np.zeros(q.shape)
+    for h in range(heads if len(k) else 0):
+        one = h // (heads // k.shape[1])
+        s = q[:, h].astype(np.float64) @ k[:, one].T / np.sqrt(d)
+        p = np.exp(s - s.max(1, keepdims=True))
+        out[:, h] = p @ v[:, one] / p.sum(1, keepdims=True)
+    return out

@@ -1,0 +1,889 @@
+// Keys and values of an encoder's states, stored once, and the attention of a decoder's
+// queries over them (kernels.h CrossView, CrossAttn), on the f16 matrix cores.
+//
+// Stored: scaled by a power of two so that the largest magnitude lies in [2^14, 2^15) --
+// of K over an image's head, of V over each dim of it -- a value is a half (kCrossF16),
+// or two, hi = f16(v) and lo = f16(v - hi), 22 bits and lo's sign (kCrossF32).  Tokens
+// that the mask leaves out are not stored, so the attention knows lengths and no mask.
+//
+// Products: S^T = K . Q^T and O^T += V^T . P^T with Q and P split the same way (Q by an
+// exponent of its own row, P held as 2^5 p), lo . lo left out: three products of
+// floats, two of halves.  Each is exact in the f32 sums of v_mfma_f32_16x16x32_f16.  A
+// stored value is off by at most 2^-25 of the half's scale, so by 2^-40 of the largest
+// where it is below 2^-18 of it.
+//
+// Layout: a block is 32 keys of a head, K and then V, in the order in which a wave wants
+// them: 1 KB, 16 bytes a lane, is one operand.  Memory to LDS, LDS to registers and
+// memory to registers are all linear.  Operand (c, t) of K: lane (li, lh) has dims 32 c
+// + 8 lh .. + 7 of key 16 t + li.  A lane then holds its own query's scores of keys 16 t
+// + 4 lh + r, which is the B operand of V^T . P^T if the 32 keys are taken in the order
+// (4 lh .. + 3 of tile 0, then of tile 1): operand df of V holds those of dim 16 df + li.
+//
+// Work is tiles of query rows (tokens times the query heads that share a head of K and
+// V), and the key steps of all tiles, end to end, in equal shares of the workgroups.  The
+// lengths are on the device: every workgroup forms the partition from them.
+#include <algorithm>
+
+#include "common.h"
+#include "kernels.h"
+#include "split_gemm.h"
+
+namespace vh {
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kPBits = 5.0f;     // P is held as 2^kPBits p
+constexpr float kMaxSlack = 8.0f;  // scores may pass the running maximum by this (base 2)
+
+template <int KIND>
+constexpr int kParts = KIND == kCrossF32 ? 2 : 1;
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// max / sum with the lanes 16 and 32 away, on the VALU: a permlane swap of two
+// copies of v leaves v in one and the partner's v in the other, in either order.
+__device__ __forceinline__ void swap16(float &a, float &b) {
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ void swap32(float &a, float &b) {
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ float max_groups(float v) {
+    float a = v, b = v;
+    swap16(a, b);
+    a = b = fmaxf(a, b);
+    swap32(a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+// Two floats to two halves, and what these leave of them (the empty asm keeps the
+// compiler from converting each again where a half is used).
+__device__ __forceinline__ f16x2 cvt_pk_f16(float a, float b) {
+    f16x2 h;
+    h[0] = (_Float16)a;
+    h[1] = (_Float16)b;
+    uint32_t u = __builtin_bit_cast(uint32_t, h);
+    asm("" : "+v"(u));
+    return __builtin_bit_cast(f16x2, u);
+}
+__device__ __forceinline__ f16x2 residual_pk_f16(f16x2 h, float a, float b) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    return cvt_pk_f16(__builtin_fmaf((float)h[0], minus, a), __builtin_fmaf((float)h[1], minus, b));
+}
+__device__ __forceinline__ void split8(f32x4 a, f32x4 b, f16x8 &hi, f16x8 &lo) {
+    f16x2 h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        h[i] = cvt_pk_f16(a[2 * i], a[2 * i + 1]);
+        l[i] = residual_pk_f16(h[i], a[2 * i], a[2 * i + 1]);
+        h[2 + i] = cvt_pk_f16(b[2 * i], b[2 * i + 1]);
+        l[2 + i] = residual_pk_f16(h[2 + i], b[2 * i], b[2 * i + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        hi[i] = h[i / 2][i % 2];
+        lo[i] = l[i / 2][i % 2];
+    }
+}
+
+__device__ __forceinline__ uint32_t finite_max(uint32_t mx, float v) {
+    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+    return max(mx, b < 0x7f800000u ? b : 0u);
+}
+
+// ---- storing ------------------------------------------------------------------------
+
+constexpr int kHeadGroup = 8;  // heads of a workgroup of range_kernel
+
+// Of a chunk of an image's tokens: the largest finite magnitudes of K of each head and of
+// V of each dim, into ranges [images][chunks][heads][1 + D], and where the seen tokens
+// go (kept [images][capacity], the tokens in order; lens).
+template <int D>
+__global__ __launch_bounds__(256) void cross_range_kernel(CrossWrite w) {
+    __shared__ uint32_t vmax[kHeadGroup * D], kmax[kHeadGroup];
+    __shared__ long long tmp[4];
+    const int tid = threadIdx.x, chunk = blockIdx.x, img = blockIdx.z;
+    const int h0 = blockIdx.y * kHeadGroup, heads = min(kHeadGroup, w.view.kv_heads - h0);
+    const int from = chunk * w.chunk, to = min(from + w.chunk, w.tokens);
+    const int *seen = w.seen ? w.seen + (size_t)img * w.tokens : nullptr;
+    for (int i = tid; i < kHeadGroup * D; i += 256) vmax[i] = 0;
+    if (tid < kHeadGroup) kmax[tid] = 0;
+    if (blockIdx.y == 0) {
+        if (seen) {
+            int n = 0;
+            for (int i = tid; i < from; i += 256) n += seen[i] != 0;
+            long long before = 0, all = 0;
+            scan_all<256>(n, tmp, &before);
+            for (int i0 = from; i0 < to; i0 += 256) {
+                const int i = i0 + tid;
+                const bool there = i < to && seen[i] != 0;
+                const long long end = before + scan_all<256>(there, tmp, &all);
+                if (there) w.kept[(size_t)img * w.view.tokens + end - 1] = i;
+                before += all;
+            }
+            if (tid == 0 && to == w.tokens) w.view.lens[img] = (int)before;
+        } else if (tid == 0 && to == w.tokens) {
+            w.view.lens[img] = w.tokens;
+        }
+    }
+    __syncthreads();
+    const int per = w.head_dim / 4, columns = heads * per;
+    int rows = 1;  // tokens at once
+    while (rows * 2 * columns <= 256) rows *= 2;
+    for (int c0 = 0; c0 < columns; c0 += 256) {
+        const int c = rows > 1 ? tid % columns : c0 + tid, first = rows > 1 ? tid / columns : 0;
+        if (c >= columns || first >= rows) continue;
+        const int h = c / per, d = 4 * (c % per);
+        const size_t off = (size_t)img * w.kv_image + (h0 + h) * w.kv_head + d;
+        uint32_t km = 0, vm[4] = {0, 0, 0, 0};
+        for (int t = from + first; t < to; t += rows) {
+            if (seen && !seen[t]) continue;
+            const f32x4 k = *reinterpret_cast<const f32x4 *>(w.k + off + t * w.kv_token);
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(w.v + off + t * w.kv_token);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                km = finite_max(km, k[i]);
+                vm[i] = finite_max(vm[i], v[i]);
+            }
+        }
+        atomicMax(&kmax[h], km);
+#pragma unroll
+        for (int i = 0; i < 4; i++) atomicMax(&vmax[h * D + d + i], vm[i]);
+    }
+    __syncthreads();
+    uint32_t *out = w.ranges + (((size_t)img * gridDim.x + chunk) * w.view.kv_heads + h0) * (1 + D);
+    for (int i = tid; i < heads * (1 + D); i += 256) {
+        const int h = i / (1 + D), d = i % (1 + D);
+        out[i] = d ? vmax[h * D + d - 1] : kmax[h];
+    }
+}
+
+// 128 keys of an image's head to their blocks, a block a wave; zeros behind the last key.
+template <int KIND, int D>
+__global__ __launch_bounds__(256) void cross_write_kernel(CrossWrite w) {
+    constexpr int NP = kParts<KIND>, C = D / 32, DF = D / 16;
+    __shared__ int exps[1 + D];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lh = lane >> 4;
+    const int g = blockIdx.y, img = blockIdx.z, len = w.view.lens[img];
+    if ((int)blockIdx.x * 128 >= len && blockIdx.x) return;
+    for (int i = tid; i < 1 + D; i += 256) {
+        uint32_t mx = 0;
+        for (int c = 0; c < w.chunks; c++)
+            mx = max(mx, w.ranges[(((size_t)img * w.chunks + c) * w.view.kv_heads + g) * (1 + D) + i]);
+        exps[i] = split_exponent(mx);
+        if (blockIdx.x == 0) {
+            if (i == 0) w.view.k_exp[(size_t)img * w.view.kv_heads + g] = exps[0];
+            else w.view.v_exp[((size_t)img * w.view.kv_heads + g) * D + i - 1] = exps[i];
+        }
+    }
+    __syncthreads();
+    const int block = blockIdx.x * 4 + wave, key0 = block * 32;
+    if ((int)blockIdx.x * 128 >= len) return;
+    char *out = w.view.at(img, g) + (size_t)block * cross_block_bytes(KIND, D) + lane * 16;
+    const int *kept = w.seen ? w.kept + (size_t)img * w.view.tokens : nullptr;
+    auto token = [&](int key) { return key < len ? (kept ? kept[key] : key) : -1; };
+    const size_t off = (size_t)img * w.kv_image + g * w.kv_head;
+    auto put = [&](int operand, f32x4 a, f32x4 b) {
+        f16x8 hi, lo;
+        split8(a, b, hi, lo);
+        *reinterpret_cast<f16x8 *>(out + (operand * NP) * 1024) = hi;
+        if constexpr (NP == 2) *reinterpret_cast<f16x8 *>(out + (operand * NP + 1) * 1024) = lo;
+    };
+    const int ke = exps[0];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int from = token(key0 + 16 * t + li);
+        const float *row = w.k + off + max(from, 0) * w.kv_token;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            f32x4 x[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int d = 32 * c + 8 * lh + 4 * e;
+                x[e] = from >= 0 && d < w.head_dim ? *reinterpret_cast<const f32x4 *>(row + d)
+                                                   : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[e][i] = __builtin_ldexpf(x[e][i], -ke);
+            }
+            put(2 * c + t, x[0], x[1]);
+        }
+    }
+    int from[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) from[j] = token(key0 + 16 * (j / 4) + 4 * lh + j % 4);
+#pragma unroll
+    for (int df = 0; df < DF; df++) {
+        const int d = 16 * df + li, e = exps[1 + d];
+        f32x4 x[2];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            x[j / 4][j % 4] = from[j] >= 0 && d < w.head_dim
+                                  ? __builtin_ldexpf(w.v[off + from[j] * w.kv_token + d], -e) : 0.0f;
+        put(2 * C + df, x[0], x[1]);
+    }
+}
+
+// What is stored, as floats [images][capacity][heads][head_dim]; zeros behind the last key.
+template <int KIND, int D>
+__global__ __launch_bounds__(256) void cross_read_kernel(CrossView view, int head_dim, float *k, float *v, int *lens) {
+    constexpr int NP = kParts<KIND>, C = D / 32, DF = D / 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lh = lane >> 4;
+    const int g = blockIdx.y, img = blockIdx.z, len = view.lens[img];
+    if (lens && tid == 0 && g == 0 && blockIdx.x == 0) lens[img] = len;
+    const int block = blockIdx.x * 4 + wave, key0 = block * 32;
+    if (key0 >= view.tokens) return;
+    const char *in = view.at(img, g) + (size_t)block * cross_block_bytes(KIND, D) + lane * 16;
+    const bool any = key0 < len;
+    const int ke = view.k_exp[(size_t)img * view.kv_heads + g];
+    auto get = [&](int operand, float (&x)[8]) {
+        const f16x8 hi = *reinterpret_cast<const f16x8 *>(in + operand * NP * 1024);
+        const f16x8 lo = *reinterpret_cast<const f16x8 *>(in + (operand * NP + NP - 1) * 1024);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)hi[i] + (NP == 2 ? (float)lo[i] : 0.0f);
+    };
+    auto row = [&](int key) { return (((size_t)img * view.tokens + key) * view.kv_heads + g) * head_dim; };
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int key = key0 + 16 * t + li;
+            float x[8] = {};
+            if (any) get(2 * c + t, x);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int d = 32 * c + 8 * lh + 4 * e;
+                f32x4 y;
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = key < len ? __builtin_ldexpf(x[4 * e + i], ke) : 0.0f;
+                if (key < view.tokens && d < head_dim) *reinterpret_cast<f32x4 *>(k + row(key) + d) = y;
+            }
+        }
+#pragma unroll
+    for (int df = 0; df < DF; df++) {
+        const int d = 16 * df + li;
+        const int ve = view.v_exp[((size_t)img * view.kv_heads + g) * D + d];
+        float x[8] = {};
+        if (any) get(2 * C + df, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int key = key0 + 16 * (j / 4) + 4 * lh + j % 4;
+            if (key < view.tokens && d < head_dim) v[row(key) + d] = key < len ? __builtin_ldexpf(x[j], ve) : 0.0f;
+        }
+    }
+}
+
+// ---- the partition --------------------------------------------------------------------
+
+// What a tile costs besides its key steps, in steps: queries fetched, first loads waited
+// for, output written.
+constexpr int kTileCost = 2;
+
+// A tile of query rows: image, head of K and V, its rows.
+struct Tile {
+    int img, g, row, rows, len, steps;
+};
+
+template <int BM>
+__device__ __forceinline__ Tile tile_of(const CrossAttn &a, int img, int len, int index, int step) {
+    Tile t;
+    t.img = img;
+    t.g = index / a.tiles;
+    t.row = (index - t.g * a.tiles) * BM;
+    t.rows = min(BM, a.queries * a.group - t.row);
+    t.len = len;
+    t.steps = (len + step - 1) / step;
+    return t;
+}
+
+// Steps of a tile of an image, with what it costs itself.
+__device__ __forceinline__ int cost_of(const CrossAttn &a, int img, int step) {
+    return (a.view.lens[img] + step - 1) / step + kTileCost;
+}
+
+// Sums over the images, and in `base` and `where` the image that unit `at(total)` is in
+// and the units before it.
+template <int THREADS, class F>
+__device__ __forceinline__ long long find_image(const CrossAttn &a, int step, F at, int &where, long long &base) {
+    __shared__ long long tmp[THREADS / 64], found[2];
+    const long long per = (long long)a.tiles * a.view.kv_heads;
+    long long total = 0, all = 0, end = 0, cost = 0;
+    for (int i0 = 0; i0 < a.images; i0 += THREADS) {
+        const int i = i0 + threadIdx.x;
+        cost = i < a.images ? per * cost_of(a, i, step) : 0;
+        end = total + scan_all<THREADS>(cost, tmp, &all);
+        total += all;
+    }
+    const long long unit = at(total);
+    if (threadIdx.x == 0) found[0] = -1;
+    __syncthreads();
+    if (a.images <= THREADS) {
+        if (end - cost <= unit && unit < end) {
+            found[0] = threadIdx.x;
+            found[1] = end - cost;
+        }
+    } else {
+        long long before = 0;
+        for (int i0 = 0; i0 < a.images; i0 += THREADS) {
+            const int i = i0 + threadIdx.x;
+            cost = i < a.images ? per * cost_of(a, i, step) : 0;
+            end = before + scan_all<THREADS>(cost, tmp, &all);
+            before += all;
+            if (end - cost <= unit && unit < end) {
+                found[0] = i;
+                found[1] = end - cost;
+            }
+        }
+    }
+    __syncthreads();
+    where = (int)found[0];
+    base = found[1];
+    return total;
+}
+
+// ---- parts ------------------------------------------------------------------------------
+
+// Where the last workgroup of a tile joins them they are read and written past the L2 of
+// an XCD (sc1), as the workgroups of a tile may be on several.
+struct Parts {
+    __amdgpu_buffer_rsrc_t base;
+    __device__ __forceinline__ explicit Parts(const CrossAttn &a)
+        : base(__builtin_amdgcn_make_buffer_rsrc(a.parts, 0, 0xffffffff, 0x00027000)) {}
+    static constexpr int kAgent = 16;
+    __device__ __forceinline__ void put(uint32_t at, f32x4 v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), base, at, 0, kAgent);
+    }
+    __device__ __forceinline__ void put(uint32_t at, float x, float y) const {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(x), __float_as_uint(y)}, base, at, 0, kAgent);
+    }
+    __device__ __forceinline__ f32x4 four(uint32_t at) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(base, at, 0, kAgent));
+    }
+    __device__ __forceinline__ u32x2 two(uint32_t at) const {
+        return __builtin_amdgcn_raw_buffer_load_b64(base, at, 0, kAgent);
+    }
+};
+// Offsets in bytes of row `in` of part x: [2 shares][BM][D] sums, then [2 shares][BM]
+// maxima and sums of weights.
+template <int BM, int D>
+__device__ __forceinline__ uint32_t sums_at(uint32_t x, int in) {
+    return (x * BM + in) * (D * 4);
+}
+template <int BM, int D>
+__device__ __forceinline__ uint32_t weights_at(const CrossAttn &a, uint32_t x, int in) {
+    return 2u * a.shares * BM * D * 4 + (x * BM + in) * 8;
+}
+
+// Row `in` of a tile, four dims from d on: the result, or a workgroup's part of it.
+template <int BM, int D>
+__device__ __forceinline__ void put_row(const CrossAttn &a, const Tile &t, int part, int in, int d, f32x4 v, float m,
+                                        float l) {
+    if (in >= t.rows) return;
+    if (part < 0) {
+        if (d >= a.head_dim) return;
+        const int row = t.row + in, token = row / a.group, head = t.g * a.group + row % a.group;
+        const float inv = 1.0f / l;
+        const int *e = a.view.v_exp + ((size_t)t.img * a.view.kv_heads + t.g) * D + d;
+        f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = l == 0.0f ? 0.0f : __builtin_ldexpf(v[i] * inv, e[i]);
+        *reinterpret_cast<f32x4 *>(a.out + t.img * a.q_image + token * a.q_token + head * a.q_head + d) = y;
+    } else {
+        const Parts parts(a);
+        parts.put(sums_at<BM, D>(part, in) + 4 * d, v);
+        if (d == 0) parts.put(weights_at<BM, D>(a, part, in), m, l);
+    }
+}
+
+// A row's four dims of a part, or of several: O on the maximum m, and the sum of weights.
+struct Sums {
+    float m, l;
+    f32x4 y;
+    __device__ __forceinline__ void join(const Sums &b) {
+        const float mn = fmaxf(m, b.m);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        const float fb = b.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(b.m - mn);
+        m = mn;
+        l = l * f + b.l * fb;
+        y = y * f + b.y * fb;
+    }
+};
+
+// The parts of shares w0 .. w1 (of w0 the one at part0) become the tile's output.  Of the
+// workgroup's groups of D / 4 lanes (a group holds a row) as many share a row as the rows
+// leave: a single query's parts are summed by all of them.
+template <int BM, int D, int THREADS>
+__device__ void join_parts(const CrossAttn &a, const Tile &t, int w0, int w1, int part0, char *smem) {
+    Sums *some = reinterpret_cast<Sums *>(smem);
+    const Parts parts(a);
+    constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
+    int rows = 1;  // at once
+    while (rows < GROUPS && rows < t.rows) rows *= 2;
+    const int sharers = GROUPS / rows;
+    const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+    for (int in = group % rows; in < (t.rows + rows - 1) / rows * rows; in += rows) {
+        auto part = [&](int w) {
+            const int x = w == w0 ? part0 : 2 * w, row = min(in, t.rows - 1);
+            const u32x2 ml = parts.two(weights_at<BM, D>(a, x, row));
+            return Sums{__uint_as_float(ml[0]), __uint_as_float(ml[1]), parts.four(sums_at<BM, D>(x, row) + 4 * d)};
+        };
+        Sums sum{-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int w = w0 + group / rows; w <= w1; w += 4 * sharers) {
+            Sums x[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = part(min(w + u * sharers, w1));
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (w + u * sharers <= w1) sum.join(x[u]);
+        }
+        if (sharers > 1) {  // all rows at once
+            some[threadIdx.x] = sum;
+            __syncthreads();
+            if (group < rows)
+                for (int i = 1; i < sharers; i++) sum.join(some[threadIdx.x + i * rows * LANES]);
+        }
+        if (group < rows && in < t.rows) put_row<BM, D>(a, t, -1, in, d, sum.y, sum.m, sum.l);
+    }
+}
+
+// Walks this workgroup's steps tile by tile: f(tile, first step, steps, part).  Without room
+// for parts (a.parts null) every workgroup takes whole tiles.  Of the workgroups that
+// hold a part of a tile the one that is done last joins them, in the order of the shares.
+// They count in the counter of the tile's first share (of which it is the last tile, so no
+// other counts there), zero before and after.
+template <int BM, int STEP, int THREADS, int D, class F>
+__device__ __forceinline__ void walk(const CrossAttn &a, char *smem, F f) {
+    __shared__ int is_last;
+    const int w = (blockIdx.x & 7) * (a.shares >> 3) + (blockIdx.x >> 3);  // neighbours on one XCD
+    const int per = a.tiles * a.view.kv_heads;
+    if (!a.parts) {
+        const long long items = (long long)per * a.images;
+        for (long long at = w; at < items; at += a.shares) {
+            const int img = (int)(at / per);
+            const Tile t = tile_of<BM>(a, img, uniform(a.view.lens[img]), (int)(at - (long long)img * per), STEP);
+            f(t, 0, t.steps, -1);
+        }
+        return;
+    }
+    int img = 0;
+    long long base = 0, share = 1;
+    const long long total = find_image<THREADS>(a, STEP, [&](long long all) {
+        share = max(1ll, (all + a.shares - 1) / a.shares);
+        return w * share;
+    }, img, base);
+    long long at = w * share;
+    const long long end = min(at + share, total);
+    if (at >= end) return;
+    img = uniform(img);
+    int len = uniform(a.view.lens[img]), cost = (len + STEP - 1) / STEP + kTileCost;
+    int index = uniform((int)((at - base) / cost)), into = uniform((int)((at - base) - (long long)index * cost));
+    for (bool first = true; at < end; first = false) {
+        const Tile t = tile_of<BM>(a, img, len, index, STEP);
+        const int steps = uniform((int)min(end - at, (long long)cost - into));
+        const bool whole = into == 0 && steps == cost;
+        const int from = max(into - kTileCost, 0), to = max(into + steps - kTileCost, 0);
+        f(t, from, to - from, whole ? -1 : 2 * w + (first ? 0 : 1));
+        if (!whole) {
+            const long long begin = at - into;
+            const int w0 = uniform((int)(begin / share)), w1 = uniform((int)((begin + cost - 1) / share));
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's parts are out
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                unsigned *counter = a.counters + w0;
+                is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                          (unsigned)(w1 - w0);
+                if (is_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (is_last) {
+                join_parts<BM, D, THREADS>(a, t, w0, w1, 2 * w0 + (begin > w0 * share ? 1 : 0), smem);
+                __syncthreads();
+            }
+        }
+        at += steps;
+        into = 0;
+        if (++index == per) {
+            index = 0;
+            if (++img < a.images) {
+                len = uniform(a.view.lens[img]);
+                cost = (len + STEP - 1) / STEP + kTileCost;
+            }
+        }
+    }
+}
+
+// ---- one wave's arithmetic --------------------------------------------------------------
+
+// QT tiles of 16 queries: their operands, running maxima and sums, and O^T: o[df][u][r] =
+// O[query 16 u + li][16 df + 4 lh + r].
+template <int KIND, int D, int QT>
+struct Queries {
+    static constexpr int C = D / 32, DF = D / 16, NP = kParts<KIND>;
+    f16x8 qh[QT][C], ql[QT][C];
+    f32x4 o[DF][QT];
+    float m[QT], l[QT], scale[QT];
+
+    // Rows first .. first + 16 QT - 1 of the tile (rows past its end: zeros).
+    __device__ __forceinline__ void load(const CrossAttn &a, const Tile &t, int first, int li, int lh) {
+        const int ke = a.view.k_exp[(size_t)t.img * a.view.kv_heads + t.g];
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            const int in = first + 16 * u + li;
+            const bool there = in < t.rows;
+            const int row = t.row + (there ? in : 0), token = row / a.group, head = t.g * a.group + row % a.group;
+            const float *src = a.q + t.img * a.q_image + token * a.q_token + head * a.q_head;
+            f32x4 x[C][2];
+            uint32_t mx = 0;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int d = 32 * c + 8 * lh + 4 * e;
+                    x[c][e] = there && d < a.head_dim ? *reinterpret_cast<const f32x4 *>(src + d)
+                                                      : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx = finite_max(mx, x[c][e][i]);
+                }
+            mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, 64));
+            mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, 64));
+            const int e = split_exponent(mx);
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[c][0][i] = __builtin_ldexpf(x[c][0][i], -e);
+                    x[c][1][i] = __builtin_ldexpf(x[c][1][i], -e);
+                }
+                split8(x[c][0], x[c][1], qh[u][c], ql[u][c]);
+            }
+            // Kept off zero and infinity: a masked score (-inf) stays -inf.
+            scale[u] = fminf(fmaxf(__builtin_ldexpf(a.scale_log2, ke + e), 0x1p-126f), 0x1p127f);
+            m[u] = -INFINITY;
+            l[u] = 0.0f;
+#pragma unroll
+            for (int df = 0; df < DF; df++) o[df][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+
+    // Scores of 32 keys, the small products first; k(operand): NP consecutive operands.
+    template <class F>
+    __device__ __forceinline__ void scores(f32x4 (&s)[2][QT], F k) const {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int u = 0; u < QT; u++) s[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            f16x8 f[2][NP];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) f[t][p] = k((2 * c + t) * NP + p);
+            if constexpr (NP == 2)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int u = 0; u < QT; u++) s[t][u] = mfma16x16x32_f16(f[t][1], qh[u][c], s[t][u]);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int u = 0; u < QT; u++) s[t][u] = mfma16x16x32_f16(f[t][0], ql[u][c], s[t][u]);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int u = 0; u < QT; u++) s[t][u] = mfma16x16x32_f16(f[t][0], qh[u][c], s[t][u]);
+        }
+    }
+
+    // Keys from `left` on are behind the last.
+    __device__ __forceinline__ void mask(f32x4 (&s)[2][QT], int left, int lh) const {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (16 * t + 4 * lh + r >= left)
+#pragma unroll
+                    for (int u = 0; u < QT; u++) s[t][u][r] = -INFINITY;
+    }
+
+    // Brings the maxima up to those of H times 32 keys' scores.  They are only raised where
+    // a score passes one by kMaxSlack, so most steps need no correction.
+    template <int H>
+    __device__ __forceinline__ void raise(const f32x4 (&s)[H][2][QT]) {
+        float mx[QT];
+        bool over = false;
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            float v = s[0][0][u][0];
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                v = fmaxf(fmaxf(v, s[h][0][u][0]), s[h][0][u][1]);
+                v = fmaxf(fmaxf(v, s[h][0][u][2]), s[h][0][u][3]);
+                v = fmaxf(fmaxf(v, s[h][1][u][0]), s[h][1][u][1]);
+                v = fmaxf(fmaxf(v, s[h][1][u][2]), s[h][1][u][3]);
+            }
+            mx[u] = v * scale[u];
+            over |= mx[u] > m[u] + kMaxSlack;
+        }
+        if (__any(over)) {
+#pragma unroll
+            for (int u = 0; u < QT; u++) {
+                const float mn = fmaxf(m[u], max_groups(mx[u]));
+                const float corr = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
+                m[u] = mn;
+                l[u] *= corr;
+#pragma unroll
+                for (int df = 0; df < DF; df++) o[df][u] *= corr;
+            }
+        }
+    }
+
+    // The scores of 32 keys become their weights, which are summed and split.
+    __device__ __forceinline__ void weights(f32x4 (&s)[2][QT], f16x8 (&ph)[QT], f16x8 (&pl)[QT]) {
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            const float off = kPBits - (m[u] == -INFINITY ? 0.0f : m[u]);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    s[t][u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][u][r], scale[u], off));
+            l[u] += ((s[0][u][0] + s[0][u][1]) + (s[0][u][2] + s[0][u][3])) +
+                    ((s[1][u][0] + s[1][u][1]) + (s[1][u][2] + s[1][u][3]));
+            split8(s[0][u], s[1][u], ph[u], pl[u]);
+        }
+    }
+
+    // O^T += V^T . P^T for 32 keys; v(operand) as in scores.
+    template <class F>
+    __device__ __forceinline__ void add(const f16x8 (&ph)[QT], const f16x8 (&pl)[QT], F v) {
+#pragma unroll
+        for (int d0 = 0; d0 < DF; d0 += 2) {
+            f16x8 f[2][NP];
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) f[k][p] = v((d0 + k) * NP + p);
+            if constexpr (NP == 2)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int u = 0; u < QT; u++) o[d0 + k][u] = mfma16x16x32_f16(f[k][1], ph[u], o[d0 + k][u]);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int u = 0; u < QT; u++) o[d0 + k][u] = mfma16x16x32_f16(f[k][0], pl[u], o[d0 + k][u]);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int u = 0; u < QT; u++) o[d0 + k][u] = mfma16x16x32_f16(f[k][0], ph[u], o[d0 + k][u]);
+        }
+    }
+};
+
+// ---- few rows: 16 a tile, each of the four waves its own 32 keys of a step ----------------
+
+template <int D>
+constexpr int few_wave_bytes() {
+    return 16 * D * 4 + 128;  // the wave's O, maxima and sums
+}
+
+template <int KIND, int D>
+__global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
+    constexpr int BM = 16, STEP = 128, NP = kParts<KIND>, C = D / 32, DF = D / 16;
+    constexpr int BLOCK = cross_block_bytes(KIND, D), WAVE = few_wave_bytes<D>();
+    __shared__ __attribute__((aligned(16))) char smem[4 * WAVE < 256 * (int)sizeof(Sums) ? 256 * sizeof(Sums) : 4 * WAVE];
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lh = lane >> 4;
+    const int wave = uniform(tid >> 6);
+    walk<BM, STEP, 256, D>(a, smem, [&](const Tile &t, int step0, int steps, int part) {
+        const char *base = a.view.at(t.img, t.g) + lane * 16;
+        auto load = [&](int step, int operand) {
+            const size_t at = (size_t)(step * 4 + wave) * BLOCK + operand * 1024;
+            return __builtin_nontemporal_load(reinterpret_cast<const f16x8 *>(base + at));
+        };
+        // K of this step is in registers; V is loaded before the scores are formed, the next K
+        // before the weights meet V.
+        f16x8 k[2 * C * NP], v[DF * NP];
+        if (steps) {
+#pragma unroll
+            for (int i = 0; i < 2 * C * NP; i++) k[i] = load(step0, i);
+        }
+        Queries<KIND, D, 1> w;
+        w.load(a, t, 0, li, lh);
+        for (int i = 0; i < steps; i++) {
+            const int step = step0 + i, left = t.len - (step * 4 + wave) * 32;
+#pragma unroll
+            for (int x = 0; x < DF * NP; x++) v[x] = load(step, 2 * C * NP + x);
+            f32x4 s[1][2][1];
+            w.scores(s[0], [&](int x) { return k[x]; });
+            const int next = min(step + 1, step0 + steps - 1);
+#pragma unroll
+            for (int x = 0; x < 2 * C * NP; x++) k[x] = load(next, x);
+            if (left < 32) w.mask(s[0], left, lh);
+            w.raise(s);
+            f16x8 ph[1], pl[1];
+            w.weights(s[0], ph, pl);
+            w.add(ph, pl, [&](int x) { return v[x]; });
+        }
+        // The four waves' sums, each on its own maximum, joined by all threads.
+        float *o = reinterpret_cast<float *>(smem + wave * WAVE);
+#pragma unroll
+        for (int df = 0; df < DF; df++) *reinterpret_cast<f32x4 *>(o + li * D + 16 * df + 4 * lh) = w.o[df][0];
+        const float l = sum_groups(w.l[0]);
+        if (lh == 0) {
+            o[16 * D + 2 * li] = w.m[0];
+            o[16 * D + 2 * li + 1] = l;
+        }
+        __syncthreads();
+        const int row = tid >> 4;
+        float m = -INFINITY, sum = 0.0f, f[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) m = fmaxf(m, reinterpret_cast<float *>(smem + x * WAVE)[16 * D + 2 * row]);
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const float *y = reinterpret_cast<float *>(smem + x * WAVE) + 16 * D + 2 * row;
+            f[x] = y[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y[0] - m);
+            sum += y[1] * f[x];
+        }
+#pragma unroll
+        for (int d = 4 * (tid & 15); d < D; d += 64) {
+            f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                y += *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(smem + x * WAVE) + row * D + d) * f[x];
+            put_row<BM, D>(a, t, part, row, d, y, m, sum);
+        }
+        __syncthreads();
+    });
+}
+
+// ---- many rows: 128 a tile, 32 a wave, K and V of a step shared in LDS ----------------------
+
+template <int KIND, int D>
+constexpr int kManyHalves = KIND == kCrossF32 && D == 128 ? 1 : 2;  // blocks of 32 keys a step
+
+template <int KIND, int D>
+__global__ __launch_bounds__(256, 2) void cross_many_kernel(CrossAttn a) {
+    constexpr int BM = 128, QT = 2, H = kManyHalves<KIND, D>, STEP = 32 * H, NP = kParts<KIND>, C = D / 32;
+    constexpr int BLOCK = cross_block_bytes(KIND, D), BYTES = H * BLOCK;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lh = lane >> 4;
+    const int wave = uniform(tid >> 6);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+    walk<BM, STEP, 256, D>(a, smem, [&](const Tile &t, int step0, int steps, int part) {
+        const char *base = a.view.at(t.img, t.g);
+        auto copy = [&](int step, int buf) {
+            const char *from = base + (size_t)step * BYTES;
+#pragma unroll
+            for (int u = 0; u < BYTES / 4096; u++)
+                copy16_to_lds(from + (4 * u + wave) * 1024, lane * 16,
+                              uniform(lds0 + buf * BYTES + (4 * u + wave) * 1024));
+        };
+        if (steps) copy(step0, 0);
+        const int first = 16 * QT * wave;
+        Queries<KIND, D, QT> w;
+        w.load(a, t, first, li, lh);
+        for (int i = 0; i < steps; i++) {
+            const int buf = i & 1, key = (step0 + i) * STEP;
+            split_wait<0>();
+            __syncthreads();  // this step's panels are there, the last one's readers done
+            if (i + 1 < steps) copy(step0 + i + 1, buf ^ 1);
+            const char *panel = smem + buf * BYTES + lane * 16;
+            auto operand = [&](int h, int x) { return *reinterpret_cast<const f16x8 *>(panel + h * BLOCK + x * 1024); };
+            f32x4 s[H][2][QT];
+#pragma unroll
+            for (int h = 0; h < H; h++) w.scores(s[h], [&](int x) { return operand(h, x); });
+            if (key + STEP > t.len)
+#pragma unroll
+                for (int h = 0; h < H; h++) w.mask(s[h], t.len - key - 32 * h, lh);
+            w.raise(s);
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                f16x8 ph[QT], pl[QT];
+                w.weights(s[h], ph, pl);
+                w.add(ph, pl, [&](int x) { return operand(h, 2 * C * NP + x); });
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < QT; u++) {
+            const float l = sum_groups(w.l[u]);
+#pragma unroll
+            for (int df = 0; df < D / 16; df++)
+                put_row<BM, D>(a, t, part, first + 16 * u + li, 16 * df + 4 * lh, w.o[df][u], w.m[u], l);
+        }
+        __syncthreads();
+    });
+}
+
+constexpr int kShares = 512;
+static_assert(kShares <= kAttnCounters, "a counter for each share");
+
+bool few_rows(const CrossAttn &a) { return (size_t)a.queries * a.group <= 16; }
+
+template <int KIND, int D>
+hipError_t run_attn(hipStream_t s, CrossAttn a) {
+    if (few_rows(a)) {
+        cross_few_kernel<KIND, D><<<a.shares, 256, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    constexpr size_t bytes = std::max<size_t>(2 * kManyHalves<KIND, D> * cross_block_bytes(KIND, D), 256 * sizeof(Sums));
+    static std::atomic<uint64_t> done{0};
+    hipError_t e = ensure_dynamic_lds(cross_many_kernel<KIND, D>, bytes, done);
+    if (e != hipSuccess) return e;
+    cross_many_kernel<KIND, D><<<a.shares, 256, bytes, s>>>(a);
+    return hipGetLastError();
+}
+
+template <int KIND, int D>
+hipError_t run_write(hipStream_t s, const CrossWrite &w) {
+    const unsigned groups = (w.view.kv_heads + kHeadGroup - 1) / kHeadGroup, images = w.view.images;
+    cross_range_kernel<D><<<dim3(w.chunks, groups, images), 256, 0, s>>>(w);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    cross_write_kernel<KIND, D><<<dim3(std::max(1, (w.tokens + 127) / 128), w.view.kv_heads, images), 256, 0, s>>>(w);
+    return hipGetLastError();
+}
+
+template <int KIND, int D>
+hipError_t run_read(hipStream_t s, const CrossView &v, int head_dim, float *k, float *vv, int *lens) {
+    cross_read_kernel<KIND, D><<<dim3((v.tokens + 127) / 128, v.kv_heads, v.images), 256, 0, s>>>(v, head_dim, k, vv, lens);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Chunks of an image's tokens in cross_range_kernel: at most 32, of 64 tokens at least.
+int cross_chunks(size_t tokens) { return (int)std::min<size_t>(std::max<size_t>((tokens + 63) / 64, 1), 32); }
+
+hipError_t launch_cross_write(hipStream_t s, CrossWrite w) {
+    w.chunks = cross_chunks(w.tokens);
+    w.chunk = (w.tokens + w.chunks - 1) / w.chunks;
+    if (w.view.kind == kCrossF32) return w.view.width == 128 ? run_write<kCrossF32, 128>(s, w) : run_write<kCrossF32, 64>(s, w);
+    return w.view.width == 128 ? run_write<kCrossF16, 128>(s, w) : run_write<kCrossF16, 64>(s, w);
+}
+
+hipError_t launch_cross_read(hipStream_t s, const CrossView &v, size_t head_dim, float *k, float *vv, int *lens) {
+    const int hd = (int)head_dim;
+    if (v.kind == kCrossF32) return v.width == 128 ? run_read<kCrossF32, 128>(s, v, hd, k, vv, lens) : run_read<kCrossF32, 64>(s, v, hd, k, vv, lens);
+    return v.width == 128 ? run_read<kCrossF16, 128>(s, v, hd, k, vv, lens) : run_read<kCrossF16, 64>(s, v, hd, k, vv, lens);
+}
+
+size_t cross_attn_floats(const CrossAttn &a) {
+    return (size_t)2 * kShares * (few_rows(a) ? 16 : 128) * (a.view.width + 2);
+}
+
+hipError_t launch_cross_attn(hipStream_t s, CrossAttn a) {
+    a.shares = kShares;
+    a.tiles = (a.queries * a.group + (few_rows(a) ? 15 : 127)) / (few_rows(a) ? 16 : 128);
+    if (a.view.kind == kCrossF32) return a.view.width == 128 ? run_attn<kCrossF32, 128>(s, a) : run_attn<kCrossF32, 64>(s, a);
+    return a.view.width == 128 ? run_attn<kCrossF16, 128>(s, a) : run_attn<kCrossF16, 64>(s, a);
+}
+
+}  // namespace vh

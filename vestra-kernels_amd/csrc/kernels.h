@@ -434,4 +434,53 @@ constexpr size_t kAttnCounters = 1024;
 size_t cache_attn_floats(const CacheView &cache, size_t tokens, size_t group, size_t requests);
 hipError_t launch_cache_attn(hipStream_t s, CacheAttn a);
 
+// ---- an encoder's states and the attention over them (k_cross.hip) -------------
+// What a value is held in: two halves (22 bits), or one.
+constexpr int kCrossF32 = 0, kCrossF16 = 1;
+// 32 keys of a head, K and then V, width = 64 or 128 (columns past head_dim are zeros).
+__host__ __device__ constexpr int cross_block_bytes(int kind, int width) {
+    return 2 * 32 * width * (kind == kCrossF32 ? 4 : 2);
+}
+struct CrossView {
+    char *blocks;  // [images][kv_heads][capacity in blocks]
+    int *lens;     // [images] keys stored
+    int *k_exp;    // [images][kv_heads]
+    int *v_exp;    // [images][kv_heads][width]
+    int kind, images, tokens, kv_heads, width;  // tokens: capacity of an image
+    // Blocks of an image's head: whole steps of 128 keys.
+    __host__ __device__ size_t head_bytes() const {
+        return ((size_t)tokens + 127) / 128 * 4 * cross_block_bytes(kind, width);
+    }
+    __device__ char *at(int image, int g) const { return blocks + ((size_t)image * kv_heads + g) * head_bytes(); }
+};
+struct CrossWrite {
+    CrossView view;
+    const float *k, *v;  // rows of head_dim floats; strides in floats
+    size_t kv_image, kv_token, kv_head;
+    const int *seen;     // [images][tokens], or null: every token
+    int tokens, head_dim;
+    uint32_t *ranges;    // [images][cross_chunks(tokens)][kv_heads][1 + width]
+    int *kept;           // [images][capacity]
+    int chunks, chunk;   // set by the launcher
+};
+int cross_chunks(size_t tokens);
+hipError_t launch_cross_write(hipStream_t s, CrossWrite w);
+hipError_t launch_cross_read(hipStream_t s, const CrossView &v, size_t head_dim, float *k, float *vv, int *lens);
+struct CrossAttn {
+    CrossView view;
+    const float *q;
+    float *out;
+    size_t q_image, q_token, q_head;  // strides of both, in floats
+    int images, queries, group, head_dim;  // group = heads / kv_heads
+    float scale_log2;                 // softmax scale times log2(e)
+    // Room for the parts of tiles that several workgroups share (cross_attn_floats())
+    // and kAttnCounters counters, zero before and after, or null: every tile is one
+    // workgroup's.  Launches sharing them must not overlap in time.
+    float *parts;
+    unsigned *counters;
+    int shares, tiles;                // set by the launcher
+};
+size_t cross_attn_floats(const CrossAttn &a);
+hipError_t launch_cross_attn(hipStream_t s, CrossAttn a);
+
 }  // namespace vh

@@ -130,6 +130,8 @@ struct RtState {
     Workspace sx;                               // split rows of a projection's input
     Workspace f8;                               // e4m3 rows of a projection's input
     unsigned long long f8_capture = 0;          // the capture that took it, where it is recorded
+    Workspace xa;                               // counters and parts of the cross attention's tiles
+    unsigned long long xa_capture = 0;
     Workspace pa;                               // counters and parts of the paged attention's tiles
     unsigned long long pa_capture = 0;          // the capture that took it, where it is recorded
     std::vector<void *> recorded;               // outgrown blocks that a graph may hold
@@ -156,7 +158,7 @@ struct RtState {
         give_back();
         hipStreamSynchronize(stream);
         for (auto &kv : rope_cache) hipFree(kv.second);
-        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx, &f8, &pa})
+        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx, &f8, &xa, &pa})
             if (w->p) hipFree(w->p);
         for (void *p : recorded) hipFree(p);
         if (tw) hipFree(tw);
@@ -348,6 +350,18 @@ struct vh_linear_fp8 {
         hipSetDevice(rt->device);
         for (void *p : {(void *)w.codes, (void *)scales, (void *)bias, (void *)gamma})
             if (p) hipFreeAsync(p, rt->stream);
+    }
+};
+
+struct vh_cross_kv {
+    Rt rt;
+    size_t head_dim = 0;
+    char *block = nullptr;  // lens, exponents, ranges, kept, blocks
+    vh::CrossWrite write{};
+    ~vh_cross_kv() {
+        if (!rt || !block) return;
+        hipSetDevice(rt->device);
+        hipFreeAsync(block, rt->stream);
     }
 };
 
@@ -4195,6 +4209,195 @@ extern "C" vh_status vh_linear_fp8_run_rows_residual(const vh_linear_fp8 *linear
     NEED(input, what);
     NEED(residual, what);
     return run_fp8(linear, nullptr, input, input->view.rows, vh::Epi::Residual, residual, what);
+}
+
+// =============================================================================
+// attention over an encoder's states
+// =============================================================================
+
+extern "C" vh_status vh_cross_kv_new(const vh_runtime *rt, int type, size_t images, size_t tokens, size_t kv_heads,
+                                     size_t head_dim, vh_cross_kv **out) {
+    const char *what = "vh_cross_kv_new";
+    NEED(rt, what);
+    NEED(out, what);
+    if (type != vh::kCrossF32 && type != vh::kCrossF16)
+        return fail(VH_ERR_KERNEL, "cross kv: type " + std::to_string(type) + " is none of 0 (two halves), 1 (one)");
+    if (head_dim == 0 || head_dim > 128 || head_dim % 4)
+        return fail(VH_ERR_KERNEL, "cross kv: head_dim must be a multiple of 4 up to 128, got " +
+                                       std::to_string(head_dim));
+    if (images == 0 || images > 65535 || kv_heads == 0 || kv_heads > 65535 || tokens == 0 || tokens > (size_t)1 << 30)
+        return fail(VH_ERR_KERNEL, "cross kv: " + std::to_string(images) + " images of " + std::to_string(tokens) +
+                                       " tokens and " + std::to_string(kv_heads) + " heads are out of range");
+    const size_t width = head_dim <= 64 ? 64 : 128, rows = images * kv_heads;
+    const size_t head_bytes = (tokens + 127) / 128 * 4 * (size_t)vh::cross_block_bytes(type, (int)width);
+    size_t bytes = 0;
+    // Below 2^32 * 2^40, so only this product can pass 64 bits; what else there is is smaller.
+    if (mul_overflows(rows, head_bytes, &bytes) || bytes > SIZE_MAX / 4)
+        return fail(VH_ERR_KERNEL, "cross kv: its size overflows");
+    GUARD_BEGIN
+    RtState &s = *rt->s;
+    TRY(set_device(s));
+    if (capturing(s.stream)) return fail(VH_ERR_KERNEL, "cross kv: not to be made inside a stream capture");
+    auto c = std::make_unique<vh_cross_kv>();
+    c->rt = rt->s;
+    c->head_dim = head_dim;
+    const auto padded = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t lens = padded(images * 4), ke = padded(rows * 4), ve = padded(rows * width * 4);
+    const size_t ranges = padded(rows * vh::cross_chunks(tokens) * (1 + width) * 4), kept = padded(images * tokens * 4);
+    TRY(dalloc(s, lens + ke + ve + ranges + kept + bytes, &c->block, "cross kv allocation"));
+    vh::CrossView &v = c->write.view;
+    char *p = c->block;
+    v.lens = reinterpret_cast<int *>(p);
+    v.k_exp = reinterpret_cast<int *>(p += lens);
+    v.v_exp = reinterpret_cast<int *>(p += ke);
+    c->write.ranges = reinterpret_cast<uint32_t *>(p += ve);
+    c->write.kept = reinterpret_cast<int *>(p += ranges);
+    v.blocks = p + kept;
+    v.kind = type;
+    v.images = (int)images;
+    v.tokens = (int)tokens;
+    v.kv_heads = (int)kv_heads;
+    v.width = (int)width;
+    // No tokens, and exponents that a scale can be formed of.
+    if (hipMemsetAsync(c->block, 0, lens + ke + ve, s.stream) != hipSuccess)
+        return fail(VH_ERR_UPLOAD, hip_msg(what, hipGetLastError()));
+    *out = c.release();
+    return VH_OK;
+    GUARD_END
+}
+
+extern "C" void vh_cross_kv_free(vh_cross_kv *kv) { delete kv; }
+
+static vh_status cross_write(vh_cross_kv *kv, vh::CrossWrite w, size_t tokens, const vh_index *seen) {
+    GUARD_BEGIN
+    RtState &s = *kv->rt;
+    TRY(set_device(s));
+    w.seen = seen ? seen->ptr : nullptr;
+    w.tokens = (int)tokens;
+    w.head_dim = (int)kv->head_dim;
+    return launch(s, "cross_kv_write", [&] { return vh::launch_cross_write(s.stream, w); });
+    GUARD_END
+}
+
+static vh_status check_cross_tokens(const vh_cross_kv *kv, size_t tokens, const vh_index *seen, const char *what) {
+    const vh::CrossView &v = kv->write.view;
+    if (tokens > (size_t)v.tokens)
+        return fail(VH_ERR_KERNEL, "cross kv: " + std::to_string(tokens) + " tokens, made for " +
+                                       std::to_string(v.tokens));
+    if (seen && seen->len != v.images * tokens) return mismatch(seen->len, v.images * tokens, what);
+    if (seen && seen->rt != kv->rt) return other_runtime(what);
+    return VH_OK;
+}
+
+extern "C" vh_status vh_cross_kv_write_f32(vh_cross_kv *kv, const vh_tensor *k, const vh_tensor *v, size_t tokens,
+                                           int token_major, const vh_index *seen) {
+    const char *what = "vh_cross_kv_write_f32";
+    NEED(kv, what);
+    NEED(k, what);
+    NEED(v, what);
+    TRY(check_cross_tokens(kv, tokens, seen, what));
+    vh::CrossWrite w = kv->write;
+    const size_t hd = kv->head_dim, heads = (size_t)w.view.kv_heads, n = w.view.images * tokens * heads * hd;
+    if (k->len != n || v->len != n) return mismatch(k->len != n ? k->len : v->len, n, what);
+    if (k->rt != kv->rt || v->rt != kv->rt) return other_runtime(what);
+    w.k = k->ptr;
+    w.v = v->ptr;
+    w.kv_image = tokens * heads * hd;
+    w.kv_token = token_major ? heads * hd : hd;
+    w.kv_head = token_major ? hd : tokens * hd;
+    return cross_write(kv, w, tokens, seen);
+}
+
+extern "C" vh_status vh_cross_kv_write_rows_f32(vh_cross_kv *kv, const vh_tensor *rows, size_t tokens,
+                                                const vh_index *seen) {
+    const char *what = "vh_cross_kv_write_rows_f32";
+    NEED(kv, what);
+    NEED(rows, what);
+    TRY(check_cross_tokens(kv, tokens, seen, what));
+    vh::CrossWrite w = kv->write;
+    const size_t hd = kv->head_dim, width = (size_t)w.view.kv_heads * hd, n = w.view.images * tokens * 2 * width;
+    if (rows->len != n) return mismatch(rows->len, n, what);
+    if (rows->rt != kv->rt) return other_runtime(what);
+    w.k = rows->ptr;
+    w.v = rows->ptr + width;
+    w.kv_image = tokens * 2 * width;
+    w.kv_token = 2 * width;
+    w.kv_head = hd;
+    return cross_write(kv, w, tokens, seen);
+}
+
+extern "C" vh_status vh_cross_kv_read_f32(const vh_cross_kv *kv, vh_tensor *k, vh_tensor *v, vh_index *lens) {
+    const char *what = "vh_cross_kv_read_f32";
+    NEED(kv, what);
+    NEED(k, what);
+    NEED(v, what);
+    const vh::CrossView &w = kv->write.view;
+    const size_t n = (size_t)w.images * w.tokens * w.kv_heads * kv->head_dim;
+    if (k->len != n || v->len != n) return mismatch(k->len != n ? k->len : v->len, n, what);
+    if (lens && lens->len != (size_t)w.images) return mismatch(lens->len, w.images, what);
+    if (k->rt != kv->rt || v->rt != kv->rt || (lens && lens->rt != kv->rt)) return other_runtime(what);
+    if (k == v) return aliased(what);
+    GUARD_BEGIN
+    RtState &s = *kv->rt;
+    TRY(set_device(s));
+    return launch(s, "cross_kv_read", [&] {
+        return vh::launch_cross_read(s.stream, w, kv->head_dim, k->ptr, v->ptr, lens ? lens->ptr : nullptr);
+    });
+    GUARD_END
+}
+
+// Room for the parts of the tiles, counters first (zeroed here; every launch leaves them
+// zero), as attn_workspace does it for the paged attention.
+static void cross_workspace(RtState &s, size_t floats, vh::CrossAttn *a) {
+    const size_t head = vh::kAttnCounters * sizeof(unsigned);
+    const size_t had = s.xa.recorded && !capturing(s.stream) ? 0 : s.xa.bytes;  // a recorded block is left to its graph
+    char *p = static_cast<char *>(graph_workspace(s, s.xa, s.xa_capture, head + floats * sizeof(float)));
+    if (!p) return;
+    if (s.xa.bytes != had && hipMemsetAsync(p, 0, head, s.stream) != hipSuccess) {
+        hipGetLastError();
+        hipFree(p);
+        s.xa = Workspace{};
+        return;
+    }
+    a->counters = reinterpret_cast<unsigned *>(p);
+    a->parts = reinterpret_cast<float *>(p + head);
+}
+
+extern "C" vh_status vh_cross_attention_f32(const vh_cross_kv *kv, const vh_tensor *q, size_t heads, size_t tokens,
+                                            int token_major, vh_tensor *out) {
+    const char *what = "vh_cross_attention_f32";
+    NEED(kv, what);
+    NEED(q, what);
+    NEED(out, what);
+    const vh::CrossView &v = kv->write.view;
+    const size_t hd = kv->head_dim, kvh = (size_t)v.kv_heads;
+    if (heads == 0 || heads > 65535 || heads % kvh != 0)
+        return fail(VH_ERR_KERNEL, "cross attention: " + std::to_string(heads) + " query heads over " +
+                                       std::to_string(kvh) + " of the states");
+    if (tokens > ((size_t)1 << 30) / heads) return fail(VH_ERR_KERNEL, "cross attention: more than 2^30 query rows");
+    const size_t n = v.images * tokens * heads * hd;
+    if (q->len != n || out->len != n) return mismatch(q->len != n ? q->len : out->len, n, what);
+    if (q->rt != kv->rt || out->rt != kv->rt) return other_runtime(what);
+    if (out == q) return aliased(what);
+    GUARD_BEGIN
+    RtState &s = *kv->rt;
+    TRY(set_device(s));
+    if (n == 0) return VH_OK;
+    vh::CrossAttn a{};
+    a.view = v;
+    a.q = q->ptr;
+    a.out = out->ptr;
+    a.q_image = tokens * heads * hd;
+    a.q_token = token_major ? heads * hd : hd;
+    a.q_head = token_major ? hd : tokens * hd;
+    a.images = v.images;
+    a.queries = (int)tokens;
+    a.group = (int)(heads / kvh);
+    a.head_dim = (int)hd;
+    a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
+    cross_workspace(s, vh::cross_attn_floats(a), &a);
+    return launch(s, "cross_attention", [&] { return vh::launch_cross_attn(s.stream, a); });
+    GUARD_END
 }
 
 // =============================================================================

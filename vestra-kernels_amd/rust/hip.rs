@@ -78,6 +78,10 @@ pub struct VhKvCache {
     _p: [u8; 0],
 }
 #[repr(C)]
+pub struct VhCrossKv {
+    _p: [u8; 0],
+}
+#[repr(C)]
 pub struct VhFp8Tensor {
     _p: [u8; 0],
 }
@@ -332,6 +336,17 @@ unsafe extern "C" {
                                    out: *mut VhTensor) -> Status;
     fn vh_linear_fp8_run_rows_residual(linear: *const VhLinearFp8, input: *const VhFp8Tensor,
                                        residual: *mut VhTensor) -> Status;
+
+    fn vh_cross_kv_new(rt: *const VhRuntime, kind: c_int, images: usize, tokens: usize, kv_heads: usize,
+                       head_dim: usize, out: *mut *mut VhCrossKv) -> Status;
+    fn vh_cross_kv_free(kv: *mut VhCrossKv);
+    fn vh_cross_kv_write_f32(kv: *mut VhCrossKv, k: *const VhTensor, v: *const VhTensor, tokens: usize,
+                             token_major: c_int, seen: *const VhIndex) -> Status;
+    fn vh_cross_kv_write_rows_f32(kv: *mut VhCrossKv, rows: *const VhTensor, tokens: usize,
+                                  seen: *const VhIndex) -> Status;
+    fn vh_cross_kv_read_f32(kv: *const VhCrossKv, k: *mut VhTensor, v: *mut VhTensor, lens: *mut VhIndex) -> Status;
+    fn vh_cross_attention_f32(kv: *const VhCrossKv, q: *const VhTensor, heads: usize, tokens: usize,
+                              token_major: c_int, out: *mut VhTensor) -> Status;
 
     fn vh_profile_enable(rt: *mut VhRuntime, enabled: c_int) -> Status;
     fn vh_profile_reset(rt: *mut VhRuntime) -> Status;
@@ -1128,6 +1143,18 @@ impl HipRuntime {
         Ok(HipLinearFp8 { raw: out, runtime: self.clone() })
     }
 
+    // -- an encoder's states -------------------------------------------------------
+
+    /// Room for the keys and values of `images` images of up to `tokens` tokens.
+    pub fn cross_kv(&self, kind: CrossType, images: usize, tokens: usize, kv_heads: usize, head_dim: usize)
+        -> Result<HipCrossKv, HipError> {
+        let raw = self.inner.raw;
+        let mut out = ptr::null_mut();
+        // SAFETY: live runtime.
+        self.call(|| unsafe { vh_cross_kv_new(raw, kind as c_int, images, tokens, kv_heads, head_dim, &mut out) })?;
+        Ok(HipCrossKv { raw: out, runtime: self.clone() })
+    }
+
     // -- profiling (device twin of DA3_FLASH_PROFILE, src/specialized.rs:1324) ----
 
     pub fn profile_enable(&self, enabled: bool) -> Result<(), HipError> {
@@ -1605,6 +1632,74 @@ impl HipLinearFp8 {
         let dst = residual.raw;
         // SAFETY: as above.
         self.runtime.call(|| unsafe { vh_linear_fp8_run_rows_residual(self.raw, input.raw, dst) })
+    }
+}
+
+// ---- an encoder's states ---------------------------------------------------------
+
+/// What stored states are held in: two halves a value, or one.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+#[repr(i32)]
+pub enum CrossType {
+    F32 = 0,
+    F16 = 1,
+}
+
+/// Keys and values of an encoder's states, stored once for the queries that read them.
+pub struct HipCrossKv {
+    raw: *mut VhCrossKv,
+    runtime: HipRuntime,
+}
+
+// SAFETY: owned device state; every use goes through the runtime's lock.
+unsafe impl Send for HipCrossKv {}
+unsafe impl Sync for HipCrossKv {}
+
+impl Drop for HipCrossKv {
+    fn drop(&mut self) {
+        let _g = self.runtime.guard();
+        // SAFETY: raw came from the library and is freed once.
+        unsafe { vh_cross_kv_free(self.raw) }
+    }
+}
+
+impl HipCrossKv {
+    /// K and V [images, kv_heads, tokens, head_dim] (or token-major); `seen`: 0 leaves a token out.
+    pub fn write(&mut self, k: &HipTensorF32, v: &HipTensorF32, tokens: usize, token_major: bool,
+                 seen: Option<&HipIndex>) -> Result<(), HipError> {
+        let raw = self.raw;
+        let mask = seen.map_or(ptr::null(), |s| s.raw.cast_const());
+        // SAFETY: live handles (or null); the states are borrowed mutably for the call.
+        self.runtime.call(|| unsafe {
+            vh_cross_kv_write_f32(raw, k.raw, v.raw, tokens, c_int::from(token_major), mask)
+        })
+    }
+
+    /// Rows of a KV projection: K and V, heads in order.
+    pub fn write_rows(&mut self, rows: &HipTensorF32, tokens: usize, seen: Option<&HipIndex>)
+        -> Result<(), HipError> {
+        let raw = self.raw;
+        let mask = seen.map_or(ptr::null(), |s| s.raw.cast_const());
+        // SAFETY: as above.
+        self.runtime.call(|| unsafe { vh_cross_kv_write_rows_f32(raw, rows.raw, tokens, mask) })
+    }
+
+    /// What is stored, as floats, the seen tokens in order; their numbers.
+    pub fn read(&self, k: &mut HipTensorF32, v: &mut HipTensorF32, lens: Option<&mut HipIndex>)
+        -> Result<(), HipError> {
+        let n = lens.map_or(ptr::null_mut(), |l| l.raw);
+        // SAFETY: live handles (or null); the outputs are borrowed mutably for the call.
+        self.runtime.call(|| unsafe { vh_cross_kv_read_f32(self.raw, k.raw, v.raw, n) })
+    }
+
+    /// Attention of q [images, heads, tokens, head_dim] (or token-major) over each image's tokens.
+    pub fn attention(&self, q: &HipTensorF32, heads: usize, tokens: usize, token_major: bool,
+                     out: &mut HipTensorF32) -> Result<(), HipError> {
+        let dst = out.raw;
+        // SAFETY: live handles; the output is borrowed mutably for the call.
+        self.runtime.call(|| unsafe {
+            vh_cross_attention_f32(self.raw, q.raw, heads, tokens, c_int::from(token_major), dst)
+        })
     }
 }
 

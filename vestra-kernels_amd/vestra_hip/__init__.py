@@ -204,6 +204,12 @@ SIGNATURES = [
     ("vh_linear_fp8_run_rows", _S, [_p, _p, _p]),
     ("vh_linear_fp8_run_rows_gelu", _S, [_p, _p, _p]),
     ("vh_linear_fp8_run_rows_residual", _S, [_p, _p, _p]),
+    ("vh_cross_kv_new", _S, [_p, ctypes.c_int, _sz, _sz, _sz, _sz, _pp]),
+    ("vh_cross_kv_free", None, [_p]),
+    ("vh_cross_kv_write_f32", _S, [_p, _p, _p, _sz, ctypes.c_int, _p]),
+    ("vh_cross_kv_write_rows_f32", _S, [_p, _p, _sz, _p]),
+    ("vh_cross_kv_read_f32", _S, [_p, _p, _p, _p]),
+    ("vh_cross_attention_f32", _S, [_p, _p, _sz, _sz, ctypes.c_int, _p]),
     ("vh_profile_enable", _S, [_p, ctypes.c_int]),
     ("vh_profile_reset", _S, [_p]),
     ("vh_profile_report", _S, [_p, ctypes.c_char_p, _sz]),
@@ -657,6 +663,46 @@ class LinearFp8:
             pass
 
 
+class CrossKv:
+    """Keys and values of an encoder's states, stored once for the queries that read them."""
+
+    TYPES = {"f32": 0, "f16": 1}
+
+    def __init__(self, runtime: "Runtime", handle: int):
+        self._rt = runtime
+        self._h = ctypes.c_void_p(handle)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def write(self, k: Tensor, v: Tensor, tokens: int, token_major: bool = False, seen: Index | None = None) -> None:
+        """K and V [images, kv_heads, tokens, head_dim] (or token-major); seen [images * tokens]: 0 leaves out."""
+        _check(lib().vh_cross_kv_write_f32(self._h, k.handle, v.handle, tokens, 1 if token_major else 0,
+                                           seen.handle if seen is not None else None))
+
+    def write_rows(self, rows: Tensor, tokens: int, seen: Index | None = None) -> None:
+        """Rows of a KV projection: K and V, heads in order."""
+        _check(lib().vh_cross_kv_write_rows_f32(self._h, rows.handle, tokens,
+                                                seen.handle if seen is not None else None))
+
+    def read(self, k: Tensor, v: Tensor, lens: Index | None = None) -> None:
+        """What is stored, as floats, the seen tokens in order; their numbers."""
+        _check(lib().vh_cross_kv_read_f32(self._h, k.handle, v.handle, lens.handle if lens is not None else None))
+
+    def attention(self, q: Tensor, heads: int, tokens: int, out: Tensor, token_major: bool = False) -> None:
+        """Attention of q [images, heads, tokens, head_dim] (or token-major) over each image's tokens."""
+        _check(lib().vh_cross_attention_f32(self._h, q.handle, heads, tokens, 1 if token_major else 0, out.handle))
+
+    def __del__(self):
+        try:
+            if self._h and self._h.value:
+                lib().vh_cross_kv_free(self._h)
+                self._h = ctypes.c_void_p(None)
+        except Exception:
+            pass
+
+
 class BlockParams(ctypes.Structure):
     _fields_ = [(n, _f32p) for n in da3.BLOCK_FIELDS + da3.QK_NORM_FIELDS]
 
@@ -1035,6 +1081,14 @@ class Runtime:
         b, g = (None if v is None else _vector(v, n) for v in (bias, gamma))
         return self._linear_fp8(lib().vh_prepare_linear_fp8_blocks, k, n, c.ctypes.data, _fp(s),
                                 _fp(b) if b is not None else None, _fp(g) if g is not None else None)
+
+    # -- an encoder's states
+    def cross_kv(self, type: str, images: int, tokens: int, kv_heads: int, head_dim: int) -> CrossKv:
+        """type: "f32" (two halves a value) or "f16"; tokens: at most so many an image."""
+        out = ctypes.c_void_p()
+        _check(lib().vh_cross_kv_new(self._h, CrossKv.TYPES.get(type, -1), images, tokens, kv_heads, head_dim,
+                                     ctypes.byref(out)))
+        return CrossKv(self, out.value)
 
     # -- profiling
     def profile_enable(self, on: bool = True) -> None:
