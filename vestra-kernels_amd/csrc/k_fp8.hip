@@ -23,6 +23,8 @@
 // registers, or memory to registers.  (Any order of k does for a product, as long as
 // both sides have it.)
 #include <algorithm>
+#include <cmath>
+#include <cstdlib>
 
 #include "common.h"
 #include "kernels.h"
@@ -33,7 +35,6 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kQuantThreads = 512;
 constexpr size_t kMaxGrid = 65536;  // of the kernels that walk their tiles
 
 // The exponent of a block whose largest finite magnitude has these bits: 448 = 1.75 * 2^8.
@@ -45,19 +46,31 @@ __device__ __forceinline__ float pow2(int e) {  // -126 <= e <= 127
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// Where dword c (values 4 c .. + 3) of row r is in a panel.
-__device__ __forceinline__ int panel_at(int r, int c) { return ((c >> 2) & 1) * 1024 + ((c >> 3) * 16 + r) * 16 + (c & 3) * 4; }
+// Where dword c (values 4 c .. + 3) of row r is in a panel in LDS, and 16 bytes of lane `lane` of
+// half h: as in memory, but for the row, which is swizzled so that the dwords of two rows
+// of 32 lanes go to different banks.
+__device__ __forceinline__ int panel_at(int r, int c) {
+    const int h = (c >> 2) & 1, lh = c >> 3;
+    return h * 1024 + (lh * 16 + (r ^ (4 * lh + 2 * h))) * 16 + (c & 3) * 4;
+}
+__device__ __forceinline__ int panel_lane(int lane, int h) {
+    return h * 1024 + (lane ^ (4 * (lane >> 4) + 2 * h)) * 16;
+}
 
-// Largest finite magnitude's bits.
+// Largest magnitude's bits, of the finite values alone.
 __device__ __forceinline__ uint32_t finite_max(uint32_t mx, float v) {
     const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
     return max(mx, b < 0x7f800000u ? b : 0u);
 }
-__device__ __forceinline__ int e4m3_of(f32x4 v, float inv) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = fabsf(v[i]) < INFINITY ? v[i] * inv : NAN;
+__device__ __forceinline__ int e4m3_of(f32x4 v) {
     const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
     return __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+}
+// For rows that may hold what is not finite.
+__device__ __forceinline__ f32x4 scaled(f32x4 v, float inv) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = fabsf(v[i]) < INFINITY ? v[i] * inv : NAN;
+    return v;
 }
 
 // Four values of a row of k floats from column d on (zeros past its end).
@@ -73,55 +86,119 @@ __device__ __forceinline__ f32x4 row4(const float *row, size_t d, size_t k) {
     return v;
 }
 
-// A workgroup takes 16 rows, its waves their blocks in turn; 32 lanes a row's block.
-// Rows past the end become zeros.
+// 16 rows' floats of a block, 32 lanes a row.
 template <bool VEC>
-__global__ __launch_bounds__(kQuantThreads) void quantize_fp8_kernel(const float *x, Fp8Rows out) {
-    __shared__ __attribute__((aligned(16))) char stage[kQuantThreads / 64][2048];
-    __shared__ int row_max[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, side = lane >> 5;
+__device__ __forceinline__ void load_panel(const float *x, const Fp8Rows &w, size_t tile, size_t b, int lane,
+                                           f32x4 (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const size_t row = tile * 16 + 2 * i + (lane >> 5), d = b * 128 + 4 * (lane & 31);
+        v[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < w.rows) v[i] = row4<VEC>(x + row * w.k, d, w.k);
+    }
+}
+// Largest of the 32 lanes of a row, in each of them.
+__device__ __forceinline__ uint32_t row_umax(uint32_t v) {
+    v = dpp_umax<0x140>(dpp_umax<0x141>(dpp_umax<0x4e>(dpp_umax<0xb1>(v))));
+    return max(v, (uint32_t)__shfl_xor((int)v, 16, kWave));
+}
+// Their codes; `to`: 2048 bytes of the wave's own.  Lanes 0 .. 7 of either half get the
+// exponents of rows 2 lane + half.
+__device__ __forceinline__ int quantize_panel(const f32x4 (&v)[8], const Fp8Rows &out, size_t tile, size_t b, int lane,
+                                              char *to) {
+    const int c = lane & 31, side = lane >> 5;
+    uint32_t mx[8];
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        mx[i] = row_umax(absmax4(0, v[i]));
+        finite &= mx[i] < 0x7f800000u;
+    }
+    int mine = -127;
+    const bool all = !__any(!finite);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (!all) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = finite_max(m, v[i][j]);
+            mx[i] = row_umax(m);
+        }
+        const int e = block_exponent(mx[i]);
+        const float inv = pow2(-e);
+        *reinterpret_cast<int *>(to + panel_at(2 * i + side, c)) = e4m3_of(all ? v[i] * inv : scaled(v[i], inv));
+        if (c == i) mine = e;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    char *at = reinterpret_cast<char *>(out.codes) + (tile * fp8_blocks(out.k) + b) * 2048 + lane * 16;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        *reinterpret_cast<u32x4 *>(at + h * 1024) = *reinterpret_cast<const u32x4 *>(to + panel_lane(lane, h));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (c < 8) out.exps[b * fp8_rows16(out.rows) + tile * 16 + 2 * c + side] = (uint8_t)(mine + 127);
+    return mine;
+}
+
+// A workgroup takes 16 rows, its waves their blocks in turn, the next block's floats on
+// their way.  Rows past the end become zeros.
+constexpr int kQuantBlocks = 256;  // whose exponents stay in LDS
+template <bool VEC, int THREADS>
+__global__ __launch_bounds__(THREADS) void quantize_fp8_kernel(const float *x, Fp8Rows out) {
+    constexpr int W = THREADS / 64;
+    __shared__ __attribute__((aligned(16))) char stage[W][2048];
+    __shared__ int wave_max[W][16];
+    __shared__ uint8_t codes[kQuantBlocks * 16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, row = 2 * c + (lane >> 5);
     const size_t kb = fp8_blocks(out.k), rows16 = fp8_rows16(out.rows);
     for (size_t tile = blockIdx.x; tile < rows16 / 16; tile += gridDim.x) {
-        if (threadIdx.x < 16) row_max[threadIdx.x] = -127;
-        __syncthreads();
-        for (size_t b = wave; b < kb; b += kQuantThreads / 64) {
-            f32x4 v[8];
+        f32x4 v[8];
+        if ((size_t)wave < kb) load_panel<VEC>(x, out, tile, wave, lane, v);
+        int most = -127;
+        for (size_t b = wave; b < kb; b += W) {
+            f32x4 now[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const size_t row = tile * 16 + 2 * i + side;
-                v[i] = row < out.rows ? row4<VEC>(x + row * out.k, b * 128 + 4 * c, out.k)
-                                      : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-            char *to = stage[wave];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                uint32_t mx = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) mx = finite_max(mx, v[i][j]);
-                mx = dpp_umax<0x140>(dpp_umax<0x141>(dpp_umax<0x4e>(dpp_umax<0xb1>(mx))));
-                mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, kWave));
-                const int e = block_exponent(mx), r = 2 * i + side;
-                *reinterpret_cast<int *>(to + panel_at(r, c)) = e4m3_of(v[i], pow2(-e));
-                if (c == 0) {
-                    out.exps[b * rows16 + tile * 16 + r] = (uint8_t)(e + 127);
-                    atomicMax(&row_max[r], e);
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            char *at = reinterpret_cast<char *>(out.codes) + (tile * kb + b) * 2048 + lane * 16;
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                *reinterpret_cast<u32x4 *>(at + h * 1024) = *reinterpret_cast<const u32x4 *>(to + h * 1024 + lane * 16);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int i = 0; i < 8; i++) now[i] = v[i];
+            if (b + W < kb) load_panel<VEC>(x, out, tile, b + W, lane, v);
+            const int e = quantize_panel(now, out, tile, b, lane, stage[wave]);
+            if (c < 8 && b < kQuantBlocks) codes[b * 16 + row] = (uint8_t)(e + 127);
+            most = max(most, e);
         }
+        if (c < 8) wave_max[wave][row] = most;
         __syncthreads();
-        if (threadIdx.x < 16) out.row_e[tile * 16 + threadIdx.x] = row_max[threadIdx.x];
-        for (size_t i = threadIdx.x; i < kb * 16; i += kQuantThreads) {
+        // Thread t writes row t % 16 of the blocks t / 16, ...
+        most = wave_max[0][tid & 15];
+#pragma unroll
+        for (int w = 1; w < W; w++) most = max(most, wave_max[w][tid & 15]);
+        if (tid < 16) out.row_e[tile * 16 + tid] = most;
+        for (size_t i = tid; i < kb * 16; i += THREADS) {
             const size_t at = (i >> 4) * rows16 + tile * 16 + (i & 15);
-            out.rel[at] = fp8_relative(out.exps[at], row_max[i & 15]);
+            out.rel[at] = fp8_relative(i < kQuantBlocks * 16 ? codes[i] : out.exps[at], most);
         }
         __syncthreads();
     }
+}
+
+// Where there are few rows: codes and exponents alone, a wave a panel; then what follows from
+// the exponents.
+template <bool VEC>
+__global__ __launch_bounds__(64) void quantize_panels_kernel(const float *x, Fp8Rows out) {
+    __shared__ __attribute__((aligned(16))) char stage[2048];
+    f32x4 v[8];
+    load_panel<VEC>(x, out, blockIdx.y, blockIdx.x, threadIdx.x, v);
+    quantize_panel(v, out, blockIdx.y, blockIdx.x, threadIdx.x, stage);
+}
+__global__ __launch_bounds__(256) void relative_fp8_kernel(Fp8Rows out) {
+    __shared__ int some[16][16];
+    const int tid = threadIdx.x, r = tid & 15, part = tid >> 4;
+    const size_t kb = fp8_blocks(out.k), rows16 = fp8_rows16(out.rows), row = (size_t)blockIdx.x * 16 + r;
+    int most = 0;
+    for (size_t b = part; b < kb; b += 16) most = max(most, (int)out.exps[b * rows16 + row]);
+    some[part][r] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; i++) most = max(most, some[i][r]);
+    if (part == 0) out.row_e[row] = most - 127;
+    for (size_t b = part; b < kb; b += 16) out.rel[b * rows16 + row] = fp8_relative(out.exps[b * rows16 + row], most - 127);
 }
 
 // The values that the codes stand for.
@@ -138,7 +215,7 @@ __global__ __launch_bounds__(256) void dequantize_fp8_kernel(Fp8Rows in, float *
         char *to = stage[wave];
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            *reinterpret_cast<u32x4 *>(to + h * 1024 + lane * 16) = *reinterpret_cast<const u32x4 *>(at + h * 1024);
+            *reinterpret_cast<u32x4 *>(to + panel_lane(lane, h)) = *reinterpret_cast<const u32x4 *>(at + h * 1024);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int r0 = 0; r0 < 8; r0++) {
@@ -196,10 +273,10 @@ __device__ __forceinline__ void put4(const Fp8Gemm &g, size_t m, size_t n, f32x4
     }
 }
 
-// C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  Two stages of 128 k in
+// C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  ST stages of 128 k in
 // LDS; D^T = B . A^T, so that a lane holds four consecutive columns of its row.
 // BLOCKS: B has float scales for 128 x 128 values (b_scales) instead of its exponents.
-template <int BM, int BN, int WM, int WN, Epi EPI, bool BLOCKS>
+template <int BM, int BN, int WM, int WN, int ST, Epi EPI, bool BLOCKS>
 __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
     constexpr int CODES = (BM + BN) * 128, STAGE = CODES + (BM + BN) * 2;
@@ -229,15 +306,15 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
             const char *from = reinterpret_cast<const char *>(is_a ? g.a.codes : g.b.codes) + (t * kb + b) * 2048 + (u & 1) * 1024;
             copy16_to_lds(from, lane * 16, __builtin_amdgcn_readfirstlane(lds0 + buf * STAGE + u * 1024));
         }
-        for (int u = wave; u < (BM + BN + 511) / 512; u += NW) {
-            // Eight rows a lane (past the end: the last eight).
-            const int r = u * 512 + lane * 8;
-            if (r < BM + BN) {
-                const bool is_a = r < BM;
-                const size_t row = is_a ? min((size_t)mt * BM + r, a16 - 8) : min((size_t)nt * BN + r - BM, b16 - 8);
-                const uint16_t *from = is_a ? g.a.rel + b * a16 + row : g.b.rel + b * b16 + row;
-                *reinterpret_cast<u32x4 *>(smem + buf * STAGE + CODES + r * 2) = *reinterpret_cast<const u32x4 *>(from);
-            }
+        // Eight rows a lane (past the end: the last eight); half of the waves A's, half B's, so that
+        // every wave has as many copies.
+        const bool is_a = wave < NW / 2;
+        const int rows = (is_a ? BM : BN) / (NW / 2), first = wave % (NW / 2) * rows;
+        if (lane < rows / 8) {
+            const size_t r16 = is_a ? a16 : b16;
+            const uint32_t at = (uint32_t)min((is_a ? (size_t)mt * BM : (size_t)nt * BN) + first + lane * 8, r16 - 8) * 2;
+            copy16_to_lds((is_a ? g.a.rel : g.b.rel) + b * r16, at,
+                          __builtin_amdgcn_readfirstlane(lds0 + buf * STAGE + CODES + ((is_a ? 0 : BM) + first) * 2));
         }
     };
     f32x4 acc[TM][TN];
@@ -245,12 +322,19 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    copy(0, 0);
+    constexpr int LD = (BM + BN) / 8 / NW + 1;  // copies of a wave and stage
+    static_assert((BM + BN) / 8 % NW == 0 && BM / (NW / 2) % 8 == 0 && BN / (NW / 2) % 8 == 0 && NW % 2 == 0);
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++)
+        if (i < (int)kb) copy(i, i);
     for (size_t b = 0; b < kb; b++) {
-        const int buf = b & 1;
-        split_wait<0>();
-        __syncthreads();
-        if (b + 1 < kb) copy(b + 1, buf ^ 1);
+        const int buf = (int)(b % ST);
+        // This stage landed; of the later ones as many as there are may be in flight.
+        if (ST > 3 && b + 2 < kb) split_wait<(ST > 3 ? 2 : 0) * LD>();
+        else if (ST > 2 && b + 1 < kb) split_wait<(ST > 2 ? 1 : 0) * LD>();
+        else split_wait<0>();
+        __builtin_amdgcn_s_barrier();
+        if (b + ST - 1 < kb) copy(b + ST - 1, (int)((b + ST - 1) % ST));
         const char *as = smem + buf * STAGE + wm * TM * 2048 + lane * 16;
         const char *bs = smem + buf * STAGE + BM * 128 + wn * TN * 2048 + lane * 16;
         const uint16_t *rs = reinterpret_cast<const uint16_t *>(smem + buf * STAGE + CODES);
@@ -260,17 +344,42 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
 #pragma unroll
         for (int j = 0; j < TN; j++)
             rb[j] = BLOCKS ? 1.0f : __uint_as_float((uint32_t)rs[BM + (wn * TN + j) * 16 + li] << 16);
-        f32x4 part[TM][TN];
         if constexpr (BLOCKS) {
+            // A block's sum from zero, a row of tiles at a time, then onto the others by its scale.
+            const size_t n_block = min(((size_t)nt * BN + wn * TN * 16) / 128, (b16 - 1) / 128);
+            const float s = g.b_scales[n_block * kb + b];
+            f16x8 fb[TN][4];
 #pragma unroll
-            for (int i = 0; i < TM; i++)
+            for (int j = 0; j < TN; j++)
 #pragma unroll
-                for (int j = 0; j < TN; j++) part[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int h = 0; h < 2; h++) {
+                    const u32x4 y = *reinterpret_cast<const u32x4 *>(bs + j * 2048 + h * 1024);
+                    fb[j][2 * h] = halves(y[0], y[1], 1.0f);
+                    fb[j][2 * h + 1] = halves(y[2], y[3], 1.0f);
+                }
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                f16x8 fa[4];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(as + i * 2048 + h * 1024);
+                    fa[2 * h] = halves(x[0], x[1], ra[i]);
+                    fa[2 * h + 1] = halves(x[2], x[3], ra[i]);
+                }
+                f32x4 part[TN];
+#pragma unroll
+                for (int j = 0; j < TN; j++) part[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int j = 0; j < TN; j++) part[j] = mfma16x16x32_f16(fb[j][e], fa[e], part[j]);
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf(part[j][r], s, acc[i][j][r]);
+            }
+            continue;
         }
-        auto &sum = [&]() -> f32x4(&)[TM][TN] {
-            if constexpr (BLOCKS) return part;
-            else return acc;
-        }();
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             u32x4 x[TM], y[TN];
@@ -287,19 +396,9 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
                 for (int i = 0; i < TM; i++) {
                     const f16x8 fa = halves(x[i][2 * e], x[i][2 * e + 1], ra[i]);
 #pragma unroll
-                    for (int j = 0; j < TN; j++) sum[i][j] = mfma16x16x32_f16(fb[j], fa, sum[i][j]);
+                    for (int j = 0; j < TN; j++) acc[i][j] = mfma16x16x32_f16(fb[j], fa, acc[i][j]);
                 }
             }
-        }
-        if constexpr (BLOCKS) {
-            const size_t n_block = min(((size_t)nt * BN + wn * TN * 16) / 128, (b16 - 1) / 128);
-            const float s = g.b_scales[n_block * kb + b];
-#pragma unroll
-            for (int i = 0; i < TM; i++)
-#pragma unroll
-                for (int j = 0; j < TN; j++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf(part[i][j][r], s, acc[i][j][r]);
         }
     }
 #pragma unroll
@@ -318,32 +417,143 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     }
 }
 
-template <int BM, int BN, int WM, int WN, Epi EPI, bool BLOCKS>
+// Few rows: 16 MT rows by 16 columns a workgroup, whose waves share K between them, memory
+// to registers; B is read once, past the caches.  A block's sum joins the others on its own
+// exponents.  FUSED (MT = 1): A are floats, which every workgroup quantises itself.
+constexpr int kFewWaves = 8;
+template <int MT, bool FUSED, bool BLOCKS, Epi EPI>
+__global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Gemm g, const float *x) {
+    __shared__ f32x4 sums[kFewWaves][MT][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lh = lane >> 4;
+    const size_t kb = fp8_blocks(g.b.k), b16 = fp8_rows16(g.b.rows), nt = blockIdx.x, mt = (size_t)blockIdx.y * MT;
+    const size_t a16 = fp8_rows16(g.m);
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (size_t b = wave; b < kb; b += kFewWaves) {
+        const char *from = reinterpret_cast<const char *>(g.b.codes) + (nt * kb + b) * 2048 + lane * 16;
+        u32x4 y[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) y[h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from + h * 1024));
+        float s = 1.0f;
+        uint32_t eb = 0x7f7f7f7f;
+        if constexpr (BLOCKS) s = g.b_scales[nt / 8 * kb + b];
+        else eb = *reinterpret_cast<const uint32_t *>(g.b.exps + b * b16 + nt * 16 + 4 * lh);
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            u32x4 a[2];
+            int ea;
+            if constexpr (FUSED) {
+                f32x4 v[8];
+                uint32_t mx = 0;
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    const size_t d = b * 128 + 32 * lh + 4 * c;
+                    v[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if ((size_t)li < g.m) v[c] = g.b.k % 4 == 0 ? row4<true>(x + li * g.b.k, d, g.b.k) : row4<false>(x + li * g.b.k, d, g.b.k);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) mx = finite_max(mx, v[c][j]);
+                }
+                mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, kWave));
+                mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, kWave));
+                ea = block_exponent(mx);
+                const float inv = pow2(-ea);
+#pragma unroll
+                for (int c = 0; c < 8; c++) a[c / 4][c % 4] = (uint32_t)e4m3_of(scaled(v[c], inv));
+            } else {
+                const size_t t = min(mt + i, a16 / 16 - 1);
+                const char *at = reinterpret_cast<const char *>(g.a.codes) + (t * kb + b) * 2048 + lane * 16;
+#pragma unroll
+                for (int h = 0; h < 2; h++) a[h] = *reinterpret_cast<const u32x4 *>(at + h * 1024);
+                ea = (int)g.a.exps[b * a16 + t * 16 + li] - 127;
+            }
+            f32x4 part{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    part = mfma16x16x32_f16(halves(y[h][2 * e], y[h][2 * e + 1], 1.0f),
+                                            halves(a[h][2 * e], a[h][2 * e + 1], 1.0f), part);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                acc[i][r] = __builtin_fmaf(BLOCKS ? s : 1.0f,
+                                           __builtin_ldexpf(part[r], ea + (int)((eb >> (8 * r)) & 255) - 127), acc[i][r]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < MT; i += kFewWaves) {
+        f32x4 v = sums[0][i][lane];
+#pragma unroll
+        for (int w = 1; w < kFewWaves; w++) v += sums[w][i][lane];
+        put4<EPI>(g, (mt + i) * 16 + li, nt * 16 + 4 * lh, v);
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int ST, Epi EPI, bool BLOCKS>
 hipError_t launch_tile(hipStream_t s, Fp8Gemm g) {
-    constexpr size_t bytes = 2 * ((BM + BN) * 128 + (BM + BN) * 2);
+    constexpr size_t bytes = ST * ((BM + BN) * 128 + (BM + BN) * 2);
     static std::atomic<uint64_t> done{0};
-    hipError_t e = ensure_dynamic_lds(fp8_gemm_kernel<BM, BN, WM, WN, EPI, BLOCKS>, bytes, done);
+    hipError_t e = ensure_dynamic_lds(fp8_gemm_kernel<BM, BN, WM, WN, ST, EPI, BLOCKS>, bytes, done);
     if (e != hipSuccess) return e;
     const size_t mt = (g.m + BM - 1) / BM, nt = (g.n + BN - 1) / BN;
     if (mt * nt > (size_t)1 << 22) return hipErrorInvalidConfiguration;
     g.m_tiles = (int)mt;
     g.n_tiles = (int)nt;
     g.tiles = (int)(mt * nt);
-    fp8_gemm_kernel<BM, BN, WM, WN, EPI, BLOCKS><<<(g.tiles + 7) / 8 * 8, WM * WN * 64, bytes, s>>>(g);
+    fp8_gemm_kernel<BM, BN, WM, WN, ST, EPI, BLOCKS><<<(g.tiles + 7) / 8 * 8, WM * WN * 64, bytes, s>>>(g);
     return hipGetLastError();
 }
 
 template <Epi EPI, bool BLOCKS>
-hipError_t launch_epi(hipStream_t s, const Fp8Gemm &g) {
-    return launch_tile<128, 128, 2, 2, EPI, BLOCKS>(s, g);
+hipError_t launch_epi(hipStream_t s, const Fp8Gemm &g, Fp8Plan plan, const float *x) {
+    if (plan == Fp8Plan::Fused || plan == Fp8Plan::Few) {
+        const dim3 grid((unsigned)((g.n + 15) / 16), (unsigned)((g.m + 63) / 64));
+        constexpr int threads = kFewWaves * 64;
+        if (plan == Fp8Plan::Fused) fp8_few_kernel<1, true, BLOCKS, EPI><<<grid, threads, 0, s>>>(g, x);
+        else if (g.m <= 16) fp8_few_kernel<1, false, BLOCKS, EPI><<<grid, threads, 0, s>>>(g, nullptr);
+        else if (g.m <= 32) fp8_few_kernel<2, false, BLOCKS, EPI><<<grid, threads, 0, s>>>(g, nullptr);
+        else fp8_few_kernel<4, false, BLOCKS, EPI><<<grid, threads, 0, s>>>(g, nullptr);
+        return hipGetLastError();
+    }
+    if (plan == Fp8Plan::Tile64) return launch_tile<64, 64, 2, 2, 2, EPI, BLOCKS>(s, g);
+    if (plan == Fp8Plan::Tile128) return launch_tile<128, 128, 2, 4, 2, EPI, BLOCKS>(s, g);
+    return launch_tile<256, 256, 2, 4, 2, EPI, BLOCKS>(s, g);
+}
+
+template <bool BLOCKS>
+hipError_t launch_blocks(hipStream_t s, const Fp8Gemm &g, Epi epi, Fp8Plan plan, const float *x) {
+    if (epi == Epi::Gelu) return launch_epi<Epi::Gelu, BLOCKS>(s, g, plan, x);
+    if (epi == Epi::Residual) return launch_epi<Epi::Residual, BLOCKS>(s, g, plan, x);
+    return launch_epi<Epi::Store, BLOCKS>(s, g, plan, x);
 }
 
 }  // namespace
 
-hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out) {
+template <int THREADS>
+static void quantize_with(hipStream_t s, const float *x, const Fp8Rows &out) {
     const unsigned grid = (unsigned)std::min(fp8_rows16(out.rows) / 16, kMaxGrid);
-    if (out.k % 4 == 0) quantize_fp8_kernel<true><<<grid, kQuantThreads, 0, s>>>(x, out);
-    else quantize_fp8_kernel<false><<<grid, kQuantThreads, 0, s>>>(x, out);
+    if (out.k % 4 == 0) quantize_fp8_kernel<true, THREADS><<<grid, THREADS, 0, s>>>(x, out);
+    else quantize_fp8_kernel<false, THREADS><<<grid, THREADS, 0, s>>>(x, out);
+}
+
+hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out, bool products_of_few) {
+    const size_t tiles = fp8_rows16(out.rows) / 16, kb = fp8_blocks(out.k);
+    // Few rows: a wave a panel (100 x 6000 in 7.8 us, two launches, against 14.2 of one workgroup for
+    // 16 rows; 865 x 768 7.0 against 4.9).  More: as many waves as two rounds leave (864 tiles
+    // of 768, two waves each, 12.7 us, of eight 19.3; 217 tiles 8.0 and 5.3).
+    if (products_of_few || (tiles <= 64 && kb > 16)) {
+        const dim3 grid((unsigned)kb, (unsigned)tiles);
+        if (out.k % 4 == 0) quantize_panels_kernel<true><<<grid, 64, 0, s>>>(x, out);
+        else quantize_panels_kernel<false><<<grid, 64, 0, s>>>(x, out);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess || products_of_few) return e;
+        relative_fp8_kernel<<<(unsigned)tiles, 256, 0, s>>>(out);
+        return hipGetLastError();
+    }
+    if (tiles >= 512) quantize_with<128>(s, x, out);
+    else quantize_with<512>(s, x, out);
     return hipGetLastError();
 }
 
@@ -355,15 +565,41 @@ hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out) {
     return hipGetLastError();
 }
 
-hipError_t launch_gemm_fp8(hipStream_t s, const Fp8Gemm &g, Epi epi) {
-    if (g.b_scales) {
-        if (epi == Epi::Gelu) return launch_epi<Epi::Gelu, true>(s, g);
-        if (epi == Epi::Residual) return launch_epi<Epi::Residual, true>(s, g);
-        return launch_epi<Epi::Store, true>(s, g);
+// By a model of the launch, in us, fitted to 24 shapes measured with each form: the few rows'
+// form takes a wave's blocks one after the other (1.0) or what all workgroups have to read and
+// multiply; tiles of 64 and 128 one tile on its own, or rounds of as many as are resident
+// (1024 and 512); tiles of 256 whole rounds of 256.
+Fp8Plan fp8_plan(size_t m, size_t n, size_t k, bool floats) {
+    const auto tiles = [&](size_t b) { return (double)((m + b - 1) / b) * (double)((n + b - 1) / b); };
+    const double kb = (double)fp8_blocks(k), groups = (double)((n + 15) / 16) * (double)((m + 63) / 64);
+    const double each = m <= 16 ? 4.2e-4 : m <= 32 ? 5.6e-4 : 8.4e-4;
+    double best = 2.6 + std::max(std::ceil(kb / kFewWaves), groups * kb * each);
+    // Fused while a wave quantises one block (one row of 768 for 2304 outputs 4.0 us, in two launches
+    // 5.8; 16 rows 5.8 and 7.3; of 3072 for 768 8.0 and 6.6).
+    Fp8Plan plan = floats && m <= 16 && kb <= kFewWaves && groups <= 1024 ? Fp8Plan::Fused : Fp8Plan::Few;
+    const auto offer = [&](Fp8Plan p, double us) {
+        if (us < best) {
+            best = us;
+            plan = p;
+        }
+    };
+    offer(Fp8Plan::Tile64, std::max(4.2 + 0.57 * kb, tiles(64) / 1024 * (5 + 1.05 * kb)));
+    offer(Fp8Plan::Tile128, std::max(7 + 1.0 * kb, tiles(128) / 512 * (8 + 1.85 * kb)));
+    offer(Fp8Plan::Tile256, std::ceil(tiles(256) / 256) * (16 + 3.0 * kb));
+    static const char *asked = getenv("VESTRA_HIP_FP8_TILE");
+    if (asked) {
+        const int a = atoi(asked);
+        if (a == 15 && floats && m <= 16) return Fp8Plan::Fused;
+        if (a == 16) return Fp8Plan::Few;
+        if (a == 64) return Fp8Plan::Tile64;
+        if (a == 128) return Fp8Plan::Tile128;
+        if (a == 256) return Fp8Plan::Tile256;
     }
-    if (epi == Epi::Gelu) return launch_epi<Epi::Gelu, false>(s, g);
-    if (epi == Epi::Residual) return launch_epi<Epi::Residual, false>(s, g);
-    return launch_epi<Epi::Store, false>(s, g);
+    return plan;
+}
+
+hipError_t launch_gemm_fp8(hipStream_t s, const Fp8Gemm &g, Epi epi, Fp8Plan plan, const float *x) {
+    return g.b_scales ? launch_blocks<true>(s, g, epi, plan, x) : launch_blocks<false>(s, g, epi, plan, x);
 }
 
 }  // namespace vh

@@ -329,7 +329,8 @@ __host__ __device__ inline uint16_t fp8_relative(int exp_code, int row_e) {
     const int e = exp_code - row_e;  // + 127
     return (uint16_t)((e > 1 ? e : 1) << 7);
 }
-hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out);
+// products_of_few: without rel and row_e, which the products of few rows do not look at.
+hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out, bool products_of_few = false);
 hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out);
 // c [m][n] = a . b^T, then the epilogue (Store: (v + bias) * gamma; Gelu: gelu(v +
 // bias); Residual: c += (v + bias) * gamma); bias and gamma may be null.  With b_scales
@@ -341,7 +342,11 @@ struct Fp8Gemm {
     size_t m, n;
     int m_tiles, n_tiles, tiles;  // set by the launcher
 };
-hipError_t launch_gemm_fp8(hipStream_t s, const Fp8Gemm &g, Epi epi);
+// Fused (16 rows at most): a is not looked at, x are floats [m][b.k], whose quantisation
+// is part of the launch.  Few: a needs no rel and row_e.
+enum class Fp8Plan : int { Fused, Few, Tile64, Tile128, Tile256 };
+Fp8Plan fp8_plan(size_t m, size_t n, size_t k, bool floats);
+hipError_t launch_gemm_fp8(hipStream_t s, const Fp8Gemm &g, Epi epi, Fp8Plan plan, const float *x = nullptr);
 
 // ---- paged cache of keys and values (k_cache.hip) ---------------------------
 // What a cache holds a value in.

@@ -3955,9 +3955,9 @@ extern "C" void vh_fp8_free(vh_fp8_tensor *tensor) { delete tensor; }
 extern "C" size_t vh_fp8_rows(const vh_fp8_tensor *tensor) { return tensor ? tensor->view.rows : 0; }
 extern "C" size_t vh_fp8_k(const vh_fp8_tensor *tensor) { return tensor ? tensor->view.k : 0; }
 
-static vh_status quantize_fp8(RtState &s, const float *x, const vh::Fp8Rows &out) {
+static vh_status quantize_fp8(RtState &s, const float *x, const vh::Fp8Rows &out, bool products_of_few = false) {
     if (out.rows == 0) return VH_OK;
-    return launch(s, "quantize_fp8", [&] { return vh::launch_quantize_fp8(s.stream, x, out); });
+    return launch(s, "quantize_fp8", [&] { return vh::launch_quantize_fp8(s.stream, x, out, products_of_few); });
 }
 
 extern "C" vh_status vh_quantize_fp8(const vh_runtime *rt, const vh_tensor *x, size_t rows, size_t k,
@@ -4037,7 +4037,9 @@ extern "C" vh_status vh_gemm_fp8_into(const vh_runtime *rt, const vh_fp8_tensor 
     g.c = c->ptr;
     g.m = a->view.rows;
     g.n = b->view.rows;
-    return launch(s, "gemm_fp8", [&] { return vh::launch_gemm_fp8(s.stream, g, vh::Epi::Store); });
+    return launch(s, "gemm_fp8", [&] {
+        return vh::launch_gemm_fp8(s.stream, g, vh::Epi::Store, vh::fp8_plan(g.m, g.n, g.a.k, false));
+    });
     GUARD_END
 }
 
@@ -4138,13 +4140,14 @@ static vh_status run_fp8(const vh_linear_fp8 *l, const vh_tensor *x, const vh_fp
     TRY(set_device(s));
     if (rows == 0) return VH_OK;
     vh::Fp8Gemm g{};
+    const vh::Fp8Plan plan = vh::fp8_plan(rows, n, k, x != nullptr);
     if (q) {
         g.a = q->view;
-    } else {
+    } else if (plan != vh::Fp8Plan::Fused) {
         void *p = graph_workspace(s, s.f8, s.f8_capture, fp8_bytes(rows, k));
         if (!p) return no_workspace(s, "fp8 activation workspace");
         g.a = fp8_view(p, rows, k);
-        TRY(quantize_fp8(s, x->ptr, g.a));
+        TRY(quantize_fp8(s, x->ptr, g.a, plan == vh::Fp8Plan::Few));
     }
     g.b = l->w;
     g.b_scales = l->scales;
@@ -4153,7 +4156,7 @@ static vh_status run_fp8(const vh_linear_fp8 *l, const vh_tensor *x, const vh_fp
     g.c = out->ptr;
     g.m = rows;
     g.n = n;
-    return launch(s, "gemm_fp8", [&] { return vh::launch_gemm_fp8(s.stream, g, epi); });
+    return launch(s, "gemm_fp8", [&] { return vh::launch_gemm_fp8(s.stream, g, epi, plan, x ? x->ptr : nullptr); });
     GUARD_END
 }
 
