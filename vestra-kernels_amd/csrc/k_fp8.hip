@@ -86,16 +86,41 @@ __device__ __forceinline__ f32x4 row4(const float *row, size_t d, size_t k) {
     return v;
 }
 
-// 16 rows' floats of a block, 32 lanes a row.
-template <bool VEC>
+// 16 rows' floats of a block, 32 lanes a row: of the nearest there are, so that no load is in a
+// branch (where every one would be waited for); clear_panel takes out what was not asked
+// for.  VEC: whole float4 at 32 bits of a lane's own, below 2^24 values a row.
+constexpr size_t kVecK = (size_t)1 << 24;
+template <bool VEC, bool NT>
 __device__ __forceinline__ void load_panel(const float *x, const Fp8Rows &w, size_t tile, size_t b, int lane,
                                            f32x4 (&v)[8]) {
+    asm volatile("" : "+v"(lane));
+    const int side = lane >> 5, c = lane & 31;
+    const int last = (int)min((size_t)16, w.rows - tile * 16) - 1;
+    if constexpr (VEC) {
+        const char *base = reinterpret_cast<const char *>(x + tile * 16 * w.k);
+        const uint32_t at = (uint32_t)min(b * 128 + 4 * c, w.k - 4) * 4, row_bytes = (uint32_t)w.k * 4;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const size_t row = tile * 16 + 2 * i + (lane >> 5), d = b * 128 + 4 * (lane & 31);
-        v[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (row < w.rows) v[i] = row4<VEC>(x + row * w.k, d, w.k);
+        for (int i = 0; i < 8; i++) {
+            const f32x4 *p = reinterpret_cast<const f32x4 *>(base + (at + min(2 * i + side, last) * row_bytes));
+            v[i] = NT ? __builtin_nontemporal_load(p) : *p;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float *row = x + (tile * 16 + min(2 * i + side, last)) * w.k;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[i][j] = row[min(b * 128 + 4 * c + j, w.k - 1)];
+        }
     }
+}
+__device__ __forceinline__ void clear_panel(const Fp8Rows &w, size_t tile, size_t b, int lane, f32x4 (&v)[8]) {
+    if (tile * 16 + 16 <= w.rows && b * 128 + 128 <= w.k) return;
+    const int side = lane >> 5, c = lane & 31;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (tile * 16 + 2 * i + side >= w.rows || b * 128 + 4 * c + j >= w.k) v[i][j] = 0.0f;
 }
 // Largest of the 32 lanes of a row, in each of them.
 __device__ __forceinline__ uint32_t row_umax(uint32_t v) {
@@ -104,29 +129,36 @@ __device__ __forceinline__ uint32_t row_umax(uint32_t v) {
 }
 // Their codes; `to`: 2048 bytes of the wave's own.  Lanes 0 .. 7 of either half get the
 // exponents of rows 2 lane + half.
-__device__ __forceinline__ int quantize_panel(const f32x4 (&v)[8], const Fp8Rows &out, size_t tile, size_t b, int lane,
+__device__ __forceinline__ int quantize_panel(f32x4 (&v)[8], const Fp8Rows &out, size_t tile, size_t b, int lane,
                                               char *to) {
+    // Opaque: what follows from the lane (addresses, masks) is formed for each panel anew, not kept
+    // over the loop in 90 registers.
+    asm volatile("" : "+v"(lane));
     const int c = lane & 31, side = lane >> 5;
-    uint32_t mx[8];
-    bool finite = true;
+    clear_panel(out, tile, b, lane, v);
+    uint32_t mx[8], most = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         mx[i] = row_umax(absmax4(0, v[i]));
-        finite &= mx[i] < 0x7f800000u;
+        most = max(most, mx[i]);
     }
-    int mine = -127;
-    const bool all = !__any(!finite);
+    if (__any(most >= 0x7f800000u)) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if (!all) {
+        for (int i = 0; i < 8; i++) {
             uint32_t m = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) m = finite_max(m, v[i][j]);
+            for (int j = 0; j < 4; j++) {
+                m = finite_max(m, v[i][j]);
+                v[i][j] = fabsf(v[i][j]) < INFINITY ? v[i][j] : NAN;
+            }
             mx[i] = row_umax(m);
         }
+    }
+    int mine = -127;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
         const int e = block_exponent(mx[i]);
-        const float inv = pow2(-e);
-        *reinterpret_cast<int *>(to + panel_at(2 * i + side, c)) = e4m3_of(all ? v[i] * inv : scaled(v[i], inv));
+        *reinterpret_cast<int *>(to + panel_at(2 * i + side, c)) = e4m3_of(v[i] * pow2(-e));
         if (c == i) mine = e;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -139,27 +171,24 @@ __device__ __forceinline__ int quantize_panel(const f32x4 (&v)[8], const Fp8Rows
     return mine;
 }
 
-// A workgroup takes 16 rows, its waves their blocks in turn, the next block's floats on
-// their way.  Rows past the end become zeros.
-constexpr int kQuantBlocks = 256;  // whose exponents stay in LDS
-template <bool VEC, int THREADS>
-__global__ __launch_bounds__(THREADS) void quantize_fp8_kernel(const float *x, Fp8Rows out) {
-    constexpr int W = THREADS / 64;
+// A workgroup takes 16 rows, its waves their blocks in turn.  Rows past the end become
+// zeros.  Bound by HBM where there are many rows (13828 x 4096 58.7 us, 4.8 TB/s); the next
+// block's floats asked for ahead, or fewer waves a workgroup, are no faster.
+constexpr int kQuantThreads = 512, kQuantBlocks = 256;  // whose exponents stay in LDS
+template <bool VEC, bool NT>
+__global__ __launch_bounds__(kQuantThreads) void quantize_fp8_kernel(const float *x, Fp8Rows out) {
+    constexpr int W = kQuantThreads / 64;
     __shared__ __attribute__((aligned(16))) char stage[W][2048];
     __shared__ int wave_max[W][16];
     __shared__ uint8_t codes[kQuantBlocks * 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, row = 2 * c + (lane >> 5);
     const size_t kb = fp8_blocks(out.k), rows16 = fp8_rows16(out.rows);
     for (size_t tile = blockIdx.x; tile < rows16 / 16; tile += gridDim.x) {
-        f32x4 v[8];
-        if ((size_t)wave < kb) load_panel<VEC>(x, out, tile, wave, lane, v);
         int most = -127;
         for (size_t b = wave; b < kb; b += W) {
-            f32x4 now[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) now[i] = v[i];
-            if (b + W < kb) load_panel<VEC>(x, out, tile, b + W, lane, v);
-            const int e = quantize_panel(now, out, tile, b, lane, stage[wave]);
+            f32x4 v[8];
+            load_panel<VEC, NT>(x, out, tile, b, lane, v);
+            const int e = quantize_panel(v, out, tile, b, lane, stage[wave]);
             if (c < 8 && b < kQuantBlocks) codes[b * 16 + row] = (uint8_t)(e + 127);
             most = max(most, e);
         }
@@ -170,7 +199,7 @@ __global__ __launch_bounds__(THREADS) void quantize_fp8_kernel(const float *x, F
 #pragma unroll
         for (int w = 1; w < W; w++) most = max(most, wave_max[w][tid & 15]);
         if (tid < 16) out.row_e[tile * 16 + tid] = most;
-        for (size_t i = tid; i < kb * 16; i += THREADS) {
+        for (size_t i = tid; i < kb * 16; i += kQuantThreads) {
             const size_t at = (i >> 4) * rows16 + tile * 16 + (i & 15);
             out.rel[at] = fp8_relative(i < kQuantBlocks * 16 ? codes[i] : out.exps[at], most);
         }
@@ -184,7 +213,7 @@ template <bool VEC>
 __global__ __launch_bounds__(64) void quantize_panels_kernel(const float *x, Fp8Rows out) {
     __shared__ __attribute__((aligned(16))) char stage[2048];
     f32x4 v[8];
-    load_panel<VEC>(x, out, blockIdx.y, blockIdx.x, threadIdx.x, v);
+    load_panel<VEC, false>(x, out, blockIdx.y, blockIdx.x, threadIdx.x, v);
     quantize_panel(v, out, blockIdx.y, blockIdx.x, threadIdx.x, stage);
 }
 __global__ __launch_bounds__(256) void relative_fp8_kernel(Fp8Rows out) {
@@ -202,7 +231,7 @@ __global__ __launch_bounds__(256) void relative_fp8_kernel(Fp8Rows out) {
 }
 
 // The values that the codes stand for.
-template <bool VEC>
+template <bool VEC, bool NT>
 __global__ __launch_bounds__(256) void dequantize_fp8_kernel(Fp8Rows in, float *out) {
     __shared__ __attribute__((aligned(16))) char stage[4][2048];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, side = lane >> 5;
@@ -227,7 +256,9 @@ __global__ __launch_bounds__(256) void dequantize_fp8_kernel(Fp8Rows in, float *
             const f32x4 v{ldexpf(lo[0], e), ldexpf(lo[1], e), ldexpf(hi[0], e), ldexpf(hi[1], e)};
             if (row >= in.rows || d >= in.k) continue;
             float *y = out + row * in.k + d;
-            if constexpr (VEC) {
+            if constexpr (VEC && NT) {
+                __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(y));
+            } else if constexpr (VEC) {
                 *reinterpret_cast<f32x4 *>(y) = v;
             } else {
 #pragma unroll
@@ -531,37 +562,39 @@ hipError_t launch_blocks(hipStream_t s, const Fp8Gemm &g, Epi epi, Fp8Plan plan,
 
 }  // namespace
 
-template <int THREADS>
-static void quantize_with(hipStream_t s, const float *x, const Fp8Rows &out) {
-    const unsigned grid = (unsigned)std::min(fp8_rows16(out.rows) / 16, kMaxGrid);
-    if (out.k % 4 == 0) quantize_fp8_kernel<true, THREADS><<<grid, THREADS, 0, s>>>(x, out);
-    else quantize_fp8_kernel<false, THREADS><<<grid, THREADS, 0, s>>>(x, out);
-}
+// Whether the floats pass by the caches (4001 x 2200 from memory 10.3 us, through the caches 12.3;
+// 13828 x 4096 58.7 and 62.1; 865 x 768 4.4 and 4.05).
+constexpr size_t kFp8StreamBytes = (size_t)32 << 20;
 
 hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out, bool products_of_few) {
     const size_t tiles = fp8_rows16(out.rows) / 16, kb = fp8_blocks(out.k);
+    const bool vec = out.k % 4 == 0 && out.k <= kVecK;
     // Few rows: a wave a panel (100 x 6000 in 7.8 us, two launches, against 14.2 of one workgroup for
-    // 16 rows; 865 x 768 7.0 against 4.9).  More: as many waves as two rounds leave (864 tiles
-    // of 768, two waves each, 12.7 us, of eight 19.3; 217 tiles 8.0 and 5.3).
+    // 16 rows; 865 x 768 7.0 against 4.9).
     if (products_of_few || (tiles <= 64 && kb > 16)) {
         const dim3 grid((unsigned)kb, (unsigned)tiles);
-        if (out.k % 4 == 0) quantize_panels_kernel<true><<<grid, 64, 0, s>>>(x, out);
+        if (vec) quantize_panels_kernel<true><<<grid, 64, 0, s>>>(x, out);
         else quantize_panels_kernel<false><<<grid, 64, 0, s>>>(x, out);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess || products_of_few) return e;
         relative_fp8_kernel<<<(unsigned)tiles, 256, 0, s>>>(out);
         return hipGetLastError();
     }
-    if (tiles >= 512) quantize_with<128>(s, x, out);
-    else quantize_with<512>(s, x, out);
+    const unsigned grid = (unsigned)std::min(tiles, kMaxGrid);
+    if (!vec) quantize_fp8_kernel<false, false><<<grid, kQuantThreads, 0, s>>>(x, out);
+    else if (out.rows * out.k * 4 >= kFp8StreamBytes) quantize_fp8_kernel<true, true><<<grid, kQuantThreads, 0, s>>>(x, out);
+    else quantize_fp8_kernel<true, false><<<grid, kQuantThreads, 0, s>>>(x, out);
     return hipGetLastError();
 }
 
 hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out) {
     const size_t tiles = fp8_rows16(in.rows) / 16 * fp8_blocks(in.k);
     const unsigned grid = (unsigned)std::min((tiles + 3) / 4, kMaxGrid);
-    if (in.k % 4 == 0) dequantize_fp8_kernel<true><<<grid, 256, 0, s>>>(in, out);
-    else dequantize_fp8_kernel<false><<<grid, 256, 0, s>>>(in, out);
+    // Whole lines past the caches (13828 x 4096 57 us, past them 44; lines in two pieces, 55312 x 1100,
+    // 71 and 76).
+    if (in.k % 32 == 0 && in.rows * in.k * 4 >= kFp8StreamBytes) dequantize_fp8_kernel<true, true><<<grid, 256, 0, s>>>(in, out);
+    else if (in.k % 4 == 0) dequantize_fp8_kernel<true, false><<<grid, 256, 0, s>>>(in, out);
+    else dequantize_fp8_kernel<false, false><<<grid, 256, 0, s>>>(in, out);
     return hipGetLastError();
 }
 
