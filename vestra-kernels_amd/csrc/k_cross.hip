@@ -101,11 +101,13 @@ __device__ __forceinline__ uint32_t finite_max(uint32_t mx, float v) {
 
 // ---- storing ------------------------------------------------------------------------
 
-constexpr int kHeadGroup = 8;  // heads of a workgroup of range_kernel
+constexpr int kHeadGroup = 8;   // heads of a workgroup of cross_range_kernel
+constexpr int kMaxChunks = 32;  // of an image's tokens there
 
 // Of a chunk of an image's tokens: the largest finite magnitudes of K of each head and of
-// V of each dim, into ranges [images][chunks][heads][1 + D], and where the seen tokens
-// go (kept [images][capacity], the tokens in order; lens).
+// V of each dim, into ranges [images][chunks][heads][1 + D]; behind the workgroups of the
+// heads one that finds where the seen tokens go (kept [images][capacity], the tokens in
+// order; lens).
 template <int D>
 __global__ __launch_bounds__(256) void cross_range_kernel(CrossWrite w) {
     __shared__ uint32_t vmax[kHeadGroup * D], kmax[kHeadGroup];
@@ -114,26 +116,24 @@ __global__ __launch_bounds__(256) void cross_range_kernel(CrossWrite w) {
     const int h0 = blockIdx.y * kHeadGroup, heads = min(kHeadGroup, w.view.kv_heads - h0);
     const int from = chunk * w.chunk, to = min(from + w.chunk, w.tokens);
     const int *seen = w.seen ? w.seen + (size_t)img * w.tokens : nullptr;
+    if (heads <= 0) {  // a workgroup of its own
+        int n = 0;
+        for (int i = tid; i < from; i += 256) n += seen[i] != 0;
+        long long before = 0, all = 0;
+        scan_all<256>(n, tmp, &before);
+        for (int i0 = from; i0 < to; i0 += 256) {
+            const int i = i0 + tid;
+            const bool there = i < to && seen[i] != 0;
+            const long long end = before + scan_all<256>(there, tmp, &all);
+            if (there) w.kept[(size_t)img * w.view.tokens + end - 1] = i;
+            before += all;
+        }
+        if (tid == 0 && to == w.tokens) w.view.lens[img] = (int)before;
+        return;
+    }
+    if (!seen && blockIdx.y == 0 && tid == 0 && to == w.tokens) w.view.lens[img] = w.tokens;
     for (int i = tid; i < kHeadGroup * D; i += 256) vmax[i] = 0;
     if (tid < kHeadGroup) kmax[tid] = 0;
-    if (blockIdx.y == 0) {
-        if (seen) {
-            int n = 0;
-            for (int i = tid; i < from; i += 256) n += seen[i] != 0;
-            long long before = 0, all = 0;
-            scan_all<256>(n, tmp, &before);
-            for (int i0 = from; i0 < to; i0 += 256) {
-                const int i = i0 + tid;
-                const bool there = i < to && seen[i] != 0;
-                const long long end = before + scan_all<256>(there, tmp, &all);
-                if (there) w.kept[(size_t)img * w.view.tokens + end - 1] = i;
-                before += all;
-            }
-            if (tid == 0 && to == w.tokens) w.view.lens[img] = (int)before;
-        } else if (tid == 0 && to == w.tokens) {
-            w.view.lens[img] = w.tokens;
-        }
-    }
     __syncthreads();
     const int per = w.head_dim / 4, columns = heads * per;
     int rows = 1;  // tokens at once
@@ -144,15 +144,24 @@ __global__ __launch_bounds__(256) void cross_range_kernel(CrossWrite w) {
         const int h = c / per, d = 4 * (c % per);
         const size_t off = (size_t)img * w.kv_image + (h0 + h) * w.kv_head + d;
         uint32_t km = 0, vm[4] = {0, 0, 0, 0};
-        for (int t = from + first; t < to; t += rows) {
-            if (seen && !seen[t]) continue;
-            const f32x4 k = *reinterpret_cast<const f32x4 *>(w.k + off + t * w.kv_token);
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(w.v + off + t * w.kv_token);
+        // Eight tokens at a time, the last one again past the end: no load waits in a branch.
+        for (int t0 = from + first; t0 < to; t0 += 8 * rows) {
+            f32x4 k[8], v[8];
+            int live[8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                km = finite_max(km, k[i]);
-                vm[i] = finite_max(vm[i], v[i]);
+            for (int u = 0; u < 8; u++) {
+                const int t = min(t0 + u * rows, to - 1);
+                k[u] = *reinterpret_cast<const f32x4 *>(w.k + off + t * w.kv_token);
+                v[u] = *reinterpret_cast<const f32x4 *>(w.v + off + t * w.kv_token);
+                live[u] = seen ? seen[t] : 1;
             }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    km = finite_max(km, live[u] ? k[u][i] : 0.0f);
+                    vm[i] = finite_max(vm[i], live[u] ? v[u][i] : 0.0f);
+                }
         }
         atomicMax(&kmax[h], km);
 #pragma unroll
@@ -166,117 +175,191 @@ __global__ __launch_bounds__(256) void cross_range_kernel(CrossWrite w) {
     }
 }
 
+template <bool NT>
+__device__ __forceinline__ f32x4 ld4(const float *p) {
+    const f32x4 *q = reinterpret_cast<const f32x4 *>(p);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+}
+
+// Four halves of column li of a 4 x 16 tile of halves in LDS, whose row r is in the lanes 4 r
+// .. 4 r + 3 of each 16-lane group (lane i gives the address of row i / 4, columns 4 (i %
+// 4) .. + 3, and receives column i).
+__device__ __forceinline__ f16x4 read_tr(const char *p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) s16x4 *)p));
+}
+
 // 128 keys of an image's head to their blocks, a block a wave; zeros behind the last key.
-template <int KIND, int D>
+// Rows are read whole; V^T comes from its rows of halves in LDS by transposing reads.
+template <int KIND, int D, bool NT>
 __global__ __launch_bounds__(256) void cross_write_kernel(CrossWrite w) {
-    constexpr int NP = kParts<KIND>, C = D / 32, DF = D / 16;
-    __shared__ int exps[1 + D];
+    constexpr int NP = kParts<KIND>, C = D / 32, DF = D / 16, PLANE = 32 * D * 2;
+    constexpr int LPR = D / 4, RPP = 64 / LPR, PASSES = 32 / RPP;  // lanes of a row of V, rows of a pass
+    __shared__ __attribute__((aligned(16))) int exps[4 + D];  // of K, then (from 4 on) of V's dims
+    __shared__ __attribute__((aligned(16))) char planes[4][NP * PLANE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lh = lane >> 4;
     const int g = blockIdx.y, img = blockIdx.z, len = w.view.lens[img];
     if ((int)blockIdx.x * 128 >= len && blockIdx.x) return;
+    const int block = blockIdx.x * 4 + wave, key0 = block * 32, last = max(len - 1, 0);
+    const bool any = (int)blockIdx.x * 128 < len, full = key0 + 32 <= len && w.head_dim == D;
+    const int *kept = w.seen ? w.kept + (size_t)img * w.view.tokens : nullptr;
+    // Loads are of the nearest key and dims there are; what was not asked for becomes zero.
+    auto token = [&](int key) { return kept ? kept[min(key, last)] : min(key, last); };
+    const size_t off = (size_t)img * w.kv_image + g * w.kv_head;
+    f32x4 k[2][C][2];
+    if (any) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const float *row = w.k + off + token(key0 + 16 * t + li) * w.kv_token;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) k[t][c][e] = ld4<NT>(row + min(32 * c + 8 * lh + 4 * e, w.head_dim - 4));
+        }
+    }
     for (int i = tid; i < 1 + D; i += 256) {
+        const uint32_t *r = w.ranges + ((size_t)img * w.chunks * w.view.kv_heads + g) * (1 + D) + i;
         uint32_t mx = 0;
-        for (int c = 0; c < w.chunks; c++)
-            mx = max(mx, w.ranges[(((size_t)img * w.chunks + c) * w.view.kv_heads + g) * (1 + D) + i]);
-        exps[i] = split_exponent(mx);
+        uint32_t some[kMaxChunks];  // all at once
+#pragma unroll
+        for (int c = 0; c < kMaxChunks; c++) some[c] = r[(size_t)min(c, w.chunks - 1) * w.view.kv_heads * (1 + D)];
+#pragma unroll
+        for (int c = 0; c < kMaxChunks; c++) mx = max(mx, some[c]);
+        const int e = split_exponent(mx);
+        exps[i ? 3 + i : 0] = e;
         if (blockIdx.x == 0) {
-            if (i == 0) w.view.k_exp[(size_t)img * w.view.kv_heads + g] = exps[0];
-            else w.view.v_exp[((size_t)img * w.view.kv_heads + g) * D + i - 1] = exps[i];
+            if (i == 0) w.view.k_exp[(size_t)img * w.view.kv_heads + g] = e;
+            else w.view.v_exp[((size_t)img * w.view.kv_heads + g) * D + i - 1] = e;
         }
     }
     __syncthreads();
-    const int block = blockIdx.x * 4 + wave, key0 = block * 32;
-    if ((int)blockIdx.x * 128 >= len) return;
+    if (!any) return;
     char *out = w.view.at(img, g) + (size_t)block * cross_block_bytes(KIND, D) + lane * 16;
-    const int *kept = w.seen ? w.kept + (size_t)img * w.view.tokens : nullptr;
-    auto token = [&](int key) { return key < len ? (kept ? kept[key] : key) : -1; };
-    const size_t off = (size_t)img * w.kv_image + g * w.kv_head;
-    auto put = [&](int operand, f32x4 a, f32x4 b) {
-        f16x8 hi, lo;
-        split8(a, b, hi, lo);
-        *reinterpret_cast<f16x8 *>(out + (operand * NP) * 1024) = hi;
-        if constexpr (NP == 2) *reinterpret_cast<f16x8 *>(out + (operand * NP + 1) * 1024) = lo;
-    };
     const int ke = exps[0];
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const int from = token(key0 + 16 * t + li);
-        const float *row = w.k + off + max(from, 0) * w.kv_token;
+    for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int c = 0; c < C; c++) {
             f32x4 x[2];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int d = 32 * c + 8 * lh + 4 * e;
-                x[e] = from >= 0 && d < w.head_dim ? *reinterpret_cast<const f32x4 *>(row + d)
-                                                   : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int e = 0; e < 2; e++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[e][i] = __builtin_ldexpf(x[e][i], -ke);
+                for (int i = 0; i < 4; i++) x[e][i] = __builtin_ldexpf(k[t][c][e][i], -ke);
+            if (!full) {
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (key0 + 16 * t + li >= len || 32 * c + 8 * lh + 4 * e >= w.head_dim)
+                        x[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            put(2 * c + t, x[0], x[1]);
+            f16x8 hi, lo;
+            split8(x[0], x[1], hi, lo);
+            *reinterpret_cast<f16x8 *>(out + (2 * c + t) * NP * 1024) = hi;
+            if constexpr (NP == 2) *reinterpret_cast<f16x8 *>(out + ((2 * c + t) * NP + 1) * 1024) = lo;
         }
+    const int vrow = lane / LPR, vd = 4 * (lane % LPR);
+    const i32x4 ve = *reinterpret_cast<const i32x4 *>(exps + 4 + vd);
+    char *plane = planes[wave];
+    f32x4 v[PASSES];
+#pragma unroll
+    for (int p = 0; p < PASSES; p++)
+        v[p] = ld4<NT>(w.v + off + token(key0 + p * RPP + vrow) * w.kv_token + min(vd, w.head_dim - 4));
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int row = p * RPP + vrow;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[p][i] = __builtin_ldexpf(v[p][i], -ve[i]);
+        if (!full && (key0 + row >= len || vd >= w.head_dim)) v[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        f16x2 h[2], l[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            h[i] = cvt_pk_f16(v[p][2 * i], v[p][2 * i + 1]);
+            l[i] = residual_pk_f16(h[i], v[p][2 * i], v[p][2 * i + 1]);
+        }
+        *reinterpret_cast<f16x4 *>(plane + (row * D + vd) * 2) = f16x4{h[0][0], h[0][1], h[1][0], h[1][1]};
+        if constexpr (NP == 2)
+            *reinterpret_cast<f16x4 *>(plane + PLANE + (row * D + vd) * 2) = f16x4{l[0][0], l[0][1], l[1][0], l[1][1]};
     }
-    int from[8];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const char *from = plane + ((4 * lh + (li >> 2)) * D + 4 * (li & 3)) * 2;
 #pragma unroll
-    for (int j = 0; j < 8; j++) from[j] = token(key0 + 16 * (j / 4) + 4 * lh + j % 4);
+    for (int df = 0; df < DF; df++)
 #pragma unroll
-    for (int df = 0; df < DF; df++) {
-        const int d = 16 * df + li, e = exps[1 + d];
-        f32x4 x[2];
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            x[j / 4][j % 4] = from[j] >= 0 && d < w.head_dim
-                                  ? __builtin_ldexpf(w.v[off + from[j] * w.kv_token + d], -e) : 0.0f;
-        put(2 * C + df, x[0], x[1]);
-    }
+        for (int p = 0; p < NP; p++) {
+            const f16x4 a = read_tr(from + p * PLANE + df * 32), b = read_tr(from + p * PLANE + 16 * D * 2 + df * 32);
+            *reinterpret_cast<f16x8 *>(out + ((2 * C + df) * NP + p) * 1024) =
+                __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
 }
 
 // What is stored, as floats [images][capacity][heads][head_dim]; zeros behind the last key.
-template <int KIND, int D>
+template <int KIND, int D, bool NT>
 __global__ __launch_bounds__(256) void cross_read_kernel(CrossView view, int head_dim, float *k, float *v, int *lens) {
-    constexpr int NP = kParts<KIND>, C = D / 32, DF = D / 16;
+    constexpr int NP = kParts<KIND>, C = D / 32, DF = D / 16, ROW = 36;  // floats of a row of 32 dims in LDS
+    __shared__ __attribute__((aligned(16))) float stage[4][32 * ROW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lh = lane >> 4;
     const int g = blockIdx.y, img = blockIdx.z, len = view.lens[img];
     if (lens && tid == 0 && g == 0 && blockIdx.x == 0) lens[img] = len;
     const int block = blockIdx.x * 4 + wave, key0 = block * 32;
     if (key0 >= view.tokens) return;
     const char *in = view.at(img, g) + (size_t)block * cross_block_bytes(KIND, D) + lane * 16;
+    // A block behind the last key is not read: its place is, and left out.
     const bool any = key0 < len;
+    if (!any) in = view.at(img, g) + lane * 16;
     const int ke = view.k_exp[(size_t)img * view.kv_heads + g];
+    const int *ves = view.v_exp + ((size_t)img * view.kv_heads + g) * D;
     auto get = [&](int operand, float (&x)[8]) {
         const f16x8 hi = *reinterpret_cast<const f16x8 *>(in + operand * NP * 1024);
         const f16x8 lo = *reinterpret_cast<const f16x8 *>(in + (operand * NP + NP - 1) * 1024);
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = (float)hi[i] + (NP == 2 ? (float)lo[i] : 0.0f);
     };
-    auto row = [&](int key) { return (((size_t)img * view.tokens + key) * view.kv_heads + g) * head_dim; };
+    auto put = [&](float *to, int key, int d, f32x4 y) {
+        if (key >= view.tokens || d >= head_dim) return;
+        if (key >= len) y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 *at = reinterpret_cast<f32x4 *>(to + (((size_t)img * view.tokens + key) * view.kv_heads + g) * head_dim + d);
+        if (NT) __builtin_nontemporal_store(y, at);
+        else *at = y;
+    };
+    float *mine = stage[wave];
+    // 32 dims at a time through LDS, so that rows are written in whole lines.
+    auto rows = [&](float *to, int d0) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int c = 0; c < C; c++)
+        for (int i = 0; i < 4; i++) {
+            const int key = 8 * i + (lane >> 3), d = 4 * (lane & 7);
+            put(to, key0 + key, d0 + d, *reinterpret_cast<const f32x4 *>(mine + key * ROW + d));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+#pragma unroll
+    for (int c = 0; c < C; c++) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const int key = key0 + 16 * t + li;
-            float x[8] = {};
-            if (any) get(2 * c + t, x);
+            float x[8];
+            get(2 * c + t, x);
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const int d = 32 * c + 8 * lh + 4 * e;
                 f32x4 y;
 #pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = key < len ? __builtin_ldexpf(x[4 * e + i], ke) : 0.0f;
-                if (key < view.tokens && d < head_dim) *reinterpret_cast<f32x4 *>(k + row(key) + d) = y;
+                for (int i = 0; i < 4; i++) y[i] = __builtin_ldexpf(x[4 * e + i], ke);
+                *reinterpret_cast<f32x4 *>(mine + (16 * t + li) * ROW + 8 * lh + 4 * e) = y;
             }
         }
+        rows(k, 32 * c);
+    }
 #pragma unroll
-    for (int df = 0; df < DF; df++) {
-        const int d = 16 * df + li;
-        const int ve = view.v_exp[((size_t)img * view.kv_heads + g) * D + d];
-        float x[8] = {};
-        if (any) get(2 * C + df, x);
+    for (int c = 0; c < C; c++) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int key = key0 + 16 * (j / 4) + 4 * lh + j % 4;
-            if (key < view.tokens && d < head_dim) v[row(key) + d] = key < len ? __builtin_ldexpf(x[j], ve) : 0.0f;
+        for (int h = 0; h < 2; h++) {
+            float x[8];
+            get(2 * C + 2 * c + h, x);
+            const int ve = ves[32 * c + 16 * h + li];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                mine[(16 * (j / 4) + 4 * lh + j % 4) * ROW + 16 * h + li] = __builtin_ldexpf(x[j], ve);
         }
+        rows(v, 32 * c);
     }
 }
 
@@ -841,26 +924,37 @@ hipError_t run_attn(hipStream_t s, CrossAttn a) {
     return hipGetLastError();
 }
 
+// Whether rows pass by the caches: those of K and V where they are read the second time, and
+// what is read back.
+constexpr size_t kCrossStreamBytes = (size_t)64 << 20;
+
 template <int KIND, int D>
 hipError_t run_write(hipStream_t s, const CrossWrite &w) {
-    const unsigned groups = (w.view.kv_heads + kHeadGroup - 1) / kHeadGroup, images = w.view.images;
+    const unsigned groups = (w.view.kv_heads + kHeadGroup - 1) / kHeadGroup + (w.seen ? 1 : 0), images = w.view.images;
+    const size_t bytes = (size_t)w.tokens * w.view.kv_heads * w.head_dim * 8;  // of an image
     cross_range_kernel<D><<<dim3(w.chunks, groups, images), 256, 0, s>>>(w);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    cross_write_kernel<KIND, D><<<dim3(std::max(1, (w.tokens + 127) / 128), w.view.kv_heads, images), 256, 0, s>>>(w);
+    const dim3 grid(std::max(1, (w.tokens + 127) / 128), w.view.kv_heads, images);
+    if (images * bytes >= kCrossStreamBytes) cross_write_kernel<KIND, D, true><<<grid, 256, 0, s>>>(w);
+    else cross_write_kernel<KIND, D, false><<<grid, 256, 0, s>>>(w);
     return hipGetLastError();
 }
 
 template <int KIND, int D>
 hipError_t run_read(hipStream_t s, const CrossView &v, int head_dim, float *k, float *vv, int *lens) {
-    cross_read_kernel<KIND, D><<<dim3((v.tokens + 127) / 128, v.kv_heads, v.images), 256, 0, s>>>(v, head_dim, k, vv, lens);
+    const dim3 grid((v.tokens + 127) / 128, v.kv_heads, v.images);
+    if (head_dim % 32 == 0 && (size_t)v.images * v.tokens * v.kv_heads * head_dim * 8 >= kCrossStreamBytes)
+        cross_read_kernel<KIND, D, true><<<grid, 256, 0, s>>>(v, head_dim, k, vv, lens);
+    else
+        cross_read_kernel<KIND, D, false><<<grid, 256, 0, s>>>(v, head_dim, k, vv, lens);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// Chunks of an image's tokens in cross_range_kernel: at most 32, of 64 tokens at least.
-int cross_chunks(size_t tokens) { return (int)std::min<size_t>(std::max<size_t>((tokens + 63) / 64, 1), 32); }
+// Chunks of an image's tokens in cross_range_kernel, of 32 tokens at least.
+int cross_chunks(size_t tokens) { return (int)std::min<size_t>(std::max<size_t>((tokens + 31) / 32, 1), kMaxChunks); }
 
 hipError_t launch_cross_write(hipStream_t s, CrossWrite w) {
     w.chunks = cross_chunks(w.tokens);
