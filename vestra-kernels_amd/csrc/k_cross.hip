@@ -23,6 +23,7 @@
 // V), and the key steps of all tiles, end to end, in equal shares of the workgroups.  The
 // lengths are on the device: every workgroup forms the partition from them.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 #include "kernels.h"
@@ -397,6 +398,13 @@ template <int THREADS, class F>
 __device__ __forceinline__ long long find_image(const CrossAttn &a, int step, F at, int &where, long long &base) {
     __shared__ long long tmp[THREADS / 64], found[2];
     const long long per = (long long)a.tiles * a.view.kv_heads;
+    if (a.images == 1) {
+        const long long total = per * cost_of(a, 0, step);
+        at(total);
+        where = 0;
+        base = 0;
+        return total;
+    }
     long long total = 0, all = 0, end = 0, cost = 0;
     for (int i0 = 0; i0 < a.images; i0 += THREADS) {
         const int i = i0 + threadIdx.x;
@@ -433,13 +441,15 @@ __device__ __forceinline__ long long find_image(const CrossAttn &a, int step, F 
 
 // ---- parts ------------------------------------------------------------------------------
 
-// Where the last workgroup of a tile joins them they are read and written past the L2 of
-// an XCD (sc1), as the workgroups of a tile may be on several.
+// Where the last workgroup of a tile joins them (HERE) they are read and written past the L2
+// of an XCD (sc1), as the workgroups of a tile may be on several; a launch of its own
+// sees them anyway.
+template <bool HERE>
 struct Parts {
     __amdgpu_buffer_rsrc_t base;
     __device__ __forceinline__ explicit Parts(const CrossAttn &a)
         : base(__builtin_amdgcn_make_buffer_rsrc(a.parts, 0, 0xffffffff, 0x00027000)) {}
-    static constexpr int kAgent = 16;
+    static constexpr int kAgent = HERE ? 16 : 0;
     __device__ __forceinline__ void put(uint32_t at, f32x4 v) const {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), base, at, 0, kAgent);
     }
@@ -465,7 +475,7 @@ __device__ __forceinline__ uint32_t weights_at(const CrossAttn &a, uint32_t x, i
 }
 
 // Row `in` of a tile, four dims from d on: the result, or a workgroup's part of it.
-template <int BM, int D>
+template <int BM, int D, bool HERE>
 __device__ __forceinline__ void put_row(const CrossAttn &a, const Tile &t, int part, int in, int d, f32x4 v, float m,
                                         float l) {
     if (in >= t.rows) return;
@@ -479,7 +489,7 @@ __device__ __forceinline__ void put_row(const CrossAttn &a, const Tile &t, int p
         for (int i = 0; i < 4; i++) y[i] = l == 0.0f ? 0.0f : __builtin_ldexpf(v[i] * inv, e[i]);
         *reinterpret_cast<f32x4 *>(a.out + t.img * a.q_image + token * a.q_token + head * a.q_head + d) = y;
     } else {
-        const Parts parts(a);
+        const Parts<HERE> parts(a);
         parts.put(sums_at<BM, D>(part, in) + 4 * d, v);
         if (d == 0) parts.put(weights_at<BM, D>(a, part, in), m, l);
     }
@@ -499,21 +509,21 @@ struct Sums {
     }
 };
 
-// The parts of shares w0 .. w1 (of w0 the one at part0) become the tile's output.  Of the
+// The parts of shares w0 .. w1 (of w0 the one at part0) become the tile's rows first .. to - 1.  Of the
 // workgroup's groups of D / 4 lanes (a group holds a row) as many share a row as the rows
 // leave: a single query's parts are summed by all of them.
-template <int BM, int D, int THREADS>
-__device__ void join_parts(const CrossAttn &a, const Tile &t, int w0, int w1, int part0, char *smem) {
+template <int BM, int D, int THREADS, bool HERE>
+__device__ void join_parts(const CrossAttn &a, const Tile &t, int w0, int w1, int part0, int first, int to, char *smem) {
     Sums *some = reinterpret_cast<Sums *>(smem);
-    const Parts parts(a);
+    const Parts<HERE> parts(a);
     constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
     int rows = 1;  // at once
-    while (rows < GROUPS && rows < t.rows) rows *= 2;
+    while (rows < GROUPS && rows < to - first) rows *= 2;
     const int sharers = GROUPS / rows;
     const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
-    for (int in = group % rows; in < (t.rows + rows - 1) / rows * rows; in += rows) {
+    for (int in = first + group % rows; in < first + (to - first + rows - 1) / rows * rows; in += rows) {
         auto part = [&](int w) {
-            const int x = w == w0 ? part0 : 2 * w, row = min(in, t.rows - 1);
+            const int x = w == w0 ? part0 : 2 * w, row = min(in, to - 1);
             const u32x2 ml = parts.two(weights_at<BM, D>(a, x, row));
             return Sums{__uint_as_float(ml[0]), __uint_as_float(ml[1]), parts.four(sums_at<BM, D>(x, row) + 4 * d)};
         };
@@ -532,16 +542,16 @@ __device__ void join_parts(const CrossAttn &a, const Tile &t, int w0, int w1, in
             if (group < rows)
                 for (int i = 1; i < sharers; i++) sum.join(some[threadIdx.x + i * rows * LANES]);
         }
-        if (group < rows && in < t.rows) put_row<BM, D>(a, t, -1, in, d, sum.y, sum.m, sum.l);
+        if (group < rows && in < to) put_row<BM, D, HERE>(a, t, -1, in, d, sum.y, sum.m, sum.l);
     }
 }
 
 // Walks this workgroup's steps tile by tile: f(tile, first step, steps, part).  Without room
-// for parts (a.parts null) every workgroup takes whole tiles.  Of the workgroups that
+// for parts (a.parts null) every workgroup takes whole tiles.  HERE: of the workgroups that
 // hold a part of a tile the one that is done last joins them, in the order of the shares.
 // They count in the counter of the tile's first share (of which it is the last tile, so no
 // other counts there), zero before and after.
-template <int BM, int STEP, int THREADS, int D, class F>
+template <int BM, int STEP, int THREADS, int D, bool HERE, class F>
 __device__ __forceinline__ void walk(const CrossAttn &a, char *smem, F f) {
     __shared__ int is_last;
     const int w = (blockIdx.x & 7) * (a.shares >> 3) + (blockIdx.x >> 3);  // neighbours on one XCD
@@ -573,7 +583,7 @@ __device__ __forceinline__ void walk(const CrossAttn &a, char *smem, F f) {
         const bool whole = into == 0 && steps == cost;
         const int from = max(into - kTileCost, 0), to = max(into + steps - kTileCost, 0);
         f(t, from, to - from, whole ? -1 : 2 * w + (first ? 0 : 1));
-        if (!whole) {
+        if (HERE && !whole) {
             const long long begin = at - into;
             const int w0 = uniform((int)(begin / share)), w1 = uniform((int)((begin + cost - 1) / share));
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's parts are out
@@ -586,7 +596,7 @@ __device__ __forceinline__ void walk(const CrossAttn &a, char *smem, F f) {
             }
             __syncthreads();
             if (is_last) {
-                join_parts<BM, D, THREADS>(a, t, w0, w1, 2 * w0 + (begin > w0 * share ? 1 : 0), smem);
+                join_parts<BM, D, THREADS, true>(a, t, w0, w1, 2 * w0 + (begin > w0 * share ? 1 : 0), 0, t.rows, smem);
                 __syncthreads();
             }
         }
@@ -785,7 +795,7 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
     __shared__ __attribute__((aligned(16))) char smem[4 * WAVE < 256 * (int)sizeof(Sums) ? 256 * sizeof(Sums) : 4 * WAVE];
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lh = lane >> 4;
     const int wave = uniform(tid >> 6);
-    walk<BM, STEP, 256, D>(a, smem, [&](const Tile &t, int step0, int steps, int part) {
+    walk<BM, STEP, 256, D, true>(a, smem, [&](const Tile &t, int step0, int steps, int part) {
         const char *base = a.view.at(t.img, t.g) + lane * 16;
         auto load = [&](int step, int operand) {
             const size_t at = (size_t)(step * 4 + wave) * BLOCK + operand * 1024;
@@ -841,7 +851,7 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
 #pragma unroll
             for (int x = 0; x < 4; x++)
                 y += *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(smem + x * WAVE) + row * D + d) * f[x];
-            put_row<BM, D>(a, t, part, row, d, y, m, sum);
+            put_row<BM, D, true>(a, t, part, row, d, y, m, sum);
         }
         __syncthreads();
     });
@@ -849,8 +859,10 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
 
 // ---- many rows: 128 a tile, 32 a wave, K and V of a step shared in LDS ----------------------
 
+// Blocks of 32 keys a step: 32 KB of LDS, twice.  (865 queries of 12 heads of 64 against 3460 halves
+// 41.6 us, with two blocks 46, with one 48.)
 template <int KIND, int D>
-constexpr int kManyHalves = KIND == kCrossF32 && D == 128 ? 1 : 2;  // blocks of 32 keys a step
+constexpr int kManyHalves = 32768 / cross_block_bytes(KIND, D);
 
 template <int KIND, int D>
 __global__ __launch_bounds__(256, 2) void cross_many_kernel(CrossAttn a) {
@@ -860,7 +872,7 @@ __global__ __launch_bounds__(256, 2) void cross_many_kernel(CrossAttn a) {
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lh = lane >> 4;
     const int wave = uniform(tid >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-    walk<BM, STEP, 256, D>(a, smem, [&](const Tile &t, int step0, int steps, int part) {
+    walk<BM, STEP, 256, D, false>(a, smem, [&](const Tile &t, int step0, int steps, int part) {
         const char *base = a.view.at(t.img, t.g);
         auto copy = [&](int step, int buf) {
             const char *from = base + (size_t)step * BYTES;
@@ -899,28 +911,73 @@ __global__ __launch_bounds__(256, 2) void cross_many_kernel(CrossAttn a) {
             const float l = sum_groups(w.l[u]);
 #pragma unroll
             for (int df = 0; df < D / 16; df++)
-                put_row<BM, D>(a, t, part, first + 16 * u + li, 16 * df + 4 * lh, w.o[df][u], w.m[u], l);
+                put_row<BM, D, false>(a, t, part, first + 16 * u + li, 16 * df + 4 * lh, w.o[df][u], w.m[u], l);
         }
         __syncthreads();
     });
 }
 
+// Rows of a workgroup of cross_join_kernel (865 queries of 12 heads of 64 against 3300 in two
+// halves: 45.3 us, with half as many 48.9, with twice 45.8).
+template <int D>
+constexpr int kJoinRows = 1024 / D;
+// Joins the parts of cross_many_kernel: of share blockIdx.x those of the tile that begins in it
+// and goes on in the next, some rows a workgroup.
+template <int BM, int STEP, int D>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossAttn a) {
+    __shared__ __attribute__((aligned(16))) char smem[256 * sizeof(Sums)];
+    const int w = blockIdx.x;
+    int img = 0;
+    long long base = 0, share = 1;
+    const long long total = find_image<256>(a, STEP, [&](long long all) {
+        share = max(1ll, (all + a.shares - 1) / a.shares);
+        return (w + 1) * share - 1;
+    }, img, base);
+    const long long end = (w + 1) * share;
+    if (end >= total) return;
+    img = uniform(img);
+    const int len = uniform(a.view.lens[img]), cost = (len + STEP - 1) / STEP + kTileCost;
+    const int index = uniform((int)((end - 1 - base) / cost));
+    const long long begin = base + (long long)index * cost;
+    if (begin < w * share || begin + cost <= end) return;
+    const Tile t = tile_of<BM>(a, img, len, index, STEP);
+    const int first = blockIdx.y * kJoinRows<D>;
+    if (first >= t.rows) return;
+    join_parts<BM, D, 256, false>(a, t, w, uniform((int)((begin + cost - 1) / share)),
+                                  2 * w + (begin > w * share ? 1 : 0), first, min(first + kJoinRows<D>, t.rows), smem);
+}
+
 constexpr int kShares = 512;
 static_assert(kShares <= kAttnCounters, "a counter for each share");
 
-bool few_rows(const CrossAttn &a) { return (size_t)a.queries * a.group <= 16; }
+// Whether a call goes to tiles of 16 rows, by the times of both in us: tiles of 128 cost more to
+// begin and to join, and do the arithmetic of 128 whatever they hold; of 16 they reach a third
+// of its rate.  (Few / many, one image of 3460 tokens, 12 heads of 64: 17 rows in halves 12.4
+// / 19, 64 12.4 / 25, 128 14 / 30, of 20000 tokens 64 35 / 35; two halves 64 16 / 27, of 20000
+// 32 46 / 40; sixteen of 4096, 32 / 8 heads of 128: 8 queries in halves 70 / 78, in two
+// 130 / 125, 16 100 / 82, 200 / 138.)  The tokens are those that the states were made for.
+bool few_rows(const CrossAttn &a) {
+    const double rows = (double)a.queries * a.group, tiles = std::ceil(rows / 128) * 128;
+    const double products = (a.view.kind == kCrossF32 ? 12e-6 : 8e-6) * a.images * a.view.kv_heads * a.view.tokens * a.view.width;
+    return 9 + rows * products / (a.view.kind == kCrossF32 ? 180 : 280) < 22 + tiles * products / 850;
+}
 
 template <int KIND, int D>
-hipError_t run_attn(hipStream_t s, CrossAttn a) {
-    if (few_rows(a)) {
+hipError_t run_attn(hipStream_t s, CrossAttn a, bool few) {
+    if (few) {
         cross_few_kernel<KIND, D><<<a.shares, 256, 0, s>>>(a);
         return hipGetLastError();
     }
-    constexpr size_t bytes = std::max<size_t>(2 * kManyHalves<KIND, D> * cross_block_bytes(KIND, D), 256 * sizeof(Sums));
+    constexpr int H = kManyHalves<KIND, D>;
+    constexpr size_t bytes = std::max<size_t>(2 * H * cross_block_bytes(KIND, D), 256 * sizeof(Sums));
     static std::atomic<uint64_t> done{0};
     hipError_t e = ensure_dynamic_lds(cross_many_kernel<KIND, D>, bytes, done);
     if (e != hipSuccess) return e;
     cross_many_kernel<KIND, D><<<a.shares, 256, bytes, s>>>(a);
+    e = hipGetLastError();
+    if (e != hipSuccess || !a.parts) return e;
+    constexpr int rows = kJoinRows<D>;
+    cross_join_kernel<128, 32 * H, D><<<dim3(a.shares, (std::min(a.queries * a.group, 128) + rows - 1) / rows), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -974,10 +1031,11 @@ size_t cross_attn_floats(const CrossAttn &a) {
 }
 
 hipError_t launch_cross_attn(hipStream_t s, CrossAttn a) {
+    const bool few = few_rows(a);
     a.shares = kShares;
-    a.tiles = (a.queries * a.group + (few_rows(a) ? 15 : 127)) / (few_rows(a) ? 16 : 128);
-    if (a.view.kind == kCrossF32) return a.view.width == 128 ? run_attn<kCrossF32, 128>(s, a) : run_attn<kCrossF32, 64>(s, a);
-    return a.view.width == 128 ? run_attn<kCrossF16, 128>(s, a) : run_attn<kCrossF16, 64>(s, a);
+    a.tiles = (a.queries * a.group + (few ? 15 : 127)) / (few ? 16 : 128);
+    if (a.view.kind == kCrossF32) return a.view.width == 128 ? run_attn<kCrossF32, 128>(s, a, few) : run_attn<kCrossF32, 64>(s, a, few);
+    return a.view.width == 128 ? run_attn<kCrossF16, 128>(s, a, few) : run_attn<kCrossF16, 64>(s, a, few);
 }
 
 }  // namespace vh
