@@ -859,10 +859,11 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
 
 // ---- many rows: 128 a tile, 32 a wave, K and V of a step shared in LDS ----------------------
 
-// Blocks of 32 keys a step: 32 KB of LDS, twice.  (865 queries of 12 heads of 64 against 3460 halves
-// 41.6 us, with two blocks 46, with one 48.)
+// Blocks of 32 keys a step; two steps in LDS.  (Halves of 64, two blocks, four, and two with three
+// workgroups a CU: 865 queries of 12 heads against 1730 keys 33 us, 40, 37, against 3460 42, 41,
+// 45, 3457 against 20742 453, 472, 443.)
 template <int KIND, int D>
-constexpr int kManyHalves = 32768 / cross_block_bytes(KIND, D);
+constexpr int kManyHalves = KIND == kCrossF32 && D == 128 ? 1 : 2;
 
 template <int KIND, int D>
 __global__ __launch_bounds__(256, 2) void cross_many_kernel(CrossAttn a) {

@@ -432,19 +432,56 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
             }
         }
     }
+    // 16 rows at a time through LDS of the wave's own, so that a row is written in one piece,
+    // whatever its alignment (1239 x 50 x 7838, no multiple of four: 63 us without, 15 with).
+    constexpr int W = TN * 16, PITCH = W + 4;
+    static_assert(NW * 16 * PITCH * 4 <= ST * STAGE, "room for every wave's rows");
+    __syncthreads();
+    float *rows = reinterpret_cast<float *>(smem) + wave * 16 * PITCH;
+    const size_t n0 = (size_t)nt * BN + wn * W;
+    const bool whole = (g.n & 3) == 0;
+    const int lanes = whole ? W / 4 : W, row0 = lane / lanes, step = 64 / lanes;
+    const size_t n = n0 + (lane % lanes) * (whole ? 4 : 1);
+    f32x4 bias{0.0f, 0.0f, 0.0f, 0.0f}, gamma{1.0f, 1.0f, 1.0f, 1.0f};
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const size_t at = min(n + (whole ? r : 0), g.n - 1);
+        if (g.bias) bias[r] = g.bias[at];
+        if (g.gamma) gamma[r] = g.gamma[at];
+    }
+    auto finish = [&](float v, int r) {
+        v += bias[r];
+        return EPI == Epi::Gelu ? gelu_fast_form(v) : v * gamma[r];
+    };
 #pragma unroll
     for (int i = 0; i < TM; i++) {
-        const size_t m = (size_t)mt * BM + (wm * TM + i) * 16 + li;
-        const int ea = g.a.row_e[min(m, a16 - 1)];
+        const size_t m0 = (size_t)mt * BM + (wm * TM + i) * 16;
+        const int ea = g.a.row_e[min(m0 + li, a16 - 1)];
 #pragma unroll
         for (int j = 0; j < TN; j++) {
-            const size_t n = (size_t)nt * BN + (wn * TN + j) * 16 + 4 * lh;
             f32x4 v = acc[i][j];
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                v[r] = ldexpf(v[r], ea + (BLOCKS ? 0 : g.b.row_e[min(n + r, b16 - 1)]));
-            put4<EPI>(g, m, n, v);
+                v[r] = ldexpf(v[r], ea + (BLOCKS ? 0 : g.b.row_e[min(n0 + 16 * j + 4 * lh + r, b16 - 1)]));
+            *reinterpret_cast<f32x4 *>(rows + li * PITCH + 16 * j + 4 * lh) = v;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (n < g.n) {
+            for (int r0 = row0; r0 < 16 && m0 + r0 < g.m; r0 += step) {
+                float *c = g.c + (m0 + r0) * g.n + n;
+                if (whole) {
+                    f32x4 v = *reinterpret_cast<const f32x4 *>(rows + r0 * PITCH + 4 * (lane % lanes));
+#pragma unroll
+                    for (int r = 0; r < 4; r++) v[r] = finish(v[r], r);
+                    if (EPI == Epi::Residual) v += *reinterpret_cast<const f32x4 *>(c);
+                    stream_store(reinterpret_cast<f32x4 *>(c), v);
+                } else {
+                    const float v = finish(rows[r0 * PITCH + lane % lanes], 0);
+                    *c = EPI == Epi::Residual ? *c + v : v;
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -600,13 +637,13 @@ hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out) {
 
 // By a model of the launch, in us, fitted to 24 shapes measured with each form: the few rows'
 // form takes a wave's blocks one after the other (1.0) or what all workgroups have to read and
-// multiply; tiles of 64 and 128 one tile on its own, or rounds of as many as are resident
+// multiply, and as long again for each round of 1024 of them; tiles of 64 and 128 one tile on its own, or rounds of as many as are resident
 // (1024 and 512); tiles of 256 whole rounds of 256.
 Fp8Plan fp8_plan(size_t m, size_t n, size_t k, bool floats) {
     const auto tiles = [&](size_t b) { return (double)((m + b - 1) / b) * (double)((n + b - 1) / b); };
     const double kb = (double)fp8_blocks(k), groups = (double)((n + 15) / 16) * (double)((m + 63) / 64);
     const double each = m <= 16 ? 4.2e-4 : m <= 32 ? 5.6e-4 : 8.4e-4;
-    double best = 2.6 + std::max(std::ceil(kb / kFewWaves), groups * kb * each);
+    double best = 2.6 + std::max(std::ceil(kb / kFewWaves), groups * kb * each) + 5 * std::max(0.0, groups / 1024 - 1);
     // Fused while a wave quantises one block (one row of 768 for 2304 outputs 4.0 us, in two launches
     // 5.8; 16 rows 5.8 and 7.3; of 3072 for 768 8.0 and 6.6).
     Fp8Plan plan = floats && m <= 16 && kb <= kFewWaves && groups <= 1024 ? Fp8Plan::Fused : Fp8Plan::Few;
