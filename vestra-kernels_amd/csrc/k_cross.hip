@@ -922,30 +922,59 @@ __global__ __launch_bounds__(256, 2) void cross_many_kernel(CrossAttn a) {
 // halves: 45.3 us, with half as many 48.9, with twice 45.8).
 template <int D>
 constexpr int kJoinRows = 1024 / D;
-// Joins the parts of cross_many_kernel: of share blockIdx.x those of the tile that begins in it
-// and goes on in the next, some rows a workgroup.
+// Joins the parts of cross_many_kernel, some rows a workgroup: of tile blockIdx.x where there
+// are fewer tiles than shares, as most workgroups would find nothing otherwise (84 tiles:
+// 6.6 us; by 512 shares 10.9), else of the tile that begins in share blockIdx.x and
+// goes on in the next.
 template <int BM, int STEP, int D>
-__global__ __launch_bounds__(256) void cross_join_kernel(CrossAttn a) {
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossAttn a, bool by_tile) {
     __shared__ __attribute__((aligned(16))) char smem[256 * sizeof(Sums)];
-    const int w = blockIdx.x;
-    int img = 0;
-    long long base = 0, share = 1;
-    const long long total = find_image<256>(a, STEP, [&](long long all) {
-        share = max(1ll, (all + a.shares - 1) / a.shares);
-        return (w + 1) * share - 1;
-    }, img, base);
-    const long long end = (w + 1) * share;
-    if (end >= total) return;
-    img = uniform(img);
-    const int len = uniform(a.view.lens[img]), cost = (len + STEP - 1) / STEP + kTileCost;
-    const int index = uniform((int)((end - 1 - base) / cost));
-    const long long begin = base + (long long)index * cost;
-    if (begin < w * share || begin + cost <= end) return;
+    __shared__ long long tmp[4];
+    const int w = blockIdx.x, per = a.tiles * a.view.kv_heads;
+    int img = 0, index = 0, len = 0, cost = 0;
+    long long base = 0, share = 1, total = 0, begin = 0;
+    const auto shared = [&](long long all) { share = max(1ll, (all + a.shares - 1) / a.shares); };
+    if (by_tile) {
+        img = w / per;
+        index = w - img * per;
+        if (a.images == 1) {
+            total = (long long)per * cost_of(a, 0, STEP);
+        } else {
+            for (int i0 = 0; i0 < a.images; i0 += 256) {
+                const int i = i0 + threadIdx.x;
+                long long sum = 0, before = 0;
+                const long long c = i < a.images ? (long long)per * cost_of(a, i, STEP) : 0;
+                scan_all<256>(c, tmp, &sum);
+                scan_all<256>(i < img ? c : 0, tmp, &before);
+                total += sum;
+                base += before;
+            }
+        }
+        shared(total);
+        len = uniform(a.view.lens[img]);
+        cost = (len + STEP - 1) / STEP + kTileCost;
+        begin = base + (long long)index * cost;
+    } else {
+        total = find_image<256>(a, STEP, [&](long long all) {
+            shared(all);
+            return (w + 1) * share - 1;
+        }, img, base);
+        const long long end = (w + 1) * share;
+        if (end >= total) return;
+        img = uniform(img);
+        len = uniform(a.view.lens[img]);
+        cost = (len + STEP - 1) / STEP + kTileCost;
+        index = uniform((int)((end - 1 - base) / cost));
+        begin = base + (long long)index * cost;
+        if (begin < w * share || begin + cost <= end) return;
+    }
+    const int w0 = uniform((int)(begin / share)), w1 = uniform((int)((begin + cost - 1) / share));
+    if (w0 == w1) return;
     const Tile t = tile_of<BM>(a, img, len, index, STEP);
     const int first = blockIdx.y * kJoinRows<D>;
     if (first >= t.rows) return;
-    join_parts<BM, D, 256, false>(a, t, w, uniform((int)((begin + cost - 1) / share)),
-                                  2 * w + (begin > w * share ? 1 : 0), first, min(first + kJoinRows<D>, t.rows), smem);
+    join_parts<BM, D, 256, false>(a, t, w0, w1, 2 * w0 + (begin > w0 * share ? 1 : 0), first,
+                                  min(first + kJoinRows<D>, t.rows), smem);
 }
 
 constexpr int kShares = 512;
@@ -978,7 +1007,10 @@ hipError_t run_attn(hipStream_t s, CrossAttn a, bool few) {
     e = hipGetLastError();
     if (e != hipSuccess || !a.parts) return e;
     constexpr int rows = kJoinRows<D>;
-    cross_join_kernel<128, 32 * H, D><<<dim3(a.shares, (std::min(a.queries * a.group, 128) + rows - 1) / rows), 256, 0, s>>>(a);
+    const size_t items = (size_t)a.tiles * a.view.kv_heads * a.images;
+    const bool by_tile = items < (size_t)a.shares;
+    const dim3 grid(by_tile ? (unsigned)items : a.shares, (std::min(a.queries * a.group, 128) + rows - 1) / rows);
+    cross_join_kernel<128, 32 * H, D><<<grid, 256, 0, s>>>(a, by_tile);
     return hipGetLastError();
 }
 
