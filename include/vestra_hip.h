@@ -623,7 +623,7 @@ vh_status vh_cross_kv_read_f32(const vh_cross_kv *kv, vh_tensor *k, vh_tensor *v
  * finite leaves no defined row of its image and head, a value none in its dim.  The same
  * call gives the same bits.  At most 2^30 query rows (tokens * heads) of an image.
  * The parts of rows whose keys several workgroups share lie in a workspace of the
- * runtime (140 MB at most).  A call inside a stream capture takes it for its graph alone, until
+ * runtime (70 MB at most).  A call inside a stream capture takes it for its graph alone, until
  * the runtime ends; where none is left (nothing as large ran since the last capture)
  * the graph goes without: slower where there are few rows, its last bits other than an
  * eager call's. */

@@ -296,3 +296,51 @@ def test_calls_refuse(rt):
             call()
     kv.read(x, y, lens)
     assert not rt.download_f32(x).any() and not rt.download_i32(lens).any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 40, 300])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e12])
+def test_scores_far_past_the_floats_between_them(rt, kind, n, size):
+    """Scores of 1e8 and up, where neighbouring floats are 8 apart: a token along whose key each query lies has
+    all of the weight.  Its score is above the others by a quarter of itself, and off by less than 2^-18 of that."""
+    tokens, hd = 700, 64
+
+    def change(k, v):
+        k[...] = np.sign(k) * np.float32(size)
+        k[0, 501, 0] = size
+
+    states = States(rt, kind, 1, tokens, 1, hd, change=change)
+    gap = states.k[0][501, 0] @ states.k[0][:, 0].T
+    assert np.sort(gap)[-2] <= 0.75 * gap[501]
+    q = np.full((1, n, 2, hd), np.float32(size))
+    q[:, :, 1] *= -1.0  # the least score there is, and the others around zero
+    q[:, :, 1, ::2] *= 0.0
+    got = states.run(q)
+    v = states.v[0][501, 0]
+    assert np.abs(got[0, :, 0] - v).max() <= 2.0 ** -18 * np.abs(v).max()
+    assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 300])
+@pytest.mark.parametrize("gap", [17.0, 20.4, 21.5, 23.0])
+def test_many_small_weights_behind_a_large_one(rt, kind, n, gap):
+    """One token that has nearly all of the weight, and 60000 whose weights are alike and e^-gap of its: what
+    these come to.  A weight is held to within 2^-34 of the largest, so 60000 to 2^-18.1 together, of values of
+    1; a score of 23 in 32 bits and its exp2 to 2^-18."""
+    tokens, hd = 60000, 64
+
+    def change(k, v):
+        k[...] = 0.0
+        k[0, 123, 0, 0] = 8.0
+        v[...] = 1.0
+        v[0, 123] = 0.0
+
+    states = States(rt, kind, 1, tokens, 1, hd, change=change)
+    q = np.zeros((1, n, 1, hd), np.float32)
+    q[..., 0] = gap
+    got = states.run(q)
+    w = (tokens - 1) * np.exp(-float(q[0, 0, 0, 0]))
+    want = w / (1 + w)
+    assert np.abs(got - want).max() <= 2.0 ** -18 * (1 + want)
