@@ -152,6 +152,34 @@ def test_rows_of_wide_range(rt, m):
     _close(rt.download_f32(c).reshape(m, n), va @ vb.T, np.abs(va) @ np.abs(vb).T, k, lost)
 
 
+@pytest.mark.parametrize("m", [1, 40, 200, 1000, 20000])
+@pytest.mark.parametrize("power", [-120, 0, 116])
+def test_block_scales_of_any_size(rt, m, power):
+    """Scales of a checkpoint whose product with a block's sum is no float, where that with the row's exponent
+    is: rows of the size that the scales are not."""
+    k, n = 300, 200
+    x = _rows(5, m, k) * np.float32(2.0 ** -power)
+    codes = ref.e4m3(seeded.normal(6, n * k, 40.0).reshape(n, k).clip(-448, 448))
+    scales = seeded.normal(7, ref.blocks(n) * ref.blocks(k)) * np.float32(2.0 ** power)
+    scales[:3] *= np.float32(2.0 ** 9)  # 128 rows of their own size
+    lin = rt.prepare_linear_fp8_blocks(k, n, codes, scales)
+    out = rt.upload_f32(np.full(m * n, np.nan))
+    lin.run(rt.upload_f32(x), m, out)
+    va, vb = ref.values(*ref.quantise(x)), ref.block_values(codes, scales)
+    _close(rt.download_f32(out).reshape(m, n), va @ vb.T, np.abs(va) @ np.abs(vb).T, k)
+
+
+def test_more_rows_than_a_launch_has_in_a_direction(rt):
+    """Of a few columns: 65536 workgroups of 16 rows, and 17 rows."""
+    m, k, n = 65536 * 16 + 17, 20, 7
+    x, w = _rows(1, m, k), seeded.normal(2, k * n, 0.1).reshape(k, n)
+    lin = rt.prepare_linear_fp8(k, n, w)
+    out = rt.upload_f32(np.full(m * n, np.nan))
+    lin.run(rt.upload_f32(x), m, out)
+    va, vb = ref.values(*ref.quantise(x)), ref.values(*ref.quantise(np.ascontiguousarray(w.T)))
+    _close(rt.download_f32(out).reshape(m, n), va @ vb.T, np.abs(va) @ np.abs(vb).T, k)
+
+
 @pytest.mark.parametrize("m", [1, 40, 200])
 def test_nan_stays_in_its_row(rt, m):
     k, n = 300, 50

@@ -36,6 +36,7 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr size_t kMaxGrid = 65536;  // of the kernels that walk their tiles
+constexpr size_t kMaxThreads = (size_t)1 << 32, kMaxGridY = 65535;  // of a launch
 
 // The exponent of a block whose largest finite magnitude has these bits: 448 = 1.75 * 2^8.
 __device__ __forceinline__ int block_exponent(uint32_t amax) {
@@ -306,7 +307,7 @@ __device__ __forceinline__ void put4(const Fp8Gemm &g, size_t m, size_t n, f32x4
 
 // C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  ST stages of 128 k in
 // LDS; D^T = B . A^T, so that a lane holds four consecutive columns of its row.
-// BLOCKS: B has float scales for 128 x 128 values (b_scales) instead of its exponents.
+// BLOCKS: B has float scales for 128 x 128 values (b_scales) on top of its rows' exponents.
 template <int BM, int BN, int WM, int WN, int ST, Epi EPI, bool BLOCKS>
 __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -462,7 +463,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
             f32x4 v = acc[i][j];
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                v[r] = ldexpf(v[r], ea + (BLOCKS ? 0 : g.b.row_e[min(n0 + 16 * j + 4 * lh + r, b16 - 1)]));
+                v[r] = ldexpf(v[r], ea + g.b.row_e[min(n0 + 16 * j + 4 * lh + r, b16 - 1)]);
             *reinterpret_cast<f32x4 *>(rows + li * PITCH + 16 * j + 4 * lh) = v;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -504,9 +505,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Gemm g, cons
 #pragma unroll
         for (int h = 0; h < 2; h++) y[h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from + h * 1024));
         float s = 1.0f;
-        uint32_t eb = 0x7f7f7f7f;
         if constexpr (BLOCKS) s = g.b_scales[nt / 8 * kb + b];
-        else eb = *reinterpret_cast<const uint32_t *>(g.b.exps + b * b16 + nt * 16 + 4 * lh);
+        const uint32_t eb = *reinterpret_cast<const uint32_t *>(g.b.exps + b * b16 + nt * 16 + 4 * lh);
 #pragma unroll
         for (int i = 0; i < MT; i++) {
             u32x4 a[2];
@@ -566,7 +566,7 @@ hipError_t launch_tile(hipStream_t s, Fp8Gemm g) {
     hipError_t e = ensure_dynamic_lds(fp8_gemm_kernel<BM, BN, WM, WN, ST, EPI, BLOCKS>, bytes, done);
     if (e != hipSuccess) return e;
     const size_t mt = (g.m + BM - 1) / BM, nt = (g.n + BN - 1) / BN;
-    if (mt * nt > (size_t)1 << 22) return hipErrorInvalidConfiguration;
+    if (mt * nt >= kMaxThreads / (WM * WN * 64)) return hipErrorInvalidConfiguration;
     g.m_tiles = (int)mt;
     g.n_tiles = (int)nt;
     g.tiles = (int)(mt * nt);
@@ -643,7 +643,10 @@ Fp8Plan fp8_plan(size_t m, size_t n, size_t k, bool floats) {
     const auto tiles = [&](size_t b) { return (double)((m + b - 1) / b) * (double)((n + b - 1) / b); };
     const double kb = (double)fp8_blocks(k), groups = (double)((n + 15) / 16) * (double)((m + 63) / 64);
     const double each = m <= 16 ? 4.2e-4 : m <= 32 ? 5.6e-4 : 8.4e-4;
-    double best = 2.6 + std::max(std::ceil(kb / kFewWaves), groups * kb * each) + 5 * std::max(0.0, groups / 1024 - 1);
+    // Where a launch has the workgroups; there is no output large enough for tiles of 256 not to.
+    const auto fits = [&](size_t b, size_t threads) { return tiles(b) < (double)(kMaxThreads / threads); };
+    const bool few = (n + 15) / 16 < kMaxThreads / (kFewWaves * 64) && (m + 15) / 16 <= kMaxGridY;
+    double best = !few ? INFINITY : 2.6 + std::max(std::ceil(kb / kFewWaves), groups * kb * each) + 5 * std::max(0.0, groups / 1024 - 1);
     // Fused while a wave quantises one block (one row of 768 for 2304 outputs 4.0 us, in two launches
     // 5.8; 16 rows 5.8 and 7.3; of 3072 for 768 8.0 and 6.6).
     Fp8Plan plan = floats && m <= 16 && kb <= kFewWaves && groups <= 1024 ? Fp8Plan::Fused : Fp8Plan::Few;
@@ -653,8 +656,8 @@ Fp8Plan fp8_plan(size_t m, size_t n, size_t k, bool floats) {
             plan = p;
         }
     };
-    offer(Fp8Plan::Tile64, std::max(4.2 + 0.57 * kb, tiles(64) / 1024 * (5 + 1.05 * kb)));
-    offer(Fp8Plan::Tile128, std::max(7 + 1.0 * kb, tiles(128) / 512 * (8 + 1.85 * kb)));
+    if (fits(64, 256)) offer(Fp8Plan::Tile64, std::max(4.2 + 0.57 * kb, tiles(64) / 1024 * (5 + 1.05 * kb)));
+    if (fits(128, 512)) offer(Fp8Plan::Tile128, std::max(7 + 1.0 * kb, tiles(128) / 512 * (8 + 1.85 * kb)));
     offer(Fp8Plan::Tile256, std::ceil(tiles(256) / 256) * (16 + 3.0 * kb));
     static const char *asked = getenv("VESTRA_HIP_FP8_TILE");
     if (asked) {

@@ -3864,16 +3864,16 @@ static size_t fp8_at(const vh::Fp8Rows &w, size_t row, size_t d) {
            (in / 32 * 16 + row % 16) * 16 + in % 16;
 }
 
-// Row-major codes [rows][k] and exponents [rows][blocks] (null: 127) to the device block of w.
-static vh_status upload_fp8(RtState &s, const vh::Fp8Rows &w, const uint8_t *codes, const uint8_t *exponents,
-                            const char *what) {
+// Row-major codes [rows][k] and exponents, at(row, block), to the device block of w.
+template <class F>
+static vh_status upload_fp8(RtState &s, const vh::Fp8Rows &w, const uint8_t *codes, F at, const char *what) {
     const size_t r16 = vh::fp8_rows16(w.rows), blocks = vh::fp8_blocks(w.k);
     std::vector<uint8_t> host(fp8_bytes(w.rows, w.k));
     const vh::Fp8Rows h = fp8_view(host.data(), w.rows, w.k);
     for (size_t r = 0; r < r16; r++) {
         int most = -127;
         for (size_t b = 0; b < blocks; b++) {
-            const int e = r < w.rows ? (exponents ? exponents[r * blocks + b] : 127) : 0;
+            const int e = r < w.rows ? at(r, b) : 0;
             h.exps[b * r16 + r] = (uint8_t)e;
             most = std::max(most, e - 127);
         }
@@ -3912,14 +3912,13 @@ extern "C" vh_status vh_fp8_upload(const vh_runtime *rt, const void *codes, cons
     GUARD_BEGIN
     RtState &s = *rt->s;
     TRY(set_device(s));
-    vh_fp8_tensor *t = nullptr;
-    TRY(new_fp8(rt->s, rows, k, &t, what));
-    vh_status st = upload_fp8(s, t->view, static_cast<const uint8_t *>(codes), e, what);
-    if (st) {
-        delete t;
-        return st;
-    }
-    *out = t;
+    vh_fp8_tensor *made = nullptr;
+    TRY(new_fp8(rt->s, rows, k, &made, what));
+    std::unique_ptr<vh_fp8_tensor> t(made);
+    const size_t blocks = vh::fp8_blocks(k);
+    TRY(upload_fp8(s, t->view, static_cast<const uint8_t *>(codes),
+                   [&](size_t r, size_t b) { return (int)e[r * blocks + b]; }, what));
+    *out = t.release();
     return VH_OK;
     GUARD_END
 }
@@ -4106,8 +4105,20 @@ extern "C" vh_status vh_prepare_linear_fp8_blocks(const vh_runtime *rt, size_t i
     char *block = nullptr;
     TRY(dalloc(s, fp8_bytes(n, k), &block, "fp8 weight allocation"));
     l->w = fp8_view(block, n, k);
-    TRY(upload_fp8(s, l->w, static_cast<const uint8_t *>(codes), nullptr, "fp8 weight upload"));
-    TRY(upload_array(s, scales, blocks, &l->scales, "fp8 scale upload"));
+    // The largest scale of 128 rows gives their exponent, and what the products meet are scales
+    // below 2: with sums and exponents of any size these stay within floats.
+    const size_t of_row = vh::fp8_blocks(k);
+    std::vector<int> exps(blocks / of_row, 0);
+    std::vector<float> below(blocks);
+    for (size_t i = 0; i < exps.size(); i++) {
+        float most = 0.0f;
+        for (size_t b = 0; b < of_row; b++) most = std::max(most, std::fabs(scales[i * of_row + b]));
+        if (most > 0.0f) exps[i] = std::max(std::ilogb(most), -127);
+        for (size_t b = 0; b < of_row; b++) below[i * of_row + b] = std::ldexp(scales[i * of_row + b], -exps[i]);
+    }
+    TRY(upload_fp8(s, l->w, static_cast<const uint8_t *>(codes), [&](size_t r, size_t) { return exps[r / 128] + 127; },
+                   "fp8 weight upload"));
+    TRY(upload_array(s, below.data(), blocks, &l->scales, "fp8 scale upload"));
     TRY(linear_fp8_vectors(s, bias, gamma, l.get()));
     *out = l.release();
     return VH_OK;
