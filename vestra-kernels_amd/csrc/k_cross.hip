@@ -107,7 +107,7 @@ __device__ __forceinline__ uint32_t finite_max(uint32_t mx, float v) {
 
 // ---- storing ------------------------------------------------------------------------
 
-constexpr int kHeadGroup = 8;   // heads of a workgroup of cross_range_kernel
+constexpr int kHeadGroup = 2;   // heads of a workgroup of cross_range_kernel (12 of 64, 865 tokens: of 8 8.4 us, of 2 5.2)
 constexpr int kMaxChunks = 32;  // of an image's tokens there
 
 // Of a chunk of an image's tokens: the largest finite magnitudes of K of each head and of
