@@ -305,6 +305,15 @@ __device__ __forceinline__ void put4(const Fp8Gemm &g, size_t m, size_t n, f32x4
     }
 }
 
+// The lane, from no register: what it gives is not kept over a loop.  (Tiles of 256 have none to spare:
+// the reload of one that was spilled waits for the copies before it: 13824 x 4096 by 8192 796 us,
+// so 735.)
+__device__ __forceinline__ int fresh_lane() {
+    int lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+    return lane;
+}
+
 // C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  ST stages of 128 k in
 // LDS; D^T = B . A^T, so that a lane holds four consecutive columns of its row.
 // BLOCKS: B has float scales for 128 x 128 values (b_scales) on top of its rows' exponents.
@@ -313,8 +322,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
     constexpr int CODES = (BM + BN) * 128, STAGE = CODES + (BM + BN) * 2;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lh = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr bool kSpare = TM * TN < 32;  // registers
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM;
 
     // Workgroups go round-robin over the 8 XCDs: each takes a run of tiles, eight
@@ -329,9 +338,10 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     const size_t kb = fp8_blocks(g.a.k), a16 = fp8_rows16(g.a.rows), b16 = fp8_rows16(g.b.rows);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
     // Units of 1 KB: halves of panels, A's then B's; then the blocks' relative exponents.
-    auto copy = [&](size_t b, int buf) {
+    auto copy = [&](size_t b, int buf, int lane) {
 #pragma unroll
-        for (int u = wave; u < (BM + BN) / 8; u += NW) {
+        for (int i = 0; i < (BM + BN) / 8 / NW; i++) {
+            const int u = wave + i * NW;
             const bool is_a = u < BM / 8;
             const size_t t = is_a ? min((size_t)mt * (BM / 16) + u / 2, a16 / 16 - 1)
                                   : min((size_t)nt * (BN / 16) + (u - BM / 8) / 2, b16 / 16 - 1);
@@ -344,7 +354,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
         const int rows = (is_a ? BM : BN) / (NW / 2), first = wave % (NW / 2) * rows;
         if (lane < rows / 8) {
             const size_t r16 = is_a ? a16 : b16;
-            const uint32_t at = (uint32_t)min((is_a ? (size_t)mt * BM : (size_t)nt * BN) + first + lane * 8, r16 - 8) * 2;
+            const uint32_t row = (uint32_t)(is_a ? mt * BM : nt * BN) + first + lane * 8;
+            const uint32_t at = min(row, (uint32_t)r16 - 8) * 2;
             copy16_to_lds((is_a ? g.a.rel : g.b.rel) + b * r16, at,
                           __builtin_amdgcn_readfirstlane(lds0 + buf * STAGE + CODES + ((is_a ? 0 : BM) + first) * 2));
         }
@@ -358,7 +369,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     static_assert((BM + BN) / 8 % NW == 0 && BM / (NW / 2) % 8 == 0 && BN / (NW / 2) % 8 == 0 && NW % 2 == 0);
 #pragma unroll
     for (int i = 0; i < ST - 1; i++)
-        if (i < (int)kb) copy(i, i);
+        if (i < (int)kb) copy(i, i, tid & 63);
     for (size_t b = 0; b < kb; b++) {
         const int buf = (int)(b % ST);
         // This stage landed; of the later ones as many as there are may be in flight.
@@ -366,7 +377,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
         else if (ST > 2 && b + 1 < kb) split_wait<(ST > 2 ? 1 : 0) * LD>();
         else split_wait<0>();
         __builtin_amdgcn_s_barrier();
-        if (b + ST - 1 < kb) copy(b + ST - 1, (int)((b + ST - 1) % ST));
+        const int lane = kSpare ? tid & 63 : fresh_lane(), li = lane & 15;
+        if (b + ST - 1 < kb) copy(b + ST - 1, (int)((b + ST - 1) % ST), lane);
         const char *as = smem + buf * STAGE + wm * TM * 2048 + lane * 16;
         const char *bs = smem + buf * STAGE + BM * 128 + wn * TN * 2048 + lane * 16;
         const uint16_t *rs = reinterpret_cast<const uint16_t *>(smem + buf * STAGE + CODES);
@@ -439,6 +451,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     static_assert(NW * 16 * PITCH * 4 <= ST * STAGE, "room for every wave's rows");
     __syncthreads();
     float *rows = reinterpret_cast<float *>(smem) + wave * 16 * PITCH;
+    const int lane = kSpare ? tid & 63 : fresh_lane(), li = lane & 15, lh = lane >> 4;
     const size_t n0 = (size_t)nt * BN + wn * W;
     const bool whole = (g.n & 3) == 0;
     const int lanes = whole ? W / 4 : W, row0 = lane / lanes, step = 64 / lanes;
