@@ -231,7 +231,8 @@ __global__ __launch_bounds__(256) void relative_fp8_kernel(Fp8Rows out) {
     for (size_t b = part; b < kb; b += 16) out.rel[b * rows16 + row] = fp8_relative(out.exps[b * rows16 + row], most - 127);
 }
 
-// The values that the codes stand for.
+// The values that the codes stand for, a wave a panel; through LDS, so that rows are written in 512
+// bytes at once.  Bound by HBM (55312 x 1100 51 us, 6.0 TB/s); 865 x 768 4.1 us, a launch and two latencies.
 template <bool VEC, bool NT>
 __global__ __launch_bounds__(256) void dequantize_fp8_kernel(Fp8Rows in, float *out) {
     __shared__ __attribute__((aligned(16))) char stage[4][2048];
@@ -317,6 +318,14 @@ __device__ __forceinline__ int fresh_lane() {
 // C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  ST stages of 128 k in
 // LDS; D^T = B . A^T, so that a lane holds four consecutive columns of its row.
 // BLOCKS: B has float scales for 128 x 128 values (b_scales) on top of its rows' exponents.
+//
+// What bounds it: tiles of 256 (waves of 128 x 64, 1.7 other vector instructions a matrix
+// instruction) the matrix cores at the clock that they leave, 13824 x 4096 by 8192 735 us, 1325
+// TFLOP/s, where a library's product of 8192^3 halves has 1139; tiles of 128 (waves of 64 x 32, 3.5,
+// with BLOCKS 4.5) the issue of instructions, 4001 x 2200 by 5001 107 us, BLOCKS 114; tiles of 64
+// (waves of 32 x 32, 5) the same and the start of a tile, 865 x 768 by 3072 11.7 us.  Waves of 64 x
+// 64 for the middle ones, in tiles of 256 x 128, 133 and 136 us, in tiles of 128 of four waves, 114.5
+// and 115: fewer waves hide less.  Three stages in LDS are no faster.
 template <int BM, int BN, int WM, int WN, int ST, Epi EPI, bool BLOCKS>
 __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -501,7 +510,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
 
 // Few rows: 16 MT rows by 16 columns a workgroup, whose waves share K between them, memory
 // to registers; B is read once, past the caches.  A block's sum joins the others on its own
-// exponents.  FUSED (MT = 1): A are floats, which every workgroup quantises itself.
+// exponents.  FUSED (MT = 1): A are floats, which every workgroup quantises itself.  Bound by a
+// launch and the latency of a block: one row of 768 by 2304 4.3 us.
 constexpr int kFewWaves = 8;
 template <int MT, bool FUSED, bool BLOCKS, Epi EPI>
 __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Gemm g, const float *x) {
@@ -650,8 +660,8 @@ hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out) {
 
 // By a model of the launch, in us, fitted to 24 shapes measured with each form: the few rows'
 // form takes a wave's blocks one after the other (1.0) or what all workgroups have to read and
-// multiply, and as long again for each round of 1024 of them; tiles of 64 and 128 one tile on its own, or rounds of as many as are resident
-// (1024 and 512); tiles of 256 whole rounds of 256.
+// multiply, and as long again for each round of 1024 of them; tiles of 64 and 128 one tile on its
+// own, or rounds of as many as are resident (1024 and 512); tiles of 256 whole rounds of 256.
 Fp8Plan fp8_plan(size_t m, size_t n, size_t k, bool floats) {
     const auto tiles = [&](size_t b) { return (double)((m + b - 1) / b) * (double)((n + b - 1) / b); };
     const double kb = (double)fp8_blocks(k), groups = (double)((n + 15) / 16) * (double)((m + 63) / 64);
