@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void relative_fp8_kernel(Fp8Rows out) {
 }
 
 // The values that the codes stand for, a wave a panel; through LDS, so that rows are written in 512
-// bytes at once.  Bound by HBM (55312 x 1100 51 us, 6.0 TB/s); 865 x 768 4.1 us, a launch and two latencies.
+// bytes at once.  Bound by HBM (13828 x 4096 44 us, 6.4 TB/s); 865 x 768 4.1 us, a launch and two latencies.
 template <bool VEC, bool NT>
 __global__ __launch_bounds__(256) void dequantize_fp8_kernel(Fp8Rows in, float *out) {
     __shared__ __attribute__((aligned(16))) char stage[4][2048];
@@ -650,9 +650,9 @@ hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out
 hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out) {
     const size_t tiles = fp8_rows16(in.rows) / 16 * fp8_blocks(in.k);
     const unsigned grid = (unsigned)std::min((tiles + 3) / 4, kMaxGrid);
-    // Whole lines past the caches (13828 x 4096 57 us, past them 44; lines in two pieces, 55312 x 1100,
-    // 71 and 76).
-    if (in.k % 32 == 0 && in.rows * in.k * 4 >= kFp8StreamBytes) dequantize_fp8_kernel<true, true><<<grid, 256, 0, s>>>(in, out);
+    // Past the caches (13828 x 4096 57 us, so 44; 55312 x 1100, whose rows are no whole lines, quantised
+    // and read back, in other memory each time, 143 and 134).
+    if (in.k % 4 == 0 && in.rows * in.k * 4 >= kFp8StreamBytes) dequantize_fp8_kernel<true, true><<<grid, 256, 0, s>>>(in, out);
     else if (in.k % 4 == 0) dequantize_fp8_kernel<true, false><<<grid, 256, 0, s>>>(in, out);
     else dequantize_fp8_kernel<false, false><<<grid, 256, 0, s>>>(in, out);
     return hipGetLastError();
