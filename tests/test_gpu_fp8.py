@@ -180,6 +180,16 @@ def test_more_rows_than_a_launch_has_in_a_direction(rt):
     _close(rt.download_f32(out).reshape(m, n), va @ vb.T, np.abs(va) @ np.abs(vb).T, k)
 
 
+@pytest.mark.parametrize("k, n", [(65535 * 32 + 65, 3), (3, 65535 * 32 + 65)])
+def test_weights_longer_than_a_launch_has_in_a_direction(rt, k, n):
+    x, w = _rows(1, 2, k), seeded.normal(2, k * n, 0.1).reshape(k, n)
+    lin = rt.prepare_linear_fp8(k, n, w)
+    out = rt.upload_f32(np.full(2 * n, np.nan))
+    lin.run(rt.upload_f32(x), 2, out)
+    va, vb = ref.values(*ref.quantise(x)), ref.values(*ref.quantise(np.ascontiguousarray(w.T)))
+    _close(rt.download_f32(out).reshape(2, n), va @ vb.T, np.abs(va) @ np.abs(vb).T, k)
+
+
 @pytest.mark.parametrize("m", [1, 40, 200])
 def test_nan_stays_in_its_row(rt, m):
     k, n = 300, 50

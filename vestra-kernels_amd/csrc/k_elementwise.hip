@@ -445,16 +445,19 @@ __global__ __launch_bounds__(256) void transpose_kernel(const float *__restrict_
                                                         float *__restrict__ out, size_t rows,
                                                         size_t cols) {
     __shared__ float tile[32][33];
-    size_t c0 = (size_t)blockIdx.x * 32, r0 = (size_t)blockIdx.y * 32;
+    const size_t c0 = (size_t)blockIdx.x * 32;
     int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int j = ty; j < 32; j += 8) {
-        size_t r = r0 + j, c = c0 + tx;
-        if (r < rows && c < cols) tile[j][tx] = in[r * cols + c];
-    }
-    __syncthreads();
-    for (int j = ty; j < 32; j += 8) {
-        size_t c = c0 + j, r = r0 + tx;
-        if (r < rows && c < cols) out[c * rows + r] = tile[tx][j];
+    for (size_t r0 = (size_t)blockIdx.y * 32; r0 < rows; r0 += (size_t)gridDim.y * 32) {
+        for (int j = ty; j < 32; j += 8) {
+            size_t r = r0 + j, c = c0 + tx;
+            if (r < rows && c < cols) tile[j][tx] = in[r * cols + c];
+        }
+        __syncthreads();
+        for (int j = ty; j < 32; j += 8) {
+            size_t c = c0 + j, r = r0 + tx;
+            if (r < rows && c < cols) out[c * rows + r] = tile[tx][j];
+        }
+        __syncthreads();
     }
 }
 
@@ -619,7 +622,7 @@ hipError_t launch_rope_table_device(hipStream_t s, const float *pos, size_t toke
 hipError_t launch_transpose(hipStream_t s, const float *in, float *out, size_t rows,
                             size_t cols) {
     if (rows == 0 || cols == 0) return hipSuccess;
-    dim3 grid((unsigned)((cols + 31) / 32), (unsigned)((rows + 31) / 32));
+    dim3 grid((unsigned)((cols + 31) / 32), (unsigned)std::min<size_t>((rows + 31) / 32, 65535));
     transpose_kernel<<<grid, 256, 0, s>>>(in, out, rows, cols);
     return hipGetLastError();
 }
