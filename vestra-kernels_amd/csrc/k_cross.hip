@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void cross_write_kernel(CrossWrite w) {
 // HBM: 16 images of 3457 tokens, 8 heads of 128, from one half 103 us, 6.6 TB/s; a frame 5.2 us.
 template <int KIND, int D, bool NT>
 __global__ __launch_bounds__(256) void cross_read_kernel(CrossView view, int head_dim, float *k, float *v, int *lens) {
-    constexpr int NP = kParts<KIND>, C = D / 32, DF = D / 16, ROW = 36;  // floats of a row of 32 dims in LDS
+    constexpr int NP = kParts<KIND>, C = D / 32, ROW = 36;  // floats of a row of 32 dims in LDS
     __shared__ __attribute__((aligned(16))) float stage[4][32 * ROW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lh = lane >> 4;
     const int g = blockIdx.y, img = blockIdx.z, len = view.lens[img];
@@ -395,6 +395,10 @@ __device__ __forceinline__ Tile tile_of(const CrossAttn &a, int img, int len, in
     t.steps = (len + step - 1) / step;
     return t;
 }
+
+// Where a tile's first step is among its units (of one without steps, the last): the share that has
+// it is the first to work on the tile, so that no workgroup begins one for its cost alone.
+__device__ __forceinline__ int first_unit(int cost) { return min(kTileCost, cost - 1); }
 
 // Steps of a tile of an image, with what it costs itself.
 __device__ __forceinline__ int cost_of(const CrossAttn &a, int img, int step) {
@@ -589,24 +593,27 @@ __device__ __forceinline__ void walk(const CrossAttn &a, char *smem, F f) {
     for (bool first = true; at < end; first = false) {
         const Tile t = tile_of<BM>(a, img, len, index, STEP);
         const int steps = uniform((int)min(end - at, (long long)cost - into));
-        const bool whole = into == 0 && steps == cost;
-        const int from = max(into - kTileCost, 0), to = max(into + steps - kTileCost, 0);
-        f(t, from, to - from, whole ? -1 : 2 * w + (first ? 0 : 1));
-        if (HERE && !whole) {
-            const long long begin = at - into;
-            const int w0 = uniform((int)(begin / share)), w1 = uniform((int)((begin + cost - 1) / share));
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's parts are out
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                unsigned *counter = a.counters + w0;
-                is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                          (unsigned)(w1 - w0);
-                if (is_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            __syncthreads();
-            if (is_last) {
-                join_parts<BM, D, THREADS, true>(a, t, w0, w1, 2 * w0 + (begin > w0 * share ? 1 : 0), 0, t.rows, smem);
+        const long long begin = at - into;
+        if (begin + first_unit(cost) < end) {
+            const bool whole = begin + first_unit(cost) >= w * share && into + steps == cost;
+            const int from = max(into - kTileCost, 0), to = max(into + steps - kTileCost, 0);
+            f(t, from, to - from, whole ? -1 : 2 * w + (first ? 0 : 1));
+            if (HERE && !whole) {
+                const int w0 = uniform((int)((begin + first_unit(cost)) / share));
+                const int w1 = uniform((int)((begin + cost - 1) / share));
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's parts are out
                 __syncthreads();
+                if (threadIdx.x == 0) {
+                    unsigned *counter = a.counters + w0;
+                    is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                              (unsigned)(w1 - w0);
+                    if (is_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                if (is_last) {
+                    join_parts<BM, D, THREADS, true>(a, t, w0, w1, 2 * w0 + (begin > w0 * share ? 1 : 0), 0, t.rows, smem);
+                    __syncthreads();
+                }
             }
         }
         at += steps;
@@ -847,21 +854,22 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
             return __builtin_nontemporal_load(reinterpret_cast<const f16x8 *>(base + at));
         };
         // K of this step is in registers; V is loaded before the scores are formed, the next K
-        // before the weights meet V.
+        // before the weights meet V.  The last step's blocks behind the last key are left out.
+        const int mine = steps - ((step0 + steps - 1) * STEP + 32 * wave >= t.len ? 1 : 0);
         f16x8 k[2 * C * NP], v[DF * NP];
-        if (steps) {
+        if (mine > 0) {
 #pragma unroll
             for (int i = 0; i < 2 * C * NP; i++) k[i] = load(step0, i);
         }
         Queries<KIND, D, 1> w;
         w.load(a, t, 0, li, lh);
-        for (int i = 0; i < steps; i++) {
+        for (int i = 0; i < mine; i++) {
             const int step = step0 + i, left = t.len - (step * 4 + wave) * 32;
 #pragma unroll
             for (int x = 0; x < DF * NP; x++) v[x] = load(step, 2 * C * NP + x);
             f32x4 s[1][2][1];
             w.scores(s[0], [&](int x) { return k[x]; });
-            const int next = min(step + 1, step0 + steps - 1);
+            const int next = min(step + 1, step0 + mine - 1);
 #pragma unroll
             for (int x = 0; x < 2 * C * NP; x++) k[x] = load(next, x);
             if (left < 32) w.mask(s[0], left, lh);
@@ -1020,10 +1028,9 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossAttn a, bool by_ti
         cost = (len + STEP - 1) / STEP + kTileCost;
         index = uniform((int)((end - 1 - base) / cost));
         begin = base + (long long)index * cost;
-        if (begin < w * share || begin + cost <= end) return;
     }
-    const int w0 = uniform((int)(begin / share)), w1 = uniform((int)((begin + cost - 1) / share));
-    if (w0 == w1) return;
+    const int w0 = uniform((int)((begin + first_unit(cost)) / share)), w1 = uniform((int)((begin + cost - 1) / share));
+    if (w0 == w1 || (!by_tile && w0 != w)) return;
     const Tile t = tile_of<BM>(a, img, len, index, STEP);
     const int first = blockIdx.y * kJoinRows<D>;
     if (first >= t.rows) return;
