@@ -161,7 +161,8 @@ SHAPES = [  # images, queries, tokens, heads, kv_heads, head_dim, seen
     (1, 128, 128, 2, 2, 64, None), (1, 129, 1, 2, 2, 64, None), (2, 200, 1000, 6, 6, 52, [0.0, 0.8]),
     (1, 865, 1730, 6, 6, 64, 0.9), (3, 257, 511, 9, 3, 96, [0.1, 1.0, 0.0]), (1, 900, 3000, 4, 2, 128, None),
     (300, 2, 40, 2, 1, 64, 0.5), (4, 1500, 65, 2, 2, 64, None),
-    (300, 100, 600, 1, 1, 64, 0.6), (290, 200, 300, 2, 1, 128, 0.9), (30, 300, 400, 4, 2, 64, 0.5)]
+    (300, 100, 600, 1, 1, 64, 0.6), (290, 200, 300, 2, 1, 128, 0.9), (30, 300, 400, 4, 2, 64, 0.5),
+    (54, 9, 44, 40, 10, 100, 0.9), (64, 8, 129, 12, 12, 64, [0.0, 0.02, 1.0, 0.5] * 16)]
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -487,16 +487,23 @@ __device__ __forceinline__ uint32_t weights_at(const CrossAttn &a, uint32_t x, i
     return 2u * a.shares * BM * D * 4 + (x * BM + in) * 8;
 }
 
+// Exponents of V's dims d .. d + 3.  Asked for before the sums are there, as a row that waited for them
+// at its end would wait for memory once more (54 images of 44 tokens, 40 / 10 heads of 100, 9
+// queries 34.4 us, so 28.9; one query against 3460 tokens 9.6 and 9.2).
+template <int D>
+__device__ __forceinline__ i32x4 dim_exponents(const CrossAttn &a, const Tile &t, int d) {
+    return *reinterpret_cast<const i32x4 *>(a.view.v_exp + ((size_t)t.img * a.view.kv_heads + t.g) * D + d);
+}
+
 // Row `in` of a tile, four dims from d on: the result, or a workgroup's part of it.
 template <int BM, int D, bool HERE>
-__device__ __forceinline__ void put_row(const CrossAttn &a, const Tile &t, int part, int in, int d, f32x4 v, float m,
-                                        float l) {
+__device__ __forceinline__ void put_row(const CrossAttn &a, const Tile &t, int part, int in, int d, i32x4 e, f32x4 v,
+                                        float m, float l) {
     if (in >= t.rows) return;
     if (part < 0) {
         if (d >= a.head_dim) return;
         const int row = t.row + in, token = row / a.group, head = t.g * a.group + row % a.group;
         const float inv = 1.0f / l;
-        const int *e = a.view.v_exp + ((size_t)t.img * a.view.kv_heads + t.g) * D + d;
         f32x4 y;
 #pragma unroll
         for (int i = 0; i < 4; i++) y[i] = l == 0.0f ? 0.0f : __builtin_ldexpf(v[i] * inv, e[i]);
@@ -534,6 +541,7 @@ __device__ void join_parts(const CrossAttn &a, const Tile &t, int w0, int w1, in
     while (rows < GROUPS && rows < to - first) rows *= 2;
     const int sharers = GROUPS / rows;
     const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+    const i32x4 e = dim_exponents<D>(a, t, d);
     for (int in = first + group % rows; in < first + (to - first + rows - 1) / rows * rows; in += rows) {
         auto part = [&](int w) {
             const int x = w == w0 ? part0 : 2 * w, row = min(in, to - 1);
@@ -555,7 +563,7 @@ __device__ void join_parts(const CrossAttn &a, const Tile &t, int w0, int w1, in
             if (group < rows)
                 for (int i = 1; i < sharers; i++) sum.join(some[threadIdx.x + i * rows * LANES]);
         }
-        if (group < rows && in < to) put_row<BM, D, HERE>(a, t, -1, in, d, sum.y, sum.m, sum.l);
+        if (group < rows && in < to) put_row<BM, D, HERE>(a, t, -1, in, d, e, sum.y, sum.m, sum.l);
     }
 }
 
@@ -652,13 +660,25 @@ struct Queries {
             const float *src = a.q + t.img * a.q_image + token * a.q_token + head * a.q_head;
             f32x4 x[C][2];
             uint32_t mx = 0;
+            // Of many rows from the nearest dims there are, so that no load waits in a branch (865 queries of
+            // 12 heads of 64 against 865 keys 26.9 us, so 26.3, against 3300 41.3 and 40.4); of few, whose
+            // K is in flight, that costs registers (16 images of 5000 tokens, two halves of 128, 109 and 119).
+            constexpr bool kAll = QT > 1;
+            const f32x4 zero{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (kAll) {
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        x[c][e] = *reinterpret_cast<const f32x4 *>(src + min(32 * c + 8 * lh + 4 * e, a.head_dim - 4));
+            }
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int d = 32 * c + 8 * lh + 4 * e;
-                    x[c][e] = there && d < a.head_dim ? *reinterpret_cast<const f32x4 *>(src + d)
-                                                      : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (kAll) x[c][e] = there && d < a.head_dim ? x[c][e] : zero;
+                    else x[c][e] = there && d < a.head_dim ? *reinterpret_cast<const f32x4 *>(src + d) : zero;
 #pragma unroll
                     for (int i = 0; i < 4; i++) mx = finite_max(mx, x[c][e][i]);
                 }
@@ -861,6 +881,9 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
 #pragma unroll
             for (int i = 0; i < 2 * C * NP; i++) k[i] = load(step0, i);
         }
+        i32x4 e[D / 64];
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) e[i] = dim_exponents<D>(a, t, 64 * i + 4 * (tid & 15));
         Queries<KIND, D, 1> w;
         w.load(a, t, 0, li, lh);
         for (int i = 0; i < mine; i++) {
@@ -901,12 +924,13 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
             sum += y[1] * f[x];
         }
 #pragma unroll
-        for (int d = 4 * (tid & 15); d < D; d += 64) {
+        for (int i = 0; i < D / 64; i++) {
+            const int d = 64 * i + 4 * (tid & 15);
             f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int x = 0; x < 4; x++)
                 y += *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(smem + x * WAVE) + row * D + d) * f[x];
-            put_row<BM, D, true>(a, t, part, row, d, y, m, sum);
+            put_row<BM, D, true>(a, t, part, row, d, e[i], y, m, sum);
         }
         __syncthreads();
     });
@@ -969,12 +993,17 @@ __global__ __launch_bounds__(256, 2) void cross_many_kernel(CrossAttn a) {
                 w.add(ph, pl, [&](int x) { return operand(h, 2 * C * NP + x); });
             }
         }
+        i32x4 e[D / 16];
+        if (part < 0) {
+#pragma unroll
+            for (int df = 0; df < D / 16; df++) e[df] = dim_exponents<D>(a, t, 16 * df + 4 * lh);
+        }
 #pragma unroll
         for (int u = 0; u < QT; u++) {
             const float l = sum_groups(w.l[u]);
 #pragma unroll
             for (int df = 0; df < D / 16; df++)
-                put_row<BM, D, false>(a, t, part, first + 16 * u + li, 16 * df + 4 * lh, w.o[df][u], w.m[u], l);
+                put_row<BM, D, false>(a, t, part, first + 16 * u + li, 16 * df + 4 * lh, e[df], w.o[df][u], w.m[u], l);
         }
         __syncthreads();
     });
