@@ -853,7 +853,7 @@ struct Queries {
 // ---- few rows: 16 a tile, each of the four waves its own 32 keys of a step ----------------
 // No barrier in the loop; blocks from memory to registers, K a step ahead, past the caches.  Bound by
 // HBM where the states are long (48 images of 5000 tokens, 32 / 8 heads of 128, in one half: 159 us, 6.2
-// TB/s), else by a chain of latencies (one query, 12 heads of 64, 3460 keys 9.5 us).
+// TB/s), else by a chain of latencies (one query, 12 heads of 64, 3460 keys 9.2 us).
 
 template <int D>
 constexpr int few_wave_bytes() {
@@ -1015,7 +1015,7 @@ template <int D>
 constexpr int kJoinRows = 1024 / D;
 // Joins the parts of cross_many_kernel, some rows a workgroup: of tile blockIdx.x where there
 // are fewer tiles than shares, as most workgroups would find nothing otherwise (84 tiles:
-// 6.6 us; by 512 shares 10.9), else of the tile that begins in share blockIdx.x and
+// 6.3 us; by 512 shares 10.9), else of the tile that begins in share blockIdx.x and
 // goes on in the next.
 template <int BM, int STEP, int D>
 __global__ __launch_bounds__(256) void cross_join_kernel(CrossAttn a, bool by_tile) {
