@@ -317,7 +317,7 @@ __device__ __forceinline__ int fresh_lane() {
 
 // C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  ST stages of 128 k in
 // LDS; D^T = B . A^T, so that a lane holds four consecutive columns of its row.
-// BLOCKS: B has float scales for 128 x 128 values (b_scales) on top of its rows' exponents.
+// BLOCKS: B has float scales for 128 x 128 values (b_rel) on top of its rows' exponents.
 //
 // What bounds it: tiles of 256 (waves of 128 x 64, 1.7 other vector instructions a matrix
 // instruction) the matrix cores at the clock that they leave, 13824 x 4096 by 8192 735 us, 1325
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
         if constexpr (BLOCKS) {
             // A block's sum from zero, a row of tiles at a time, then onto the others by its scale.
             const size_t n_block = min(((size_t)nt * BN + wn * TN * 16) / 128, (b16 - 1) / 128);
-            const float s = g.b_scales[n_block * kb + b];
+            const float s = g.b_rel[n_block * kb + b];
             f16x8 fb[TN][4];
 #pragma unroll
             for (int j = 0; j < TN; j++)
@@ -508,6 +508,35 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     }
 }
 
+// What joins a block's sum of 16 columns of B (panel nt) to the others: exponents of the columns 4 lh .. + 3,
+// or a checkpoint's scale as a significand in [1, 2) and an exponent (far below every sum for a zero), so
+// that no intermediate is larger than the product: with the scale multiplied in behind the exponents of rows
+// whose other scales are far above it, a finite product passed the floats on its way.
+struct Scale {
+    float significand;
+    int e[4];
+};
+template <bool BLOCKS>
+__device__ __forceinline__ Scale block_scale(const Fp8Gemm &g, size_t nt, size_t b, int lh) {
+    Scale s{1.0f, {}};
+    if constexpr (BLOCKS) {
+        const float v = g.b_scales[nt / 8 * fp8_blocks(g.b.k) + b];
+        s.significand = 2.0f * __builtin_amdgcn_frexp_mantf(v);
+        const int e = v == 0.0f ? -1000 : __builtin_amdgcn_frexp_expf(v) - 1;
+#pragma unroll
+        for (int r = 0; r < 4; r++) s.e[r] = e;
+    } else {
+        const uint32_t e = *reinterpret_cast<const uint32_t *>(g.b.exps + b * fp8_rows16(g.b.rows) + nt * 16 + 4 * lh);
+#pragma unroll
+        for (int r = 0; r < 4; r++) s.e[r] = (int)((e >> (8 * r)) & 255) - 127;
+    }
+    return s;
+}
+__device__ __forceinline__ void join_block(f32x4 &acc, f32x4 part, int ea, const Scale &s) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(s.significand, __builtin_ldexpf(part[r], ea + s.e[r]), acc[r]);
+}
+
 // Few rows: 16 MT rows by 16 columns a workgroup, whose waves share K between them, memory
 // to registers; B is read once, past the caches.  A block's sum joins the others on its own
 // exponents.  FUSED (MT = 1): A are floats, which every workgroup quantises itself.  Bound by a
@@ -517,7 +546,7 @@ template <int MT, bool FUSED, bool BLOCKS, Epi EPI>
 __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Gemm g, const float *x) {
     __shared__ f32x4 sums[kFewWaves][MT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lh = lane >> 4;
-    const size_t kb = fp8_blocks(g.b.k), b16 = fp8_rows16(g.b.rows), nt = blockIdx.x, mt = (size_t)blockIdx.y * MT;
+    const size_t kb = fp8_blocks(g.b.k), nt = blockIdx.x, mt = (size_t)blockIdx.y * MT;
     const size_t a16 = fp8_rows16(g.m);
     f32x4 acc[MT];
 #pragma unroll
@@ -527,9 +556,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Gemm g, cons
         u32x4 y[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) y[h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from + h * 1024));
-        float s = 1.0f;
-        if constexpr (BLOCKS) s = g.b_scales[nt / 8 * kb + b];
-        const uint32_t eb = *reinterpret_cast<const uint32_t *>(g.b.exps + b * b16 + nt * 16 + 4 * lh);
+        const Scale s = block_scale<BLOCKS>(g, nt, b, lh);
 #pragma unroll
         for (int i = 0; i < MT; i++) {
             u32x4 a[2];
@@ -565,10 +592,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Gemm g, cons
                 for (int e = 0; e < 2; e++)
                     part = mfma16x16x32_f16(halves(y[h][2 * e], y[h][2 * e + 1], 1.0f),
                                             halves(a[h][2 * e], a[h][2 * e + 1], 1.0f), part);
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                acc[i][r] = __builtin_fmaf(BLOCKS ? s : 1.0f,
-                                           __builtin_ldexpf(part[r], ea + (int)((eb >> (8 * r)) & 255) - 127), acc[i][r]);
+            join_block(acc[i], part, ea, s);
         }
     }
 #pragma unroll

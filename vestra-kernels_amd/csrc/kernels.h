@@ -334,11 +334,11 @@ hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out
 hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out);
 // c [m][n] = a . b^T, then the epilogue (Store: (v + bias) * gamma; Gelu: gelu(v +
 // bias); Residual: c += (v + bias) * gamma); bias and gamma may be null.  With b_scales
-// [ceil(n / 128)][blocks] these are the scales of b's codes, for 128 x 128 values, over
-// 2^exponent, which b then has for all blocks of a row.
+// [ceil(n / 128)][blocks] these are the scales of b's codes, for 128 x 128 values, and
+// b_rel the same over 2^exponent, which b then has for all blocks of a row.
 struct Fp8Gemm {
     Fp8Rows a, b;
-    const float *b_scales, *bias, *gamma;
+    const float *b_scales, *b_rel, *bias, *gamma;
     float *c;
     size_t m, n;
     int m_tiles, n_tiles, tiles;  // set by the launcher

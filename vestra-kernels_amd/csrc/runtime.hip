@@ -343,7 +343,7 @@ struct vh_fp8_tensor {
 struct vh_linear_fp8 {
     Rt rt;
     vh::Fp8Rows w{};
-    float *scales = nullptr;  // for 128 x 128 codes, or null
+    float *scales = nullptr;  // for 128 x 128 codes, then the same over their rows' exponents; or null
     float *bias = nullptr, *gamma = nullptr;
     ~vh_linear_fp8() {
         if (!rt) return;
@@ -4105,11 +4105,13 @@ extern "C" vh_status vh_prepare_linear_fp8_blocks(const vh_runtime *rt, size_t i
     char *block = nullptr;
     TRY(dalloc(s, fp8_bytes(n, k), &block, "fp8 weight allocation"));
     l->w = fp8_view(block, n, k);
-    // The largest scale of 128 rows gives their exponent, and what the products meet are scales
-    // below 2: with sums and exponents of any size these stay within floats.
+    // The largest scale of 128 rows gives their exponent, and what the sums of tiles meet are scales
+    // below 2; few rows meet them as they are.
     const size_t of_row = vh::fp8_blocks(k);
     std::vector<int> exps(blocks / of_row, 0);
-    std::vector<float> below(blocks);
+    std::vector<float> both(scales, scales + blocks);
+    both.resize(2 * blocks);
+    float *below = both.data() + blocks;
     for (size_t i = 0; i < exps.size(); i++) {
         float most = 0.0f;
         for (size_t b = 0; b < of_row; b++) most = std::max(most, std::fabs(scales[i * of_row + b]));
@@ -4118,7 +4120,7 @@ extern "C" vh_status vh_prepare_linear_fp8_blocks(const vh_runtime *rt, size_t i
     }
     TRY(upload_fp8(s, l->w, static_cast<const uint8_t *>(codes), [&](size_t r, size_t) { return exps[r / 128] + 127; },
                    "fp8 weight upload"));
-    TRY(upload_array(s, below.data(), blocks, &l->scales, "fp8 scale upload"));
+    TRY(upload_array(s, both.data(), 2 * blocks, &l->scales, "fp8 scale upload"));
     TRY(linear_fp8_vectors(s, bias, gamma, l.get()));
     *out = l.release();
     return VH_OK;
@@ -4162,6 +4164,7 @@ static vh_status run_fp8(const vh_linear_fp8 *l, const vh_tensor *x, const vh_fp
     }
     g.b = l->w;
     g.b_scales = l->scales;
+    if (l->scales) g.b_rel = l->scales + (n + 127) / 128 * vh::fp8_blocks(k);
     g.bias = l->bias;
     g.gamma = l->gamma;
     g.c = out->ptr;
