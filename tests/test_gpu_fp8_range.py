@@ -43,3 +43,15 @@ def test_scales_far_below_the_largest_of_their_rows(rt, m, powers, scales):
     lin.run(rt.upload_f32(x), m, out)
     vx = ref.values(*ref.quantise(x))
     _close(rt.download_f32(out).reshape(m, n), vx @ vw.T, np.abs(vx) @ np.abs(vw).T, k)
+
+
+@pytest.mark.parametrize("extra", [1, 12])
+@pytest.mark.parametrize("m, k, n", [(2000, 520, 1088), (3000, 520, 2080), (3500, 384, 4288), (1999, 130, 1280)])
+def test_columns_past_the_end_leave_the_others_rows_alone(rt, m, k, n, extra):
+    """The last columns' tiles, in tiles of 64, 128 and 256: most lanes of a wave have nothing to write, and
+    its strips of 16 rows go through the same LDS."""
+    a, b = _sized(3, m, [0] * ref.blocks(k), k), _sized(4, n + extra, [0] * ref.blocks(k), k)
+    va, vb = (ref.values(*ref.quantise(x)) for x in (a, b))
+    c = rt.upload_f32(np.full(m * (n + extra), np.nan))
+    rt.gemm_fp8_into(*(rt.quantize_fp8(rt.upload_f32(x), *x.shape) for x in (a, b)), c)
+    _close(rt.download_f32(c).reshape(m, n + extra), va @ vb.T, np.abs(va) @ np.abs(vb).T, k)

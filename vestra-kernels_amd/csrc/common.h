@@ -98,6 +98,16 @@ __device__ __forceinline__ void stream_store(T *p, T v) {
     __builtin_nontemporal_store(v, p);
 }
 
+// Between a wave's writes to LDS and its other lanes' reads, and before the next writes there: no instruction, but all
+// lanes come together here.  A fence alone orders a lane's own accesses: lanes that a branch keeps from the
+// reads may be let go on to the next writes first (a product of 1100 columns, the last tile's strips: the rows of
+// one overwritten by the next one's while lanes were yet to read them).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // One DPP lane permutation (a VALU modifier, no LDS round trip).
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float v) {

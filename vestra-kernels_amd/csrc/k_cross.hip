@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256) void cross_write_kernel(CrossWrite w) {
         if constexpr (NP == 2)
             *reinterpret_cast<f16x4 *>(plane + PLANE + (row * D + vd) * 2) = f16x4{l[0][0], l[0][1], l[1][0], l[1][1]};
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    wave_sync();
     const char *from = plane + ((4 * lh + (li >> 2)) * D + 4 * (li & 3)) * 2;
 #pragma unroll
     for (int df = 0; df < DF; df++)
@@ -334,13 +334,13 @@ __global__ __launch_bounds__(256) void cross_read_kernel(CrossView view, int hea
     float *mine = stage[wave];
     // 32 dims at a time through LDS, so that rows are written in whole lines.
     auto rows = [&](float *to, int d0) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        wave_sync();
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int key = 8 * i + (lane >> 3), d = 4 * (lane & 7);
             put(to, key0 + key, d0 + d, *reinterpret_cast<const f32x4 *>(mine + key * ROW + d));
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        wave_sync();
     };
 #pragma unroll
     for (int c = 0; c < C; c++) {

@@ -162,12 +162,12 @@ __device__ __forceinline__ int quantize_panel(f32x4 (&v)[8], const Fp8Rows &out,
         *reinterpret_cast<int *>(to + panel_at(2 * i + side, c)) = e4m3_of(v[i] * pow2(-e));
         if (c == i) mine = e;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    wave_sync();
     char *at = reinterpret_cast<char *>(out.codes) + (tile * fp8_blocks(out.k) + b) * 2048 + lane * 16;
 #pragma unroll
     for (int h = 0; h < 2; h++)
         *reinterpret_cast<u32x4 *>(at + h * 1024) = *reinterpret_cast<const u32x4 *>(to + panel_lane(lane, h));
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    wave_sync();
     if (c < 8) out.exps[b * fp8_rows16(out.rows) + tile * 16 + 2 * c + side] = (uint8_t)(mine + 127);
     return mine;
 }
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(256) void dequantize_fp8_kernel(Fp8Rows in, float *
 #pragma unroll
         for (int h = 0; h < 2; h++)
             *reinterpret_cast<u32x4 *>(to + panel_lane(lane, h)) = *reinterpret_cast<const u32x4 *>(at + h * 1024);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        wave_sync();
 #pragma unroll
         for (int r0 = 0; r0 < 8; r0++) {
             const int r = 2 * r0 + side;
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(256) void dequantize_fp8_kernel(Fp8Rows in, float *
                     if (d + j < in.k) y[j] = v[j];
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        wave_sync();
     }
 }
 
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
                 v[r] = ldexpf(v[r], ea + g.b.row_e[min(n0 + 16 * j + 4 * lh + r, b16 - 1)]);
             *reinterpret_cast<f32x4 *>(rows + li * PITCH + 16 * j + 4 * lh) = v;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        wave_sync();
         if (n < g.n) {
             for (int r0 = row0; r0 < 16 && m0 + r0 < g.m; r0 += step) {
                 float *c = g.c + (m0 + r0) * g.n + n;
@@ -504,7 +504,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
                 }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        wave_sync();
     }
 }
 
