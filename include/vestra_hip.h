@@ -553,9 +553,8 @@ vh_status vh_quantize_fp8_into(const vh_runtime *rt, const vh_tensor *x, size_t 
                                vh_fp8_tensor *out);
 /* The values that the codes stand for, out [rows, k]. */
 vh_status vh_dequantize_fp8_into(const vh_runtime *rt, const vh_fp8_tensor *tensor, vh_tensor *out);
-/* c [a.rows, b.rows] = a . b^T of the values, in 32-bit sums.  A value counts to within
- * 2^-25 of 2^E, E the largest exponent of its row: exactly, unless exponents of a
- * row differ by more than 15. */
+/* c [a.rows, b.rows] = a . b^T of the values: exact products in 32-bit sums.  Where a row's
+ * exponents differ by more than 15 (blocks of zeros aside) its outputs take longer. */
 vh_status vh_gemm_fp8_into(const vh_runtime *rt, const vh_fp8_tensor *a, const vh_fp8_tensor *b, vh_tensor *c);
 
 /* A projection with e4m3 weights, as vh_linear_q8_0 is one with Q8_0's: weight row-major

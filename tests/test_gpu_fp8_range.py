@@ -55,3 +55,90 @@ def test_columns_past_the_end_leave_the_others_rows_alone(rt, m, k, n, extra):
     c = rt.upload_f32(np.full(m * (n + extra), np.nan))
     rt.gemm_fp8_into(*(rt.quantize_fp8(rt.upload_f32(x), *x.shape) for x in (a, b)), c)
     _close(rt.download_f32(c).reshape(m, n + extra), va @ vb.T, np.abs(va) @ np.abs(vb).T, k)
+
+
+# Rows of few, of tiles of 64, of 128 and of 256, as the model of a launch has them.
+FORMS = [(1, 512, 700), (12, 1100, 70), (40, 512, 300), (2000, 520, 1100), (700, 2300, 2000), (3000, 520, 2100),
+         (3500, 384, 4300)]
+
+
+def _powers(blocks, low, high):
+    """Sizes of a row's blocks, the largest first, the others far below: what the other side has there is far above."""
+    p = np.full(blocks, low)
+    p[0] = high
+    return p
+
+
+@pytest.mark.parametrize("m, k, n", FORMS)
+@pytest.mark.parametrize("gap", [16, 24, 70])
+def test_a_small_block_against_a_large_one(rt, m, k, n, gap):
+    """The outputs come from the blocks that are small in one side's rows and large in the other's."""
+    nb = ref.blocks(k)
+    a, b = _sized(1, m, _powers(nb, -gap, 0), k), _sized(2, n, -_powers(nb, -gap, 0), k)
+    a[:, :128] *= (np.arange(m) % 3 == 0)[:, None]  # zeros: rows whose exponents are alike
+    va, vb = (ref.values(*ref.quantise(x)) for x in (a, b))
+    c = rt.upload_f32(np.full(m * n, np.nan))
+    qa, qb = (rt.quantize_fp8(rt.upload_f32(x), *x.shape) for x in (a, b))
+    rt.gemm_fp8_into(qa, qb, c)
+    want, size = va @ vb.T, np.abs(va) @ np.abs(vb).T
+    got = rt.download_f32(c).reshape(m, n)
+    _close(got, want, size, k)
+    # Rows that came as codes.
+    up = [rt.fp8_upload(*rt.fp8_download(q), *x.shape) for q, x in ((qa, a), (qb, b))]
+    again = rt.upload_f32(np.full(m * n, np.nan))
+    rt.gemm_fp8_into(*up, again)
+    assert np.array_equal(rt.download_f32(again).reshape(m, n), got)
+
+
+@pytest.mark.parametrize("m, k, n", FORMS)
+def test_projections_of_rows_of_wide_range(rt, m, k, n):
+    """From floats and from rows, with every epilogue: one row in seven has a block 2^40 above the others, where the
+    weights are 2^40 below theirs."""
+    nb = ref.blocks(k)
+    x = _sized(1, m, np.zeros(nb), k)
+    wide = np.arange(m) % 7 == 0
+    x[wide, :128] *= np.float32(2.0 ** 40)
+    w = np.ascontiguousarray(_sized(2, n, _powers(nb, -4, -44), k).T)
+    bias, gamma, res = seeded.normal(5, n), seeded.normal(6, n), seeded.normal(7, m * n)
+    vx, vw = ref.values(*ref.quantise(x)), ref.values(*ref.quantise(np.ascontiguousarray(w.T)))
+    xt, rows = rt.upload_f32(x), rt.quantize_fp8(rt.upload_f32(x), m, k)
+    y, size = vx @ vw.T + bias, np.abs(vx) @ np.abs(vw).T + np.abs(bias)
+    lin, r = rt.prepare_linear_fp8(k, n, w, bias, gamma), res.reshape(m, n)
+    for run, arg in ((lin.run_residual, (xt, m)), (lin.run_rows_residual, (rows,))):
+        out = rt.upload_f32(res)
+        run(*arg, out)
+        _close(rt.download_f32(out).reshape(m, n), y * gamma + r, size * np.abs(gamma) + np.abs(r), k)
+    lin, out = rt.prepare_linear_fp8(k, n, w, bias), rt.upload_f32(res)
+    lin.run_gelu(xt, m, out)
+    _close(rt.download_f32(out).reshape(m, n), ref.gelu(y), 1.13 * size, k, 1e-6 * np.maximum(1, np.abs(y)))
+
+
+@pytest.mark.parametrize("m, k, n", FORMS)
+@pytest.mark.parametrize("gap", [24, 100])
+def test_block_scales_of_wide_range(rt, m, k, n, gap):
+    """A checkpoint's scales that run the other way than the rows' blocks, and are zero for the largest of them."""
+    nb = ref.blocks(k)
+    x = _sized(1, m, _powers(nb, 10 - gap, 10), k)
+    scales = np.exp2(-_powers(nb, 10 - gap, 10)) * np.exp(seeded.normal(3, ref.blocks(n) * nb, 0.3).reshape(-1, nb))
+    scales[::2, 0] = 0.0
+    lin, vw = _checkpoint(rt, 6, k, n, scales.astype(np.float32).reshape(-1))
+    out = rt.upload_f32(np.full(m * n, np.nan))
+    lin.run(rt.upload_f32(x), m, out)
+    vx = ref.values(*ref.quantise(x))
+    _close(rt.download_f32(out).reshape(m, n), vx @ vw.T, np.abs(vx) @ np.abs(vw).T, k)
+
+
+@pytest.mark.parametrize("m, k, n", FORMS[3:])
+def test_nan_stays_in_its_row_of_wide_range(rt, m, k, n):
+    nb = ref.blocks(k)
+    a, b = _sized(1, m, _powers(nb, -30, 0), k), _sized(2, n, np.zeros(nb), k)
+    want = ref.values(*ref.quantise(a)) @ ref.values(*ref.quantise(b)).T
+    size = np.abs(a).astype(np.float64) @ np.abs(b).T.astype(np.float64)
+    a[m // 2, k - 1], b[n // 3, 7] = np.inf, np.nan
+    c = rt.upload_f32(np.zeros(m * n))
+    rt.gemm_fp8_into(*(rt.quantize_fp8(rt.upload_f32(x), *x.shape) for x in (a, b)), c)
+    got = rt.download_f32(c).reshape(m, n)
+    bad = np.zeros((m, n), bool)
+    bad[m // 2], bad[:, n // 3] = True, True
+    assert np.isnan(got[bad]).all()
+    _close(got[~bad], want[~bad], 1.13 * size[~bad], k)  # the codes' values: each within 2^-4 of its own

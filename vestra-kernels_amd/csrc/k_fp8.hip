@@ -13,9 +13,10 @@
 // the scaled and the plain form), which is no 32-bit sum.  The conversion
 // (v_cvt_scalef32_pk_f16_fp8) takes a power-of-two scale: a block's exponent relative to
 // the largest of its row, so that one f32 sum runs over all of K and the rows' exponents
-// join behind it.  A value is then off by at most 2^-25 of 2^E, E the row's largest
-// exponent (448 * 2^E the largest value it can hold): nothing while a row's
-// exponents are within 15 of each other, and 2^-33 of the largest value at the worst.
+// join behind it.  That is exact while a row's exponents are within 15 of each other (blocks
+// of zeros aside).  Rows that are wider say so (fp8_row), and a wave of a tile that meets one forms
+// its 16 rows' sums again, each block's on its own exponents, as the products of few rows do
+// it: what is small in one side's row may stand against what is large in the other's.
 //
 // Storage, "panels": 16 rows x 128 values are 2048 bytes, [half 2][lane 64][16]: lane
 // (row li, lh) of half h holds values 32 lh + 16 h .. + 15 of its row, so that a
@@ -129,7 +130,8 @@ __device__ __forceinline__ uint32_t row_umax(uint32_t v) {
     return max(v, (uint32_t)__shfl_xor((int)v, 16, kWave));
 }
 // Their codes; `to`: 2048 bytes of the wave's own.  Lanes 0 .. 7 of either half get the
-// exponents of rows 2 lane + half.
+// exponents of rows 2 lane + half, kEmpty where all values are zeros.
+constexpr int kEmpty = -128;
 __device__ __forceinline__ int quantize_panel(f32x4 (&v)[8], const Fp8Rows &out, size_t tile, size_t b, int lane,
                                               char *to) {
     // Opaque: what follows from the lane (addresses, masks) is formed for each panel anew, not kept
@@ -155,12 +157,12 @@ __device__ __forceinline__ int quantize_panel(f32x4 (&v)[8], const Fp8Rows &out,
             mx[i] = row_umax(m);
         }
     }
-    int mine = -127;
+    int mine = kEmpty;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int e = block_exponent(mx[i]);
         *reinterpret_cast<int *>(to + panel_at(2 * i + side, c)) = e4m3_of(v[i] * pow2(-e));
-        if (c == i) mine = e;
+        if (c == i) mine = mx[i] ? e : kEmpty;
     }
     wave_sync();
     char *at = reinterpret_cast<char *>(out.codes) + (tile * fp8_blocks(out.k) + b) * 2048 + lane * 16;
@@ -168,7 +170,7 @@ __device__ __forceinline__ int quantize_panel(f32x4 (&v)[8], const Fp8Rows &out,
     for (int h = 0; h < 2; h++)
         *reinterpret_cast<u32x4 *>(at + h * 1024) = *reinterpret_cast<const u32x4 *>(to + panel_lane(lane, h));
     wave_sync();
-    if (c < 8) out.exps[b * fp8_rows16(out.rows) + tile * 16 + 2 * c + side] = (uint8_t)(mine + 127);
+    if (c < 8) out.exps[b * fp8_rows16(out.rows) + tile * 16 + 2 * c + side] = (uint8_t)(max(mine, -127) + 127);
     return mine;
 }
 
@@ -180,26 +182,34 @@ template <bool VEC, bool NT>
 __global__ __launch_bounds__(kQuantThreads) void quantize_fp8_kernel(const float *x, Fp8Rows out) {
     constexpr int W = kQuantThreads / 64;
     __shared__ __attribute__((aligned(16))) char stage[W][2048];
-    __shared__ int wave_max[W][16];
+    __shared__ int wave_max[W][16], wave_min[W][16];
     __shared__ uint8_t codes[kQuantBlocks * 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, row = 2 * c + (lane >> 5);
     const size_t kb = fp8_blocks(out.k), rows16 = fp8_rows16(out.rows);
     for (size_t tile = blockIdx.x; tile < rows16 / 16; tile += gridDim.x) {
-        int most = -127;
+        int most = -127, least = 127;
         for (size_t b = wave; b < kb; b += W) {
             f32x4 v[8];
             load_panel<VEC, NT>(x, out, tile, b, lane, v);
             const int e = quantize_panel(v, out, tile, b, lane, stage[wave]);
-            if (c < 8 && b < kQuantBlocks) codes[b * 16 + row] = (uint8_t)(e + 127);
+            if (c < 8 && b < kQuantBlocks) codes[b * 16 + row] = (uint8_t)(max(e, -127) + 127);
             most = max(most, e);
+            if (e != kEmpty) least = min(least, e);
         }
-        if (c < 8) wave_max[wave][row] = most;
+        if (c < 8) {
+            wave_max[wave][row] = most;
+            wave_min[wave][row] = least;
+        }
         __syncthreads();
         // Thread t writes row t % 16 of the blocks t / 16, ...
         most = wave_max[0][tid & 15];
+        least = wave_min[0][tid & 15];
 #pragma unroll
-        for (int w = 1; w < W; w++) most = max(most, wave_max[w][tid & 15]);
-        if (tid < 16) out.row_e[tile * 16 + tid] = most;
+        for (int w = 1; w < W; w++) {
+            most = max(most, wave_max[w][tid & 15]);
+            least = min(least, wave_min[w][tid & 15]);
+        }
+        if (tid < 16) out.row_e[tile * 16 + tid] = fp8_row(most, least);
         for (size_t i = tid; i < kb * 16; i += kQuantThreads) {
             const size_t at = (i >> 4) * rows16 + tile * 16 + (i & 15);
             out.rel[at] = fp8_relative(i < kQuantBlocks * 16 ? codes[i] : out.exps[at], most);
@@ -209,25 +219,35 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_fp8_kernel(const float
 }
 
 // Where there are few rows: codes and exponents alone, a wave a panel; then what follows from
-// the exponents.
+// the exponents, until when `rel` says which blocks are all zeros.
 template <bool VEC>
 __global__ __launch_bounds__(64) void quantize_panels_kernel(const float *x, Fp8Rows out) {
     __shared__ __attribute__((aligned(16))) char stage[2048];
     f32x4 v[8];
     load_panel<VEC, false>(x, out, blockIdx.y, blockIdx.x, threadIdx.x, v);
-    quantize_panel(v, out, blockIdx.y, blockIdx.x, threadIdx.x, stage);
+    const int e = quantize_panel(v, out, blockIdx.y, blockIdx.x, threadIdx.x, stage);
+    const int c = threadIdx.x & 31, row = 2 * c + (threadIdx.x >> 5);
+    if (c < 8) out.rel[blockIdx.x * fp8_rows16(out.rows) + blockIdx.y * 16 + row] = e == kEmpty;
 }
 __global__ __launch_bounds__(256) void relative_fp8_kernel(Fp8Rows out) {
-    __shared__ int some[16][16];
+    __shared__ int some[16][16], low[16][16];
     const int tid = threadIdx.x, r = tid & 15, part = tid >> 4;
     const size_t kb = fp8_blocks(out.k), rows16 = fp8_rows16(out.rows), row = (size_t)blockIdx.x * 16 + r;
-    int most = 0;
-    for (size_t b = part; b < kb; b += 16) most = max(most, (int)out.exps[b * rows16 + row]);
+    int most = 0, least = 254;
+    for (size_t b = part; b < kb; b += 16) {
+        const int e = out.exps[b * rows16 + row];
+        most = max(most, e);
+        if (!out.rel[b * rows16 + row]) least = min(least, e);
+    }
     some[part][r] = most;
+    low[part][r] = least;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; i++) most = max(most, some[i][r]);
-    if (part == 0) out.row_e[row] = most - 127;
+    for (int i = 0; i < 16; i++) {
+        most = max(most, some[i][r]);
+        least = min(least, low[i][r]);
+    }
+    if (part == 0) out.row_e[row] = fp8_row(most - 127, least - 127);
     for (size_t b = part; b < kb; b += 16) out.rel[b * rows16 + row] = fp8_relative(out.exps[b * rows16 + row], most - 127);
 }
 
@@ -303,6 +323,75 @@ __device__ __forceinline__ void put4(const Fp8Gemm &g, size_t m, size_t n, f32x4
 #pragma unroll
         for (int r = 0; r < 4; r++)
             if (r < count) c[r] = EPI == Epi::Residual ? c[r] + v[r] : v[r];
+    }
+}
+
+// What joins a block's sum of 16 columns of B (panel nt) to the others: exponents of the columns 4 lh .. + 3,
+// or a checkpoint's scale as a significand in [1, 2) and an exponent (far below every sum for a zero), so
+// that no intermediate is larger than the product: with the scale multiplied in behind the exponents of rows
+// whose other scales are far above it, a finite product passed the floats on its way.
+struct Scale {
+    float significand;
+    int e[4];
+};
+template <bool BLOCKS>
+__device__ __forceinline__ Scale block_scale(const Fp8Gemm &g, size_t nt, size_t b, int lh) {
+    Scale s{1.0f, {}};
+    if constexpr (BLOCKS) {
+        const float v = g.b_scales[nt / 8 * fp8_blocks(g.b.k) + b];
+        s.significand = 2.0f * __builtin_amdgcn_frexp_mantf(v);
+        const int e = v == 0.0f ? -1000 : __builtin_amdgcn_frexp_expf(v) - 1;
+#pragma unroll
+        for (int r = 0; r < 4; r++) s.e[r] = e;
+    } else {
+        const uint32_t e = *reinterpret_cast<const uint32_t *>(g.b.exps + b * fp8_rows16(g.b.rows) + nt * 16 + 4 * lh);
+#pragma unroll
+        for (int r = 0; r < 4; r++) s.e[r] = (int)((e >> (8 * r)) & 255) - 127;
+    }
+    return s;
+}
+__device__ __forceinline__ void join_block(f32x4 &acc, f32x4 part, int ea, const Scale &s) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(s.significand, __builtin_ldexpf(part[r], ea + s.e[r]), acc[r]);
+}
+
+// The sums of 16 rows (panel mt of A) by 16 TN columns (panels nt .. of B; past the end the last), a block after the
+// other on its own exponents, from memory: of rows too wide for the sums of a tile.  The loads of a block's
+// panels are in flight together (865 x 768 by 3072 with a wide row in every 16 20.9 us, without 12.7; 13828 x 4096 by
+// 8192 2.35 ms and 0.85).
+template <int TN, bool BLOCKS>
+__device__ __forceinline__ void wide_sums(const Fp8Gemm &g, size_t mt, size_t nt, int lane, f32x4 (&acc)[TN]) {
+    const size_t kb = fp8_blocks(g.a.k), a16 = fp8_rows16(g.a.rows), last = fp8_rows16(g.b.rows) / 16 - 1;
+    mt = min(mt, a16 / 16 - 1);
+#pragma unroll
+    for (int j = 0; j < TN; j++) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (size_t b = 0; b < kb; b++) {
+        u32x4 x[2], y[TN][2];
+        Scale s[TN];
+        const int ea = (int)g.a.exps[b * a16 + mt * 16 + (lane & 15)] - 127;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            x[h] = *reinterpret_cast<const u32x4 *>(g.a.codes + (mt * kb + b) * 2048 + h * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+            const size_t panel = min(nt + j, last);
+            s[j] = block_scale<BLOCKS>(g, panel, b, lane >> 4);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                y[j][h] = *reinterpret_cast<const u32x4 *>(g.b.codes + (panel * kb + b) * 2048 + h * 1024 + lane * 16);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+            f32x4 part{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    part = mfma16x16x32_f16(halves(y[j][h][2 * e], y[j][h][2 * e + 1], 1.0f),
+                                            halves(x[h][2 * e], x[h][2 * e + 1], 1.0f), part);
+            join_block(acc[j], part, ea, s[j]);
+        }
     }
 }
 
@@ -476,18 +565,32 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
         v += bias[r];
         return EPI == Epi::Gelu ? gelu_fast_form(v) : v * gamma[r];
     };
+    // The rows' exponents join the sums, those of wide rows are formed again.
+    int row_a[TM], row_b[TN][4], wide_a = 0, wide_b = 0;
+#pragma unroll
+    for (int i = 0; i < TM; i++) wide_a |= row_a[i] = g.a.row_e[min((size_t)mt * BM + (wm * TM + i) * 16 + li, a16 - 1)];
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) wide_b |= row_b[j][r] = g.b.row_e[min(n0 + 16 * j + 4 * lh + r, b16 - 1)];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                acc[i][j][r] = ldexpf(acc[i][j][r], fp8_row_exponent(row_a[i]) + fp8_row_exponent(row_b[j][r]));
+    if (__any((wide_a | wide_b) & 1)) {
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+            if (__any((row_a[i] | wide_b) & 1))
+                wide_sums<TN, BLOCKS>(g, (size_t)mt * (BM / 16) + wm * TM + i, n0 / 16, lane, acc[i]);
+    }
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         const size_t m0 = (size_t)mt * BM + (wm * TM + i) * 16;
-        const int ea = g.a.row_e[min(m0 + li, a16 - 1)];
 #pragma unroll
-        for (int j = 0; j < TN; j++) {
-            f32x4 v = acc[i][j];
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                v[r] = ldexpf(v[r], ea + g.b.row_e[min(n0 + 16 * j + 4 * lh + r, b16 - 1)]);
-            *reinterpret_cast<f32x4 *>(rows + li * PITCH + 16 * j + 4 * lh) = v;
-        }
+        for (int j = 0; j < TN; j++) *reinterpret_cast<f32x4 *>(rows + li * PITCH + 16 * j + 4 * lh) = acc[i][j];
         wave_sync();
         if (n < g.n) {
             for (int r0 = row0; r0 < 16 && m0 + r0 < g.m; r0 += step) {
@@ -506,35 +609,6 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
         }
         wave_sync();
     }
-}
-
-// What joins a block's sum of 16 columns of B (panel nt) to the others: exponents of the columns 4 lh .. + 3,
-// or a checkpoint's scale as a significand in [1, 2) and an exponent (far below every sum for a zero), so
-// that no intermediate is larger than the product: with the scale multiplied in behind the exponents of rows
-// whose other scales are far above it, a finite product passed the floats on its way.
-struct Scale {
-    float significand;
-    int e[4];
-};
-template <bool BLOCKS>
-__device__ __forceinline__ Scale block_scale(const Fp8Gemm &g, size_t nt, size_t b, int lh) {
-    Scale s{1.0f, {}};
-    if constexpr (BLOCKS) {
-        const float v = g.b_scales[nt / 8 * fp8_blocks(g.b.k) + b];
-        s.significand = 2.0f * __builtin_amdgcn_frexp_mantf(v);
-        const int e = v == 0.0f ? -1000 : __builtin_amdgcn_frexp_expf(v) - 1;
-#pragma unroll
-        for (int r = 0; r < 4; r++) s.e[r] = e;
-    } else {
-        const uint32_t e = *reinterpret_cast<const uint32_t *>(g.b.exps + b * fp8_rows16(g.b.rows) + nt * 16 + 4 * lh);
-#pragma unroll
-        for (int r = 0; r < 4; r++) s.e[r] = (int)((e >> (8 * r)) & 255) - 127;
-    }
-    return s;
-}
-__device__ __forceinline__ void join_block(f32x4 &acc, f32x4 part, int ea, const Scale &s) {
-#pragma unroll
-    for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(s.significand, __builtin_ldexpf(part[r], ea + s.e[r]), acc[r]);
 }
 
 // Few rows: 16 MT rows by 16 columns a workgroup, whose waves share K between them, memory

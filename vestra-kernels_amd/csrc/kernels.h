@@ -321,7 +321,7 @@ struct Fp8Rows {
     uint8_t *codes;  // [rows16 / 16][blocks] panels of 2048 bytes (k_fp8.hip)
     uint8_t *exps;   // [blocks][rows16] exponent + 127
     uint16_t *rel;   // [blocks][rows16] 2^(exponent - row_e), at least 2^-126, as the upper half of a float
-    int *row_e;      // [rows16] largest exponent of the row
+    int *row_e;      // [rows16] fp8_row() of the row's exponents
 };
 __host__ __device__ inline size_t fp8_rows16(size_t rows) { return (rows + 15) & ~(size_t)15; }
 __host__ __device__ inline size_t fp8_blocks(size_t k) { return (k + 127) / 128; }
@@ -329,13 +329,19 @@ __host__ __device__ inline uint16_t fp8_relative(int exp_code, int row_e) {
     const int e = exp_code - row_e;  // + 127
     return (uint16_t)((e > 1 ? e : 1) << 7);
 }
+// A row's largest exponent, and whether it is wide: the least of its blocks that are not all zeros is so far below it that
+// codes times 2^(exponent - largest) are no halves any more (4 bits, the least of them 2^-9: exact down to 2^-15).
+__host__ __device__ inline int fp8_row(int largest, int least) { return 2 * largest + (largest - least > 15 ? 1 : 0); }
+__host__ __device__ inline int fp8_row_exponent(int row) { return row >> 1; }
 // products_of_few: without rel and row_e, which the products of few rows do not look at.
 hipError_t launch_quantize_fp8(hipStream_t s, const float *x, const Fp8Rows &out, bool products_of_few = false);
 hipError_t launch_dequantize_fp8(hipStream_t s, const Fp8Rows &in, float *out);
 // c [m][n] = a . b^T, then the epilogue (Store: (v + bias) * gamma; Gelu: gelu(v +
 // bias); Residual: c += (v + bias) * gamma); bias and gamma may be null.  With b_scales
 // [ceil(n / 128)][blocks] these are the scales of b's codes, for 128 x 128 values, and
-// b_rel the same over 2^exponent, which b then has for all blocks of a row.
+// b_rel the same over 2^exponent, which b then has for all blocks of a row; its rows are wide
+// where a scale over 2^exponent is below kFp8LeastScale.
+constexpr float kFp8LeastScale = 0x1p-90f;  // sums of tiles are multiples of 2^-33 (2^-15 2^-9 by 2^-9): normal floats
 struct Fp8Gemm {
     Fp8Rows a, b;
     const float *b_scales, *b_rel, *bias, *gamma;

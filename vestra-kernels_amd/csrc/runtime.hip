@@ -3864,20 +3864,24 @@ static size_t fp8_at(const vh::Fp8Rows &w, size_t row, size_t d) {
            (in / 32 * 16 + row % 16) * 16 + in % 16;
 }
 
-// Row-major codes [rows][k] and exponents, at(row, block), to the device block of w.
-template <class F>
-static vh_status upload_fp8(RtState &s, const vh::Fp8Rows &w, const uint8_t *codes, F at, const char *what) {
+// Row-major codes [rows][k] and exponents, at(row, block), to the device block of w.  wide(row): whether a row is to
+// be taken for a wide one, whatever its exponents.
+template <class F, class G>
+static vh_status upload_fp8(RtState &s, const vh::Fp8Rows &w, const uint8_t *codes, F at, G wide, const char *what) {
     const size_t r16 = vh::fp8_rows16(w.rows), blocks = vh::fp8_blocks(w.k);
     std::vector<uint8_t> host(fp8_bytes(w.rows, w.k));
     const vh::Fp8Rows h = fp8_view(host.data(), w.rows, w.k);
     for (size_t r = 0; r < r16; r++) {
-        int most = -127;
+        int most = -127, least = 127;
         for (size_t b = 0; b < blocks; b++) {
             const int e = r < w.rows ? at(r, b) : 0;
             h.exps[b * r16 + r] = (uint8_t)e;
             most = std::max(most, e - 127);
+            const uint8_t *c = codes + r * w.k + b * 128;
+            if (r < w.rows && e - 127 < least && std::any_of(c, c + std::min((size_t)128, w.k - b * 128), [](uint8_t v) { return v & 127; }))
+                least = e - 127;
         }
-        h.row_e[r] = most;
+        h.row_e[r] = vh::fp8_row(most, r < w.rows && wide(r) ? most - 1000 : least);
         for (size_t b = 0; b < blocks; b++) h.rel[b * r16 + r] = vh::fp8_relative(h.exps[b * r16 + r], most);
         if (r >= w.rows) continue;
         for (size_t d = 0; d < w.k; d += 16) {
@@ -3917,7 +3921,7 @@ extern "C" vh_status vh_fp8_upload(const vh_runtime *rt, const void *codes, cons
     std::unique_ptr<vh_fp8_tensor> t(made);
     const size_t blocks = vh::fp8_blocks(k);
     TRY(upload_fp8(s, t->view, static_cast<const uint8_t *>(codes),
-                   [&](size_t r, size_t b) { return (int)e[r * blocks + b]; }, what));
+                   [&](size_t r, size_t b) { return (int)e[r * blocks + b]; }, [](size_t) { return false; }, what));
     *out = t.release();
     return VH_OK;
     GUARD_END
@@ -4109,6 +4113,7 @@ extern "C" vh_status vh_prepare_linear_fp8_blocks(const vh_runtime *rt, size_t i
     // below 2; few rows meet them as they are.
     const size_t of_row = vh::fp8_blocks(k);
     std::vector<int> exps(blocks / of_row, 0);
+    std::vector<char> wide(exps.size(), 0);
     std::vector<float> both(scales, scales + blocks);
     both.resize(2 * blocks);
     float *below = both.data() + blocks;
@@ -4116,10 +4121,13 @@ extern "C" vh_status vh_prepare_linear_fp8_blocks(const vh_runtime *rt, size_t i
         float most = 0.0f;
         for (size_t b = 0; b < of_row; b++) most = std::max(most, std::fabs(scales[i * of_row + b]));
         if (most > 0.0f) exps[i] = std::max(std::ilogb(most), -127);
-        for (size_t b = 0; b < of_row; b++) below[i * of_row + b] = std::ldexp(scales[i * of_row + b], -exps[i]);
+        for (size_t b = 0; b < of_row; b++) {
+            below[i * of_row + b] = std::ldexp(scales[i * of_row + b], -exps[i]);
+            if (scales[i * of_row + b] != 0.0f && std::fabs(below[i * of_row + b]) < vh::kFp8LeastScale) wide[i] = 1;
+        }
     }
     TRY(upload_fp8(s, l->w, static_cast<const uint8_t *>(codes), [&](size_t r, size_t) { return exps[r / 128] + 127; },
-                   "fp8 weight upload"));
+                   [&](size_t r) { return wide[r / 128] != 0; }, "fp8 weight upload"));
     TRY(upload_array(s, both.data(), 2 * blocks, &l->scales, "fp8 scale upload"));
     TRY(linear_fp8_vectors(s, bias, gamma, l.get()));
     *out = l.release();
