@@ -518,11 +518,11 @@ vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *cached, const
  * give finite rows; larger ones may pass the floats on the way.  The same call gives the
  * same bits.  At most 4096 requests, 65535 heads and 2^30 query rows (tokens * heads).
  * The parts of rows whose keys several workgroups share lie in a workspace of the
- * runtime (35 MB at most).  A call inside a stream capture takes it for its graph
- * alone, until the runtime ends, and the next call outside gets another: replays may
- * overlap with other graphs and calls.  Where none is left (nothing as large ran since
- * the last capture) the graph goes without: slower where there are few rows, its last
- * bits other than an eager call's. */
+ * runtime (35 MB at most, and as much again for the next capture).  A capture gets a
+ * block that no call has used, for its graph alone, until the runtime ends: replays may
+ * overlap with other graphs and with calls, queued ones too.  Where none is left (nothing
+ * as large ran since the last capture, or there was no memory for it) the graph goes
+ * without: slower where there are few rows, its last bits other than an eager call's. */
 vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const vh_tensor *q, size_t heads,
                                     size_t tokens, size_t requests, const vh_index *table,
                                     size_t max_pages, const vh_index *starts, const vh_index *lens,
@@ -572,9 +572,11 @@ size_t vh_linear_fp8_input_features(const vh_linear_fp8 *linear);
 size_t vh_linear_fp8_output_features(const vh_linear_fp8 *linear);
 /* out [rows, N] = (quantize(input) . W + bias) * gamma, input rows of floats quantised as
  * vh_quantize_fp8 does; gelu(quantize(input) . W + bias), without a gamma; residual +=
- * (quantize(input) . W + bias) * gamma.  The quantised rows lie in a workspace of the
- * runtime.  A call inside a stream capture takes it for its graph alone, until the
- * runtime ends; where none is left (nothing as large ran since the last capture) it is
+ * (quantize(input) . W + bias) * gamma; products and sums as vh_gemm_fp8_into forms them.
+ * The quantised rows lie in a workspace of the runtime, with a block as large for the next
+ * capture, which gets it for its graph alone, until the runtime ends: replays may overlap with
+ * other graphs and with calls, queued ones too.  Where none is left (nothing as large ran
+ * since the last capture, or there was no memory for it) a call inside a capture is
  * refused with VH_ERR_UPLOAD. */
 vh_status vh_linear_fp8_run(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows, vh_tensor *out);
 vh_status vh_linear_fp8_run_gelu(const vh_linear_fp8 *linear, const vh_tensor *input, size_t rows, vh_tensor *out);
@@ -622,10 +624,8 @@ vh_status vh_cross_kv_read_f32(const vh_cross_kv *kv, vh_tensor *k, vh_tensor *v
  * finite leaves no defined row of its image and head, a value none in its dim.  The same
  * call gives the same bits.  At most 2^30 query rows (tokens * heads) of an image.
  * The parts of rows whose keys several workgroups share lie in a workspace of the
- * runtime (70 MB at most).  A call inside a stream capture takes it for its graph alone, until
- * the runtime ends; where none is left (nothing as large ran since the last capture)
- * the graph goes without: slower where there are few rows, its last bits other than an
- * eager call's. */
+ * runtime (70 MB at most, and as much again for the next capture), for captures as that of
+ * vh_kv_cache_attention_f32. */
 vh_status vh_cross_attention_f32(const vh_cross_kv *kv, const vh_tensor *q, size_t heads, size_t tokens,
                                  int token_major, vh_tensor *out);
 

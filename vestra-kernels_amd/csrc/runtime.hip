@@ -114,6 +114,15 @@ struct Workspace {
     bool recorded = false;  // a captured graph may hold it
 };
 
+// A workspace of calls that may be captured (graph_workspace): the block of the calls outside a capture,
+// and one as large that no call has used, which the next capture takes.
+struct GraphWorkspace {
+    Workspace own, spare;
+    Workspace taken;                 // the last capture's (RtState::recorded owns it)
+    unsigned long long capture = 0;  // and that capture
+    size_t without = 0;              // own.bytes for which there was no memory for a spare
+};
+
 struct RtState {
     int device = 0;
     hipStream_t stream = nullptr;
@@ -128,12 +137,9 @@ struct RtState {
     Workspace fcnt;                             // and the in-kernel merge's arrival counters
     Workspace aq;                               // Q8_0 activation blocks
     Workspace sx;                               // split rows of a projection's input
-    Workspace f8;                               // e4m3 rows of a projection's input
-    unsigned long long f8_capture = 0;          // the capture that took it, where it is recorded
-    Workspace xa;                               // counters and parts of the cross attention's tiles
-    unsigned long long xa_capture = 0;
-    Workspace pa;                               // counters and parts of the paged attention's tiles
-    unsigned long long pa_capture = 0;          // the capture that took it, where it is recorded
+    GraphWorkspace f8;                          // e4m3 rows of a projection's input
+    GraphWorkspace xa;                          // counters and parts of the cross attention's tiles
+    GraphWorkspace pa;                          // and of the paged attention's
     std::vector<void *> recorded;               // outgrown blocks that a graph may hold
     float *tw = nullptr;                        // balanced-tail GEMM partials
     unsigned *tcnt = nullptr;                   // and arrival counters (zeroed once)
@@ -158,7 +164,7 @@ struct RtState {
         give_back();
         hipStreamSynchronize(stream);
         for (auto &kv : rope_cache) hipFree(kv.second);
-        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx, &f8, &xa, &pa})
+        for (Workspace *w : {&ws, &sk, &fw, &fcnt, &aq, &sx, &f8.own, &f8.spare, &xa.own, &xa.spare, &pa.own, &pa.spare})
             if (w->p) hipFree(w->p);
         for (void *p : recorded) hipFree(p);
         if (tw) hipFree(tw);
@@ -175,9 +181,10 @@ struct RtState {
 };
 
 // After an allocation of s has failed: the tensor blocks that the runtimes of its
-// device hold go back, what the stream-ordered pool keeps with them, and the split
+// device hold go back, what the stream-ordered pool keeps with them, the split
 // rows of s (as large as its largest call's, and taken after every other
-// allocation of a call, so that none is using them here).  A runtime that is being captured keeps its blocks.  Another thread may begin a
+// allocation of a call, so that none is using them here) and the blocks that it keeps for
+// captures.  A runtime that is being captured keeps its blocks.  Another thread may begin a
 // capture of its runtime at any moment, and a free on that stream would become
 // part of the graph: its work is waited for, and the blocks, which nothing
 // uses any more, are freed on the stream of s.  (A capture that begins during
@@ -198,6 +205,12 @@ void give_back_all(RtState &s) {
     if (s.sx.p && !s.sx.recorded) {
         hipFree(s.sx.p);
         s.sx = Workspace{};
+    }
+    for (GraphWorkspace *w : {&s.f8, &s.xa, &s.pa}) {
+        if (!w->spare.p) continue;
+        hipFree(w->spare.p);
+        w->spare = Workspace{};
+        w->without = w->own.bytes;
     }
     hipMemPool_t pool = nullptr;
     if (hipDeviceGetDefaultMemPool(&pool, s.device) == hipSuccess && pool) hipMemPoolTrimTo(pool, 0);
@@ -582,25 +595,52 @@ vh_status no_workspace(RtState &s, const char *what) {
     return fail(VH_ERR_UPLOAD, hip_msg(what, hipErrorOutOfMemory));
 }
 
-// The workspace w for a call that may be captured, or null.  A capture takes the block for
-// its graph alone: the next call outside gets another, so replays of the graph, on
-// whatever stream, and other graphs never meet in it.
-void *graph_workspace(RtState &s, Workspace &w, unsigned long long &owner, size_t bytes) {
+// The workspace w for a call that may be captured, or null; its first `zeros` bytes are zero when it is new, and every
+// call leaves them zero.  A capture takes the spare block, for its graph alone: no call outside has used it, so
+// replays of the graph, on whatever stream, meet neither a call that is still queued on the
+// runtime's nor another graph.  The next call outside makes another.
+void *graph_workspace(RtState &s, GraphWorkspace &w, size_t bytes, size_t zeros) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     unsigned long long id = 0;
     if (hipStreamGetCaptureInfo(s.stream, &st, &id) != hipSuccess) {
         hipGetLastError();
         return nullptr;
     }
-    const bool captured = st != hipStreamCaptureStatusNone;
-    if (!captured && w.recorded) {
-        s.recorded.push_back(w.p);
-        w = Workspace{};
+    if (st != hipStreamCaptureStatusNone) {
+        if (w.capture != id || w.taken.bytes < bytes) {
+            if (w.spare.bytes < bytes) return nullptr;
+            s.recorded.push_back(w.spare.p);
+            w.taken = w.spare;
+            w.spare = Workspace{};
+            w.capture = id;
+        }
+        return w.taken.p;
     }
-    if (captured && w.recorded && owner != id) return nullptr;
-    void *p = grow_workspace(s, w, bytes);
-    if (captured && p) owner = id;
-    return p;
+    const size_t had = w.own.bytes;
+    if (!grow_workspace(s, w.own, bytes)) return nullptr;
+    if (zeros && w.own.bytes != had && hipMemsetAsync(w.own.p, 0, zeros, s.stream) != hipSuccess) {
+        hipGetLastError();
+        hipFree(w.own.p);
+        w.own = Workspace{};
+        return nullptr;
+    }
+    if (w.spare.bytes < w.own.bytes && w.without != w.own.bytes) {
+        if (w.spare.p) hipFree(w.spare.p);
+        w.spare = Workspace{};
+        hipError_t e = hipMalloc(&w.spare.p, w.own.bytes);
+        // Done before a replay on another stream can begin.
+        if (e == hipSuccess && zeros) e = hipMemsetAsync(w.spare.p, 0, zeros, s.stream);
+        if (e == hipSuccess && zeros) e = hipStreamSynchronize(s.stream);
+        if (e == hipSuccess) {
+            w.spare.bytes = w.own.bytes;
+        } else {
+            hipGetLastError();
+            if (w.spare.p) hipFree(w.spare.p);
+            w.spare = Workspace{};
+            w.without = w.own.bytes;
+        }
+    }
+    return w.own.p;
 }
 
 vh_status workspace(RtState &s, size_t floats, float **out) {
@@ -3744,34 +3784,14 @@ extern "C" vh_status vh_kv_pages_assign(const vh_runtime *rt, const vh_index *ca
     GUARD_END
 }
 
-// Room for the parts of the paged attention's tiles, counters first (zeroed here;
-// every launch leaves them zero).  A capture takes the runtime's block for its graph
-// alone: the next call outside gets another, so replays of the graph, on whatever
-// stream, and other graphs never meet in it.  Without room (a capture of a size that
-// has not run since the last capture) a tile's keys stay with one workgroup.
-static void attn_workspace(RtState &s, size_t floats, vh::CacheAttn *a) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    unsigned long long id = 0;
-    if (hipStreamGetCaptureInfo(s.stream, &st, &id) != hipSuccess) {
-        hipGetLastError();
-        return;
-    }
-    const bool captured = st != hipStreamCaptureStatusNone;
-    if (!captured && s.pa.recorded) {
-        s.recorded.push_back(s.pa.p);
-        s.pa = Workspace{};
-    }
-    if (captured && s.pa.recorded && s.pa_capture != id) return;
-    const size_t head = vh::kAttnCounters * sizeof(unsigned), had = s.pa.bytes;
-    char *p = static_cast<char *>(grow_workspace(s, s.pa, head + floats * sizeof(float)));
+// Room for the parts of an attention's tiles, counters first (zero when new; every launch
+// leaves them zero).  Without room (a capture of a size that has not run since the last
+// capture) a tile's keys stay with one workgroup.
+template <class Attn>
+static void attn_workspace(RtState &s, GraphWorkspace &w, size_t floats, Attn *a) {
+    const size_t head = vh::kAttnCounters * sizeof(unsigned);
+    char *p = static_cast<char *>(graph_workspace(s, w, head + floats * sizeof(float), head));
     if (!p) return;
-    if (s.pa.bytes != had && hipMemsetAsync(p, 0, head, s.stream) != hipSuccess) {
-        hipGetLastError();
-        hipFree(p);
-        s.pa = Workspace{};
-        return;
-    }
-    if (captured) s.pa_capture = id;
     a->counters = reinterpret_cast<unsigned *>(p);
     a->parts = reinterpret_cast<float *>(p + head);
 }
@@ -3828,7 +3848,7 @@ extern "C" vh_status vh_kv_cache_attention_f32(const vh_kv_cache *cache, const v
     a.window = window < (size_t)INT32_MAX ? (int)window : 0;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.cache = cache->view;
-    attn_workspace(s, vh::cache_attn_floats(a.cache, tokens, heads / kvh, requests), &a);
+    attn_workspace(s, s.pa, vh::cache_attn_floats(a.cache, tokens, heads / kvh, requests), &a);
     return launch(s, "kv_attention", [&] { return vh::launch_cache_attn(s.stream, a); });
     GUARD_END
 }
@@ -4165,7 +4185,7 @@ static vh_status run_fp8(const vh_linear_fp8 *l, const vh_tensor *x, const vh_fp
     if (q) {
         g.a = q->view;
     } else if (plan != vh::Fp8Plan::Fused) {
-        void *p = graph_workspace(s, s.f8, s.f8_capture, fp8_bytes(rows, k));
+        void *p = graph_workspace(s, s.f8, fp8_bytes(rows, k), 0);
         if (!p) return no_workspace(s, "fp8 activation workspace");
         g.a = fp8_view(p, rows, k);
         TRY(quantize_fp8(s, x->ptr, g.a, plan == vh::Fp8Plan::Few));
@@ -4371,23 +4391,6 @@ extern "C" vh_status vh_cross_kv_read_f32(const vh_cross_kv *kv, vh_tensor *k, v
     GUARD_END
 }
 
-// Room for the parts of the tiles, counters first (zeroed here; every launch leaves them
-// zero), as attn_workspace does it for the paged attention.
-static void cross_workspace(RtState &s, size_t floats, vh::CrossAttn *a) {
-    const size_t head = vh::kAttnCounters * sizeof(unsigned);
-    const size_t had = s.xa.recorded && !capturing(s.stream) ? 0 : s.xa.bytes;  // a recorded block is left to its graph
-    char *p = static_cast<char *>(graph_workspace(s, s.xa, s.xa_capture, head + floats * sizeof(float)));
-    if (!p) return;
-    if (s.xa.bytes != had && hipMemsetAsync(p, 0, head, s.stream) != hipSuccess) {
-        hipGetLastError();
-        hipFree(p);
-        s.xa = Workspace{};
-        return;
-    }
-    a->counters = reinterpret_cast<unsigned *>(p);
-    a->parts = reinterpret_cast<float *>(p + head);
-}
-
 extern "C" vh_status vh_cross_attention_f32(const vh_cross_kv *kv, const vh_tensor *q, size_t heads, size_t tokens,
                                             int token_major, vh_tensor *out) {
     const char *what = "vh_cross_attention_f32";
@@ -4420,7 +4423,7 @@ extern "C" vh_status vh_cross_attention_f32(const vh_cross_kv *kv, const vh_tens
     a.group = (int)(heads / kvh);
     a.head_dim = (int)hd;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
-    cross_workspace(s, vh::cross_attn_floats(a), &a);
+    attn_workspace(s, s.xa, vh::cross_attn_floats(a), &a);
     return launch(s, "cross_attention", [&] { return vh::launch_cross_attn(s.stream, a); });
     GUARD_END
 }
