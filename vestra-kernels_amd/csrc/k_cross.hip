@@ -143,11 +143,11 @@ __global__ __launch_bounds__(256) void cross_range_kernel(CrossWrite w) {
     if (tid < kHeadGroup) kmax[tid] = 0;
     __syncthreads();
     const int per = w.head_dim / 4, columns = heads * per;
+    static_assert(kHeadGroup * D / 4 <= 256, "a thread for each column");
     int rows = 1;  // tokens at once
     while (rows * 2 * columns <= 256) rows *= 2;
-    for (int c0 = 0; c0 < columns; c0 += 256) {
-        const int c = rows > 1 ? tid % columns : c0 + tid, first = rows > 1 ? tid / columns : 0;
-        if (c >= columns || first >= rows) continue;
+    const int c = tid % columns, first = tid / columns;
+    if (first < rows) {
         const int h = c / per, d = 4 * (c % per);
         const size_t off = (size_t)img * w.kv_image + (h0 + h) * w.kv_head + d;
         uint32_t km = 0, vm[4] = {0, 0, 0, 0};
@@ -864,7 +864,8 @@ template <int KIND, int D>
 __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
     constexpr int BM = 16, STEP = 128, NP = kParts<KIND>, C = D / 32, DF = D / 16;
     constexpr int BLOCK = cross_block_bytes(KIND, D), WAVE = few_wave_bytes<D>();
-    __shared__ __attribute__((aligned(16))) char smem[4 * WAVE < 256 * (int)sizeof(Sums) ? 256 * sizeof(Sums) : 4 * WAVE];
+    __shared__ __attribute__((aligned(16))) char smem[4 * WAVE];
+    static_assert(4 * WAVE >= 256 * sizeof(Sums), "room for join_parts");
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lh = lane >> 4;
     const int wave = uniform(tid >> 6);
     walk<BM, STEP, 256, D, true>(a, smem, [&](const Tile &t, int step0, int steps, int part) {
@@ -1089,7 +1090,7 @@ hipError_t run_attn(hipStream_t s, CrossAttn a, bool few) {
         return hipGetLastError();
     }
     constexpr int H = kManyHalves<KIND, D>;
-    constexpr size_t bytes = std::max<size_t>(2 * H * cross_block_bytes(KIND, D), 256 * sizeof(Sums));
+    constexpr size_t bytes = 2 * H * cross_block_bytes(KIND, D);
     static std::atomic<uint64_t> done{0};
     hipError_t e = ensure_dynamic_lds(cross_many_kernel<KIND, D>, bytes, done);
     if (e != hipSuccess) return e;

@@ -404,7 +404,7 @@ __device__ __forceinline__ int fresh_lane() {
     return lane;
 }
 
-// C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  ST stages of 128 k in
+// C = A . B^T, a workgroup of WM x WN waves a tile of BM x BN.  Two stages of 128 k in
 // LDS; D^T = B . A^T, so that a lane holds four consecutive columns of its row.
 // BLOCKS: B has float scales for 128 x 128 values (b_rel) on top of its rows' exponents.
 //
@@ -415,10 +415,13 @@ __device__ __forceinline__ int fresh_lane() {
 // (waves of 32 x 32, 5) the same and the start of a tile, 865 x 768 by 3072 11.7 us.  Waves of 64 x
 // 64 for the middle ones, in tiles of 256 x 128, 133 and 136 us, in tiles of 128 of four waves, 114.5
 // and 115: fewer waves hide less.  Three stages in LDS are no faster.
-template <int BM, int BN, int WM, int WN, int ST, Epi EPI, bool BLOCKS>
+constexpr int kStages = 2;
+template <int BM, int BN>
+constexpr int kStageBytes = (BM + BN) * 128 + (BM + BN) * 2;  // codes, relative exponents
+template <int BM, int BN, int WM, int WN, Epi EPI, bool BLOCKS>
 __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-    constexpr int CODES = (BM + BN) * 128, STAGE = CODES + (BM + BN) * 2;
+    constexpr int CODES = (BM + BN) * 128, STAGE = kStageBytes<BM, BN>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr bool kSpare = TM * TN < 32;  // registers
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -463,20 +466,14 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int LD = (BM + BN) / 8 / NW + 1;  // copies of a wave and stage
     static_assert((BM + BN) / 8 % NW == 0 && BM / (NW / 2) % 8 == 0 && BN / (NW / 2) % 8 == 0 && NW % 2 == 0);
-#pragma unroll
-    for (int i = 0; i < ST - 1; i++)
-        if (i < (int)kb) copy(i, i, tid & 63);
+    copy(0, 0, tid & 63);
     for (size_t b = 0; b < kb; b++) {
-        const int buf = (int)(b % ST);
-        // This stage landed; of the later ones as many as there are may be in flight.
-        if (ST > 3 && b + 2 < kb) split_wait<(ST > 3 ? 2 : 0) * LD>();
-        else if (ST > 2 && b + 1 < kb) split_wait<(ST > 2 ? 1 : 0) * LD>();
-        else split_wait<0>();
+        const int buf = (int)(b % kStages);
+        split_wait<0>();  // this stage landed
         __builtin_amdgcn_s_barrier();
         const int lane = kSpare ? tid & 63 : fresh_lane(), li = lane & 15;
-        if (b + ST - 1 < kb) copy(b + ST - 1, (int)((b + ST - 1) % ST), lane);
+        if (b + 1 < kb) copy(b + 1, buf ^ 1, lane);
         const char *as = smem + buf * STAGE + wm * TM * 2048 + lane * 16;
         const char *bs = smem + buf * STAGE + BM * 128 + wn * TN * 2048 + lane * 16;
         const uint16_t *rs = reinterpret_cast<const uint16_t *>(smem + buf * STAGE + CODES);
@@ -546,7 +543,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
     // 16 rows at a time through LDS of the wave's own, so that a row is written in one piece,
     // whatever its alignment (1239 x 50 x 7838, no multiple of four: 63 us without, 15 with).
     constexpr int W = TN * 16, PITCH = W + 4;
-    static_assert(NW * 16 * PITCH * 4 <= ST * STAGE, "room for every wave's rows");
+    static_assert(NW * 16 * PITCH * 4 <= kStages * STAGE, "room for every wave's rows");
     __syncthreads();
     float *rows = reinterpret_cast<float *>(smem) + wave * 16 * PITCH;
     const int lane = kSpare ? tid & 63 : fresh_lane(), li = lane & 15, lh = lane >> 4;
@@ -680,18 +677,18 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Gemm g, cons
     }
 }
 
-template <int BM, int BN, int WM, int WN, int ST, Epi EPI, bool BLOCKS>
+template <int BM, int BN, int WM, int WN, Epi EPI, bool BLOCKS>
 hipError_t launch_tile(hipStream_t s, Fp8Gemm g) {
-    constexpr size_t bytes = ST * ((BM + BN) * 128 + (BM + BN) * 2);
+    constexpr size_t bytes = kStages * kStageBytes<BM, BN>;
     static std::atomic<uint64_t> done{0};
-    hipError_t e = ensure_dynamic_lds(fp8_gemm_kernel<BM, BN, WM, WN, ST, EPI, BLOCKS>, bytes, done);
+    hipError_t e = ensure_dynamic_lds(fp8_gemm_kernel<BM, BN, WM, WN, EPI, BLOCKS>, bytes, done);
     if (e != hipSuccess) return e;
     const size_t mt = (g.m + BM - 1) / BM, nt = (g.n + BN - 1) / BN;
     if (mt * nt >= kMaxThreads / (WM * WN * 64)) return hipErrorInvalidConfiguration;
     g.m_tiles = (int)mt;
     g.n_tiles = (int)nt;
     g.tiles = (int)(mt * nt);
-    fp8_gemm_kernel<BM, BN, WM, WN, ST, EPI, BLOCKS><<<(g.tiles + 7) / 8 * 8, WM * WN * 64, bytes, s>>>(g);
+    fp8_gemm_kernel<BM, BN, WM, WN, EPI, BLOCKS><<<(g.tiles + 7) / 8 * 8, WM * WN * 64, bytes, s>>>(g);
     return hipGetLastError();
 }
 
@@ -706,9 +703,9 @@ hipError_t launch_epi(hipStream_t s, const Fp8Gemm &g, Fp8Plan plan, const float
         else fp8_few_kernel<4, false, BLOCKS, EPI><<<grid, threads, 0, s>>>(g, nullptr);
         return hipGetLastError();
     }
-    if (plan == Fp8Plan::Tile64) return launch_tile<64, 64, 2, 2, 2, EPI, BLOCKS>(s, g);
-    if (plan == Fp8Plan::Tile128) return launch_tile<128, 128, 2, 4, 2, EPI, BLOCKS>(s, g);
-    return launch_tile<256, 256, 2, 4, 2, EPI, BLOCKS>(s, g);
+    if (plan == Fp8Plan::Tile64) return launch_tile<64, 64, 2, 2, EPI, BLOCKS>(s, g);
+    if (plan == Fp8Plan::Tile128) return launch_tile<128, 128, 2, 4, EPI, BLOCKS>(s, g);
+    return launch_tile<256, 256, 2, 4, EPI, BLOCKS>(s, g);
 }
 
 template <bool BLOCKS>
