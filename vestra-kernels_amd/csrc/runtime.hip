@@ -120,7 +120,7 @@ struct GraphWorkspace {
     Workspace own, spare;
     Workspace taken;                 // the last capture's (RtState::recorded owns it)
     unsigned long long capture = 0;  // and that capture
-    size_t without = 0;              // own.bytes for which there was no memory for a spare
+    bool wanted = true;              // a spare; false once there is one, or was no memory for it
 };
 
 struct RtState {
@@ -210,7 +210,7 @@ void give_back_all(RtState &s) {
         if (!w->spare.p) continue;
         hipFree(w->spare.p);
         w->spare = Workspace{};
-        w->without = w->own.bytes;
+        w->wanted = true;
     }
     hipMemPool_t pool = nullptr;
     if (hipDeviceGetDefaultMemPool(&pool, s.device) == hipSuccess && pool) hipMemPoolTrimTo(pool, 0);
@@ -608,6 +608,7 @@ void *graph_workspace(RtState &s, GraphWorkspace &w, size_t bytes, size_t zeros)
     }
     if (st != hipStreamCaptureStatusNone) {
         if (w.capture != id || w.taken.bytes < bytes) {
+            w.wanted = true;
             if (w.spare.bytes < bytes) return nullptr;
             s.recorded.push_back(w.spare.p);
             w.taken = w.spare;
@@ -624,10 +625,12 @@ void *graph_workspace(RtState &s, GraphWorkspace &w, size_t bytes, size_t zeros)
         w.own = Workspace{};
         return nullptr;
     }
-    if (w.spare.bytes < w.own.bytes && w.without != w.own.bytes) {
+    if (w.own.bytes != had) w.wanted = true;
+    if (w.wanted && w.spare.bytes < w.own.bytes) {
         if (w.spare.p) hipFree(w.spare.p);
         w.spare = Workspace{};
         hipError_t e = hipMalloc(&w.spare.p, w.own.bytes);
+        if (e != hipSuccess) w.spare.p = nullptr;
         // Done before a replay on another stream can begin.
         if (e == hipSuccess && zeros) e = hipMemsetAsync(w.spare.p, 0, zeros, s.stream);
         if (e == hipSuccess && zeros) e = hipStreamSynchronize(s.stream);
@@ -637,9 +640,9 @@ void *graph_workspace(RtState &s, GraphWorkspace &w, size_t bytes, size_t zeros)
             hipGetLastError();
             if (w.spare.p) hipFree(w.spare.p);
             w.spare = Workspace{};
-            w.without = w.own.bytes;
         }
     }
+    w.wanted = false;
     return w.own.p;
 }
 
