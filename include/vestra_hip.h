@@ -620,7 +620,8 @@ vh_status vh_cross_kv_read_f32(const vh_cross_kv *kv, vh_tensor *k, vh_tensor *v
  * [images, tokens, heads, head_dim] when token_major; heads % kv_heads == 0 and query head
  * h reads head h / (heads / kv_heads).  The number of queries has nothing to do with
  * that of the states.  Zeros where an image has no token to see.  A query row is scaled and
- * held in two halves as type 0 is; statistics and sums are 32 bits.  A key that is not
+ * held in two halves as type 0 is; statistics and sums are 32 bits, weights are held to within
+ * 2^-34 of the largest of their row before they meet the values.  A key that is not
  * finite leaves no defined row of its image and head, a value none in its dim.  The same
  * call gives the same bits.  At most 2^30 query rows (tokens * heads) of an image.
  * The parts of rows whose keys several workgroups share lie in a workspace of the

@@ -939,8 +939,8 @@ __global__ __launch_bounds__(256, 2) void cross_few_kernel(CrossAttn a) {
 
 // ---- many rows: 128 a tile, 32 a wave, K and V of a step shared in LDS ----------------------
 // Bound by the matrix cores and the vector instructions of the softmax at the clock that both leave
-// (1.9 GHz): in halves 49% and 60% of the cycles, 3457 queries of 12 heads of 64 against 20742 keys
-// 447 us, 960 TFLOP/s; in two halves 53% and 50%, of 128 62% and 39%, 1030 TFLOP/s (2 x 865
+// (1.9 to 2 GHz): in halves 49% and 60% of the cycles, 3457 queries of 12 heads of 64 against 20742 keys
+// 447 us, 986 TFLOP/s; in two halves 53% and 50%, of 128 62% and 39%, 1030 TFLOP/s (2 x 865
 // queries of 32 / 8 heads against 4000 keys 331 us).  The next step's scores between this step's
 // weights, an instruction of the one to four or five of the other, take 5% longer (469, 340).
 

@@ -409,8 +409,9 @@ __device__ __forceinline__ int fresh_lane() {
 // BLOCKS: B has float scales for 128 x 128 values (b_rel) on top of its rows' exponents.
 //
 // What bounds it: tiles of 256 (waves of 128 x 64, 1.7 other vector instructions a matrix
-// instruction) the matrix cores at the clock that they leave, 13824 x 4096 by 8192 735 us, 1325
-// TFLOP/s, where a library's product of 8192^3 halves has 1139; tiles of 128 (waves of 64 x 32, 3.5,
+// instruction) the matrix cores at the clock that they leave, 13824 x 4096 by 8192 721 us, 1286
+// TFLOP/s at 2.15 GHz in a row of a hundred (the first ones after a pause take 750 to 910 us, at 2.06 down
+// to 1.7 GHz), where a library's product of 8192^3 halves has 1139; tiles of 128 (waves of 64 x 32, 3.5,
 // with BLOCKS 4.5) the issue of instructions, 4001 x 2200 by 5001 107 us, BLOCKS 114; tiles of 64
 // (waves of 32 x 32, 5) the same and the start of a tile, 865 x 768 by 3072 11.7 us.  Waves of 64 x
 // 64 for the middle ones, in tiles of 256 x 128, 133 and 136 us, in tiles of 128 of four waves, 114.5
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_gemm_kernel(Fp8Gemm g) {
         }
     }
     // 16 rows at a time through LDS of the wave's own, so that a row is written in one piece,
-    // whatever its alignment (1239 x 50 x 7838, no multiple of four: 63 us without, 15 with).
+    // whatever its alignment (1239 x 50 x 7838, no multiple of four, from floats: 63 us without, 25 with).
     constexpr int W = TN * 16, PITCH = W + 4;
     static_assert(NW * 16 * PITCH * 4 <= kStages * STAGE, "room for every wave's rows");
     __syncthreads();
