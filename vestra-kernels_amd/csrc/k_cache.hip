@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(CacheRows a) {
             if (rope.pairs) {
                 float *buf = exchange[wave][u];
                 reinterpret_cast<f32x4 *>(buf)[lane] = y;
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                wave_sync();
                 const float *mine = buf + sub * a.head_dim;
                 const bool turned = row < a.heads + a.kv_heads;
 #pragma unroll
@@ -150,6 +150,7 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(CacheRows a) {
                     const float r = add_rn(mul_rn(y[e], sc[1]), mul_rn(w, s));
                     if (turned && pair[e] >= 0) y[e] = r;
                 }
+                wave_sync();
             }
             const bool live = used && row < total_rows;
             if (row < a.heads && live) {

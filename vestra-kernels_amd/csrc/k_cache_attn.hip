@@ -130,7 +130,6 @@ __device__ __forceinline__ bf16x4 read_tr(const char *p) {
     return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                           (__attribute__((address_space(3))) s16x4 *)p));
 }
-__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 __device__ __forceinline__ bool finite8(f32x4 a, f32x4 b) {
     uint32_t m = 0;
@@ -928,7 +927,7 @@ __global__ __launch_bounds__(256, (few_workgroups<KIND, D>())) void few_rows_ker
             load(a.cache.v, a.cache.vd, slot);
             const int next = slot_of(a, key_of(i + 1), next_page);
             next_page = page_of(a, t, key_of(i + 2));
-            wave_fence();
+            wave_sync();
             f32x4 sx[1][2][1];
             f32x4(&s)[2][1] = sx[0];
             s[0][0] = s[1][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -962,7 +961,7 @@ __global__ __launch_bounds__(256, (few_workgroups<KIND, D>())) void few_rows_ker
                         s[j][0] = y[j];
                     }
             }
-            wave_fence();
+            wave_sync();
             if (partial) w.mask(s, key, present, lh);
             w.raise(sx, a.scale_log2);
             w.weights(s, a.scale_log2);
@@ -981,7 +980,7 @@ __global__ __launch_bounds__(256, (few_workgroups<KIND, D>())) void few_rows_ker
             }
             slot = next;
             load(a.cache.k, a.cache.kd, slot);
-            wave_fence();
+            wave_sync();
             const int vrow = 4 * lh + (li >> 2);
             const char *v = mine + vrow * (D * 2) + (li & 1) * 8;
             const int vx = v_swizzle<D>(vrow), vg = (li & 3) >> 1;
@@ -1003,7 +1002,7 @@ __global__ __launch_bounds__(256, (few_workgroups<KIND, D>())) void few_rows_ker
                 split3(s[0][0], s[1][0], p[0]);
                 w.template add<NP, 0, D / 16>(v, PLANE, vx, vg, p);
             }
-            wave_fence();
+            wave_sync();
             if (__any(dropped)) add_not_finite<KIND>(a, t, g, w, key, lh);
         }
         // The four waves' sums, each on its own maximum, joined by all threads.
