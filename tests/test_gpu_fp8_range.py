@@ -142,3 +142,19 @@ def test_nan_stays_in_its_row_of_wide_range(rt, m, k, n):
     bad[m // 2], bad[:, n // 3] = True, True
     assert np.isnan(got[bad]).all()
     _close(got[~bad], want[~bad], 1.13 * size[~bad], k)  # the codes' values: each within 2^-4 of its own
+
+
+@pytest.mark.parametrize("m, k, n", [(40, 512, 300), (2000, 520, 1100), (3000, 520, 2100), (3500, 384, 4300)])
+@pytest.mark.parametrize("gap", [14, 15, 16, 17])
+def test_the_least_codes_at_the_border_of_wide_rows(rt, m, k, n, gap):
+    """Blocks `gap` powers of two below the first one of their row, of the least codes there are, whose sums are
+    what comes out, to the bit: every product is a multiple of 2^-9 by one of 1, 2 or 4, below 2^24 of them in all."""
+    a = np.zeros((m, k), np.float32)
+    a[:, 0], a[:, 128::128] = 448.0 * 2.0 ** gap, 448.0  # the exponents gap and 0
+    a[:, 129:160] = (1 + (np.arange(m)[:, None] + np.arange(31)) % 7) * 2.0 ** -9
+    b = np.zeros((n, k), np.float32)
+    b[:, 129:160] = 2.0 ** ((np.arange(n)[:, None] + np.arange(31)) % 3)
+    want = a[:, 129:160].astype(np.float64) @ b[:, 129:160].T.astype(np.float64)
+    c = rt.upload_f32(np.full(m * n, np.nan))
+    rt.gemm_fp8_into(*(rt.quantize_fp8(rt.upload_f32(x), *x.shape) for x in (a, b)), c)
+    assert np.array_equal(rt.download_f32(c).reshape(m, n), want)
